@@ -115,6 +115,23 @@ class PermuteArgs(ctypes.Structure):
     _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p)]
 
 
+class KvDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("B", "T", "S_q", "H", "H_kv", "D", "n_pages", "page_size", "max_pages",
+                                            "format", "dtype", "causal", "ld_q", "ld_k", "ld_v")]
+
+
+class KvWriteArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("K", "V", "cache", "row_start", "kv_len", "table")]
+
+
+class KvReadArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("cache", "row_start", "kv_len", "table", "K", "V")]
+
+
+class KvAttnArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("Q", "cache", "row_start", "kv_len", "table", "O", "lse", "workspace")]
+
+
 class Timing(ctypes.Structure):
     _fields_ = [("total_ms", ctypes.c_double), ("kernel_ms", ctypes.c_double * 4), ("n_kernels", ctypes.c_int),
                 ("kernel_names", (ctypes.c_char * 64) * 4)]
@@ -158,6 +175,13 @@ SIGNATURES = {
     "mtk_conv_run": (ctypes.c_int, [_VP, ctypes.POINTER(ConvArgs)]),
     "mtk_permute_plan": (ctypes.c_int, [_VP, ctypes.POINTER(PermuteDesc), _PP]),
     "mtk_permute_run": (ctypes.c_int, [_VP, ctypes.POINTER(PermuteArgs)]),
+    "mtk_kv_cache_bytes": (ctypes.c_int, [ctypes.POINTER(KvDesc), ctypes.POINTER(ctypes.c_size_t)]),
+    "mtk_kv_write_plan": (ctypes.c_int, [_VP, ctypes.POINTER(KvDesc), _PP]),
+    "mtk_kv_write_run": (ctypes.c_int, [_VP, ctypes.POINTER(KvWriteArgs)]),
+    "mtk_kv_read_plan": (ctypes.c_int, [_VP, ctypes.POINTER(KvDesc), _PP]),
+    "mtk_kv_read_run": (ctypes.c_int, [_VP, ctypes.POINTER(KvReadArgs)]),
+    "mtk_kv_attn_plan": (ctypes.c_int, [_VP, ctypes.POINTER(KvDesc), _PP]),
+    "mtk_kv_attn_run": (ctypes.c_int, [_VP, ctypes.POINTER(KvAttnArgs)]),
     "mtk_plan_workspace_bytes": (ctypes.c_size_t, [_VP]),
     "mtk_plan_describe": (ctypes.c_int, [_VP, ctypes.c_char_p, ctypes.c_size_t]),
     "mtk_plan_work": (ctypes.c_int, [_VP, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]),
@@ -534,6 +558,99 @@ class ConvPlan(_Plan):
         self._run(self.args(x, w, bias, y, workspace))
 
 
+# ------------------------------------------------------------------ paged key/value cache in few bits
+
+KV_FP4, KV_FP8 = 0, 1
+_KV_FORMATS = {"fp4": KV_FP4, "fp8": KV_FP8}
+
+
+def kv_cache_bytes(n_pages, page_size, H_kv, D, format="fp4") -> int:
+    """Bytes of a cache of n_pages pages of page_size positions (mtk_kv_cache_bytes)."""
+    d = KvDesc(n_pages=n_pages, page_size=page_size, H_kv=H_kv, D=D, format=_KV_FORMATS[format])
+    n = ctypes.c_size_t()
+    _check(lib().mtk_kv_cache_bytes(ctypes.byref(d), ctypes.byref(n)))
+    return int(n.value)
+
+
+class _KvPlan(_Plan):
+    _plan_fn = None
+
+    def __init__(self, device: Device | None, **fields):
+        fields["format"], fields["dtype"] = _KV_FORMATS[fields["format"]], _DT[fields["dtype"]]
+        self.desc = KvDesc(**fields)
+        h = ctypes.c_void_p()
+        _check(getattr(lib(), self._plan_fn)(device.handle if device else None, ctypes.byref(self.desc), ctypes.byref(h)))
+        super().__init__(h)
+
+
+class KvWritePlan(_KvPlan):
+    """Rows of K and V ([T][H_kv][D], ld_k / ld_v elements apart) into a paged cache in few bits. row_start [B + 1],
+    kv_len [B] and table [B][max_pages] are int32 on the device: row i of sequence b is position
+    kv_len[b] - (its rows) + i. include/mtk.h has the format."""
+
+    _args_type = KvWriteArgs
+    _run_fn = "mtk_kv_write_run"
+    _plan_fn = "mtk_kv_write_plan"
+
+    def __init__(self, device: Device | None, B, T, H_kv, D, *, n_pages, page_size, max_pages, format="fp4", dtype="f16",
+                 ld_k=0, ld_v=0):
+        super().__init__(device, B=B, T=T, H_kv=H_kv, D=D, n_pages=n_pages, page_size=page_size, max_pages=max_pages,
+                         format=format, dtype=dtype, ld_k=ld_k, ld_v=ld_v)
+
+    @staticmethod
+    def args(K, V, cache, row_start, kv_len, table) -> KvWriteArgs:
+        return KvWriteArgs(K=_ptr(K), V=_ptr(V), cache=_ptr(cache), row_start=_ptr(row_start), kv_len=_ptr(kv_len),
+                           table=_ptr(table))
+
+    def run(self, K, V, cache, row_start, kv_len, table):
+        self._run(self.args(K, V, cache, row_start, kv_len, table))
+
+
+class KvReadPlan(_KvPlan):
+    """The cached rows back in 16 bits, packed as KvWritePlan takes them (with row_start over whole sequences: a
+    cached prefix)."""
+
+    _args_type = KvReadArgs
+    _run_fn = "mtk_kv_read_run"
+    _plan_fn = "mtk_kv_read_plan"
+
+    def __init__(self, device: Device | None, B, T, H_kv, D, *, n_pages, page_size, max_pages, format="fp4", dtype="f16",
+                 ld_k=0, ld_v=0):
+        super().__init__(device, B=B, T=T, H_kv=H_kv, D=D, n_pages=n_pages, page_size=page_size, max_pages=max_pages,
+                         format=format, dtype=dtype, ld_k=ld_k, ld_v=ld_v)
+
+    @staticmethod
+    def args(cache, row_start, kv_len, table, K, V) -> KvReadArgs:
+        return KvReadArgs(cache=_ptr(cache), row_start=_ptr(row_start), kv_len=_ptr(kv_len), table=_ptr(table), K=_ptr(K),
+                          V=_ptr(V))
+
+    def run(self, cache, row_start, kv_len, table, K, V):
+        self._run(self.args(cache, row_start, kv_len, table, K, V))
+
+
+class KvAttentionPlan(_KvPlan):
+    """O = softmax(Q K^T / sqrt(D)) V over the positions of a paged cache: Q [T][H][D] (ld_q elements between rows),
+    O [T][H][D], lse [T][H] fp32 if given; at most S_q rows per sequence (0: T). causal: row i sees the positions up to
+    its own. Needs a workspace where the keys may be split over workgroups."""
+
+    _args_type = KvAttnArgs
+    _run_fn = "mtk_kv_attn_run"
+    _plan_fn = "mtk_kv_attn_plan"
+
+    def __init__(self, device: Device | None, B, T, H, H_kv, D, *, n_pages, page_size, max_pages, S_q=0, format="fp4",
+                 dtype="f16", causal=True, ld_q=0):
+        super().__init__(device, B=B, T=T, S_q=S_q, H=H, H_kv=H_kv, D=D, n_pages=n_pages, page_size=page_size,
+                         max_pages=max_pages, format=format, dtype=dtype, causal=1 if causal else 0, ld_q=ld_q)
+
+    @staticmethod
+    def args(Q, cache, row_start, kv_len, table, O, lse=None, workspace=None) -> KvAttnArgs:
+        return KvAttnArgs(Q=_ptr(Q), cache=_ptr(cache), row_start=_ptr(row_start), kv_len=_ptr(kv_len), table=_ptr(table),
+                          O=_ptr(O), lse=_ptr(lse), workspace=_ptr(workspace))
+
+    def run(self, Q, cache, row_start, kv_len, table, O, lse=None, workspace=None):
+        self._run(self.args(Q, cache, row_start, kv_len, table, O, lse, workspace))
+
+
 # ------------------------------------------------------------------ harness-level calls
 
 def gemm(dev: Device, A, B, bias=None, *, trans_b=True, dtype="f16", split_k=1, tile=0,
@@ -625,5 +742,5 @@ def validate(actual, expected, abs_tol: float, dtype="f16") -> dict:
     return {"rel_frobenius": v.rel_frobenius, "max_abs_error": v.max_abs_error, "mismatches": int(v.mismatches)}
 
 
-__all__ = ["Device", "DeviceBuffer", "GemmPlan", "AttentionPlan", "ConvPlan", "conv_desc", "gemm", "attention",
-           "conv", "validate", "MtkError", "lib", "SIGNATURES"]
+__all__ = ["Device", "DeviceBuffer", "GemmPlan", "AttentionPlan", "ConvPlan", "KvWritePlan", "KvReadPlan",
+           "KvAttentionPlan", "kv_cache_bytes", "conv_desc", "gemm", "attention", "conv", "validate", "MtkError", "lib", "SIGNATURES"]

@@ -9,7 +9,7 @@
 
 #include <stdint.h>
 
-#define MTK_KARGS_VERSION 16
+#define MTK_KARGS_VERSION 17
 
 /* In-workgroup split-K: bytes of workspace slot per output tile of BM x BM (256 or 128). Each
  * wavefront keeps these accumulator blocks (32 x 32 fp32, 4 KB) of its running sum in the slot,
@@ -143,5 +143,39 @@ typedef struct {
   void *dst;       /* [KD][KH][KW][C][O] */
   int32_t O, C, T; /* T = KD * KH * KW */
 } mtk_permute_args;
+
+/* Rows written into, or read back from, a paged cache in few bits (kv_cache.h has its layout). */
+typedef struct {
+  const void *K, *V; /* write: rows in; read: rows out (written through) */
+  void *cache;
+  const int32_t *row_start, *kv_len, *table;
+  int64_t ld_k, ld_v; /* elements between rows */
+  int32_t B, T, H_kv, D;
+  int32_t blocks;     /* blocks of 32 dims of a head */
+  int32_t page_shift; /* log2 of the positions per page */
+  int32_t n_pages, max_pages;
+  int32_t parts; /* wavefronts that share a row */
+} mtk_kv_move_kargs;
+
+/* Attention over a paged cache in few bits. */
+typedef struct {
+  const void *Q;
+  const void *cache;
+  const int32_t *row_start, *kv_len, *table;
+  void *O;
+  float *lse; /* [T][H] or NULL */
+  float *part, *part_ml;
+  int64_t ld_q; /* elements between rows of Q */
+  int32_t B, T, S_q, H, H_kv, D;
+  int32_t blocks, page_shift, n_pages, max_pages;
+  int32_t causal;
+  float scale_log2; /* log2(e) / sqrt(D) */
+  /* the sequences of this launch: those with more than rows_above and at most rows_most (row, query head)
+   * pairs per K/V head */
+  int32_t rows_above, rows_most;
+  /* splits of the keys (kv_cache.h): workgroups wanted, least steps of a split, most workgroups */
+  int32_t units, least, max_units;
+  int32_t part_ld; /* floats per row of part */
+} mtk_kv_attn_kargs;
 
 #endif

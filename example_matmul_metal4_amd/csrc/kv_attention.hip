@@ -1,0 +1,436 @@
+// Attention over a paged key/value cache in few bits (fp4 or fp8 blocks of 32 dims with a power-of-two scale,
+// kv_cache.h), ragged batch, grouped heads: few rows per sequence (a decode step, drafted tokens).
+//
+//   O[i][h] = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(q_i . k_j / sqrt(D)),  j <= position of row i (causal)
+//
+// with k_j, v_j the cached values. One pass over the keys with a running exponent offset and sum per row (fp32).
+//   * A workgroup has one (sequence, K/V head, 16 NR rows of (row, query head) pairs, split of the keys); its 4
+//     wavefronts take every 4th tile of 32 keys. Which split is found on the device from the lengths themselves
+//     (find_unit), so that a captured launch serves any lengths.
+//   * K: a lane has the codes of one key and a quarter of the head's dims: exactly an operand of the 16x16x32
+//     MFMA (the dims may be summed in any order, Q is loaded in the same one). They go from the load through
+//     v_cvt_scalef32_pk (two codes and their scale per instruction, exact) into S^T = K Q^T without LDS.
+//   * S^T leaves each lane with 4 keys of one row per 16 keys, which is the operand layout of P^T in
+//     O^T = V^T P^T. V^T needs 8 keys of one dim per lane: V is converted the same way, written to the
+//     wavefront's own LDS tile and read back transposed (ds_read_b64_tr_b16).
+//   * P is rounded to the 16-bit type for the MFMA (2^-9 or 2^-12 of its value, averaged over the keys); scores,
+//     offsets and sums stay in fp32.
+//   * Keys past the length have their V codes zeroed (a page's unused rows may hold anything); a NaN block's V is
+//     zeroed too and its dims set to NaN only for the rows that see the key, so that nothing masked reaches O.
+#include "kv_device.hpp"
+
+namespace mtk {
+
+constexpr int kKvTile = 32;               // keys per tile
+constexpr int kKvWaves = 4;               // wavefronts per workgroup
+constexpr int kKvStep = kKvTile * kKvWaves;
+constexpr float kKvSlack = 8.0f;          // log2-domain headroom before O is rescaled
+
+// max over the lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float quarters_max(float x) {
+  x = half_max(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  const uint32_t r0 = r[0], r1 = r[1];
+  return __builtin_elementwise_maximum(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
+}
+__device__ __forceinline__ float quarters_sum(float x) {
+  x = half_sum(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  const uint32_t r0 = r[0], r1 = r[1];
+  return __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
+}
+
+// Sums of some keys of a row (4 dims), unscaled, with their exponent offset (log2) and the sum of the weights.
+struct KvPart {
+  float m = -INFINITY, l = 0.0f;
+  f32x4 x = f32x4{};
+};
+__device__ __forceinline__ void add_part(KvPart &s, const KvPart &t) {
+  const float m = fmaxf(s.m, t.m);
+  const float m0 = m == -INFINITY ? 0.0f : m;
+  const float f = __builtin_amdgcn_exp2f(s.m - m0), g = __builtin_amdgcn_exp2f(t.m - m0);
+  // an offset of -inf has no keys, or only NaN scores: its sums count as they are
+  s.l = s.l * (s.m == -INFINITY ? 1.0f : f) + t.l * (t.m == -INFINITY ? 1.0f : g);
+  s.x = s.x * (s.m == -INFINITY ? 1.0f : f) + t.x * (t.m == -INFINITY ? 1.0f : g);
+  s.m = m;
+}
+
+// 4 dims of (packed row, query head) from d on; the row's log-sum-exp with d == 0.
+template <int DT>
+__device__ __forceinline__ void store_out(const mtk_kv_attn_kargs &a, int row, int h, int d, const KvPart &s) {
+  const float inv = s.l != 0.0f ? 1.0f / s.l : 0.0f;  // no key: 0; NaN stays
+  if (d < a.D)
+    *(u32x2 *)((uint16_t *)a.O + ((size_t)row * a.H + h) * a.D + d) =
+        u32x2{pack2<DT>(s.x.x * inv, s.x.y * inv), pack2<DT>(s.x.z * inv, s.x.w * inv)};
+  if (d == 0 && a.lse)
+    a.lse[(size_t)row * a.H + h] = s.l == 0.0f ? -INFINITY : (s.m == -INFINITY ? s.l : s.m + __builtin_amdgcn_logf(s.l)) * 0.6931471805599453f;
+}
+
+template <int DT, int FMT, int DP, int NR>
+__device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
+  constexpr int kRows = 16 * NR;
+  constexpr int kFr = DP / 32;                // operands of 8 dims per lane and key
+  constexpr int kW8 = kWords8<FMT>;
+  constexpr int kRaw = kFr * kW8;             // words of codes per lane and key
+  constexpr int kSc = DP == 256 ? 2 : 1;      // scales per lane and key
+  constexpr int kKb = kKvTile / 16;           // 16-key blocks per tile
+  constexpr int kDb = DP / 16;                // 16-dim blocks of O
+  constexpr int kVRowB = 2 * DP;
+  constexpr int kWaveB = kKvTile * kVRowB;
+  constexpr int kPitch = DP + 4;              // floats per parked row
+  constexpr int kParkB = 16 * kPitch * 4;
+  __shared__ __attribute__((aligned(1024))) char smem[kKvWaves * (kWaveB > kParkB ? kWaveB : kParkB)];
+  __shared__ float sm_m[kKvWaves][16], sm_l[kKvWaves][16];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 15, j = lane >> 4;
+  const int G = a.H / a.H_kv;
+
+  int id = -1;
+  const KvUnit u = find_unit<kRows, kKvStep>(a, lane, -1, [&](int total) {
+    total = min(total, a.max_units);
+    return id = (int)blockIdx.x < total ? xcd_remap(blockIdx.x, total) : -1;
+  });
+  if (u.b < 0) return;
+  int rest = id - u.base;
+  const int hk = rest % a.H_kv;
+  rest /= a.H_kv;
+  const int rb = rest % u.share.blocks, split = rest / u.share.blocks;
+  const kv_seq seq = u.seq;
+  const int rows = min(seq.rows, a.S_q) * G;
+  const int32_t *table = a.table + (size_t)u.b * a.max_pages;
+  const int row_b = kv_row_bytes(FMT, a.blocks);
+  const uint64_t region = kv_region_bytes(FMT, a.blocks, a.page_shift);
+  const int page_mask = (1 << a.page_shift) - 1;
+  const uint32_t k_scales = (uint32_t)(2 * row_b) << a.page_shift, v_codes = (uint32_t)row_b << a.page_shift;
+  const uint32_t v_scales = k_scales + ((uint32_t)a.blocks << a.page_shift);
+
+  // ---- Q, as the operand of S^T: row c of each 16, this lane's dims
+  auto dim = [&](int f) { return DP == 64 ? 16 * j + 8 * f : 128 * (f >> 2) + 32 * j + 8 * (f & 3); };
+  u32x4 qf[NR][kFr];
+  int lim[NR];  // the last key that this lane's row sees
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const int r = rb * kRows + 16 * n + c;
+    const int i = r / G;
+    const int64_t pos = a.causal ? seq.pos0 + i : (int64_t)seq.keys - 1;
+    lim[n] = r < rows && pos >= 0 ? (int)min(pos, (int64_t)seq.keys - 1) : -1;
+    const uint16_t *q = (const uint16_t *)a.Q + (size_t)(seq.first + i) * a.ld_q + (size_t)(hk * G + r - i * G) * a.D;
+#pragma unroll
+    for (int f = 0; f < kFr; ++f)
+      qf[n][f] = r < rows && dim(f) < a.D ? *(const u32x4 *)(q + dim(f)) : u32x4{0u, 0u, 0u, 0u};
+  }
+  // keys that the rows of this workgroup see at all, and those that every one of them sees
+  const int r_last = min(rb * kRows + kRows, rows) - 1;
+  const int64_t p_first = a.causal ? seq.pos0 + rb * kRows / G : (int64_t)seq.keys - 1;
+  const int64_t p_last = a.causal ? seq.pos0 + r_last / G : (int64_t)seq.keys - 1;
+  const int n_keys = (int)max((int64_t)0, min((int64_t)seq.keys, p_last + 1));
+  const int all_see = (int)max((int64_t)0, min((int64_t)seq.keys, p_first + 1));
+  const int per = u.share.per * kKvStep;
+  const int key_end = min(n_keys, (split + 1) * per);
+
+  // ---- this lane's place in a row of codes
+  constexpr int kHalf = FMT == KV_FP4 ? 8 : 16;  // bytes of half a block
+  const int blk0 = DP == 64 ? j >> 1 : j;
+  const uint32_t code_at = DP == 64 ? (uint32_t)(blk0 * 2 * kHalf + (j & 1) * kHalf) : (uint32_t)(blk0 * 2 * kHalf);
+  struct Tile {
+    uint32_t k[kKb][kRaw], v[kKb][kRaw], ks[kKb][kSc], vs[kKb][kSc];
+    uint32_t bad = 0;  // 16-key blocks whose page is not one
+  };
+  auto load = [&](Tile &t, int key0) {
+    t.bad = 0;
+#pragma unroll
+    for (int kb = 0; kb < kKb; ++kb) {
+      const int key = key0 + 16 * kb;
+      const int page = key < n_keys && !seq.bad ? kv_page(table, key, a.n_pages, a.max_pages, a.page_shift) : -1;
+      const int at = __builtin_amdgcn_readfirstlane(page);
+      if (at < 0 && key < n_keys) t.bad |= 1u << kb;
+      const char *p = (const char *)a.cache + ((uint64_t)(uint32_t)max(at, 0) * a.H_kv + hk) * region;
+      const uint32_t off = (uint32_t)((key & page_mask) + c);
+#pragma unroll
+      for (int s = 0; s < kSc; ++s) {
+        const int blk = blk0 + 4 * s;
+        constexpr int kN = kRaw / kSc;
+        uint32_t *kw = t.k[kb] + s * kN, *vw = t.v[kb] + s * kN;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) kw[i] = vw[i] = 0;
+        t.ks[kb][s] = t.vs[kb][s] = 127;
+        if (at >= 0 && blk < a.blocks) {
+          const uint32_t o = off * (uint32_t)row_b + code_at + (DP == 256 ? s * 8u * kHalf : 0u);
+          const uint32_t so = off * (uint32_t)a.blocks + (uint32_t)blk;
+          if constexpr (kN == 2) {
+            const u32x2 x = *(const u32x2 *)(p + o), y = *(const u32x2 *)(p + v_codes + o);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) kw[i] = x[i], vw[i] = y[i];
+          } else {
+#pragma unroll
+            for (int q = 0; q < kN / 4; ++q) {
+              const u32x4 x = *(const u32x4 *)(p + o + 16 * q), y = *(const u32x4 *)(p + v_codes + o + 16 * q);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) kw[4 * q + i] = x[i], vw[4 * q + i] = y[i];
+            }
+          }
+          t.ks[kb][s] = *(const uint8_t *)(p + k_scales + so);
+          t.vs[kb][s] = *(const uint8_t *)(p + v_scales + so);
+        }
+      }
+    }
+  };
+
+  char *vt = smem + wave * kWaveB;
+  auto vswz = [](int r) {
+    return DP == 64 ? (((r >> 1) & 3) << 1) | ((r >> 3) & 1) : ((r & 7) << 1) | ((r >> 3) & 1);
+  };
+  const float cl = a.scale_log2;
+  float m_off[NR], l_run[NR];
+  f32x4 o[NR][kDb];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    m_off[n] = -INFINITY;
+    l_run[n] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < kDb; ++d) o[n][d] = f32x4{};
+  }
+
+  Tile t;
+  int key0 = split * per + wave * kKvTile;
+  if (key0 < key_end) load(t, key0);
+  for (; key0 < key_end; key0 += kKvStep) {
+    // ---- NaN blocks and pages that are none: bit k of kn (vn[s]) is key k of the tile
+    uint32_t kn = 0, vn[kSc][4] = {};
+    bool nan = t.bad != 0;
+#pragma unroll
+    for (int kb = 0; kb < kKb; ++kb)
+#pragma unroll
+      for (int s = 0; s < kSc; ++s) nan |= max(t.ks[kb][s], t.vs[kb][s]) == kNanScale;
+    const bool rare = __any(nan);
+    if (rare) {
+#pragma unroll
+      for (int kb = 0; kb < kKb; ++kb) {
+        const bool none = (t.bad >> kb) & 1;
+#pragma unroll
+        for (int s = 0; s < kSc; ++s) {
+          const uint64_t x = none ? ~0ull : __ballot(t.ks[kb][s] == kNanScale), y = none ? ~0ull : __ballot(t.vs[kb][s] == kNanScale);
+          kn |= (uint32_t)((x | x >> 16 | x >> 32 | x >> 48) & 0xffff) << (16 * kb);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) vn[s][q] |= (uint32_t)((y >> (16 * q)) & 0xffff) << (16 * kb);
+          if (t.ks[kb][s] == kNanScale) t.ks[kb][s] = 127;
+          if (t.vs[kb][s] == kNanScale) {
+            t.vs[kb][s] = 127;
+#pragma unroll
+            for (int i = 0; i < kRaw / kSc; ++i) t.v[kb][s * (kRaw / kSc) + i] = 0;
+          }
+        }
+      }
+    }
+    if (key0 + kKvTile > n_keys) {  // rows of a page past the length may hold anything
+#pragma unroll
+      for (int kb = 0; kb < kKb; ++kb)
+        if (key0 + 16 * kb + c >= n_keys) {
+#pragma unroll
+          for (int i = 0; i < kRaw; ++i) t.v[kb][i] = 0;
+#pragma unroll
+          for (int s = 0; s < kSc; ++s) t.vs[kb][s] = 127;
+        }
+    }
+
+    // ---- S^T = K Q^T
+    f32x4 s[NR][kKb];
+#pragma unroll
+    for (int kb = 0; kb < kKb; ++kb) {
+#pragma unroll
+      for (int n = 0; n < NR; ++n) s[n][kb] = f32x4{};
+#pragma unroll
+      for (int f = 0; f < kFr; ++f) {
+        const u32x4 kf = values8<DT, FMT>(t.k[kb] + f * kW8, scale_of(t.ks[kb][kSc == 2 ? f >> 2 : 0]));
+#pragma unroll
+        for (int n = 0; n < NR; ++n) s[n][kb] = mfma16x16x32<DT>(kf, qf[n][f], s[n][kb]);
+      }
+    }
+    // ---- V in 16 bits to LDS: chunk (8 dims) ch of key r at r * row + ((ch ^ vswz(r)) * 16)
+#pragma unroll
+    for (int kb = 0; kb < kKb; ++kb) {
+      const int r = 16 * kb + c;
+#pragma unroll
+      for (int f = 0; f < kFr; ++f)
+        *(u32x4 *)(vt + r * kVRowB + (((dim(f) >> 3) ^ vswz(r)) << 4)) =
+            values8<DT, FMT>(t.v[kb] + f * kW8, scale_of(t.vs[kb][kSc == 2 ? f >> 2 : 0]));
+    }
+    const bool masked = key0 + kKvTile > all_see;
+    const int k0 = key0;
+    if (key0 + kKvStep < key_end) load(t, key0 + kKvStep);
+    // the tile is this wavefront's own: its LDS accesses complete in order, only the compiler has to keep the
+    // reads (of other lanes' chunks) behind the writes
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+
+    // ---- softmax of the tile: this lane has keys 16 kb + 4 j + i of row c
+    u32x4 pf[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      if (rare) {
+#pragma unroll
+        for (int kb = 0; kb < kKb; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if ((kn >> (16 * kb + 4 * j + i)) & 1) s[n][kb][i] = __builtin_nanf("");
+      }
+      if (masked) {
+#pragma unroll
+        for (int kb = 0; kb < kKb; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][kb][i] = k0 + 16 * kb + 4 * j + i <= lim[n] ? s[n][kb][i] : -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < kKb; ++kb) mx = vmax3(vmax3(mx, s[n][kb][0], s[n][kb][1]), s[n][kb][2], s[n][kb][3]);
+      const float m_tile = quarters_max(mx) * cl;
+      float alpha = 1.0f;
+      if (m_tile > m_off[n] + kKvSlack) {
+        alpha = __builtin_amdgcn_exp2f(m_off[n] - m_tile);
+        m_off[n] = m_tile;
+      }
+      const float moff = m_off[n] == -INFINITY ? 0.0f : m_off[n];
+      if (__any(alpha != 1.0f)) {
+#pragma unroll
+        for (int d = 0; d < kDb; ++d) o[n][d] *= alpha;
+      }
+      float p[8], sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i >> 2][i & 3], cl, -moff));
+        sum += p[i];
+      }
+      l_run[n] = __builtin_fmaf(l_run[n], alpha, sum);
+      pf[n] = u32x4{pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7])};
+    }
+
+    // ---- O^T += V^T P^T: two transposed reads (keys 4 j .. + 3 of each 16) per 16 dims
+#pragma unroll
+    for (int d = 0; d < kDb; ++d) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 16 * e + 4 * j + (c >> 2), ch = 2 * d + ((c & 3) >> 1);
+        const char *p = vt + r * kVRowB + ((ch ^ vswz(r)) << 4) + 8 * (c & 1);
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
+        const u32x2 y = __builtin_bit_cast(u32x2, x);
+        w[2 * e] = y.x;
+        w[2 * e + 1] = y.y;
+      }
+      const u32x4 vf = u32x4{w[0], w[1], w[2], w[3]};
+#pragma unroll
+      for (int n = 0; n < NR; ++n) o[n][d] = mfma16x16x32<DT>(vf, pf[n], o[n][d]);
+    }
+    if (rare) {  // the dims of a NaN block, for the rows that see the key
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        const int seen = lim[n] - k0 + 1;
+        const uint32_t vis = seen >= 32 ? ~0u : seen <= 0 ? 0u : (1u << seen) - 1;
+#pragma unroll
+        for (int d = 0; d < kDb; ++d) {
+          // 32-dim block d / 2: lane quarter (d / 2) & 3 of scale d / 8; DP 64: quarters 2 (d / 2), + 1
+          const uint32_t nm = DP == 64 ? vn[0][(d >> 1) * 2] : vn[d >> 3][(d >> 1) & 3];
+          if (nm & vis) o[n][d] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+        }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+
+  // ---- the wavefronts' sums, 16 rows at a time, in wavefront order
+  const bool alone = u.share.splits == 1;
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const float l_tot = quarters_sum(l_run[n]);
+    __syncthreads();  // the staging tiles, or the last rows, have been read
+    if (j == 0) {
+      sm_m[wave][c] = m_off[n];
+      sm_l[wave][c] = l_tot;
+    }
+    float *park = (float *)smem + wave * (kParkB / 4);
+#pragma unroll
+    for (int d = 0; d < kDb; ++d) *(f32x4 *)(park + c * kPitch + 16 * d + 4 * j) = o[n][d];
+    __syncthreads();
+    for (int it = tid; it < 16 * (DP / 4); it += 64 * kKvWaves) {
+      const int rr = it / (DP / 4), d0 = 4 * (it % (DP / 4));
+      const int r = rb * kRows + 16 * n + rr;
+      if (r >= rows) continue;
+      KvPart sum;
+#pragma unroll
+      for (int w = 0; w < kKvWaves; ++w)
+        add_part(sum, KvPart{sm_m[w][rr], sm_l[w][rr], *(const f32x4 *)((const float *)smem + w * (kParkB / 4) + rr * kPitch + d0)});
+      if (alone) {
+        const int i = r / G;
+        store_out<DT>(a, seq.first + i, hk * G + r - i * G, d0, sum);
+      } else {
+        const size_t at = (size_t)id * kRows + 16 * n + rr;
+        if (d0 < a.part_ld) *(f32x4 *)(a.part + at * a.part_ld + d0) = sum.x;
+        if (d0 == 0) *(f32x2 *)(a.part_ml + 2 * at) = f32x2{sum.m, sum.l};
+      }
+    }
+  }
+}
+
+// The splits' sums of each row of a split sequence, in split order: one wavefront per packed row and as many query
+// heads as it has groups of D / 4 lanes.
+template <int DT, int ROWS>
+__device__ __forceinline__ void kv_combine(const mtk_kv_attn_kargs &a) {
+  const int lane = threadIdx.x, G = a.H / a.H_kv;
+  const int chunks = a.part_ld / 4, heads = max(1, 64 / chunks);
+  const int groups = (a.H + heads - 1) / heads;
+  for (int w = blockIdx.x; w < a.T * groups; w += gridDim.x) {
+    const int t = w / groups, h = (w - t * groups) * heads + lane / chunks;
+    const int b = seq_of_row(a, t, lane);
+    if (b < 0) continue;
+    const KvUnit u = find_unit<ROWS, kKvStep>(a, lane, b, [](int) { return -1; });
+    const int i = t - u.seq.first;
+    if (u.share.blocks == 0 || u.share.splits == 1 || i >= min(u.seq.rows, a.S_q)) continue;
+    if (h >= a.H || lane >= chunks * heads) continue;
+    const int hk = h / G, r = i * G + h - hk * G, d = 4 * (lane % chunks);
+    KvPart sum;
+    for (int s = 0; s < u.share.splits; ++s) {
+      const int id = u.base + (s * u.share.blocks + r / ROWS) * a.H_kv + hk;
+      if (id >= a.max_units) break;
+      const size_t at = (size_t)id * ROWS + r % ROWS;
+      const f32x2 ml = *(const f32x2 *)(a.part_ml + 2 * at);
+      add_part(sum, KvPart{ml.x, ml.y, *(const f32x4 *)(a.part + at * a.part_ld + d)});
+    }
+    store_out<DT>(a, t, h, d, sum);
+  }
+}
+
+}  // namespace mtk
+
+using namespace mtk;
+
+#define MTK_KV_ATTEND(NAME, DT, FMT, DP, NR) \
+  extern "C" __global__ void __launch_bounds__(256) NAME(const mtk_kv_attn_kargs a) { kv_attend<DT, FMT, DP, NR>(a); }
+#define MTK_KV_ATTEND_DT(DP, NR)                                                        \
+  MTK_KV_ATTEND(mtk_kv_attend_fp4_d##DP##_r##NR##_f16, DT_F16, KV_FP4, DP, NR)          \
+  MTK_KV_ATTEND(mtk_kv_attend_fp4_d##DP##_r##NR##_bf16, DT_BF16, KV_FP4, DP, NR)        \
+  MTK_KV_ATTEND(mtk_kv_attend_fp8_d##DP##_r##NR##_f16, DT_F16, KV_FP8, DP, NR)          \
+  MTK_KV_ATTEND(mtk_kv_attend_fp8_d##DP##_r##NR##_bf16, DT_BF16, KV_FP8, DP, NR)
+
+// mtk_kv_attend_<format>_d<padded head dimension>_r<16-row blocks per workgroup>_<type>
+MTK_KV_ATTEND_DT(64, 1)
+MTK_KV_ATTEND_DT(64, 2)
+MTK_KV_ATTEND_DT(64, 4)
+MTK_KV_ATTEND_DT(128, 1)
+MTK_KV_ATTEND_DT(128, 2)
+MTK_KV_ATTEND_DT(128, 4)
+MTK_KV_ATTEND_DT(256, 1)
+MTK_KV_ATTEND_DT(256, 2)
+
+#define MTK_KV_COMBINE(NR)                                                                                  \
+  extern "C" __global__ void __launch_bounds__(64) mtk_kv_combine_r##NR##_f16(const mtk_kv_attn_kargs a) {  \
+    kv_combine<DT_F16, 16 * NR>(a);                                                                         \
+  }                                                                                                         \
+  extern "C" __global__ void __launch_bounds__(64) mtk_kv_combine_r##NR##_bf16(const mtk_kv_attn_kargs a) { \
+    kv_combine<DT_BF16, 16 * NR>(a);                                                                        \
+  }
+MTK_KV_COMBINE(1)
+MTK_KV_COMBINE(2)
+MTK_KV_COMBINE(4)

@@ -1,0 +1,277 @@
+// Plans of the paged key/value cache in few bits (include/mtk.h, kv_cache.h): checks, kernel choice and argument
+// blocks. Part of runtime.cpp's translation unit, inside its unnamed namespace.
+
+constexpr int kKvMaxPositions = 1 << 30;  // of a table row
+
+bool is_kv(const mtk_plan *p) { return p->kind == PLAN_KV_WRITE || p->kind == PLAN_KV_READ || p->kind == PLAN_KV_ATTN; }
+
+int kv_blocks_of(const mtk_kv_desc &d) { return (d.D + 31) / 32; }
+int kv_shift_of(const mtk_kv_desc &d) { return __builtin_ctz((unsigned)d.page_size); }
+uint64_t kv_cache_size(const mtk_kv_desc &d) {
+  return (uint64_t)d.n_pages * (uint64_t)d.H_kv * kv_region_bytes(d.format, kv_blocks_of(d), kv_shift_of(d));
+}
+
+int check_kv_geometry(const mtk_kv_desc &d) {
+  if (d.H_kv <= 0 || d.n_pages <= 0) return fail(MTK_ERR_INVALID, "H_kv and n_pages must be positive (got %d, %d)", d.H_kv, d.n_pages);
+  if (d.D <= 0 || d.D > 256 || d.D % 8 != 0)
+    return fail(MTK_ERR_UNSUPPORTED, "head dimension must be a multiple of 8 up to 256 (got %d)", d.D);
+  if (d.page_size < 16 || d.page_size > 1024 || (d.page_size & (d.page_size - 1)) != 0)
+    return fail(MTK_ERR_INVALID, "page_size must be a power of two from 16 to 1024 (got %d)", d.page_size);
+  if (d.format != MTK_KV_FP4 && d.format != MTK_KV_FP8) return fail(MTK_ERR_INVALID, "format must be MTK_KV_FP4 or MTK_KV_FP8");
+  if (d.H_kv > (1 << 20)) return fail(MTK_ERR_UNSUPPORTED, "H_kv above %d is not supported", 1 << 20);
+  if ((double)d.n_pages * d.H_kv * (double)kv_region_bytes(d.format, kv_blocks_of(d), kv_shift_of(d)) > 9e18)
+    return fail(MTK_ERR_UNSUPPORTED, "a cache of this size cannot be addressed");
+  return MTK_OK;
+}
+
+// What the three plans have in common.
+int check_kv_batch(const mtk_kv_desc &d) {
+  const int s = check_kv_geometry(d);
+  if (s != MTK_OK) return s;
+  if (d.B <= 0 || d.T <= 0 || d.max_pages <= 0)
+    return fail(MTK_ERR_INVALID, "B, T and max_pages must be positive (got %d, %d, %d)", d.B, d.T, d.max_pages);
+  if ((long long)d.max_pages * d.page_size > kKvMaxPositions)
+    return fail(MTK_ERR_UNSUPPORTED, "a table row of more than 2^30 positions is not supported");
+  if (d.dtype != MTK_F16 && d.dtype != MTK_BF16) return fail(MTK_ERR_INVALID, "dtype must be MTK_F16 or MTK_BF16");
+  return MTK_OK;
+}
+
+int kv_ld(int ld, int width, const char *name, int64_t *out) {
+  *out = ld ? ld : width;
+  if (ld != 0 && (ld < width || ld % 8 != 0))
+    return fail(MTK_ERR_INVALID, "%s must be 0 or a multiple of 8 of at least %d (got %d)", name, width, ld);
+  return MTK_OK;
+}
+
+std::string kv_suffix(const mtk_kv_desc &d) { return d.dtype == MTK_F16 ? "f16" : "bf16"; }
+const char *kv_format(const mtk_kv_desc &d) { return d.format == MTK_KV_FP4 ? "fp4" : "fp8"; }
+
+int finish_kv(mtk_plan *p, mtk_plan **out) {
+  const int s = resolve(p);
+  if (s != MTK_OK) {
+    delete p;
+    return s;
+  }
+  *out = p;
+  return MTK_OK;
+}
+
+int plan_kv_move(mtk_ctx *ctx, const mtk_kv_desc *d_in, PlanKind kind, mtk_plan **out) {
+  if (!d_in || !out) return fail(MTK_ERR_INVALID, "null descriptor or output");
+  const mtk_kv_desc d = *d_in;
+  int s = check_kv_batch(d);
+  if (s != MTK_OK) return s;
+  if ((long long)d.H_kv * d.D > INT32_MAX) return fail(MTK_ERR_UNSUPPORTED, "rows of more than 2^31 elements are not supported");
+  mtk_kv_move_kargs a{};
+  if ((s = kv_ld(d.ld_k, d.H_kv * d.D, "ld_k", &a.ld_k)) != MTK_OK || (s = kv_ld(d.ld_v, d.H_kv * d.D, "ld_v", &a.ld_v)) != MTK_OK) return s;
+  a.B = d.B;
+  a.T = d.T;
+  a.H_kv = d.H_kv;
+  a.D = d.D;
+  a.blocks = kv_blocks_of(d);
+  a.page_shift = kv_shift_of(d);
+  a.n_pages = d.n_pages;
+  a.max_pages = d.max_pages;
+  const long long items = 8LL * d.H_kv * a.blocks;  // of 16 bytes of K or V, per row
+  if (items > (1 << 28)) return fail(MTK_ERR_UNSUPPORTED, "rows of this size are not supported");
+  // wavefronts per row: enough to fill the device with few rows, at least one item per lane
+  const int cus = ctx ? ctx->prop.multiProcessorCount : 256;
+  a.parts = (int)std::max(1LL, std::min((items + 63) / 64, (16LL * cus + d.T - 1) / d.T));
+  const long long waves = (long long)a.parts * d.T;
+  if ((waves + 3) / 4 > INT32_MAX / 256) return fail(MTK_ERR_UNSUPPORTED, "T of %d is not supported", d.T);
+  mtk_plan *p = new mtk_plan();
+  p->ctx = ctx;
+  p->kind = kind;
+  p->kv = d;
+  Launch g;
+  g.name = std::string(kind == PLAN_KV_WRITE ? "mtk_kv_write_" : "mtk_kv_read_") + kv_format(d) + "_" + kv_suffix(d);
+  g.grid = (unsigned)((waves + 3) / 4);
+  set_args(g, a);
+  p->launches.push_back(g);
+  p->bytes = (double)d.T * d.H_kv * (4.0 * d.D + 2.0 * (kv_row_bytes(d.format, a.blocks) + a.blocks)) + 4.0 * (2.0 * d.B + 1);
+  char desc[256];
+  snprintf(desc, sizeof desc, "kv %s %s %s B=%d T=%d H_kv=%d D=%d pages=%dx%d max_pages=%d waves/row=%d grid=%u",
+           kind == PLAN_KV_WRITE ? "write" : "read", kv_format(d), kv_suffix(d).c_str(), d.B, d.T, d.H_kv, d.D, d.n_pages,
+           d.page_size, d.max_pages, a.parts, g.grid);
+  p->description = desc;
+  return finish_kv(p, out);
+}
+
+int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
+  if (!d_in || !out) return fail(MTK_ERR_INVALID, "null descriptor or output");
+  mtk_kv_desc d = *d_in;
+  int s = check_kv_batch(d);
+  if (s != MTK_OK) return s;
+  if (d.H <= 0 || d.H % d.H_kv != 0) return fail(MTK_ERR_INVALID, "H must be a positive multiple of H_kv (got H=%d, H_kv=%d)", d.H, d.H_kv);
+  if (d.S_q == 0) d.S_q = d.T;
+  if (d.S_q < 0 || d.S_q > d.T) return fail(MTK_ERR_INVALID, "S_q must be 0 to T (got %d, T=%d)", d.S_q, d.T);
+  if ((long long)d.H * d.D > INT32_MAX || (long long)d.T * d.H > INT32_MAX / 64)
+    return fail(MTK_ERR_UNSUPPORTED, "T x H of more than 2^25 rows, or rows of more than 2^31 elements, are not supported");
+  mtk_kv_attn_kargs a{};
+  if ((s = kv_ld(d.ld_q, d.H * d.D, "ld_q", &a.ld_q)) != MTK_OK) return s;
+  const int G = d.H / d.H_kv, cus = ctx ? ctx->prop.multiProcessorCount : 256;
+  const int dp = d.D <= 64 ? 64 : d.D <= 128 ? 128 : 256;
+  a.B = d.B;
+  a.T = d.T;
+  a.S_q = d.S_q;
+  a.H = d.H;
+  a.H_kv = d.H_kv;
+  a.D = d.D;
+  a.blocks = kv_blocks_of(d);
+  a.page_shift = kv_shift_of(d);
+  a.n_pages = d.n_pages;
+  a.max_pages = d.max_pages;
+  a.causal = d.causal ? 1 : 0;
+  a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)d.D));
+  a.rows_above = 0;
+  a.rows_most = INT32_MAX;
+  const long long pairs = (long long)d.S_q * G;
+  const int nr = pairs <= 16 ? 1 : pairs <= 32 || dp == 256 ? 2 : 4, rows = 16 * nr, step = 128;
+  a.units = cus * (nr == 1 ? 4 : 2);
+  a.least = 2;
+  const long long blocks = kv_max_blocks(d.B, d.T, d.S_q, G, rows) * d.H_kv;
+  if (blocks > (1 << 27)) return fail(MTK_ERR_UNSUPPORTED, "a batch of more than 2^27 row blocks is not supported");
+  a.max_units = (int)(a.units + blocks);
+  a.part_ld = a.blocks * 32;
+  const long long steps = ((long long)d.max_pages * d.page_size + step - 1) / step;
+  const bool split = steps > a.least;
+  if (!split) a.max_units = (int)blocks;
+  mtk_plan *p = new mtk_plan();
+  p->ctx = ctx;
+  p->kind = PLAN_KV_ATTN;
+  p->kv = d;
+  char name[96];
+  Launch g;
+  snprintf(name, sizeof name, "mtk_kv_attend_%s_d%d_r%d_%s", kv_format(d), dp, nr, kv_suffix(d).c_str());
+  g.name = name;
+  g.grid = (unsigned)a.max_units;
+  set_args(g, a);
+  p->launches.push_back(g);
+  if (split) {
+    Launch c = g;
+    snprintf(name, sizeof name, "mtk_kv_combine_r%d_%s", nr, kv_suffix(d).c_str());
+    c.name = name;
+    c.block = 64;
+    const int heads = std::max(1, 64 / (a.part_ld / 4));
+    c.grid = (unsigned)std::min<long long>((long long)d.T * ((d.H + heads - 1) / heads), 8LL * cus);
+    p->launches.push_back(c);
+    p->part_ml_at = (size_t)a.max_units * rows * a.part_ld * sizeof(float);
+    p->workspace = p->part_ml_at + (size_t)a.max_units * rows * 2 * sizeof(float);
+  }
+  const double cap = (double)d.max_pages * d.page_size;
+  p->flops = 4.0 * d.T * d.H * d.D * cap;
+  p->bytes = d.B * cap * d.H_kv * 2.0 * (kv_row_bytes(d.format, a.blocks) + a.blocks) + 4.0 * d.T * d.H * d.D +
+             4.0 * (2.0 * d.B + 1 + (double)d.B * d.max_pages);
+  char desc[320];
+  snprintf(desc, sizeof desc,
+           "kv attention %s %s B=%d T=%d S_q=%d H=%d H_kv=%d D=%d pages=%dx%d max_pages=%d causal=%d rows/wg=%d workgroups=%d, most %d",
+           kv_format(d), kv_suffix(d).c_str(), d.B, d.T, d.S_q, d.H, d.H_kv, d.D, d.n_pages, d.page_size, d.max_pages, a.causal, rows,
+           a.units, a.max_units);
+  p->description = desc;
+  return finish_kv(p, out);
+}
+
+// ------------------------------------------------------------------ run-time arguments
+
+bool overlap(const void *a, uint64_t a_bytes, const void *b, uint64_t b_bytes) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return x < y ? a_bytes > y - x : b_bytes > x - y;
+}
+
+// Bytes that `rows` rows of `width` elements with `ld` between them span.
+uint64_t kv_span(int rows, int64_t ld, int64_t width) { return 2 * ((uint64_t)(rows - 1) * (uint64_t)ld + (uint64_t)width); }
+
+int check_kv_args(const mtk_plan *p, const void *argset) {
+  const mtk_kv_desc &d = p->kv;
+  const int32_t *ints[3];
+  const void *cache;
+  if (!argset) return fail(MTK_ERR_INVALID, "null arguments");
+  if (p->kind == PLAN_KV_ATTN) {
+    const mtk_kv_attn_args *t = (const mtk_kv_attn_args *)argset;
+    cache = t->cache;
+    ints[0] = t->row_start, ints[1] = t->kv_len, ints[2] = t->table;
+    if (!t->Q || !t->O) return fail(MTK_ERR_INVALID, "Q and O must be non-null");
+    if (!aligned(t->Q, 16) || !aligned(t->O, 16)) return fail(MTK_ERR_INVALID, "Q and O must be 16-byte aligned");
+    if (t->lse && !aligned(t->lse, 4)) return fail(MTK_ERR_INVALID, "lse must be 4-byte aligned");
+    if (p->workspace && (!t->workspace || !aligned(t->workspace, 16)))
+      return fail(MTK_ERR_INVALID, "this plan needs a 16-byte aligned workspace of %zu bytes", p->workspace);
+    const int64_t width = (int64_t)d.H * d.D;
+    if (overlap(t->Q, kv_span(d.T, d.ld_q ? d.ld_q : width, width), t->O, kv_span(d.T, width, width)))
+      return fail(MTK_ERR_INVALID, "Q and O overlap");
+  } else {
+    const bool write = p->kind == PLAN_KV_WRITE;
+    const mtk_kv_write_args *w = (const mtk_kv_write_args *)argset;
+    const mtk_kv_read_args *r = (const mtk_kv_read_args *)argset;
+    const void *K = write ? w->K : r->K, *V = write ? w->V : r->V;
+    cache = write ? w->cache : r->cache;
+    ints[0] = write ? w->row_start : r->row_start, ints[1] = write ? w->kv_len : r->kv_len, ints[2] = write ? w->table : r->table;
+    if (!K || !V) return fail(MTK_ERR_INVALID, "K and V must be non-null");
+    if (!aligned(K, 16) || !aligned(V, 16)) return fail(MTK_ERR_INVALID, "K and V must be 16-byte aligned");
+    const int64_t width = (int64_t)d.H_kv * d.D;
+    if (cache && (overlap(K, kv_span(d.T, d.ld_k ? d.ld_k : width, width), cache, kv_cache_size(d)) ||
+                  overlap(V, kv_span(d.T, d.ld_v ? d.ld_v : width, width), cache, kv_cache_size(d))))
+      return fail(MTK_ERR_INVALID, "K or V overlaps the cache");
+  }
+  if (!cache || !aligned(cache, 16)) return fail(MTK_ERR_INVALID, "the cache must be non-null and 16-byte aligned");
+  for (const int32_t *x : ints)
+    if (!x || !aligned(x, 4)) return fail(MTK_ERR_INVALID, "row_start, kv_len and table must be non-null and 4-byte aligned");
+  return MTK_OK;
+}
+
+// Writes the run-time pointers of a launch into `block`, a copy of its argument block.
+void patch_kv(const mtk_plan *p, const Launch &, char *block, const void *argset) {
+  if (p->kind == PLAN_KV_ATTN) {
+    const mtk_kv_attn_args *t = (const mtk_kv_attn_args *)argset;
+    mtk_kv_attn_kargs &a = *(mtk_kv_attn_kargs *)block;
+    a.Q = t->Q;
+    a.cache = t->cache;
+    a.row_start = t->row_start;
+    a.kv_len = t->kv_len;
+    a.table = t->table;
+    a.O = t->O;
+    a.lse = t->lse;
+    a.part = p->workspace ? (float *)t->workspace : nullptr;
+    a.part_ml = p->workspace ? (float *)((char *)t->workspace + p->part_ml_at) : nullptr;
+    return;
+  }
+  mtk_kv_move_kargs &a = *(mtk_kv_move_kargs *)block;
+  if (p->kind == PLAN_KV_WRITE) {
+    const mtk_kv_write_args *t = (const mtk_kv_write_args *)argset;
+    a.K = t->K;
+    a.V = t->V;
+    a.cache = t->cache;
+    a.row_start = t->row_start;
+    a.kv_len = t->kv_len;
+    a.table = t->table;
+  } else {
+    const mtk_kv_read_args *t = (const mtk_kv_read_args *)argset;
+    a.K = t->K;
+    a.V = t->V;
+    a.cache = const_cast<void *>(t->cache);
+    a.row_start = t->row_start;
+    a.kv_len = t->kv_len;
+    a.table = t->table;
+  }
+}
+
+// A run: argument blocks on the stack, nothing is allocated.
+int run_kv(const mtk_plan *p, PlanKind kind, const void *argset) {
+  if (!p) return fail(MTK_ERR_INVALID, "null plan");
+  if (p->kind != kind)
+    return fail(MTK_ERR_INVALID, "not a plan for %s",
+                kind == PLAN_KV_WRITE ? "writing a cache" : kind == PLAN_KV_READ ? "reading a cache" : "attention over a cache");
+  if (!p->ctx) return fail(MTK_ERR_INVALID, "plan was created without a context (dry plan)");
+  const int s = check_kv_args(p, argset);
+  if (s != MTK_OK) return s;
+  alignas(16) char block[512];
+  HIP_TRY(hipSetDevice(p->ctx->device));
+  for (const Launch &l : p->launches) {
+    if (l.args.size() > sizeof block) return fail(MTK_ERR_INVALID, "argument block of %s too large", l.name.c_str());
+    memcpy(block, l.args.data(), l.args.size());
+    patch_kv(p, l, block, argset);
+    void *params[] = {block};
+    const hipError_t e = hipModuleLaunchKernel(l.fn, l.grid, 1, 1, l.block, 1, 1, 0, p->ctx->stream, params, nullptr);
+    if (e != hipSuccess) return fail(MTK_ERR_LAUNCH, "launch of %s failed: %s", l.name.c_str(), hipGetErrorString(e));
+  }
+  return MTK_OK;
+}

@@ -27,6 +27,7 @@
 
 #include "../../include/mtk.h"
 #include "kargs.h"
+#include "kv_cache.h"
 #include "scratch.h"
 
 namespace {
@@ -168,7 +169,8 @@ struct mtk_ctx {
 
 namespace {
 
-enum PlanKind { PLAN_GEMM = 1, PLAN_ATTN = 2, PLAN_CONV = 3, PLAN_ATTN_BWD = 4, PLAN_PERMUTE = 5 };
+enum PlanKind { PLAN_GEMM = 1, PLAN_ATTN = 2, PLAN_CONV = 3, PLAN_ATTN_BWD = 4, PLAN_PERMUTE = 5,
+                PLAN_KV_WRITE = 6, PLAN_KV_READ = 7, PLAN_KV_ATTN = 8 };
 
 enum LaunchRole { ROLE_MAIN = 0, ROLE_REDUCE = 1, ROLE_PERMUTE = 2 };
 
@@ -189,6 +191,7 @@ struct mtk_plan {
   mtk_attn_desc attn{};
   mtk_conv_desc conv{};
   mtk_permute_desc perm{};
+  mtk_kv_desc kv{};
   std::vector<Launch> launches;
   // attention with the keys split over workgroups: `launches` need a partial-sum buffer of the
   // library's; `plain` is the plan without one (one kernel that walks the splits in turn, the same bits),
@@ -1313,6 +1316,8 @@ int plan_attn(mtk_ctx *ctx, const mtk_attn_desc *d_in, mtk_plan **out) {
   return MTK_OK;
 }
 
+#include "kv_plans.hpp"
+
 // ------------------------------------------------------------------ binding run-time pointers
 
 int check_gemm_args(const mtk_plan *p, const mtk_gemm_args *g) {
@@ -1408,6 +1413,10 @@ int bind_args(const mtk_plan *p, const void *argset, std::vector<Launch> &ls, vo
     mtk_permute_args &a = args_of<mtk_permute_args>(ls[0]);
     a.src = t->src;
     a.dst = t->dst;
+  } else if (is_kv(p)) {
+    const int s = check_kv_args(p, argset);
+    if (s != MTK_OK) return s;
+    for (Launch &l : ls) patch_kv(p, l, l.args.data(), argset);
   } else if (p->kind == PLAN_ATTN_BWD) {
     const mtk_attn_bwd_args *t = (const mtk_attn_bwd_args *)argset;
     if (!t || !t->Q || !t->K || !t->V || !t->O || !t->dO || !t->lse || !t->dQ || !t->dK || !t->dV)
@@ -1464,6 +1473,12 @@ size_t argset_size(const mtk_plan *p) {
       return sizeof(mtk_attn_bwd_args);
     case PLAN_PERMUTE:
       return sizeof(mtk_permute_run_args);
+    case PLAN_KV_WRITE:
+      return sizeof(mtk_kv_write_args);
+    case PLAN_KV_READ:
+      return sizeof(mtk_kv_read_args);
+    case PLAN_KV_ATTN:
+      return sizeof(mtk_kv_attn_args);
     default:
       return sizeof(mtk_attn_args);
   }
@@ -1787,6 +1802,24 @@ int mtk_conv_run(const mtk_plan *plan, const mtk_conv_args *args) {
   if (plan && plan->kind != PLAN_CONV) return fail(MTK_ERR_INVALID, "not a convolution plan");
   return run_plan(plan, args);
 }
+
+int mtk_kv_cache_bytes(const mtk_kv_desc *desc, size_t *bytes) {
+  if (!desc || !bytes) return fail(MTK_ERR_INVALID, "null argument");
+  const int s = check_kv_geometry(*desc);
+  if (s != MTK_OK) return s;
+  *bytes = (size_t)kv_cache_size(*desc);
+  return MTK_OK;
+}
+int mtk_kv_write_plan(mtk_ctx *ctx, const mtk_kv_desc *desc, mtk_plan **out) {
+  return plan_kv_move(ctx, desc, PLAN_KV_WRITE, out);
+}
+int mtk_kv_read_plan(mtk_ctx *ctx, const mtk_kv_desc *desc, mtk_plan **out) {
+  return plan_kv_move(ctx, desc, PLAN_KV_READ, out);
+}
+int mtk_kv_attn_plan(mtk_ctx *ctx, const mtk_kv_desc *desc, mtk_plan **out) { return plan_kv_attn(ctx, desc, out); }
+int mtk_kv_write_run(const mtk_plan *plan, const mtk_kv_write_args *args) { return run_kv(plan, PLAN_KV_WRITE, args); }
+int mtk_kv_read_run(const mtk_plan *plan, const mtk_kv_read_args *args) { return run_kv(plan, PLAN_KV_READ, args); }
+int mtk_kv_attn_run(const mtk_plan *plan, const mtk_kv_attn_args *args) { return run_kv(plan, PLAN_KV_ATTN, args); }
 
 size_t mtk_plan_workspace_bytes(const mtk_plan *plan) { return plan ? plan->workspace : 0; }
 

@@ -315,13 +315,94 @@ typedef struct {
 
 int mtk_permute_run(const mtk_plan *plan, const mtk_permute_run_args *args);
 
+/* ------------------------------------------------------------------ paged key/value cache in few bits */
+
+/* A cache of keys and values for serving: paged, one length per sequence, held in 4 or 8 bits. No counterpart in the
+ * reference, whose attention takes K and V whole, in 16 bits, at one length (Sources/attention/attention.swift:466-468).
+ *
+ * Format: a block is 32 dims of one position and K/V head (the last block of a head of D dims is filled with zeros).
+ * Its values are held as e2m1 (MTK_KV_FP4: 0, 0.5, 1, 1.5, 2, 3, 4, 6) or e4m3 (MTK_KV_FP8: up to 448) times a power
+ * of two 2^e, the smallest that brings the block's largest magnitude to at most 6 or 448 (and at least 2^-126), rounded
+ * to nearest, ties to the even code. A Gaussian row is off by 12 % (fp4) or 2.7 % (fp8) in the 2-norm. Magnitudes
+ * above the largest such value that the 16-bit type holds (f16: 49152 and 61440) are limited to it. A block with a NaN
+ * or an infinity reads back as NaN, all of it.
+ *
+ * Layout: page p holds page_size positions (a power of two, 16 to 1024); the region of (page, K/V head) is
+ * [K codes][V codes][K scales][V scales]: codes [position][ceil(D / 32)][16 (fp4) or 32 (fp8) bytes], two e2m1 codes per
+ * byte with the even dim in the low half; scales [position][ceil(D / 32)], a byte e + 127, 255 for a NaN block. Regions
+ * lie [page][head]. A page can be copied or moved as it is; mtk_kv_cache_bytes is the size of n_pages of them.
+ *
+ * Batch: B sequences, described on the device, so that one plan (or one graph) serves any lengths:
+ *   row_start [B + 1]         sequence b has rows row_start[b] .. row_start[b + 1] - 1 of the packed tensors (n of
+ *                             them, none allowed); ascending, within [0, T]. Rows of no sequence are left as they were.
+ *   kv_len [B]                its positions, those of its rows included: row i is position kv_len[b] - n + i
+ *   table [B][max_pages]      its pages in order; entries past its length are not read
+ * The kernels check all of it: a position whose page is out of [0, n_pages), or past the table, or below 0 is not written,
+ * reads as NaN, and makes the attention of the rows that see it NaN. Two sequences may share pages; where both are
+ * written at one position of one page in one call, its bytes are some mix of the two.
+ *
+ * One descriptor for the three plans. */
+#define MTK_KV_FP4 0
+#define MTK_KV_FP8 1
+typedef struct {
+  int B, T;       /* sequences; rows of the packed tensors */
+  int S_q;        /* attention: most rows of a sequence, 0 = T (rows past it are left as they were) */
+  int H, H_kv, D; /* query heads (attention only), a multiple of H_kv; D: a multiple of 8 up to 256 */
+  int n_pages, page_size, max_pages; /* of the cache; positions per page; entries per row of the table */
+  int format;     /* MTK_KV_FP4 or MTK_KV_FP8 */
+  int dtype;      /* of Q, K, V, O: MTK_F16 or MTK_BF16; the type that the cache was written from */
+  int causal;     /* attention: row i sees the positions up to its own; 0: every position of its sequence */
+  int ld_q, ld_k, ld_v; /* elements between rows of Q; of K and V: 0 = packed, else a multiple of 8 (slices of a
+                           fused projection) */
+} mtk_kv_desc;
+
+/* Bytes of a cache of n_pages pages (page_size, H_kv, D, format of the descriptor). Zeroed or not: no position is read
+ * that kv_len does not cover. */
+int mtk_kv_cache_bytes(const mtk_kv_desc *desc, size_t *bytes);
+
+/* Rows of K and V ([T][H_kv][D]) into the cache. */
+int mtk_kv_write_plan(mtk_ctx *ctx, const mtk_kv_desc *desc, mtk_plan **out);
+typedef struct {
+  const void *K, *V; /* 16-byte aligned, as the cache */
+  void *cache;
+  const int32_t *row_start, *kv_len, *table;
+} mtk_kv_write_args;
+int mtk_kv_write_run(const mtk_plan *plan, const mtk_kv_write_args *args);
+
+/* And back to 16 bits, each value exactly (f16 values below 2^-14 to the nearest subnormal). With row_start covering
+ * whole sequences, this gathers a cached prefix into packed rows. */
+int mtk_kv_read_plan(mtk_ctx *ctx, const mtk_kv_desc *desc, mtk_plan **out);
+typedef struct {
+  const void *cache;
+  const int32_t *row_start, *kv_len, *table;
+  void *K, *V;
+} mtk_kv_read_args;
+int mtk_kv_read_run(const mtk_plan *plan, const mtk_kv_read_args *args);
+
+/* O = softmax(Q K^T / sqrt(D)) V over the cached positions, Q [T][H][D] (ld_q), O [T][H][D] packed, query head h on
+ * K/V head h / (H / H_kv). The new rows' own K and V are read from the cache: write them first. A row that sees no
+ * position gives zeros and a log-sum-exp of -inf. The keys of long sequences are split over workgroups, whose partial
+ * sums lie in the workspace until a second kernel adds them in a fixed order: the result does not vary from run to run,
+ * and runs that may overlap need a workspace each. O may not overlap Q. */
+int mtk_kv_attn_plan(mtk_ctx *ctx, const mtk_kv_desc *desc, mtk_plan **out);
+typedef struct {
+  const void *Q;
+  const void *cache;
+  const int32_t *row_start, *kv_len, *table;
+  void *O;
+  float *lse;      /* [T][H] natural-log log-sum-exp of each row's scaled scores, or NULL */
+  void *workspace; /* >= mtk_plan_workspace_bytes(plan), 16-byte aligned, or NULL if 0 */
+} mtk_kv_attn_args;
+int mtk_kv_attn_run(const mtk_plan *plan, const mtk_kv_attn_args *args);
+
 /* ------------------------------------------------------------------ plans, validate, profile */
 
 size_t mtk_plan_workspace_bytes(const mtk_plan *plan);
 /* Human-readable kernel-select result (kernel names, grid, tile, split-K). */
 int mtk_plan_describe(const mtk_plan *plan, char *buf, size_t len);
 /* Algorithmic work of one run: FLOPs (2*M*N*K; conv 2*N*OD*OH*OW*O*KD*KH*KW*C with padded taps
- * counted; attention 4*B*H*S_q*S_kv*D, halved-by-mask count for causal) and minimum HBM bytes. */
+ * counted; attention 4*B*H*S_q*S_kv*D, halved-by-mask count for causal) and minimum HBM bytes. The paged cache's
+ * lengths are not known to its plans: attention counts T rows against full tables. */
 int mtk_plan_work(const mtk_plan *plan, double *flops, double *bytes);
 int mtk_plan_destroy(mtk_plan *plan);
 
@@ -330,7 +411,7 @@ int mtk_plan_destroy(mtk_plan *plan);
  * Runs `warmup` untimed iterations, then `iters` timed ones, cycling through `nsets` argument sets
  * (so a large operand can be rotated to defeat the 256 MB Infinity Cache). Each set is the op's
  * args struct (mtk_gemm_args / mtk_attn_args / mtk_attn_bwd_args / mtk_conv_args /
- * mtk_permute_run_args). HIP events on the plan's stream
+ * mtk_permute_run_args / mtk_kv_write_args / mtk_kv_read_args / mtk_kv_attn_args). HIP events on the plan's stream
  * bracket each kernel; results are averages per iteration, in milliseconds. */
 typedef struct {
   double total_ms;      /* per iteration, first launch start to last launch end */
