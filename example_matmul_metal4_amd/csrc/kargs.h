@@ -154,7 +154,8 @@ typedef struct {
   int32_t blocks;     /* blocks of 32 dims of a head */
   int32_t page_shift; /* log2 of the positions per page */
   int32_t n_pages, max_pages;
-  int32_t parts; /* wavefronts that share a row */
+  int32_t parts, rows_per_wave; /* wavefronts that share a row; rows of a wavefront (1 with several parts) */
+  uint32_t mul_blocks;          /* n / blocks = umulhi(n, mul_blocks), 0: blocks is 1 */
 } mtk_kv_move_kargs;
 
 /* Attention over a paged cache in few bits. */
@@ -166,7 +167,7 @@ typedef struct {
   float *lse; /* [T][H] or NULL */
   float *part, *part_ml;
   int64_t ld_q; /* elements between rows of Q */
-  int32_t B, T, S_q, H, H_kv, D;
+  int32_t B, T, S_q, H, H_kv, G, D; /* G: H / H_kv */
   int32_t blocks, page_shift, n_pages, max_pages;
   int32_t causal;
   float scale_log2; /* log2(e) / sqrt(D) */

@@ -21,10 +21,10 @@
 
 namespace mtk {
 
-constexpr int kKvTile = 32;               // keys per tile
-constexpr int kKvWaves = 4;               // wavefronts per workgroup
-constexpr int kKvStep = kKvTile * kKvWaves;
-constexpr float kKvSlack = 8.0f;          // log2-domain headroom before O is rescaled
+constexpr int kKvBlocks = 2;  // 16-key blocks per tile
+constexpr int kKvTile = 16 * kKvBlocks;
+constexpr float kKvSlack = 8.0f;  // log2-domain headroom before O is rescaled
+constexpr int kWindow = 56;       // table entries between the starts of two windows (below)
 
 // max over the lanes l, l ^ 16, l ^ 32, l ^ 48
 __device__ __forceinline__ float quarters_max(float x) {
@@ -66,26 +66,26 @@ __device__ __forceinline__ void store_out(const mtk_kv_attn_kargs &a, int row, i
     a.lse[(size_t)row * a.H + h] = s.l == 0.0f ? -INFINITY : (s.m == -INFINITY ? s.l : s.m + __builtin_amdgcn_logf(s.l)) * 0.6931471805599453f;
 }
 
-template <int DT, int FMT, int DP, int NR>
+template <int DT, int FMT, int DP, int NR, int W>
 __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
-  constexpr int kRows = 16 * NR;
+  constexpr int kRows = 16 * NR, kKvStep = kKvTile * W;  // W wavefronts per workgroup
   constexpr int kFr = DP / 32;                // operands of 8 dims per lane and key
   constexpr int kW8 = kWords8<FMT>;
   constexpr int kRaw = kFr * kW8;             // words of codes per lane and key
   constexpr int kSc = DP == 256 ? 2 : 1;      // scales per lane and key
-  constexpr int kKb = kKvTile / 16;           // 16-key blocks per tile
+  constexpr int kKb = kKvBlocks;
   constexpr int kDb = DP / 16;                // 16-dim blocks of O
   constexpr int kVRowB = 2 * DP;
-  constexpr int kWaveB = kKvTile * kVRowB;
+  constexpr int kWaveB = 32 * kVRowB;         // V is staged 32 keys at a time
   constexpr int kPitch = DP + 4;              // floats per parked row
   constexpr int kParkB = 16 * kPitch * 4;
-  __shared__ __attribute__((aligned(1024))) char smem[kKvWaves * (kWaveB > kParkB ? kWaveB : kParkB)];
-  __shared__ float sm_m[kKvWaves][16], sm_l[kKvWaves][16];
+  __shared__ __attribute__((aligned(1024))) char smem[W * (kWaveB > kParkB ? kWaveB : kParkB)];
+  __shared__ float sm_m[W][16], sm_l[W][16];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 15, j = lane >> 4;
-  const int G = a.H / a.H_kv;
+  const int G = a.G;
 
   int id = -1;
   const KvUnit u = find_unit<kRows, kKvStep>(a, lane, -1, [&](int total) {
@@ -96,15 +96,30 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
   int rest = id - u.base;
   const int hk = rest % a.H_kv;
   rest /= a.H_kv;
-  const int rb = rest % u.share.blocks, split = rest / u.share.blocks;
+  const int rb = u.share.blocks == 1 ? 0 : rest % u.share.blocks, split = u.share.blocks == 1 ? rest : rest / u.share.blocks;
   const kv_seq seq = u.seq;
   const int rows = min(seq.rows, a.S_q) * G;
+
+  // keys that the rows of this workgroup see at all, and those that every one of them sees
+  const int r_last = min(rb * kRows + kRows, rows) - 1;
+  const int64_t p_first = a.causal ? seq.pos0 + rb * kRows / G : (int64_t)seq.keys - 1;
+  const int64_t p_last = a.causal ? seq.pos0 + r_last / G : (int64_t)seq.keys - 1;
+  const int n_keys = (int)max((int64_t)0, min((int64_t)seq.keys, p_last + 1));
+  const int all_see = (int)max((int64_t)0, min((int64_t)seq.keys, p_first + 1));
+  const int per = u.share.per * kKvStep;
+  const int key_end = min(n_keys, (split + 1) * per);
+  int key0 = split * per + wave * kKvTile;
+
+  // ---- pages: a lane holds one table entry of a window of 64 (-1: no page), and one of the next window, which
+  // starts kWindow entries on, so that a tile lies in one of the two
   const int32_t *table = a.table + (size_t)u.b * a.max_pages;
-  const int row_b = kv_row_bytes(FMT, a.blocks);
-  const uint64_t region = kv_region_bytes(FMT, a.blocks, a.page_shift);
-  const int page_mask = (1 << a.page_shift) - 1;
-  const uint32_t k_scales = (uint32_t)(2 * row_b) << a.page_shift, v_codes = (uint32_t)row_b << a.page_shift;
-  const uint32_t v_scales = k_scales + ((uint32_t)a.blocks << a.page_shift);
+  const int last_entry = n_keys > 0 && !seq.bad ? (n_keys - 1) >> a.page_shift : -1;
+  auto entry = [&](int e) {
+    const int page = e <= last_entry ? table[e] : -1;
+    return page < a.n_pages ? page : -1;
+  };
+  int e0 = key0 >> a.page_shift;
+  int window = entry(e0 + lane), next_window = entry(e0 + kWindow + lane);
 
   // ---- Q, as the operand of S^T: row c of each 16, this lane's dims
   auto dim = [&](int f) { return DP == 64 ? 16 * j + 8 * f : 128 * (f >> 2) + 32 * j + 8 * (f & 3); };
@@ -121,59 +136,60 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
     for (int f = 0; f < kFr; ++f)
       qf[n][f] = r < rows && dim(f) < a.D ? *(const u32x4 *)(q + dim(f)) : u32x4{0u, 0u, 0u, 0u};
   }
-  // keys that the rows of this workgroup see at all, and those that every one of them sees
-  const int r_last = min(rb * kRows + kRows, rows) - 1;
-  const int64_t p_first = a.causal ? seq.pos0 + rb * kRows / G : (int64_t)seq.keys - 1;
-  const int64_t p_last = a.causal ? seq.pos0 + r_last / G : (int64_t)seq.keys - 1;
-  const int n_keys = (int)max((int64_t)0, min((int64_t)seq.keys, p_last + 1));
-  const int all_see = (int)max((int64_t)0, min((int64_t)seq.keys, p_first + 1));
-  const int per = u.share.per * kKvStep;
-  const int key_end = min(n_keys, (split + 1) * per);
 
-  // ---- this lane's place in a row of codes
-  constexpr int kHalf = FMT == KV_FP4 ? 8 : 16;  // bytes of half a block
-  const int blk0 = DP == 64 ? j >> 1 : j;
-  const uint32_t code_at = DP == 64 ? (uint32_t)(blk0 * 2 * kHalf + (j & 1) * kHalf) : (uint32_t)(blk0 * 2 * kHalf);
+  // ---- this lane's place in 16 positions of codes and scales. Lanes of blocks past the head's last read the last
+  // one: Q is zero there, and those dims of O are not stored.
+  const uint32_t row_b = (uint32_t)kv_row_bytes(FMT, a.blocks);
+  const uint64_t region = kv_region_bytes(FMT, a.blocks, a.page_shift), page_b = region * (uint64_t)a.H_kv;
+  const int page_mask = (1 << a.page_shift) - 1;
+  const uint32_t k_scales = (2 * row_b) << a.page_shift, v_codes = row_b << a.page_shift;
+  const uint32_t v_scales = k_scales + ((uint32_t)a.blocks << a.page_shift);
+  constexpr uint32_t kHalf = FMT == KV_FP4 ? 8 : 16;  // bytes of half a block
+  uint32_t code_at[kSc], scale_at[kSc];
+#pragma unroll
+  for (int s = 0; s < kSc; ++s) {
+    const int blk = min(DP == 64 ? j >> 1 : j + 4 * s, a.blocks - 1);
+    code_at[s] = c * row_b + blk * 2 * kHalf + (DP == 64 ? (j & 1) * kHalf : 0u);
+    scale_at[s] = (uint32_t)(c * a.blocks + blk);
+  }
+  const char *head = (const char *)a.cache + (uint64_t)hk * region;
   struct Tile {
     uint32_t k[kKb][kRaw], v[kKb][kRaw], ks[kKb][kSc], vs[kKb][kSc];
     uint32_t bad = 0;  // 16-key blocks whose page is not one
   };
+  const int last_block = (n_keys - 1) & ~15;
   auto load = [&](Tile &t, int key0) {
+    if ((min(key0 + kKvTile - 16, last_block) >> a.page_shift) - e0 >= 64) {
+      e0 += kWindow;
+      window = next_window;
+      next_window = entry(e0 + kWindow + lane);
+    }
     t.bad = 0;
 #pragma unroll
     for (int kb = 0; kb < kKb; ++kb) {
-      const int key = key0 + 16 * kb;
-      const int page = key < n_keys && !seq.bad ? kv_page(table, key, a.n_pages, a.max_pages, a.page_shift) : -1;
-      const int at = __builtin_amdgcn_readfirstlane(page);
-      if (at < 0 && key < n_keys) t.bad |= 1u << kb;
-      const char *p = (const char *)a.cache + ((uint64_t)(uint32_t)max(at, 0) * a.H_kv + hk) * region;
-      const uint32_t off = (uint32_t)((key & page_mask) + c);
+      const int key = min(key0 + 16 * kb, last_block);  // blocks past the keys: any, they are masked
+      const int page = __builtin_amdgcn_readlane(window, (key >> a.page_shift) - e0);
+      t.bad |= page < 0 ? 1u << kb : 0u;
+      const char *p = head + (uint64_t)(uint32_t)max(page, 0) * page_b;
+      const char *code = p + (uint32_t)(key & page_mask) * row_b, *scale = p + k_scales + (uint32_t)(key & page_mask) * (uint32_t)a.blocks;
 #pragma unroll
       for (int s = 0; s < kSc; ++s) {
-        const int blk = blk0 + 4 * s;
         constexpr int kN = kRaw / kSc;
         uint32_t *kw = t.k[kb] + s * kN, *vw = t.v[kb] + s * kN;
+        if constexpr (kN == 2) {
+          const u32x2 x = *(const u32x2 *)(code + code_at[s]), y = *(const u32x2 *)(code + v_codes + code_at[s]);
 #pragma unroll
-        for (int i = 0; i < kN; ++i) kw[i] = vw[i] = 0;
-        t.ks[kb][s] = t.vs[kb][s] = 127;
-        if (at >= 0 && blk < a.blocks) {
-          const uint32_t o = off * (uint32_t)row_b + code_at + (DP == 256 ? s * 8u * kHalf : 0u);
-          const uint32_t so = off * (uint32_t)a.blocks + (uint32_t)blk;
-          if constexpr (kN == 2) {
-            const u32x2 x = *(const u32x2 *)(p + o), y = *(const u32x2 *)(p + v_codes + o);
+          for (int i = 0; i < 2; ++i) kw[i] = x[i], vw[i] = y[i];
+        } else {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) kw[i] = x[i], vw[i] = y[i];
-          } else {
+          for (int q = 0; q < kN / 4; ++q) {
+            const u32x4 x = *(const u32x4 *)(code + code_at[s] + 16 * q), y = *(const u32x4 *)(code + v_codes + code_at[s] + 16 * q);
 #pragma unroll
-            for (int q = 0; q < kN / 4; ++q) {
-              const u32x4 x = *(const u32x4 *)(p + o + 16 * q), y = *(const u32x4 *)(p + v_codes + o + 16 * q);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) kw[4 * q + i] = x[i], vw[4 * q + i] = y[i];
-            }
+            for (int i = 0; i < 4; ++i) kw[4 * q + i] = x[i], vw[4 * q + i] = y[i];
           }
-          t.ks[kb][s] = *(const uint8_t *)(p + k_scales + so);
-          t.vs[kb][s] = *(const uint8_t *)(p + v_scales + so);
         }
+        t.ks[kb][s] = *(const uint8_t *)(scale + scale_at[s]);
+        t.vs[kb][s] = *(const uint8_t *)(scale + (v_scales - k_scales) + scale_at[s]);
       }
     }
   };
@@ -194,17 +210,17 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
   }
 
   Tile t;
-  int key0 = split * per + wave * kKvTile;
   if (key0 < key_end) load(t, key0);
+#pragma unroll 1
   for (; key0 < key_end; key0 += kKvStep) {
-    // ---- NaN blocks and pages that are none: bit k of kn (vn[s]) is key k of the tile
-    uint32_t kn = 0, vn[kSc][4] = {};
-    bool nan = t.bad != 0;
+    // ---- NaN blocks and pages that are none: bit k of kn (vn[s][q]) is key k of the tile
+    uint64_t kn = 0, vn[kSc][4] = {};
+    uint32_t top = t.bad ? kNanScale : 0;
 #pragma unroll
     for (int kb = 0; kb < kKb; ++kb)
 #pragma unroll
-      for (int s = 0; s < kSc; ++s) nan |= max(t.ks[kb][s], t.vs[kb][s]) == kNanScale;
-    const bool rare = __any(nan);
+      for (int s = 0; s < kSc; ++s) top = max(top, max(t.ks[kb][s], t.vs[kb][s]));
+    const bool rare = __any(top == kNanScale);
     if (rare) {
 #pragma unroll
       for (int kb = 0; kb < kKb; ++kb) {
@@ -212,11 +228,11 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
 #pragma unroll
         for (int s = 0; s < kSc; ++s) {
           const uint64_t x = none ? ~0ull : __ballot(t.ks[kb][s] == kNanScale), y = none ? ~0ull : __ballot(t.vs[kb][s] == kNanScale);
-          kn |= (uint32_t)((x | x >> 16 | x >> 32 | x >> 48) & 0xffff) << (16 * kb);
+          kn |= ((x | x >> 16 | x >> 32 | x >> 48) & 0xffff) << (16 * kb);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) vn[s][q] |= (uint32_t)((y >> (16 * q)) & 0xffff) << (16 * kb);
-          if (t.ks[kb][s] == kNanScale) t.ks[kb][s] = 127;
-          if (t.vs[kb][s] == kNanScale) {
+          for (int q = 0; q < 4; ++q) vn[s][q] |= ((y >> (16 * q)) & 0xffff) << (16 * kb);
+          if (none || t.ks[kb][s] == kNanScale) t.ks[kb][s] = 127;
+          if (none || t.vs[kb][s] == kNanScale) {
             t.vs[kb][s] = 127;
 #pragma unroll
             for (int i = 0; i < kRaw / kSc; ++i) t.v[kb][s * (kRaw / kSc) + i] = 0;
@@ -249,24 +265,28 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
       }
     }
     // ---- V in 16 bits to LDS: chunk (8 dims) ch of key r at r * row + ((ch ^ vswz(r)) * 16)
+    auto stage = [&](int h) {
 #pragma unroll
-    for (int kb = 0; kb < kKb; ++kb) {
-      const int r = 16 * kb + c;
+      for (int kb = 2 * h; kb < 2 * h + 2; ++kb) {
+        const int r = 16 * (kb & 1) + c;
 #pragma unroll
-      for (int f = 0; f < kFr; ++f)
-        *(u32x4 *)(vt + r * kVRowB + (((dim(f) >> 3) ^ vswz(r)) << 4)) =
-            values8<DT, FMT>(t.v[kb] + f * kW8, scale_of(t.vs[kb][kSc == 2 ? f >> 2 : 0]));
-    }
+        for (int f = 0; f < kFr; ++f)
+          *(u32x4 *)(vt + r * kVRowB + (((dim(f) >> 3) ^ vswz(r)) << 4)) =
+              values8<DT, FMT>(t.v[kb] + f * kW8, scale_of(t.vs[kb][kSc == 2 ? f >> 2 : 0]));
+      }
+      // the tile is this wavefront's own: its LDS accesses complete in order, only the compiler has to keep the
+      // reads (of other lanes' chunks) behind the writes
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    };
+    stage(0);
     const bool masked = key0 + kKvTile > all_see;
-    const int k0 = key0;
-    if (key0 + kKvStep < key_end) load(t, key0 + kKvStep);
-    // the tile is this wavefront's own: its LDS accesses complete in order, only the compiler has to keep the
-    // reads (of other lanes' chunks) behind the writes
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    if constexpr (kKb == 2) {
+      if (key0 + kKvStep < key_end) load(t, key0 + kKvStep);
+    }
 
     // ---- softmax of the tile: this lane has keys 16 kb + 4 j + i of row c
-    u32x4 pf[NR];
+    u32x4 pf[NR][kKb / 2];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       if (rare) {
@@ -280,7 +300,7 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
 #pragma unroll
         for (int kb = 0; kb < kKb; ++kb)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][kb][i] = k0 + 16 * kb + 4 * j + i <= lim[n] ? s[n][kb][i] : -INFINITY;
+          for (int i = 0; i < 4; ++i) s[n][kb][i] = key0 + 16 * kb + 4 * j + i <= lim[n] ? s[n][kb][i] : -INFINITY;
       }
       float mx = -INFINITY;
 #pragma unroll
@@ -296,48 +316,59 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
 #pragma unroll
         for (int d = 0; d < kDb; ++d) o[n][d] *= alpha;
       }
-      float p[8], sum = 0.0f;
+      float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i >> 2][i & 3], cl, -moff));
-        sum += p[i];
+      for (int h = 0; h < kKb / 2; ++h) {
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][2 * h + (i >> 2)][i & 3], cl, -moff));
+          sum += p[i];
+        }
+        pf[n][h] = u32x4{pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7])};
       }
       l_run[n] = __builtin_fmaf(l_run[n], alpha, sum);
-      pf[n] = u32x4{pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7])};
     }
 
     // ---- O^T += V^T P^T: two transposed reads (keys 4 j .. + 3 of each 16) per 16 dims
 #pragma unroll
-    for (int d = 0; d < kDb; ++d) {
-      uint32_t w[4];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = 16 * e + 4 * j + (c >> 2), ch = 2 * d + ((c & 3) >> 1);
-        const char *p = vt + r * kVRowB + ((ch ^ vswz(r)) << 4) + 8 * (c & 1);
-        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
-        const u32x2 y = __builtin_bit_cast(u32x2, x);
-        w[2 * e] = y.x;
-        w[2 * e + 1] = y.y;
+    for (int h = 0; h < kKb / 2; ++h) {
+      if (h > 0) stage(h);
+      if constexpr (kKb > 2) {
+        if (h == kKb / 2 - 1 && key0 + kKvStep < key_end) load(t, key0 + kKvStep);
       }
-      const u32x4 vf = u32x4{w[0], w[1], w[2], w[3]};
 #pragma unroll
-      for (int n = 0; n < NR; ++n) o[n][d] = mfma16x16x32<DT>(vf, pf[n], o[n][d]);
+      for (int d = 0; d < kDb; ++d) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = 16 * e + 4 * j + (c >> 2), ch = 2 * d + ((c & 3) >> 1);
+          const char *p = vt + r * kVRowB + ((ch ^ vswz(r)) << 4) + 8 * (c & 1);
+          const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
+          const u32x2 y = __builtin_bit_cast(u32x2, x);
+          w[2 * e] = y.x;
+          w[2 * e + 1] = y.y;
+        }
+        const u32x4 vf = u32x4{w[0], w[1], w[2], w[3]};
+#pragma unroll
+        for (int n = 0; n < NR; ++n) o[n][d] = mfma16x16x32<DT>(vf, pf[n][h], o[n][d]);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
     }
     if (rare) {  // the dims of a NaN block, for the rows that see the key
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
-        const int seen = lim[n] - k0 + 1;
-        const uint32_t vis = seen >= 32 ? ~0u : seen <= 0 ? 0u : (1u << seen) - 1;
+        const int seen = lim[n] - key0 + 1;
+        const uint64_t vis = seen >= 64 ? ~0ull : seen <= 0 ? 0ull : (1ull << seen) - 1;
 #pragma unroll
         for (int d = 0; d < kDb; ++d) {
           // 32-dim block d / 2: lane quarter (d / 2) & 3 of scale d / 8; DP 64: quarters 2 (d / 2), + 1
-          const uint32_t nm = DP == 64 ? vn[0][(d >> 1) * 2] : vn[d >> 3][(d >> 1) & 3];
+          const uint64_t nm = DP == 64 ? vn[0][(d >> 1) * 2] : vn[d >> 3][(d >> 1) & 3];
           if (nm & vis) o[n][d] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
         }
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
   }
 
   // ---- the wavefronts' sums, 16 rows at a time, in wavefront order
@@ -354,13 +385,13 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
 #pragma unroll
     for (int d = 0; d < kDb; ++d) *(f32x4 *)(park + c * kPitch + 16 * d + 4 * j) = o[n][d];
     __syncthreads();
-    for (int it = tid; it < 16 * (DP / 4); it += 64 * kKvWaves) {
+    for (int it = tid; it < 16 * (DP / 4); it += 64 * W) {
       const int rr = it / (DP / 4), d0 = 4 * (it % (DP / 4));
       const int r = rb * kRows + 16 * n + rr;
       if (r >= rows) continue;
       KvPart sum;
 #pragma unroll
-      for (int w = 0; w < kKvWaves; ++w)
+      for (int w = 0; w < W; ++w)
         add_part(sum, KvPart{sm_m[w][rr], sm_l[w][rr], *(const f32x4 *)((const float *)smem + w * (kParkB / 4) + rr * kPitch + d0)});
       if (alone) {
         const int i = r / G;
@@ -374,31 +405,66 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
   }
 }
 
-// The splits' sums of each row of a split sequence, in split order: one wavefront per packed row and as many query
-// heads as it has groups of D / 4 lanes.
-template <int DT, int ROWS>
+// The splits' sums of each (row, query head) of a split sequence, in an order that the splits' number fixes: a group
+// of D / 4 lanes (4 dims each) adds every NGth split, a workgroup's NG groups are added in turn.
+constexpr int kKvCombine = 256;  // threads
+template <int DT, int ROWS, int STEP>
 __device__ __forceinline__ void kv_combine(const mtk_kv_attn_kargs &a) {
-  const int lane = threadIdx.x, G = a.H / a.H_kv;
-  const int chunks = a.part_ld / 4, heads = max(1, 64 / chunks);
-  const int groups = (a.H + heads - 1) / heads;
-  for (int w = blockIdx.x; w < a.T * groups; w += gridDim.x) {
-    const int t = w / groups, h = (w - t * groups) * heads + lane / chunks;
-    const int b = seq_of_row(a, t, lane);
-    if (b < 0) continue;
-    const KvUnit u = find_unit<ROWS, kKvStep>(a, lane, b, [](int) { return -1; });
-    const int i = t - u.seq.first;
-    if (u.share.blocks == 0 || u.share.splits == 1 || i >= min(u.seq.rows, a.S_q)) continue;
-    if (h >= a.H || lane >= chunks * heads) continue;
-    const int hk = h / G, r = i * G + h - hk * G, d = 4 * (lane % chunks);
-    KvPart sum;
-    for (int s = 0; s < u.share.splits; ++s) {
-      const int id = u.base + (s * u.share.blocks + r / ROWS) * a.H_kv + hk;
-      if (id >= a.max_units) break;
-      const size_t at = (size_t)id * ROWS + r % ROWS;
-      const f32x2 ml = *(const f32x2 *)(a.part_ml + 2 * at);
-      add_part(sum, KvPart{ml.x, ml.y, *(const f32x4 *)(a.part + at * a.part_ld + d)});
+  __shared__ f32x4 sm_x[kKvCombine];
+  __shared__ f32x2 sm_ml[kKvCombine];
+  const int tid = threadIdx.x, lane = tid & 63, G = a.G;
+  const int chunks = a.part_ld / 4, groups = kKvCombine / chunks;
+  const int g = tid / chunks, d = 4 * (tid - g * chunks);
+  const int items = a.T * a.H, per = (items + gridDim.x - 1) / gridDim.x;
+  const int end = min(items, ((int)blockIdx.x + 1) * per);
+  KvUnit u;
+  u.seq.rows = 0;
+  u.seq.first = 0;
+  for (int it = blockIdx.x * per; it < end; ++it) {  // uniform: every wavefront takes the same items
+    const int t = it / a.H, h = it - t * a.H;
+    if (u.b < 0 || t >= u.seq.first + u.seq.rows) {
+      const int b = seq_of_row(a, t, lane);
+      if (b < 0) {
+        it = (t + 1) * a.H - 1;
+        continue;
+      }
+      u = find_unit<ROWS, STEP>(a, lane, b, [](int) { return -1; });
     }
-    store_out<DT>(a, t, h, d, sum);
+    if (u.share.blocks == 0 || u.share.splits == 1 || t - u.seq.first >= a.S_q) {
+      if ((int64_t)(u.seq.first + u.seq.rows) * a.H >= end) return;
+      it = (u.seq.first + u.seq.rows) * a.H - 1;
+      continue;
+    }
+    const int hk = h / G, r = (t - u.seq.first) * G + h - hk * G;
+    const int S = u.share.splits, stride = u.share.blocks * a.H_kv;
+    const int id0 = u.base + (r / ROWS) * a.H_kv + hk;
+    KvPart sum;
+    constexpr int kAhead = 4;  // splits in flight
+    for (int s0 = g; s0 < S; s0 += kAhead * groups) {
+      KvPart p[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int s = s0 + i * groups, id = id0 + s * stride;
+        if (s < S && id < a.max_units) {
+          const size_t at = (size_t)id * ROWS + r % ROWS;
+          const f32x2 ml = *(const f32x2 *)(a.part_ml + 2 * at);
+          p[i] = KvPart{ml.x, ml.y, *(const f32x4 *)(a.part + at * a.part_ld + d)};
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) add_part(sum, p[i]);
+    }
+    __syncthreads();
+    sm_x[tid] = sum.x;
+    sm_ml[tid] = f32x2{sum.m, sum.l};
+    __syncthreads();
+    if (tid < chunks) {
+      for (int i = 1; i < min(groups, S); ++i) {
+        const int k = tid + i * chunks;
+        add_part(sum, KvPart{sm_ml[k].x, sm_ml[k].y, sm_x[k]});
+      }
+      store_out<DT>(a, t, h, d, sum);
+    }
   }
 }
 
@@ -406,31 +472,35 @@ __device__ __forceinline__ void kv_combine(const mtk_kv_attn_kargs &a) {
 
 using namespace mtk;
 
-#define MTK_KV_ATTEND(NAME, DT, FMT, DP, NR) \
-  extern "C" __global__ void __launch_bounds__(256) NAME(const mtk_kv_attn_kargs a) { kv_attend<DT, FMT, DP, NR>(a); }
-#define MTK_KV_ATTEND_DT(DP, NR)                                                        \
-  MTK_KV_ATTEND(mtk_kv_attend_fp4_d##DP##_r##NR##_f16, DT_F16, KV_FP4, DP, NR)          \
-  MTK_KV_ATTEND(mtk_kv_attend_fp4_d##DP##_r##NR##_bf16, DT_BF16, KV_FP4, DP, NR)        \
-  MTK_KV_ATTEND(mtk_kv_attend_fp8_d##DP##_r##NR##_f16, DT_F16, KV_FP8, DP, NR)          \
-  MTK_KV_ATTEND(mtk_kv_attend_fp8_d##DP##_r##NR##_bf16, DT_BF16, KV_FP8, DP, NR)
+#define MTK_KV_ATTEND(NAME, DT, FMT, DP, NR, W, EU)                                                              \
+  extern "C" __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(EU, EU)))              \
+  NAME(const mtk_kv_attn_kargs a) { kv_attend<DT, FMT, DP, NR, W>(a); }
+#define MTK_KV_ATTEND_DT(DP, NR, W, EU)                                                              \
+  MTK_KV_ATTEND(mtk_kv_attend_fp4_d##DP##_r##NR##_f16, DT_F16, KV_FP4, DP, NR, W, EU)                \
+  MTK_KV_ATTEND(mtk_kv_attend_fp4_d##DP##_r##NR##_bf16, DT_BF16, KV_FP4, DP, NR, W, EU)              \
+  MTK_KV_ATTEND(mtk_kv_attend_fp8_d##DP##_r##NR##_f16, DT_F16, KV_FP8, DP, NR, W, EU)                \
+  MTK_KV_ATTEND(mtk_kv_attend_fp8_d##DP##_r##NR##_bf16, DT_BF16, KV_FP8, DP, NR, W, EU)
 
-// mtk_kv_attend_<format>_d<padded head dimension>_r<16-row blocks per workgroup>_<type>
-MTK_KV_ATTEND_DT(64, 1)
-MTK_KV_ATTEND_DT(64, 2)
-MTK_KV_ATTEND_DT(64, 4)
-MTK_KV_ATTEND_DT(128, 1)
-MTK_KV_ATTEND_DT(128, 2)
-MTK_KV_ATTEND_DT(128, 4)
-MTK_KV_ATTEND_DT(256, 1)
-MTK_KV_ATTEND_DT(256, 2)
+// mtk_kv_attend_<format>_d<padded head dimension>_r<16-row blocks per workgroup>_<type>: wavefronts per workgroup
+// and per SIMD by what their registers allow
+MTK_KV_ATTEND_DT(64, 1, 8, 4)
+MTK_KV_ATTEND_DT(64, 2, 8, 2)
+MTK_KV_ATTEND_DT(64, 4, 4, 2)
+MTK_KV_ATTEND_DT(128, 1, 8, 4)
+MTK_KV_ATTEND_DT(128, 2, 8, 2)
+MTK_KV_ATTEND_DT(128, 4, 4, 1)
+MTK_KV_ATTEND_DT(256, 1, 4, 2)
+MTK_KV_ATTEND_DT(256, 2, 4, 1)
 
-#define MTK_KV_COMBINE(NR)                                                                                  \
-  extern "C" __global__ void __launch_bounds__(64) mtk_kv_combine_r##NR##_f16(const mtk_kv_attn_kargs a) {  \
-    kv_combine<DT_F16, 16 * NR>(a);                                                                         \
-  }                                                                                                         \
-  extern "C" __global__ void __launch_bounds__(64) mtk_kv_combine_r##NR##_bf16(const mtk_kv_attn_kargs a) { \
-    kv_combine<DT_BF16, 16 * NR>(a);                                                                        \
+#define MTK_KV_COMBINE(NR, W)                                                                                          \
+  extern "C" __global__ void __launch_bounds__(kKvCombine) mtk_kv_combine_r##NR##_w##W##_f16(const mtk_kv_attn_kargs a) {  \
+    kv_combine<DT_F16, 16 * NR, kKvTile * W>(a);                                                                        \
+  }                                                                                                                 \
+  extern "C" __global__ void __launch_bounds__(kKvCombine) mtk_kv_combine_r##NR##_w##W##_bf16(const mtk_kv_attn_kargs a) { \
+    kv_combine<DT_BF16, 16 * NR, kKvTile * W>(a);                                                                       \
   }
-MTK_KV_COMBINE(1)
-MTK_KV_COMBINE(2)
-MTK_KV_COMBINE(4)
+MTK_KV_COMBINE(1, 8)
+MTK_KV_COMBINE(2, 8)
+MTK_KV_COMBINE(1, 4)
+MTK_KV_COMBINE(2, 4)
+MTK_KV_COMBINE(4, 4)

@@ -104,7 +104,7 @@ __device__ __forceinline__ int seq_of_row(const A &a, int t, int lane) {
 // unit(total) falls into, or sequence `want_b` if that is not negative. One wavefront's lanes hold 64 sequences.
 template <int ROWS, int STEP, typename F>
 __device__ __forceinline__ KvUnit find_unit(const mtk_kv_attn_kargs &a, int lane, int want_b, F &&unit) {
-  const int G = a.H / a.H_kv;
+  const int G = a.G;
   KvUnit u;
   auto share_of = [&](const kv_seq &s) { return kv_blocks(s, a.S_q, G, ROWS, STEP, a.rows_above, a.rows_most); };
   // work -> steps per workgroup

@@ -77,7 +77,10 @@ int plan_kv_move(mtk_ctx *ctx, const mtk_kv_desc *d_in, PlanKind kind, mtk_plan 
   // wavefronts per row: enough to fill the device with few rows, at least one item per lane
   const int cus = ctx ? ctx->prop.multiProcessorCount : 256;
   a.parts = (int)std::max(1LL, std::min((items + 63) / 64, (16LL * cus + d.T - 1) / d.T));
-  const long long waves = (long long)a.parts * d.T;
+  // rows per wavefront: as many (up to 8) as leave 16 wavefronts per CU
+  a.rows_per_wave = a.parts > 1 ? 1 : (int)std::max(1LL, std::min(8LL, d.T / (16LL * cus)));
+  a.mul_blocks = a.blocks == 1 ? 0u : (uint32_t)((0x100000000ull + a.blocks - 1) / a.blocks);
+  const long long waves = (long long)a.parts * ((d.T + a.rows_per_wave - 1) / a.rows_per_wave);
   if ((waves + 3) / 4 > INT32_MAX / 256) return fail(MTK_ERR_UNSUPPORTED, "T of %d is not supported", d.T);
   mtk_plan *p = new mtk_plan();
   p->ctx = ctx;
@@ -90,9 +93,9 @@ int plan_kv_move(mtk_ctx *ctx, const mtk_kv_desc *d_in, PlanKind kind, mtk_plan 
   p->launches.push_back(g);
   p->bytes = (double)d.T * d.H_kv * (4.0 * d.D + 2.0 * (kv_row_bytes(d.format, a.blocks) + a.blocks)) + 4.0 * (2.0 * d.B + 1);
   char desc[256];
-  snprintf(desc, sizeof desc, "kv %s %s %s B=%d T=%d H_kv=%d D=%d pages=%dx%d max_pages=%d waves/row=%d grid=%u",
+  snprintf(desc, sizeof desc, "kv %s %s %s B=%d T=%d H_kv=%d D=%d pages=%dx%d max_pages=%d waves/row=%d rows/wave=%d grid=%u",
            kind == PLAN_KV_WRITE ? "write" : "read", kv_format(d), kv_suffix(d).c_str(), d.B, d.T, d.H_kv, d.D, d.n_pages,
-           d.page_size, d.max_pages, a.parts, g.grid);
+           d.page_size, d.max_pages, a.parts, a.rows_per_wave, g.grid);
   p->description = desc;
   return finish_kv(p, out);
 }
@@ -116,6 +119,7 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
   a.S_q = d.S_q;
   a.H = d.H;
   a.H_kv = d.H_kv;
+  a.G = G;
   a.D = d.D;
   a.blocks = kv_blocks_of(d);
   a.page_shift = kv_shift_of(d);
@@ -126,9 +130,10 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
   a.rows_above = 0;
   a.rows_most = INT32_MAX;
   const long long pairs = (long long)d.S_q * G;
-  const int nr = pairs <= 16 ? 1 : pairs <= 32 || dp == 256 ? 2 : 4, rows = 16 * nr, step = 128;
-  a.units = cus * (nr == 1 ? 4 : 2);
-  a.least = 2;
+  const int nr = pairs <= 16 ? 1 : pairs <= 32 || dp == 256 ? 2 : 4, rows = 16 * nr;
+  const int waves = nr == 4 || dp == 256 ? 4 : 8, step = 32 * waves;
+  a.units = cus * (nr == 1 ? 2 : 1);
+  a.least = 32 / waves;
   const long long blocks = kv_max_blocks(d.B, d.T, d.S_q, G, rows) * d.H_kv;
   if (blocks > (1 << 27)) return fail(MTK_ERR_UNSUPPORTED, "a batch of more than 2^27 row blocks is not supported");
   a.max_units = (int)(a.units + blocks);
@@ -145,15 +150,15 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
   snprintf(name, sizeof name, "mtk_kv_attend_%s_d%d_r%d_%s", kv_format(d), dp, nr, kv_suffix(d).c_str());
   g.name = name;
   g.grid = (unsigned)a.max_units;
+  g.block = 64 * waves;
   set_args(g, a);
   p->launches.push_back(g);
   if (split) {
     Launch c = g;
-    snprintf(name, sizeof name, "mtk_kv_combine_r%d_%s", nr, kv_suffix(d).c_str());
+    snprintf(name, sizeof name, "mtk_kv_combine_r%d_w%d_%s", nr, waves, kv_suffix(d).c_str());
     c.name = name;
-    c.block = 64;
-    const int heads = std::max(1, 64 / (a.part_ld / 4));
-    c.grid = (unsigned)std::min<long long>((long long)d.T * ((d.H + heads - 1) / heads), 8LL * cus);
+    c.block = 256;
+    c.grid = (unsigned)std::min<long long>((long long)d.T * d.H, 8LL * cus);
     p->launches.push_back(c);
     p->part_ml_at = (size_t)a.max_units * rows * a.part_ld * sizeof(float);
     p->workspace = p->part_ml_at + (size_t)a.max_units * rows * 2 * sizeof(float);

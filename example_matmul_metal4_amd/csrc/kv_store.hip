@@ -7,7 +7,8 @@
 // so that nothing reads back as an infinity. A block with a NaN or an infinity gets scale 255 and reads as NaN.
 // Read: value times scale, two per instruction, exact.
 //
-// `parts` wavefronts share a row: a lane has 8 dims (16 bytes of K or V) at a time, 4 neighbours a block.
+// A lane has 8 dims (16 bytes of K or V) at a time, 4 neighbours a block. Few rows: `parts` wavefronts share one; many:
+// a wavefront has several in turn, whose places it looks up once.
 #include "kv_device.hpp"
 
 namespace mtk {
@@ -20,58 +21,71 @@ __device__ __forceinline__ uint32_t block_max(uint32_t x) {
   return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xf, 0xf, true));  // lane ^ 2
 }
 
-// Where a lane's item (8 dims of K or V of one head of a row) lies.
+// n / d, d's multiplier ceil(2^32 / d) (0: d is 1); exact for n * d < 2^32.
+__device__ __forceinline__ int div_by(int n, uint32_t mul) { return mul ? (int)__umulhi((uint32_t)n, mul) : n; }
+
+// Where a lane's item (8 dims of K or V of one head of a row) lies in a row of K or V and in a page of the cache.
 template <int FMT>
 struct KvItem {
-  int d, head, blk, quarter, v;
+  int d, head, quarter, v;
+  uint64_t code, scale;  // byte offsets of position 0's codes and scale from the page
   __device__ __forceinline__ KvItem(const mtk_kv_move_kargs &a, int it) {
-    quarter = it & 3;
-    int rest = it >> 2;
-    blk = rest % a.blocks;
-    rest /= a.blocks;
-    head = rest % a.H_kv;
-    v = rest / a.H_kv;
-    d = 32 * blk + 8 * quarter;
-  }
-  // byte offsets of the codes and the scale in the cache
-  __device__ __forceinline__ void place(const mtk_kv_move_kargs &a, int page, int off, uint64_t &code, uint64_t &scale) const {
     const uint32_t row_b = (uint32_t)kv_row_bytes(FMT, a.blocks);
-    const uint64_t base = ((uint64_t)(uint32_t)page * a.H_kv + head) * kv_region_bytes(FMT, a.blocks, a.page_shift);
+    quarter = it & 3;
+    const int block = it >> 2, both = div_by(block, a.mul_blocks), blk = block - both * a.blocks;
+    v = both >= a.H_kv ? 1 : 0;
+    head = both - v * a.H_kv;
+    d = 32 * blk + 8 * quarter;
+    const uint64_t at = (uint64_t)(uint32_t)head * kv_region_bytes(FMT, a.blocks, a.page_shift);
     constexpr uint32_t kQ = FMT == KV_FP4 ? 4 : 8;
-    code = base + (v ? row_b << a.page_shift : 0u) + off * row_b + blk * 4 * kQ + quarter * kQ;
-    scale = base + ((2 * row_b + (v ? a.blocks : 0)) << a.page_shift) + off * a.blocks + blk;
+    code = at + (v ? row_b << a.page_shift : 0u) + blk * 4 * kQ + quarter * kQ;
+    scale = at + ((2 * row_b + (v ? a.blocks : 0)) << a.page_shift) + blk;
   }
 };
 
-// The row of this wavefront, and where it lies in the cache (page -1: nowhere).
-__device__ __forceinline__ int kv_place(const mtk_kv_move_kargs &a, int t, int lane, int &off) {
-  const int b = seq_of_row(a, t, lane);
-  off = 0;
-  if (b < 0) return -2;
-  const kv_seq s = load_seq(a, b);
-  const int64_t pos = s.pos0 + (t - s.first);
-  off = (int)(pos & ((1 << a.page_shift) - 1));
-  return __builtin_amdgcn_readfirstlane(kv_page(a.table + (size_t)b * a.max_pages, pos, a.n_pages, a.max_pages, a.page_shift));
-}
+// The rows of this wavefront: [t0, t0 + n), part `part` of each; lane i has the page of row t0 + i (-1: no page, -2:
+// a row of no sequence) and its place in it. Rows of one sequence, the common case, are looked up at once.
+struct KvRows {
+  int t0, n = 0, part, page, off;
+  __device__ __forceinline__ KvRows(const mtk_kv_move_kargs &a, int lane) {
+    const int64_t w = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t group = a.parts == 1 ? w : w / a.parts;
+    part = (int)(w - group * a.parts);
+    if (group * a.rows_per_wave >= a.T) return;
+    t0 = (int)(group * a.rows_per_wave);
+    n = min(a.rows_per_wave, a.T - t0);
+    page = -2;
+    off = 0;
+    for (int i = 0; i < n;) {
+      const int b = seq_of_row(a, t0 + i, lane);
+      if (b < 0) {
+        ++i;
+        continue;
+      }
+      const kv_seq s = load_seq(a, b);
+      const int end = min(n, s.first + s.rows - t0);
+      if (lane >= i && lane < end) {
+        const int64_t pos = s.pos0 + (t0 + lane - s.first);
+        off = (int)(pos & ((1 << a.page_shift) - 1));
+        page = kv_page(a.table + (size_t)b * a.max_pages, pos, a.n_pages, a.max_pages, a.page_shift);
+      }
+      i = max(end, i + 1);
+    }
+  }
+};
+
+constexpr int kMoveAhead = 4;  // items of a lane whose loads are in flight at once
 
 template <int DT, int FMT>
 __device__ __forceinline__ void kv_write(const mtk_kv_move_kargs &a) {
   const int lane = threadIdx.x & 63;
-  const int64_t w = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t t64 = w / a.parts;
-  if (t64 >= a.T) return;
-  const int t = (int)t64, part = (int)(w - t64 * a.parts);
-  int off;
-  const int page = kv_place(a, t, lane, off);
-  if (page < 0) return;
+  const KvRows rows(a, lane);
   const int items = 8 * a.H_kv * a.blocks;
+  const uint64_t page_b = kv_region_bytes(FMT, a.blocks, a.page_shift) * (uint64_t)a.H_kv;
+  const uint32_t row_b = (uint32_t)kv_row_bytes(FMT, a.blocks);
   constexpr uint32_t kInf = DT == DT_F16 ? 0x7C00u : 0x7F80u;
   constexpr uint32_t kMost = DT == DT_F16 ? (FMT == KV_FP4 ? 0x7A00u : 0x7B80u) : (FMT == KV_FP4 ? 0x7F40u : 0x7F70u);
-  for (int it = part * 64 + lane; it < items; it += 64 * a.parts) {  // items are whole blocks of 4 lanes
-    const KvItem<FMT> x(a, it);
-    u32x4 v = u32x4{0u, 0u, 0u, 0u};
-    const uint16_t *src = (const uint16_t *)(x.v ? a.V : a.K) + (size_t)t * (x.v ? a.ld_v : a.ld_k) + (size_t)x.head * a.D + x.d;
-    if (x.d < a.D) v = *(const u32x4 *)src;
+  auto one = [&](const KvItem<FMT> &x, char *at, int off, u32x4 v) {
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -93,83 +107,108 @@ __device__ __forceinline__ void kv_write(const mtk_kv_move_kargs &a) {
     int byte = FMT == KV_FP4 ? (int)(f >> 23) - 2 + ((f & 0x7fffffu) > 0x400000u) : (int)(f >> 23) - 8 + ((f & 0x7fffffu) > 0x600000u);
     byte = max(byte, 1);
     const float scale = scale_of((uint32_t)byte);
-    uint64_t code, at;
-    x.place(a, page, off, code, at);
-    char *c = (char *)a.cache;
-    auto pair = [&](uint32_t w) {
-      if constexpr (DT == DT_F16)
-        return __builtin_bit_cast(f16x2, w);
-      else
-        return __builtin_bit_cast(bf16x2, w);
-    };
+    const uint32_t v0 = v[0], v1 = v[1], v2 = v[2], v3 = v[3];
+    char *code = at + x.code + (uint32_t)off * row_b;
     if constexpr (FMT == KV_FP4) {
       uint32_t r = 0;
-      const uint32_t v0 = v[0], v1 = v[1], v2 = v[2], v3 = v[3];
       if constexpr (DT == DT_F16) {
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, pair(v0), scale, 0);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, pair(v1), scale, 1);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, pair(v2), scale, 2);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, pair(v3), scale, 3);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, v0), scale, 0);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, v1), scale, 1);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, v2), scale, 2);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, __builtin_bit_cast(f16x2, v3), scale, 3);
       } else {
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, pair(v0), scale, 0);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, pair(v1), scale, 1);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, pair(v2), scale, 2);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, pair(v3), scale, 3);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, v0), scale, 0);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, v1), scale, 1);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, v2), scale, 2);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, v3), scale, 3);
       }
-      *(uint32_t *)(c + code) = r;
+      *(uint32_t *)code = r;
     } else {
       s16x2 r0 = s16x2{0, 0}, r1 = s16x2{0, 0};
-      const uint32_t v0 = v[0], v1 = v[1], v2 = v[2], v3 = v[3];
       if constexpr (DT == DT_F16) {
-        r0 = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r0, pair(v0), scale, false);
-        r0 = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r0, pair(v1), scale, true);
-        r1 = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r1, pair(v2), scale, false);
-        r1 = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r1, pair(v3), scale, true);
+        r0 = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r0, __builtin_bit_cast(f16x2, v0), scale, false);
+        r0 = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r0, __builtin_bit_cast(f16x2, v1), scale, true);
+        r1 = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r1, __builtin_bit_cast(f16x2, v2), scale, false);
+        r1 = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r1, __builtin_bit_cast(f16x2, v3), scale, true);
       } else {
-        r0 = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r0, pair(v0), scale, false);
-        r0 = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r0, pair(v1), scale, true);
-        r1 = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r1, pair(v2), scale, false);
-        r1 = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r1, pair(v3), scale, true);
+        r0 = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r0, __builtin_bit_cast(bf16x2, v0), scale, false);
+        r0 = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r0, __builtin_bit_cast(bf16x2, v1), scale, true);
+        r1 = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r1, __builtin_bit_cast(bf16x2, v2), scale, false);
+        r1 = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r1, __builtin_bit_cast(bf16x2, v3), scale, true);
       }
-      *(u32x2 *)(c + code) = u32x2{__builtin_bit_cast(uint32_t, r0), __builtin_bit_cast(uint32_t, r1)};
+      *(u32x2 *)code = u32x2{__builtin_bit_cast(uint32_t, r0), __builtin_bit_cast(uint32_t, r1)};
     }
-    if (x.quarter == 0) *(uint8_t *)(c + at) = (uint8_t)(bad ? kNanScale : byte);
+    if (x.quarter == 0) *(uint8_t *)(at + x.scale + (uint32_t)off * (uint32_t)a.blocks) = (uint8_t)(bad ? kNanScale : byte);
+  };
+  for (int it0 = rows.part * 64 + lane; it0 < items; it0 += 64 * a.parts * kMoveAhead) {  // 4 lanes are a whole block
+    for (int i = 0; i < rows.n; ++i) {
+      const int page = __builtin_amdgcn_readlane(rows.page, i), off = __builtin_amdgcn_readlane(rows.off, i);
+      if (page < 0) continue;
+      const size_t t = (size_t)(rows.t0 + i);
+      char *at = (char *)a.cache + (uint64_t)(uint32_t)page * page_b;
+      u32x4 v[kMoveAhead];
+#pragma unroll
+      for (int k = 0; k < kMoveAhead; ++k) {
+        const int it = it0 + 64 * a.parts * k;
+        v[k] = u32x4{0u, 0u, 0u, 0u};
+        if (it < items) {
+          const KvItem<FMT> x(a, it);
+          if (x.d < a.D)
+            v[k] = *(const u32x4 *)((const uint16_t *)(x.v ? a.V : a.K) + t * (x.v ? a.ld_v : a.ld_k) + (size_t)x.head * a.D + x.d);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kMoveAhead; ++k) {
+        const int it = it0 + 64 * a.parts * k;
+        if (it < items) one(KvItem<FMT>(a, it), at, off, v[k]);
+      }
+    }
   }
 }
 
 template <int DT, int FMT>
 __device__ __forceinline__ void kv_read(const mtk_kv_move_kargs &a) {
   const int lane = threadIdx.x & 63;
-  const int64_t w = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t t64 = w / a.parts;
-  if (t64 >= a.T) return;
-  const int t = (int)t64, part = (int)(w - t64 * a.parts);
-  int off;
-  const int page = kv_place(a, t, lane, off);
-  if (page == -2) return;  // no sequence's row: left as it was
+  const KvRows rows(a, lane);
   const int items = 8 * a.H_kv * a.blocks;
+  const uint64_t page_b = kv_region_bytes(FMT, a.blocks, a.page_shift) * (uint64_t)a.H_kv;
+  const uint32_t row_b = (uint32_t)kv_row_bytes(FMT, a.blocks);
   constexpr uint32_t kNan = DT == DT_F16 ? 0x7E007E00u : 0x7FC07FC0u;
-  const char *c = (const char *)a.cache;
-  for (int it = part * 64 + lane; it < items; it += 64 * a.parts) {
-    const KvItem<FMT> x(a, it);
-    if (x.d >= a.D) continue;
-    u32x4 v = u32x4{kNan, kNan, kNan, kNan};
-    if (page >= 0) {
-      uint64_t code, at;
-      x.place(a, page, off, code, at);
-      uint32_t words[kWords8<FMT>];
-      if constexpr (FMT == KV_FP4) {
-        words[0] = *(const uint32_t *)(c + code);
-      } else {
-        const u32x2 y = *(const u32x2 *)(c + code);
-        words[0] = y.x;
-        words[1] = y.y;
+  for (int it0 = rows.part * 64 + lane; it0 < items; it0 += 64 * a.parts * kMoveAhead) {
+    for (int i = 0; i < rows.n; ++i) {
+      const int page = __builtin_amdgcn_readlane(rows.page, i), off = __builtin_amdgcn_readlane(rows.off, i);
+      if (page == -2) continue;  // no sequence's row: left as it was
+      const size_t t = (size_t)(rows.t0 + i);
+      const char *at = (const char *)a.cache + (uint64_t)(uint32_t)max(page, 0) * page_b;  // page -1 is not looked at
+      uint32_t words[kMoveAhead][kWords8<FMT>], s[kMoveAhead];
+#pragma unroll
+      for (int k = 0; k < kMoveAhead; ++k) {
+        const int it = it0 + 64 * a.parts * k;
+        s[k] = kNanScale;
+        if (it < items && page >= 0) {
+          const KvItem<FMT> x(a, it);
+          const char *code = at + x.code + (uint32_t)off * row_b;
+          if constexpr (FMT == KV_FP4) {
+            words[k][0] = *(const uint32_t *)code;
+          } else {
+            const u32x2 y = *(const u32x2 *)code;
+            words[k][0] = y.x;
+            words[k][1] = y.y;
+          }
+          s[k] = *(const uint8_t *)(at + x.scale + (uint32_t)off * (uint32_t)a.blocks);
+        }
       }
-      const uint32_t s = *(const uint8_t *)(c + at);
-      if (s != kNanScale) v = values8<DT, FMT>(words, scale_of(s));
+#pragma unroll
+      for (int k = 0; k < kMoveAhead; ++k) {
+        const int it = it0 + 64 * a.parts * k;
+        if (it >= items) continue;
+        const KvItem<FMT> x(a, it);
+        if (x.d >= a.D) continue;
+        u32x4 v = u32x4{kNan, kNan, kNan, kNan};
+        if (s[k] != kNanScale) v = values8<DT, FMT>(words[k], scale_of(s[k]));
+        *(u32x4 *)((uint16_t *)(x.v ? a.V : a.K) + t * (x.v ? a.ld_v : a.ld_k) + (size_t)x.head * a.D + x.d) = v;
+      }
     }
-    uint16_t *dst = (uint16_t *)(x.v ? a.V : a.K) + (size_t)t * (x.v ? a.ld_v : a.ld_k) + (size_t)x.head * a.D + x.d;
-    *(u32x4 *)dst = v;
   }
 }
 
