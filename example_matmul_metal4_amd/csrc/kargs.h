@@ -165,6 +165,8 @@ typedef struct {
   const int32_t *row_start, *kv_len, *table;
   void *O;
   float *lse; /* [T][H] or NULL */
+  /* partial sums of the pairs that a workgroup has part of: [workgroup][2][rows of a block][part_ld], and the rows'
+   * (exponent offset in log2, sum of weights). Place 0: the part that the workgroup's range starts with, 1: any other. */
   float *part, *part_ml;
   int64_t ld_q; /* elements between rows of Q */
   int32_t B, T, S_q, H, H_kv, G, D; /* G: H / H_kv */
@@ -174,8 +176,8 @@ typedef struct {
   /* the sequences of this launch: those with more than rows_above and at most rows_most (row, query head)
    * pairs per K/V head */
   int32_t rows_above, rows_most;
-  /* splits of the keys (kv_cache.h): workgroups wanted, least steps of a split, most workgroups */
-  int32_t units, least, max_units;
+  /* who does what (kv_cache.h): workgroups wanted (at most), least steps of one, or one for each pair */
+  int32_t units, least, whole;
   int32_t part_ld; /* floats per row of part */
 } mtk_kv_attn_kargs;
 

@@ -21,8 +21,6 @@
 
 namespace mtk {
 
-constexpr int kKvBlocks = 2;  // 16-key blocks per tile
-constexpr int kKvTile = 16 * kKvBlocks;
 constexpr float kKvSlack = 8.0f;  // log2-domain headroom before O is rescaled
 constexpr int kWindow = 56;       // table entries between the starts of two windows (below)
 
@@ -66,14 +64,14 @@ __device__ __forceinline__ void store_out(const mtk_kv_attn_kargs &a, int row, i
     a.lse[(size_t)row * a.H + h] = s.l == 0.0f ? -INFINITY : (s.m == -INFINITY ? s.l : s.m + __builtin_amdgcn_logf(s.l)) * 0.6931471805599453f;
 }
 
-template <int DT, int FMT, int DP, int NR, int W>
+template <int DT, int FMT, int DP, int NR, int KB, int W>
 __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
-  constexpr int kRows = 16 * NR, kKvStep = kKvTile * W;  // W wavefronts per workgroup
+  constexpr int kRows = 16 * NR, kKvTile = 16 * KB, kKvStep = kKvTile * W;
   constexpr int kFr = DP / 32;                // operands of 8 dims per lane and key
   constexpr int kW8 = kWords8<FMT>;
   constexpr int kRaw = kFr * kW8;             // words of codes per lane and key
   constexpr int kSc = DP == 256 ? 2 : 1;      // scales per lane and key
-  constexpr int kKb = kKvBlocks;
+  constexpr int kKb = KB;                     // 16-key blocks per tile
   constexpr int kDb = DP / 16;                // 16-dim blocks of O
   constexpr int kVRowB = 2 * DP;
   constexpr int kWaveB = 32 * kVRowB;         // V is staged 32 keys at a time
@@ -87,55 +85,14 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
   const int c = lane & 15, j = lane >> 4;
   const int G = a.G;
 
-  int id = -1;
-  const KvUnit u = find_unit<kRows, kKvStep>(a, lane, -1, [&](int total) {
-    total = min(total, a.max_units);
-    return id = (int)blockIdx.x < total ? xcd_remap(blockIdx.x, total) : -1;
-  });
-  if (u.b < 0) return;
-  int rest = id - u.base;
-  const int hk = rest % a.H_kv;
-  rest /= a.H_kv;
-  const int rb = u.share.blocks == 1 ? 0 : rest % u.share.blocks, split = u.share.blocks == 1 ? rest : rest / u.share.blocks;
-  const kv_seq seq = u.seq;
-  const int rows = min(seq.rows, a.S_q) * G;
-
-  // keys that the rows of this workgroup see at all, and those that every one of them sees
-  const int r_last = min(rb * kRows + kRows, rows) - 1;
-  const int64_t p_first = a.causal ? seq.pos0 + rb * kRows / G : (int64_t)seq.keys - 1;
-  const int64_t p_last = a.causal ? seq.pos0 + r_last / G : (int64_t)seq.keys - 1;
-  const int n_keys = (int)max((int64_t)0, min((int64_t)seq.keys, p_last + 1));
-  const int all_see = (int)max((int64_t)0, min((int64_t)seq.keys, p_first + 1));
-  const int per = u.share.per * kKvStep;
-  const int key_end = min(n_keys, (split + 1) * per);
-  int key0 = split * per + wave * kKvTile;
-
-  // ---- pages: a lane holds one table entry of a window of 64 (-1: no page), and one of the next window, which
-  // starts kWindow entries on, so that a tile lies in one of the two
-  const int32_t *table = a.table + (size_t)u.b * a.max_pages;
-  const int last_entry = n_keys > 0 && !seq.bad ? (n_keys - 1) >> a.page_shift : -1;
-  auto entry = [&](int e) {
-    const int page = e <= last_entry ? table[e] : -1;
-    return page < a.n_pages ? page : -1;
-  };
-  int e0 = key0 >> a.page_shift;
-  int window = entry(e0 + lane), next_window = entry(e0 + kWindow + lane);
-
-  // ---- Q, as the operand of S^T: row c of each 16, this lane's dims
-  auto dim = [&](int f) { return DP == 64 ? 16 * j + 8 * f : 128 * (f >> 2) + 32 * j + 8 * (f & 3); };
-  u32x4 qf[NR][kFr];
-  int lim[NR];  // the last key that this lane's row sees
-#pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    const int r = rb * kRows + 16 * n + c;
-    const int i = r / G;
-    const int64_t pos = a.causal ? seq.pos0 + i : (int64_t)seq.keys - 1;
-    lim[n] = r < rows && pos >= 0 ? (int)min(pos, (int64_t)seq.keys - 1) : -1;
-    const uint16_t *q = (const uint16_t *)a.Q + (size_t)(seq.first + i) * a.ld_q + (size_t)(hk * G + r - i * G) * a.D;
-#pragma unroll
-    for (int f = 0; f < kFr; ++f)
-      qf[n][f] = r < rows && dim(f) < a.D ? *(const u32x4 *)(q + dim(f)) : u32x4{0u, 0u, 0u, 0u};
-  }
+  __shared__ int sm_line[W][kLineWords];
+  KvLine<kRows, kKvStep> line(a, lane, sm_line[wave]);
+  const int wgs = kv_div(line.total + line.cut.each - 1, line.cut.each);
+  if ((int)blockIdx.x >= wgs) return;
+  const int wg = xcd_remap(blockIdx.x, wgs);
+  const int line_from = wg * line.cut.each, line_to = min(line.total, line_from + line.cut.each);
+  KvSegment seg = line.at(line_from, line_to);
+  if (seg.b < 0) return;
 
   // ---- this lane's place in 16 positions of codes and scales. Lanes of blocks past the head's last read the last
   // one: Q is zero there, and those dims of O are not stored.
@@ -152,74 +109,178 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
     code_at[s] = c * row_b + blk * 2 * kHalf + (DP == 64 ? (j & 1) * kHalf : 0u);
     scale_at[s] = (uint32_t)(c * a.blocks + blk);
   }
-  const char *head = (const char *)a.cache + (uint64_t)hk * region;
   struct Tile {
     uint32_t k[kKb][kRaw], v[kKb][kRaw], ks[kKb][kSc], vs[kKb][kSc];
     uint32_t bad = 0;  // 16-key blocks whose page is not one
   };
-  const int last_block = (n_keys - 1) & ~15;
-  auto load = [&](Tile &t, int key0) {
-    if ((min(key0 + kKvTile - 16, last_block) >> a.page_shift) - e0 >= 64) {
-      e0 += kWindow;
-      window = next_window;
-      next_window = entry(e0 + kWindow + lane);
+
+  // ---- what the loads of a segment need: its pages, as table entries that the lanes hold, 64 in a window and 64 in
+  // the next window, which starts kWindow entries on, so that a tile lies in one of the two
+  struct Source {
+    const char *head;     // the K/V head's region of page 0
+    const int32_t *table;
+    uint32_t pages;       // entries below it are pages
+    int last_entry, last_block, e0, window, next_window;
+    int key0, key_end, n_keys;  // this wavefront's first key, the segment's end, the keys that its rows see
+  };
+  auto source = [&](const KvSegment &g) {
+    Source x;
+    const int rows = min(g.seq.rows, a.S_q) * G, r_last = min(g.rb * kRows + kRows, rows) - 1;
+    const int64_t p_last = a.causal ? g.seq.pos0 + kv_div(r_last, G) : (int64_t)g.seq.keys - 1;
+    x.n_keys = (int)max((int64_t)0, min((int64_t)g.seq.keys, p_last + 1));
+    x.key_end = min(x.n_keys, g.to * kKvStep);
+    x.key0 = g.from * kKvStep + wave * kKvTile;
+    x.head = (const char *)a.cache + (uint64_t)(uint32_t)g.hk * region;
+    x.table = a.table + (size_t)(uint32_t)g.b * (uint32_t)a.max_pages;
+    x.pages = g.seq.bad ? 0u : (uint32_t)a.n_pages;
+    x.last_block = (max(x.n_keys, 1) - 1) & ~15;
+    x.last_entry = x.last_block >> a.page_shift;
+    x.e0 = min(x.key0, x.last_block) >> a.page_shift;
+    x.window = x.table[min(x.e0 + lane, x.last_entry)];
+    x.next_window = x.table[min(x.e0 + kWindow + lane, x.last_entry)];
+    return x;
+  };
+  // Where the blocks of a tile are. The range of the loads is the page's region.
+  struct Place {
+    rsrc_t r[kKb];
+    uint32_t at[kKb];
+  };
+  auto locate = [&](Tile &t, Source &x, int key0) {
+    if ((min(key0 + kKvTile - 16, x.last_block) >> a.page_shift) - x.e0 >= 64) {
+      x.e0 += kWindow;
+      x.window = x.next_window;
+      x.next_window = x.table[min(x.e0 + kWindow + lane, x.last_entry)];
     }
     t.bad = 0;
+    Place p;
 #pragma unroll
     for (int kb = 0; kb < kKb; ++kb) {
-      const int key = min(key0 + 16 * kb, last_block);  // blocks past the keys: any, they are masked
-      const int page = __builtin_amdgcn_readlane(window, (key >> a.page_shift) - e0);
-      t.bad |= page < 0 ? 1u << kb : 0u;
-      const char *p = head + (uint64_t)(uint32_t)max(page, 0) * page_b;
-      const char *code = p + (uint32_t)(key & page_mask) * row_b, *scale = p + k_scales + (uint32_t)(key & page_mask) * (uint32_t)a.blocks;
+      const int key = min(key0 + 16 * kb, x.last_block);  // blocks past the keys: any, they are masked
+      uint32_t page = (uint32_t)__builtin_amdgcn_readlane(x.window, (key >> a.page_shift) - x.e0);
+      if (page >= x.pages) {
+        t.bad |= 1u << kb;
+        page = 0;
+      }
+      p.r[kb] = make_rsrc(x.head + (uint64_t)page * page_b, (uint32_t)region);
+      p.at[kb] = (uint32_t)(key & page_mask);
+    }
+    return p;
+  };
+  auto load_scales = [&](Tile &t, const Place &p) {
+#pragma unroll
+    for (int kb = 0; kb < kKb; ++kb)
+#pragma unroll
+      for (int s = 0; s < kSc; ++s) {
+        const uint32_t at = p.at[kb] * (uint32_t)a.blocks;
+        t.ks[kb][s] = __builtin_amdgcn_raw_buffer_load_b8(p.r[kb], scale_at[s], k_scales + at, 0);
+        t.vs[kb][s] = __builtin_amdgcn_raw_buffer_load_b8(p.r[kb], scale_at[s], v_scales + at, 0);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // Codes of K (which 0) or V (1) of blocks b0 to b1 - 1.
+  auto load = [&](Tile &t, const Place &p, int which, int b0, int b1) {
+#pragma unroll
+    for (int kb = b0; kb < b1; ++kb)
 #pragma unroll
       for (int s = 0; s < kSc; ++s) {
         constexpr int kN = kRaw / kSc;
-        uint32_t *kw = t.k[kb] + s * kN, *vw = t.v[kb] + s * kN;
+        uint32_t *w = (which ? t.v[kb] : t.k[kb]) + s * kN;
+        const uint32_t so = (which ? v_codes : 0u) + p.at[kb] * row_b;
         if constexpr (kN == 2) {
-          const u32x2 x = *(const u32x2 *)(code + code_at[s]), y = *(const u32x2 *)(code + v_codes + code_at[s]);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) kw[i] = x[i], vw[i] = y[i];
+          const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(p.r[kb], code_at[s], so, 0);
+          w[0] = x[0], w[1] = x[1];
         } else {
 #pragma unroll
           for (int q = 0; q < kN / 4; ++q) {
-            const u32x4 x = *(const u32x4 *)(code + code_at[s] + 16 * q), y = *(const u32x4 *)(code + v_codes + code_at[s] + 16 * q);
+            const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(p.r[kb], code_at[s] + 16 * q, so, 0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) kw[4 * q + i] = x[i], vw[4 * q + i] = y[i];
+            for (int i = 0; i < 4; ++i) w[4 * q + i] = x[i];
           }
         }
-        t.ks[kb][s] = *(const uint8_t *)(scale + scale_at[s]);
-        t.vs[kb][s] = *(const uint8_t *)(scale + (v_scales - k_scales) + scale_at[s]);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto load_tile = [&](Tile &t, Source &x, int key0) {
+    const Place p = locate(t, x, key0);
+    load_scales(t, p);
+    load(t, p, 0, 0, kKb);
+    load(t, p, 1, 0, kKb);
+  };
+
+  // V in 16 bits in LDS: chunk (8 dims) ch of key r at r * row + ((ch ^ swz(r)) * 16), swz(r) from bits 0 to 3 of r: the
+  // chunks that 16 lanes write, and those that 32 lanes read transposed, lie in different banks. An operand's or a
+  // block's chunk differs from the first one's in bits of its own, so that its address is the first one's with those
+  // bits flipped (rows of 16 more keys: an offset).
+  auto vswz = [](int r) {
+    return DP == 64 ? (((r >> 1) & 3) << 1) | ((r >> 3) & 1) : ((r & 7) << 1) | ((r >> 3) & 1);
+  };
+  const int tr = 4 * j + (c >> 2);
+  uint32_t v_put = (uint32_t)(wave * kWaveB + c * kVRowB + (((DP == 64 ? 2 * j : 4 * j) ^ vswz(c)) << 4));
+  uint32_t v_get = (uint32_t)(wave * kWaveB + tr * kVRowB + ((((c & 3) >> 1) ^ vswz(tr)) << 4) + 8 * (c & 1));
+  const float cl = a.scale_log2;
+
+  // ---- Q, as the operand of S^T: row c of each 16, this lane's dims
+  auto dim = [&](int f) { return DP == 64 ? 16 * j + 8 * f : 128 * (f >> 2) + 32 * j + 8 * (f & 3); };
+  u32x4 qf[NR][kFr];
+  int lim[NR];  // the last key that this lane's row sees
+  auto load_q = [&](const KvSegment &g) {
+    const int rows = min(g.seq.rows, a.S_q) * G;
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      const int r = g.rb * kRows + 16 * n + c, i = kv_div(r, G);
+      const int64_t pos = a.causal ? g.seq.pos0 + i : (int64_t)g.seq.keys - 1;
+      lim[n] = r < rows && pos >= 0 ? (int)min(pos, (int64_t)g.seq.keys - 1) : -1;
+      const uint16_t *q = (const uint16_t *)a.Q + (size_t)(g.seq.first + i) * a.ld_q + (size_t)(g.hk * G + r - i * G) * a.D;
+#pragma unroll
+      for (int f = 0; f < kFr; ++f) {
+        qf[n][f] = u32x4{0u, 0u, 0u, 0u};
+        if (r < rows && dim(f) < a.D) qf[n][f] = *(const u32x4 *)(q + dim(f));
       }
     }
   };
 
-  char *vt = smem + wave * kWaveB;
-  auto vswz = [](int r) {
-    return DP == 64 ? (((r >> 1) & 3) << 1) | ((r >> 3) & 1) : ((r & 7) << 1) | ((r >> 3) & 1);
-  };
-  const float cl = a.scale_log2;
-  float m_off[NR], l_run[NR];
-  f32x4 o[NR][kDb];
-#pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    m_off[n] = -INFINITY;
-    l_run[n] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < kDb; ++d) o[n][d] = f32x4{};
-  }
-
+  Source src = source(seg);
+  load_q(seg);
   Tile t;
-  if (key0 < key_end) load(t, key0);
+  if (src.key0 < src.key_end) load_tile(t, src, src.key0);
+
+  for (;;) {
+    // the next segment's table entries, ahead of their use
+    const bool more = seg.start + seg.to < line_to && !line.cut.padded;
+    int window = 0, next_window = 0;
+    if (more) {
+      const Source x = source(line.at(seg.start + seg.to, line_to));
+      window = x.window;
+      next_window = x.next_window;
+    }
+    float m_off[NR], l_run[NR];
+    f32x4 o[NR][kDb];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      m_off[n] = -INFINITY;
+      l_run[n] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < kDb; ++d) o[n][d] = f32x4{};
+    }
+    const int n_keys = src.n_keys, key_end = src.key_end;
+    // keys that every row of the workgroup sees
+    const int64_t p_first = a.causal ? seg.seq.pos0 + kv_div(seg.rb * kRows, G) : (int64_t)seg.seq.keys - 1;
+    const int all_see = (int)max((int64_t)0, min((int64_t)seg.seq.keys, p_first + 1));
 #pragma unroll 1
-  for (; key0 < key_end; key0 += kKvStep) {
+  for (int key0 = src.key0; key0 < key_end; key0 += kKvStep) {
+    asm volatile("" : "+v"(v_put), "+v"(v_get));  // the flips are done in the loop: their results would fill registers
     // ---- NaN blocks and pages that are none: bit k of kn (vn[s][q]) is key k of the tile
     uint64_t kn = 0, vn[kSc][4] = {};
+    uint32_t vs[kKb][kSc];  // the next tile's are loaded before this one's have been used
+#pragma unroll
+    for (int kb = 0; kb < kKb; ++kb)
+#pragma unroll
+      for (int s = 0; s < kSc; ++s) vs[kb][s] = t.vs[kb][s];
     uint32_t top = t.bad ? kNanScale : 0;
 #pragma unroll
     for (int kb = 0; kb < kKb; ++kb)
 #pragma unroll
-      for (int s = 0; s < kSc; ++s) top = max(top, max(t.ks[kb][s], t.vs[kb][s]));
+      for (int s = 0; s < kSc; ++s) top = max(top, max(t.ks[kb][s], vs[kb][s]));
     const bool rare = __any(top == kNanScale);
     if (rare) {
 #pragma unroll
@@ -227,13 +288,13 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
         const bool none = (t.bad >> kb) & 1;
 #pragma unroll
         for (int s = 0; s < kSc; ++s) {
-          const uint64_t x = none ? ~0ull : __ballot(t.ks[kb][s] == kNanScale), y = none ? ~0ull : __ballot(t.vs[kb][s] == kNanScale);
+          const uint64_t x = none ? ~0ull : __ballot(t.ks[kb][s] == kNanScale), y = none ? ~0ull : __ballot(vs[kb][s] == kNanScale);
           kn |= ((x | x >> 16 | x >> 32 | x >> 48) & 0xffff) << (16 * kb);
 #pragma unroll
           for (int q = 0; q < 4; ++q) vn[s][q] |= ((y >> (16 * q)) & 0xffff) << (16 * kb);
           if (none || t.ks[kb][s] == kNanScale) t.ks[kb][s] = 127;
-          if (none || t.vs[kb][s] == kNanScale) {
-            t.vs[kb][s] = 127;
+          if (none || vs[kb][s] == kNanScale) {
+            vs[kb][s] = 127;
 #pragma unroll
             for (int i = 0; i < kRaw / kSc; ++i) t.v[kb][s * (kRaw / kSc) + i] = 0;
           }
@@ -247,7 +308,7 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
 #pragma unroll
           for (int i = 0; i < kRaw; ++i) t.v[kb][i] = 0;
 #pragma unroll
-          for (int s = 0; s < kSc; ++s) t.vs[kb][s] = 127;
+          for (int s = 0; s < kSc; ++s) vs[kb][s] = 127;
         }
     }
 
@@ -268,22 +329,27 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
     auto stage = [&](int h) {
 #pragma unroll
       for (int kb = 2 * h; kb < 2 * h + 2; ++kb) {
-        const int r = 16 * (kb & 1) + c;
 #pragma unroll
         for (int f = 0; f < kFr; ++f)
-          *(u32x4 *)(vt + r * kVRowB + (((dim(f) >> 3) ^ vswz(r)) << 4)) =
-              values8<DT, FMT>(t.v[kb] + f * kW8, scale_of(t.vs[kb][kSc == 2 ? f >> 2 : 0]));
+          *(u32x4 *)(smem + ((v_put ^ (uint32_t)((f < 4 ? f : f + 12) << 4)) + 16 * (kb & 1) * kVRowB)) =
+              values8<DT, FMT>(t.v[kb] + f * kW8, scale_of(vs[kb][kSc == 2 ? f >> 2 : 0]));
       }
       // the tile is this wavefront's own: its LDS accesses complete in order, only the compiler has to keep the
       // reads (of other lanes' chunks) behind the writes
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     };
-    stage(0);
-    const bool masked = key0 + kKvTile > all_see;
-    if constexpr (kKb == 2) {
-      if (key0 + kKvStep < key_end) load(t, key0 + kKvStep);
+    // the next tile's loads, each as soon as its registers are free
+    const bool ahead = key0 + kKvStep < key_end;
+    Place place;
+    if (ahead) {
+      place = locate(t, src, key0 + kKvStep);
+      load_scales(t, place);
+      load(t, place, 0, 0, kKb);
     }
+    stage(0);
+    if (ahead) load(t, place, 1, 0, 2);
+    const bool masked = key0 + kKvTile > all_see;
 
     // ---- softmax of the tile: this lane has keys 16 kb + 4 j + i of row c
     u32x4 pf[NR][kKb / 2];
@@ -291,10 +357,11 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
     for (int n = 0; n < NR; ++n) {
       if (rare) {
 #pragma unroll
-        for (int kb = 0; kb < kKb; ++kb)
+        for (int kb = 0; kb < kKb; ++kb) {
+          const uint32_t mine = (uint32_t)(kn >> (16 * kb)) >> (4 * j);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if ((kn >> (16 * kb + 4 * j + i)) & 1) s[n][kb][i] = __builtin_nanf("");
+          for (int i = 0; i < 4; ++i) s[n][kb][i] = (mine >> i) & 1 ? __builtin_nanf("") : s[n][kb][i];
+        }
       }
       if (masked) {
 #pragma unroll
@@ -333,17 +400,16 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
     // ---- O^T += V^T P^T: two transposed reads (keys 4 j .. + 3 of each 16) per 16 dims
 #pragma unroll
     for (int h = 0; h < kKb / 2; ++h) {
-      if (h > 0) stage(h);
-      if constexpr (kKb > 2) {
-        if (h == kKb / 2 - 1 && key0 + kKvStep < key_end) load(t, key0 + kKvStep);
+      if (h > 0) {
+        stage(h);
+        if (ahead) load(t, place, 1, 2 * h, 2 * h + 2);
       }
 #pragma unroll
       for (int d = 0; d < kDb; ++d) {
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int r = 16 * e + 4 * j + (c >> 2), ch = 2 * d + ((c & 3) >> 1);
-          const char *p = vt + r * kVRowB + ((ch ^ vswz(r)) << 4) + 8 * (c & 1);
+          const char *p = smem + ((v_get ^ (uint32_t)(d << 5)) + 16 * e * kVRowB);
           const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
           const u32x2 y = __builtin_bit_cast(u32x2, x);
           w[2 * e] = y.x;
@@ -371,42 +437,59 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
     }
   }
 
-  // ---- the wavefronts' sums, 16 rows at a time, in wavefront order
-  const bool alone = u.share.splits == 1;
-#pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    const float l_tot = quarters_sum(l_run[n]);
-    __syncthreads();  // the staging tiles, or the last rows, have been read
-    if (j == 0) {
-      sm_m[wave][c] = m_off[n];
-      sm_l[wave][c] = l_tot;
+    // the next segment's first tile and Q are on their way while this one's sums are joined
+    KvSegment next = seg;
+    if (more) {
+      next = line.at(seg.start + seg.to, line_to);
+      src = source(next);
+      src.window = window;
+      src.next_window = next_window;
+      load_q(next);
+      if (src.key0 < src.key_end) load_tile(t, src, src.key0);
     }
-    float *park = (float *)smem + wave * (kParkB / 4);
+
+    // ---- the wavefronts' sums, 16 rows at a time, in wavefront order
+    const bool alone = seg.from == 0 && seg.to == seg.steps;
+    const int rows = min(seg.seq.rows, a.S_q) * G;
+    const size_t place = (size_t)wg * 2 + (seg.start + seg.from == line_from ? 0 : 1);
 #pragma unroll
-    for (int d = 0; d < kDb; ++d) *(f32x4 *)(park + c * kPitch + 16 * d + 4 * j) = o[n][d];
-    __syncthreads();
-    for (int it = tid; it < 16 * (DP / 4); it += 64 * W) {
-      const int rr = it / (DP / 4), d0 = 4 * (it % (DP / 4));
-      const int r = rb * kRows + 16 * n + rr;
-      if (r >= rows) continue;
-      KvPart sum;
+    for (int n = 0; n < NR; ++n) {
+      const float l_tot = quarters_sum(l_run[n]);
+      __syncthreads();  // the staging tiles, or the last rows, have been read
+      if (j == 0) {
+        sm_m[wave][c] = m_off[n];
+        sm_l[wave][c] = l_tot;
+      }
+      float *park = (float *)smem + wave * (kParkB / 4);
 #pragma unroll
-      for (int w = 0; w < W; ++w)
-        add_part(sum, KvPart{sm_m[w][rr], sm_l[w][rr], *(const f32x4 *)((const float *)smem + w * (kParkB / 4) + rr * kPitch + d0)});
-      if (alone) {
-        const int i = r / G;
-        store_out<DT>(a, seq.first + i, hk * G + r - i * G, d0, sum);
-      } else {
-        const size_t at = (size_t)id * kRows + 16 * n + rr;
-        if (d0 < a.part_ld) *(f32x4 *)(a.part + at * a.part_ld + d0) = sum.x;
-        if (d0 == 0) *(f32x2 *)(a.part_ml + 2 * at) = f32x2{sum.m, sum.l};
+      for (int d = 0; d < kDb; ++d) *(f32x4 *)(park + c * kPitch + 16 * d + 4 * j) = o[n][d];
+      __syncthreads();
+      for (int it = tid; it < 16 * (DP / 4); it += 64 * W) {
+        const int rr = it / (DP / 4), d0 = 4 * (it % (DP / 4));
+        const int r = seg.rb * kRows + 16 * n + rr;
+        if (r >= rows) continue;
+        KvPart sum;
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+          add_part(sum, KvPart{sm_m[w][rr], sm_l[w][rr], *(const f32x4 *)((const float *)smem + w * (kParkB / 4) + rr * kPitch + d0)});
+        if (alone) {
+          const int i = kv_div(r, G);
+          store_out<DT>(a, seg.seq.first + i, seg.hk * G + r - i * G, d0, sum);
+        } else {
+          const size_t at = place * kRows + 16 * n + rr;
+          if (d0 < a.part_ld) *(f32x4 *)(a.part + at * a.part_ld + d0) = sum.x;
+          if (d0 == 0) *(f32x2 *)(a.part_ml + 2 * at) = f32x2{sum.m, sum.l};
+        }
       }
     }
+    if (!more) break;
+    seg = next;
+    __syncthreads();  // the parked sums have been read
   }
 }
 
-// The splits' sums of each (row, query head) of a split sequence, in an order that the splits' number fixes: a group
-// of D / 4 lanes (4 dims each) adds every NGth split, a workgroup's NG groups are added in turn.
+// The partial sums of each (row, query head) of a pair that workgroups share, in an order that their number fixes: a group
+// of D / 4 lanes (4 dims each) adds every NGth part, a workgroup's NG groups are added in turn.
 constexpr int kKvCombine = 256;  // threads
 template <int DT, int ROWS, int STEP>
 __device__ __forceinline__ void kv_combine(const mtk_kv_attn_kargs &a) {
@@ -417,36 +500,44 @@ __device__ __forceinline__ void kv_combine(const mtk_kv_attn_kargs &a) {
   const int g = tid / chunks, d = 4 * (tid - g * chunks);
   const int items = a.T * a.H, per = (items + gridDim.x - 1) / gridDim.x;
   const int end = min(items, ((int)blockIdx.x + 1) * per);
-  KvUnit u;
-  u.seq.rows = 0;
-  u.seq.first = 0;
-  for (int it = blockIdx.x * per; it < end; ++it) {  // uniform: every wavefront takes the same items
+  int it = blockIdx.x * per;
+  if (it >= end) return;
+  __shared__ int sm_line[kKvCombine / 64][kLineWords];
+  KvLine<ROWS, STEP> line(a, lane, sm_line[tid >> 6]);
+  if (line.cut.padded && line.cut.each >= line.total) return;
+  int b = -1, base = 0, length = 1;
+  KvSegment seq{};
+  for (; it < end; ++it) {  // uniform: every wavefront takes the same items
     const int t = it / a.H, h = it - t * a.H;
-    if (u.b < 0 || t >= u.seq.first + u.seq.rows) {
-      const int b = seq_of_row(a, t, lane);
-      if (b < 0) {
+    if (b < 0 || t >= seq.seq.first + seq.seq.rows) {
+      const int at = line.find_row(t);
+      b = at;
+      if (at < 0) {
         it = (t + 1) * a.H - 1;
         continue;
       }
-      u = find_unit<ROWS, STEP>(a, lane, b, [](int) { return -1; });
+      int pairs;
+      seq = line.sequence(at, length, base, pairs);
+      if (pairs == 0) length = 0;
     }
-    if (u.share.blocks == 0 || u.share.splits == 1 || t - u.seq.first >= a.S_q) {
-      if ((int64_t)(u.seq.first + u.seq.rows) * a.H >= end) return;
-      it = (u.seq.first + u.seq.rows) * a.H - 1;
+    if (length == 0 || t - seq.seq.first >= a.S_q || (line.cut.padded && length == line.cut.each)) {
+      it = min((int64_t)end, (int64_t)(seq.seq.first + seq.seq.rows) * a.H) - 1;  // none of the sequence's, or none left
       continue;
     }
-    const int hk = h / G, r = (t - u.seq.first) * G + h - hk * G;
-    const int S = u.share.splits, stride = u.share.blocks * a.H_kv;
-    const int id0 = u.base + (r / ROWS) * a.H_kv + hk;
+    const int hk = h / G, r = (t - seq.seq.first) * G + h - hk * G;
+    const int start = base + (r / ROWS * a.H_kv + hk) * length;
+    const int w0 = kv_div(start, line.cut.each), w1 = min(kv_div(start + seq.steps - 1, line.cut.each), a.units - 1);
+    if (w0 >= w1) continue;  // one workgroup's
+    const int first = start == w0 * line.cut.each ? 0 : 1;
     KvPart sum;
-    constexpr int kAhead = 4;  // splits in flight
-    for (int s0 = g; s0 < S; s0 += kAhead * groups) {
+    constexpr int kAhead = 8;  // parts in flight
+    for (int s0 = w0 + g; s0 <= w1; s0 += kAhead * groups) {
       KvPart p[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const int s = s0 + i * groups, id = id0 + s * stride;
-        if (s < S && id < a.max_units) {
-          const size_t at = (size_t)id * ROWS + r % ROWS;
+        const int w = s0 + i * groups;
+        if (w <= w1) {
+          const size_t at = ((size_t)w * 2 + (w == w0 ? first : 0)) * ROWS + r % ROWS;
           const f32x2 ml = *(const f32x2 *)(a.part_ml + 2 * at);
           p[i] = KvPart{ml.x, ml.y, *(const f32x4 *)(a.part + at * a.part_ld + d)};
         }
@@ -459,7 +550,7 @@ __device__ __forceinline__ void kv_combine(const mtk_kv_attn_kargs &a) {
     sm_ml[tid] = f32x2{sum.m, sum.l};
     __syncthreads();
     if (tid < chunks) {
-      for (int i = 1; i < min(groups, S); ++i) {
+      for (int i = 1; i < min(groups, w1 - w0 + 1); ++i) {
         const int k = tid + i * chunks;
         add_part(sum, KvPart{sm_ml[k].x, sm_ml[k].y, sm_x[k]});
       }
@@ -472,35 +563,43 @@ __device__ __forceinline__ void kv_combine(const mtk_kv_attn_kargs &a) {
 
 using namespace mtk;
 
-#define MTK_KV_ATTEND(NAME, DT, FMT, DP, NR, W, EU)                                                              \
-  extern "C" __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(EU, EU)))              \
-  NAME(const mtk_kv_attn_kargs a) { kv_attend<DT, FMT, DP, NR, W>(a); }
-#define MTK_KV_ATTEND_DT(DP, NR, W, EU)                                                              \
-  MTK_KV_ATTEND(mtk_kv_attend_fp4_d##DP##_r##NR##_f16, DT_F16, KV_FP4, DP, NR, W, EU)                \
-  MTK_KV_ATTEND(mtk_kv_attend_fp4_d##DP##_r##NR##_bf16, DT_BF16, KV_FP4, DP, NR, W, EU)              \
-  MTK_KV_ATTEND(mtk_kv_attend_fp8_d##DP##_r##NR##_f16, DT_F16, KV_FP8, DP, NR, W, EU)                \
-  MTK_KV_ATTEND(mtk_kv_attend_fp8_d##DP##_r##NR##_bf16, DT_BF16, KV_FP8, DP, NR, W, EU)
+#define MTK_KV_ATTEND(NAME, DT, FMT, DP, NR, KB, W, EU)                                              \
+  extern "C" __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(EU, EU))) \
+  NAME(const mtk_kv_attn_kargs a) { kv_attend<DT, FMT, DP, NR, KB, W>(a); }
+#define MTK_KV_ATTEND_FMT(NAME, FMT, DP, NR, KB, W, EU)                                 \
+  MTK_KV_ATTEND(mtk_kv_attend_##NAME##_d##DP##_r##NR##_f16, DT_F16, FMT, DP, NR, KB, W, EU)   \
+  MTK_KV_ATTEND(mtk_kv_attend_##NAME##_d##DP##_r##NR##_bf16, DT_BF16, FMT, DP, NR, KB, W, EU)
 
-// mtk_kv_attend_<format>_d<padded head dimension>_r<16-row blocks per workgroup>_<type>: wavefronts per workgroup
-// and per SIMD by what their registers allow
-MTK_KV_ATTEND_DT(64, 1, 8, 4)
-MTK_KV_ATTEND_DT(64, 2, 8, 2)
-MTK_KV_ATTEND_DT(64, 4, 4, 2)
-MTK_KV_ATTEND_DT(128, 1, 8, 4)
-MTK_KV_ATTEND_DT(128, 2, 8, 2)
-MTK_KV_ATTEND_DT(128, 4, 4, 1)
-MTK_KV_ATTEND_DT(256, 1, 4, 2)
-MTK_KV_ATTEND_DT(256, 2, 4, 1)
+// mtk_kv_attend_<format>_d<padded head dimension>_r<16-row blocks per workgroup>_<type>: 16-key blocks per tile,
+// wavefronts per workgroup, wavefronts per SIMD as the registers allow. runtime: kv_kernel_shape.
+MTK_KV_ATTEND_FMT(fp4, KV_FP4, 64, 1, 4, 4, 4)
+MTK_KV_ATTEND_FMT(fp4, KV_FP4, 64, 2, 4, 8, 2)
+MTK_KV_ATTEND_FMT(fp4, KV_FP4, 64, 4, 2, 4, 2)
+MTK_KV_ATTEND_FMT(fp4, KV_FP4, 128, 1, 2, 4, 4)
+MTK_KV_ATTEND_FMT(fp4, KV_FP4, 128, 2, 2, 8, 2)
+MTK_KV_ATTEND_FMT(fp4, KV_FP4, 128, 4, 2, 4, 1)
+MTK_KV_ATTEND_FMT(fp4, KV_FP4, 256, 1, 2, 8, 2)
+MTK_KV_ATTEND_FMT(fp4, KV_FP4, 256, 2, 2, 4, 1)
+MTK_KV_ATTEND_FMT(fp8, KV_FP8, 64, 1, 4, 4, 3)
+MTK_KV_ATTEND_FMT(fp8, KV_FP8, 64, 2, 4, 8, 2)
+MTK_KV_ATTEND_FMT(fp8, KV_FP8, 64, 4, 2, 4, 2)
+MTK_KV_ATTEND_FMT(fp8, KV_FP8, 128, 1, 2, 4, 3)
+MTK_KV_ATTEND_FMT(fp8, KV_FP8, 128, 2, 2, 8, 2)
+MTK_KV_ATTEND_FMT(fp8, KV_FP8, 128, 4, 2, 4, 1)
+MTK_KV_ATTEND_FMT(fp8, KV_FP8, 256, 1, 2, 8, 2)
+MTK_KV_ATTEND_FMT(fp8, KV_FP8, 256, 2, 2, 4, 1)
 
-#define MTK_KV_COMBINE(NR, W)                                                                                          \
-  extern "C" __global__ void __launch_bounds__(kKvCombine) mtk_kv_combine_r##NR##_w##W##_f16(const mtk_kv_attn_kargs a) {  \
-    kv_combine<DT_F16, 16 * NR, kKvTile * W>(a);                                                                        \
-  }                                                                                                                 \
-  extern "C" __global__ void __launch_bounds__(kKvCombine) mtk_kv_combine_r##NR##_w##W##_bf16(const mtk_kv_attn_kargs a) { \
-    kv_combine<DT_BF16, 16 * NR, kKvTile * W>(a);                                                                       \
+#define MTK_KV_COMBINE(NR, STEP)                                                                                                 \
+  extern "C" __global__ void __launch_bounds__(kKvCombine) mtk_kv_combine_r##NR##_k##STEP##_f16(const mtk_kv_attn_kargs a) {  \
+    kv_combine<DT_F16, 16 * NR, STEP>(a);                                                                                        \
+  }                                                                                                                              \
+  extern "C" __global__ void __launch_bounds__(kKvCombine) mtk_kv_combine_r##NR##_k##STEP##_bf16(const mtk_kv_attn_kargs a) { \
+    kv_combine<DT_BF16, 16 * NR, STEP>(a);                                                                                       \
   }
-MTK_KV_COMBINE(1, 8)
-MTK_KV_COMBINE(2, 8)
-MTK_KV_COMBINE(1, 4)
-MTK_KV_COMBINE(2, 4)
-MTK_KV_COMBINE(4, 4)
+MTK_KV_COMBINE(1, 512)
+MTK_KV_COMBINE(1, 256)
+MTK_KV_COMBINE(1, 128)
+MTK_KV_COMBINE(2, 512)
+MTK_KV_COMBINE(2, 256)
+MTK_KV_COMBINE(2, 128)
+MTK_KV_COMBINE(4, 128)

@@ -54,45 +54,67 @@ MTK_KV_FN int kv_page(const int32_t *row_of_table, int64_t pos, int n_pages, int
   return page >= 0 && page < n_pages ? page : -1;
 }
 
-// Key splits. A sequence has blocks of `rows` (row, query head) pairs of a K/V head and ceil(keys / step) steps
-// of keys; one workgroup takes at most c steps of one block and head. c is the least (from `least` on) that keeps
-// the launch at about `units` workgroups: work / units, then raised while the rounding up of short sequences
-// still adds too many (which is looked at for up to 64 sequences).
+// x / d for 0 <= x < 2^31, 0 < d < 2^24.
+MTK_KV_FN int kv_div(int x, int d) {
+#ifdef __HIP_DEVICE_COMPILE__
+  // by a reciprocal in 32 bits: at most x 2^-22 / d + 1 off, so a second estimate of the rest is at most one off
+  const float inv = __builtin_amdgcn_rcpf((float)d);
+  int q = (int)((float)x * inv);
+  int r = x - q * d;
+  const int e = (int)((float)r * inv);
+  q += e;
+  r -= e * d;
+  return q + (r < 0 ? -1 : r >= d ? 1 : 0);
+#else
+  return x / d;
+#endif
+}
+
+// Who does what in attention. A sequence has `blocks` blocks of `rows` (row, query head) pairs for each K/V head, and
+// `steps` steps of keys (at least one). The (block, head) pairs of all sequences, sequence after sequence, lie on a
+// line; workgroup w has the steps from w * each to (w + 1) * each of it, so that all of them have the same work, whatever
+// the lengths. A pair that a boundary cuts leaves partial sums.
+//   each = max(least, work / units), so that there are at most `units` workgroups.
+// Where so little work is left that pairs of their own workgroups (ceil(steps / least) each) are no more than `units`,
+// a pair's length on the line is rounded up to a multiple of `each` = least: no workgroup has parts of two pairs.
 typedef struct {
-  int blocks; /* row blocks */
-  int steps;
-  int splits, per; /* workgroups per block and head, steps of each */
+  int blocks, steps;
 } kv_share;
 
 MTK_KV_FN kv_share kv_blocks(kv_seq s, int S_q, int G, int rows, int step, int rows_above, int rows_most) {
   kv_share r;
-  const int64_t pairs = (int64_t)(s.rows < S_q ? s.rows : S_q) * G;
-  const int mine = pairs > rows_above && pairs <= rows_most;
-  r.blocks = mine ? (int)((pairs + rows - 1) / rows) : 0;
-  r.steps = (int)(((int64_t)s.keys + step - 1) / step);
-  r.splits = 1;
-  r.per = r.steps;
+  const uint32_t pairs = (uint32_t)(s.rows < S_q ? s.rows : S_q) * (uint32_t)G;  // S_q * G < 2^31
+  const int mine = pairs > (uint32_t)rows_above && pairs <= (uint32_t)rows_most;
+  r.blocks = mine ? (int)((pairs + (uint32_t)rows - 1) / (uint32_t)rows) : 0;
+  r.steps = (int)(((uint32_t)s.keys + (uint32_t)step - 1) / (uint32_t)step);
+  if (r.steps < 1) r.steps = 1;
   return r;
 }
 
-MTK_KV_FN void kv_split(kv_share *r, int c) {
-  if (r->steps <= c) {
-    r->splits = 1;
-    r->per = r->steps;
-    return;
+// Workgroups of a pair's own, of `least` steps each.
+MTK_KV_FN int kv_own(kv_share r, int least) { return kv_div(r.steps + least - 1, least); }
+
+typedef struct {
+  int each;   /* steps of a workgroup */
+  int padded; /* a pair's length is a multiple of it */
+} kv_cut;
+
+// From the sums over all sequences of blocks * heads * steps and blocks * heads * kv_own. whole: every pair has one
+// workgroup (its steps are at most `least`), however many.
+MTK_KV_FN kv_cut kv_cut_of(int work, int own, int units, int least, int whole) {
+  kv_cut c;
+  c.padded = whole || own <= units;
+  c.each = least;
+  if (!c.padded) {
+    const int n = kv_div(work + units - 1, units);
+    if (n > least) c.each = n;
   }
-  const int n = (r->steps + c - 1) / c;
-  r->per = (r->steps + n - 1) / n;
-  r->splits = (r->steps + r->per - 1) / r->per;
+  return c;
 }
 
-// The next c to try when `total` workgroups came out.
-MTK_KV_FN int kv_next_c(int c, int total, int units) {
-  const int64_t n = (int64_t)c * total / (units > 0 ? units : 1);
-  return n > c ? (n < (1 << 30) ? (int)n : (1 << 30)) : c + 1;
-}
+MTK_KV_FN int kv_length(kv_share r, kv_cut c) { return c.padded ? kv_div(r.steps + c.each - 1, c.each) * c.each : r.steps; }
 
-// Most workgroups of a launch with these limits: each row block and head rounds its splits up by less than one.
+// Most row blocks per K/V head of a launch.
 MTK_KV_FN int64_t kv_max_blocks(int B, int T, int S_q, int G, int rows) {
   const int64_t each = (int64_t)B * (((int64_t)S_q * G + rows - 1) / rows);
   const int64_t all = (int64_t)T * G / rows + B;

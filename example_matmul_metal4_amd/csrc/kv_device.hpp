@@ -70,15 +70,6 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
-// A wavefront's view of the batch: which sequence has unit `id` (or packed row `id`).
-struct KvUnit {
-  int b = -1;     // sequence, -1: none
-  int total = 0;  // units of the launch
-  int base = 0;   // the sequence's first unit
-  kv_seq seq;
-  kv_share share;
-};
-
 template <typename A>
 __device__ __forceinline__ kv_seq load_seq(const A &a, int b) {
   if (b >= a.B) return kv_sequence(0, 0, 0, 0, a.max_pages, a.page_shift);
@@ -100,68 +91,110 @@ __device__ __forceinline__ int seq_of_row(const A &a, int t, int lane) {
   return __builtin_amdgcn_readfirstlane(found);
 }
 
-// The shares of the sequences in kernels of ROWS rows per block and STEP keys per step, and the sequence that
-// unit(total) falls into, or sequence `want_b` if that is not negative. One wavefront's lanes hold 64 sequences.
-template <int ROWS, int STEP, typename F>
-__device__ __forceinline__ KvUnit find_unit(const mtk_kv_attn_kargs &a, int lane, int want_b, F &&unit) {
-  const int G = a.G;
-  KvUnit u;
-  auto share_of = [&](const kv_seq &s) { return kv_blocks(s, a.S_q, G, ROWS, STEP, a.rows_above, a.rows_most); };
-  // work -> steps per workgroup
-  float work = 0.0f;
-  kv_seq s0 = load_seq(a, lane);
-  kv_share h0 = share_of(s0);
-  work = (float)h0.blocks * (float)h0.steps;
-  for (int b0 = 64; b0 < a.B; b0 += 64) {
-    const kv_share h = share_of(load_seq(a, b0 + lane));
-    work += (float)h.blocks * (float)h.steps;
+// Some steps of one pair (kv_cache.h).
+struct KvSegment {
+  int b = -1;       // sequence, -1: none
+  int hk, rb;       // K/V head, row block
+  int from, to;     // steps
+  int steps;        // of the pair
+  int start;        // the pair's place on the line
+  kv_seq seq;
+};
+
+// A wavefront's view of the line: 64 sequences at a time, in LDS words of its own (registers are what the kernel is
+// short of). ROWS rows per block, STEP keys per step.
+constexpr int kLineWords = 4 * 64;
+template <int ROWS, int STEP>
+struct KvLine {
+  const mtk_kv_attn_kargs &a;
+  const int lane;
+  int *const sm;  // [4][64]: where the sequence's pairs end, first row, rows, length
+  kv_cut cut;
+  int total;              // length of the line
+  int b0 = 0, before = 0; // the first of the 64, and where its pairs start
+
+  __device__ __forceinline__ kv_share share_of(const kv_seq &x) const {
+    return kv_blocks(x, a.S_q, a.G, ROWS, STEP, a.rows_above, a.rows_most);
   }
-  const float each = ceilf(wave_sum(work) * (float)a.H_kv / (float)a.units);
-  int c = max(a.least, each < 1e9f ? (int)each : 1000000000);
-  if (a.B <= 64) {
-    int scan = 0;
+  __device__ __forceinline__ int len_of(int b) const { return b < a.B ? a.kv_len[b] : 0; }
+  __device__ __forceinline__ void place(const kv_seq &s, int len, const kv_share &h) {
+    sm[lane] = before + wave_scan(h.blocks * a.H_kv * kv_length(h, cut));
+    sm[64 + lane] = s.first;
+    sm[128 + lane] = s.rows;
+    sm[192 + lane] = len;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  __device__ __forceinline__ KvLine(const mtk_kv_attn_kargs &args, int lane_, int *words) : a(args), lane(lane_), sm(words) {
+    const kv_seq s = load_seq(a, lane);
+    const int len = len_of(lane);
+    const kv_share h = share_of(s);
+    int work = h.blocks * a.H_kv * h.steps, own = h.blocks * a.H_kv * kv_own(h, a.least);
 #pragma unroll 1
-    for (int i = 0;; ++i) {
-      kv_split(&h0, c);
-      scan = wave_scan(h0.blocks * h0.splits * a.H_kv);
-      u.total = __builtin_amdgcn_readlane(scan, 63);
-      if (u.total <= a.units || i == 2) break;
-      c = kv_next_c(c, u.total, a.units);
+    for (int b = 64; b < a.B; b += 64) {
+      const kv_share x = share_of(load_seq(a, b + lane));
+      work += x.blocks * a.H_kv * x.steps;
+      own += x.blocks * a.H_kv * kv_own(x, a.least);
     }
-    const int id = unit(u.total);
-    const uint64_t past = want_b >= 0 ? 1ull << want_b : __ballot(scan > id);
-    if (!past || (want_b < 0 && id < 0)) return u;
-    const int at = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
-    u.b = at;
-    u.base = __builtin_amdgcn_readlane(scan - h0.blocks * h0.splits * a.H_kv, at);
-  } else {
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-      kv_share h = share_of(load_seq(a, b0 + lane));
-      kv_split(&h, c);
-      u.total += __builtin_amdgcn_readlane(wave_scan(h.blocks * h.splits * a.H_kv), 63);
-    }
-    const int id = unit(u.total);
-    if (want_b < 0 && (id < 0 || id >= u.total)) return u;
-    int before = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-      kv_share h = share_of(load_seq(a, b0 + lane));
-      kv_split(&h, c);
-      const int n = h.blocks * h.splits * a.H_kv, scan = before + wave_scan(n);
-      const uint64_t past = want_b >= 0 ? (want_b - b0 < 64 ? 1ull << (want_b - b0) : 0ull) : __ballot(scan > id);
-      if (past) {
-        const int at = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
-        u.b = b0 + at;
-        u.base = __builtin_amdgcn_readlane(scan - n, at);
-        break;
-      }
-      before = __builtin_amdgcn_readlane(scan, 63);
-    }
-    if (u.b < 0) return u;
+    work = __builtin_amdgcn_readlane(wave_scan(work), 63);
+    own = __builtin_amdgcn_readlane(wave_scan(own), 63);
+    cut = kv_cut_of(work, own, a.units, a.least, a.whole);
+    cut.each = __builtin_amdgcn_readfirstlane(cut.each);
+    total = cut.padded ? own * a.least : work;
+    place(s, len, h);
   }
-  u.seq = load_seq(a, u.b);
-  u.share = share_of(u.seq);
-  kv_split(&u.share, c);
-  return u;
-}
+  __device__ __forceinline__ void next() {  // the next 64
+    before = __builtin_amdgcn_readfirstlane(sm[63]);
+    b0 += 64;
+    const kv_seq s = load_seq(a, b0 + lane);
+    place(s, len_of(b0 + lane), share_of(s));
+  }
+  // The lane of the sequence that pos falls into, or -1. pos ascends from call to call.
+  __device__ __forceinline__ int find(int pos) {
+    for (;;) {
+      const uint64_t in = __ballot(sm[lane] > pos);
+      if (in) return __builtin_amdgcn_readfirstlane(__builtin_ctzll(in));
+      if (b0 + 64 >= a.B) return -1;
+      next();
+    }
+  }
+  // The lane of the sequence that packed row t belongs to, or -1. t ascends from call to call.
+  __device__ __forceinline__ int find_row(int t) {
+    for (;;) {
+      const int first = sm[64 + lane];
+      const uint64_t in = __ballot(b0 + lane < a.B && first <= t && t < first + sm[128 + lane]);
+      if (in) return __builtin_amdgcn_readfirstlane(__builtin_ctzll(in));
+      if (b0 + 64 >= a.B) return -1;
+      next();
+    }
+  }
+  // That sequence; the length of its pairs and where they start.
+  __device__ __forceinline__ KvSegment sequence(int at, int &length, int &base, int &pairs) const {
+    KvSegment g;
+    g.b = b0 + at;
+    const int first = __builtin_amdgcn_readfirstlane(sm[64 + at]), rows = __builtin_amdgcn_readfirstlane(sm[128 + at]);
+    g.seq = kv_sequence(first, first + rows, __builtin_amdgcn_readfirstlane(sm[192 + at]), a.T, a.max_pages, a.page_shift);
+    const kv_share h = share_of(g.seq);
+    g.steps = h.steps;
+    length = __builtin_amdgcn_readfirstlane(kv_length(h, cut));
+    pairs = h.blocks * a.H_kv;
+    base = __builtin_amdgcn_readfirstlane(sm[at]) - pairs * length;
+    return g;
+  }
+  // The pair at pos, pos < end, and its steps before `end`. Steps past a padded pair's own: none (from >= to).
+  __device__ __forceinline__ KvSegment at(int pos, int end) {
+    const int l = find(pos);
+    if (l < 0) return KvSegment{};
+    int length, base, pairs;
+    KvSegment g = sequence(l, length, base, pairs);
+    const int pair = __builtin_amdgcn_readfirstlane(kv_div(pos - base, length));
+    g.start = base + pair * length;
+    g.from = pos - g.start;
+    g.to = min(g.steps, end - g.start);
+    g.rb = __builtin_amdgcn_readfirstlane(kv_div(pair, a.H_kv));
+    g.hk = pair - g.rb * a.H_kv;
+    return g;
+  }
+};
 
 }  // namespace mtk

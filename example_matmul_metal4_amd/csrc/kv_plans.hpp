@@ -100,6 +100,19 @@ int plan_kv_move(mtk_ctx *ctx, const mtk_kv_desc *d_in, PlanKind kind, mtk_plan 
   return finish_kv(p, out);
 }
 
+// Of the attention kernels (kv_attention.hip): keys per tile, wavefronts per workgroup, workgroups per CU.
+struct KvShape {
+  int tile, waves, per_cu;
+  int step() const { return tile * waves; }
+};
+KvShape kv_kernel_shape(int fmt, int dp, int nr) {
+  const bool fp4 = fmt == MTK_KV_FP4;
+  if (nr == 4) return {32, 4, dp == 64 ? 2 : 1};
+  if (dp == 64) return nr == 1 ? KvShape{64, 4, fp4 ? 4 : 3} : KvShape{64, 8, 1};
+  if (dp == 128) return nr == 1 ? KvShape{32, 4, fp4 ? 4 : 3} : KvShape{32, 8, 1};
+  return nr == 1 ? KvShape{32, 8, 1} : KvShape{32, 4, 1};
+}
+
 int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
   if (!d_in || !out) return fail(MTK_ERR_INVALID, "null descriptor or output");
   mtk_kv_desc d = *d_in;
@@ -108,6 +121,8 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
   if (d.H <= 0 || d.H % d.H_kv != 0) return fail(MTK_ERR_INVALID, "H must be a positive multiple of H_kv (got H=%d, H_kv=%d)", d.H, d.H_kv);
   if (d.S_q == 0) d.S_q = d.T;
   if (d.S_q < 0 || d.S_q > d.T) return fail(MTK_ERR_INVALID, "S_q must be 0 to T (got %d, T=%d)", d.S_q, d.T);
+  if ((long long)d.S_q * (d.H / d.H_kv) > INT32_MAX / 2)
+    return fail(MTK_ERR_UNSUPPORTED, "S_q x H / H_kv of %lld is not supported", (long long)d.S_q * (d.H / d.H_kv));
   if ((long long)d.H * d.D > INT32_MAX || (long long)d.T * d.H > INT32_MAX / 64)
     return fail(MTK_ERR_UNSUPPORTED, "T x H of more than 2^25 rows, or rows of more than 2^31 elements, are not supported");
   mtk_kv_attn_kargs a{};
@@ -131,16 +146,17 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
   a.rows_most = INT32_MAX;
   const long long pairs = (long long)d.S_q * G;
   const int nr = pairs <= 16 ? 1 : pairs <= 32 || dp == 256 ? 2 : 4, rows = 16 * nr;
-  const int waves = nr == 4 || dp == 256 ? 4 : 8, step = 32 * waves;
-  a.units = cus * (nr == 1 ? 2 : 1);
-  a.least = 32 / waves;
-  const long long blocks = kv_max_blocks(d.B, d.T, d.S_q, G, rows) * d.H_kv;
-  if (blocks > (1 << 27)) return fail(MTK_ERR_UNSUPPORTED, "a batch of more than 2^27 row blocks is not supported");
-  a.max_units = (int)(a.units + blocks);
+  const KvShape shape = kv_kernel_shape(d.format, dp, nr);
+  a.units = cus * shape.per_cu;
+  a.least = 1024 / shape.step();
+  const long long steps = std::max(1LL, ((long long)d.max_pages * d.page_size + shape.step() - 1) / shape.step());
+  const long long each = ((pairs + rows - 1) / rows) * d.B * d.H_kv;  // blocks, whatever row_start holds
+  if (each * (steps + a.least) > INT32_MAX)
+    return fail(MTK_ERR_UNSUPPORTED, "a batch of %lld row blocks over %lld positions is not supported", each, (long long)d.max_pages * d.page_size);
+  a.whole = steps <= a.least ? 1 : 0;
   a.part_ld = a.blocks * 32;
-  const long long steps = ((long long)d.max_pages * d.page_size + step - 1) / step;
-  const bool split = steps > a.least;
-  if (!split) a.max_units = (int)blocks;
+  const bool split = !a.whole;
+  const int grid = a.whole ? (int)(kv_max_blocks(d.B, d.T, d.S_q, G, rows) * d.H_kv) : a.units;
   mtk_plan *p = new mtk_plan();
   p->ctx = ctx;
   p->kind = PLAN_KV_ATTN;
@@ -149,19 +165,19 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
   Launch g;
   snprintf(name, sizeof name, "mtk_kv_attend_%s_d%d_r%d_%s", kv_format(d), dp, nr, kv_suffix(d).c_str());
   g.name = name;
-  g.grid = (unsigned)a.max_units;
-  g.block = 64 * waves;
+  g.grid = (unsigned)grid;
+  g.block = 64u * (unsigned)shape.waves;
   set_args(g, a);
   p->launches.push_back(g);
   if (split) {
     Launch c = g;
-    snprintf(name, sizeof name, "mtk_kv_combine_r%d_w%d_%s", nr, waves, kv_suffix(d).c_str());
+    snprintf(name, sizeof name, "mtk_kv_combine_r%d_k%d_%s", nr, shape.step(), kv_suffix(d).c_str());
     c.name = name;
     c.block = 256;
     c.grid = (unsigned)std::min<long long>((long long)d.T * d.H, 8LL * cus);
     p->launches.push_back(c);
-    p->part_ml_at = (size_t)a.max_units * rows * a.part_ld * sizeof(float);
-    p->workspace = p->part_ml_at + (size_t)a.max_units * rows * 2 * sizeof(float);
+    p->part_ml_at = (size_t)a.units * 2 * rows * a.part_ld * sizeof(float);
+    p->workspace = p->part_ml_at + (size_t)a.units * 2 * rows * 2 * sizeof(float);
   }
   const double cap = (double)d.max_pages * d.page_size;
   p->flops = 4.0 * d.T * d.H * d.D * cap;
@@ -169,9 +185,9 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
              4.0 * (2.0 * d.B + 1 + (double)d.B * d.max_pages);
   char desc[320];
   snprintf(desc, sizeof desc,
-           "kv attention %s %s B=%d T=%d S_q=%d H=%d H_kv=%d D=%d pages=%dx%d max_pages=%d causal=%d rows/wg=%d workgroups=%d, most %d",
+           "kv attention %s %s B=%d T=%d S_q=%d H=%d H_kv=%d D=%d pages=%dx%d max_pages=%d causal=%d rows/wg=%d grid=%d%s",
            kv_format(d), kv_suffix(d).c_str(), d.B, d.T, d.S_q, d.H, d.H_kv, d.D, d.n_pages, d.page_size, d.max_pages, a.causal, rows,
-           a.units, a.max_units);
+           grid, a.whole ? "" : ", equal shares of all keys");
   p->description = desc;
   return finish_kv(p, out);
 }
