@@ -178,6 +178,7 @@ typedef struct {
   int32_t rows_above, rows_most;
   /* who does what (kv_cache.h): workgroups wanted (at most), least steps of one, or one for each pair */
   int32_t units, least, whole;
+  int32_t most_blocks; /* whole: row blocks of a sequence, at most */
   int32_t part_ld; /* floats per row of part */
 } mtk_kv_attn_kargs;
 

@@ -85,14 +85,31 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
   const int c = lane & 15, j = lane >> 4;
   const int G = a.G;
 
-  __shared__ int sm_line[W][kLineWords];
-  KvLine<kRows, kKvStep> line(a, lane, sm_line[wave]);
-  const int wgs = kv_div(line.total + line.cut.each - 1, line.cut.each);
-  if ((int)blockIdx.x >= wgs) return;
-  const int wg = xcd_remap(blockIdx.x, wgs);
-  const int line_from = wg * line.cut.each, line_to = min(line.total, line_from + line.cut.each);
-  KvSegment seg = line.at(line_from, line_to);
-  if (seg.b < 0) return;
+  __shared__ int sm_line[W == 16 ? 1 : W][kLineWords];  // 16 wavefronts: pairs are whole
+  KvLine<kRows, kKvStep> line(a, lane, sm_line[W == 16 ? 0 : wave]);
+  int wg = 0, line_from = 0, line_to = 0;
+  KvSegment seg;
+  const bool whole = W == 16 || a.whole;
+  if (whole) {  // a workgroup for each pair, by its number: nothing to look up
+    const int q = kv_div(blockIdx.x, a.H_kv);
+    seg.hk = blockIdx.x - q * a.H_kv;
+    seg.b = a.most_blocks == 1 ? q : kv_div(q, a.most_blocks);
+    seg.rb = q - seg.b * a.most_blocks;
+    seg.seq = load_seq(a, seg.b);
+    const kv_share h = line.share_of(seg.seq);
+    seg.from = seg.start = 0;
+    seg.to = seg.steps = h.steps;
+    if (seg.rb >= h.blocks) return;
+  } else {
+    line.lay();
+    const int wgs = kv_div(line.total + line.cut.each - 1, line.cut.each);
+    if ((int)blockIdx.x >= wgs) return;
+    wg = xcd_remap(blockIdx.x, wgs);
+    line_from = wg * line.cut.each;
+    line_to = min(line.total, line_from + line.cut.each);
+    seg = line.at(line_from, line_to);
+    if (seg.b < 0) return;
+  }
 
   // ---- this lane's place in 16 positions of codes and scales. Lanes of blocks past the head's last read the last
   // one: Q is zero there, and those dims of O are not stored.
@@ -120,7 +137,7 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
     const char *head;     // the K/V head's region of page 0
     const int32_t *table;
     uint32_t pages;       // entries below it are pages
-    int last_entry, last_block, e0, window, next_window;
+    int last_block, e0, window, next_window;
     int key0, key_end, n_keys;  // this wavefront's first key, the segment's end, the keys that its rows see
   };
   auto source = [&](const KvSegment &g) {
@@ -134,10 +151,9 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
     x.table = a.table + (size_t)(uint32_t)g.b * (uint32_t)a.max_pages;
     x.pages = g.seq.bad ? 0u : (uint32_t)a.n_pages;
     x.last_block = (max(x.n_keys, 1) - 1) & ~15;
-    x.last_entry = x.last_block >> a.page_shift;
-    x.e0 = min(x.key0, x.last_block) >> a.page_shift;
-    x.window = x.table[min(x.e0 + lane, x.last_entry)];
-    x.next_window = x.table[min(x.e0 + kWindow + lane, x.last_entry)];
+    x.e0 = x.key0 >> a.page_shift;
+    x.window = x.table[min(x.e0 + lane, a.max_pages - 1)];
+    x.next_window = x.table[min(x.e0 + kWindow + lane, a.max_pages - 1)];
     return x;
   };
   // Where the blocks of a tile are. The range of the loads is the page's region.
@@ -149,7 +165,7 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
     if ((min(key0 + kKvTile - 16, x.last_block) >> a.page_shift) - x.e0 >= 64) {
       x.e0 += kWindow;
       x.window = x.next_window;
-      x.next_window = x.table[min(x.e0 + kWindow + lane, x.last_entry)];
+      x.next_window = x.table[min(x.e0 + kWindow + lane, a.max_pages - 1)];
     }
     t.bad = 0;
     Place p;
@@ -246,7 +262,7 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
 
   for (;;) {
     // the next segment's table entries, ahead of their use
-    const bool more = seg.start + seg.to < line_to && !line.cut.padded;
+    const bool more = !whole && !line.cut.padded && seg.start + seg.to < line_to;
     int window = 0, next_window = 0;
     if (more) {
       const Source x = source(line.at(seg.start + seg.to, line_to));
@@ -470,8 +486,16 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
         if (r >= rows) continue;
         KvPart sum;
 #pragma unroll
-        for (int w = 0; w < W; ++w)
-          add_part(sum, KvPart{sm_m[w][rr], sm_l[w][rr], *(const f32x4 *)((const float *)smem + w * (kParkB / 4) + rr * kPitch + d0)});
+        for (int w = 0; w < W; ++w) sum.m = fmaxf(sum.m, sm_m[w][rr]);
+        const float m0 = sum.m == -INFINITY ? 0.0f : sum.m;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const float m = sm_m[w][rr], f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m0);  // no keys, or NaN scores
+          sum.l = __builtin_fmaf(f, sm_l[w][rr], sum.l);
+          const f32x4 x = *(const f32x4 *)((const float *)smem + w * (kParkB / 4) + rr * kPitch + d0);
+          sum.x = f32x4{__builtin_fmaf(f, x.x, sum.x.x), __builtin_fmaf(f, x.y, sum.x.y), __builtin_fmaf(f, x.z, sum.x.z),
+                        __builtin_fmaf(f, x.w, sum.x.w)};
+        }
         if (alone) {
           const int i = kv_div(r, G);
           store_out<DT>(a, seg.seq.first + i, seg.hk * G + r - i * G, d0, sum);
@@ -504,7 +528,7 @@ __device__ __forceinline__ void kv_combine(const mtk_kv_attn_kargs &a) {
   if (it >= end) return;
   __shared__ int sm_line[kKvCombine / 64][kLineWords];
   KvLine<ROWS, STEP> line(a, lane, sm_line[tid >> 6]);
-  if (line.cut.padded && line.cut.each >= line.total) return;
+  line.lay();
   int b = -1, base = 0, length = 1;
   KvSegment seq{};
   for (; it < end; ++it) {  // uniform: every wavefront takes the same items
@@ -588,6 +612,14 @@ MTK_KV_ATTEND_FMT(fp8, KV_FP8, 128, 2, 2, 8, 2)
 MTK_KV_ATTEND_FMT(fp8, KV_FP8, 128, 4, 2, 4, 1)
 MTK_KV_ATTEND_FMT(fp8, KV_FP8, 256, 1, 2, 8, 2)
 MTK_KV_ATTEND_FMT(fp8, KV_FP8, 256, 2, 2, 4, 1)
+// ..._w16: 16 wavefronts, for few pairs of short sequences, where a tile's latency counts
+#define MTK_KV_ATTEND_W16(NAME, FMT, DP, KB)                                            \
+  MTK_KV_ATTEND(mtk_kv_attend_##NAME##_d##DP##_r1_w16_f16, DT_F16, FMT, DP, 1, KB, 16, 4)     \
+  MTK_KV_ATTEND(mtk_kv_attend_##NAME##_d##DP##_r1_w16_bf16, DT_BF16, FMT, DP, 1, KB, 16, 4)
+MTK_KV_ATTEND_W16(fp4, KV_FP4, 64, 2)
+MTK_KV_ATTEND_W16(fp4, KV_FP4, 128, 2)
+MTK_KV_ATTEND_W16(fp8, KV_FP8, 64, 2)
+MTK_KV_ATTEND_W16(fp8, KV_FP8, 128, 2)
 
 #define MTK_KV_COMBINE(NR, STEP)                                                                                                 \
   extern "C" __global__ void __launch_bounds__(kKvCombine) mtk_kv_combine_r##NR##_k##STEP##_f16(const mtk_kv_attn_kargs a) {  \

@@ -109,8 +109,8 @@ struct KvLine {
   const mtk_kv_attn_kargs &a;
   const int lane;
   int *const sm;  // [4][64]: where the sequence's pairs end, first row, rows, length
-  kv_cut cut;
-  int total;              // length of the line
+  kv_cut cut{};
+  int total = 0;          // length of the line
   int b0 = 0, before = 0; // the first of the 64, and where its pairs start
 
   __device__ __forceinline__ kv_share share_of(const kv_seq &x) const {
@@ -125,7 +125,8 @@ struct KvLine {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
-  __device__ __forceinline__ KvLine(const mtk_kv_attn_kargs &args, int lane_, int *words) : a(args), lane(lane_), sm(words) {
+  __device__ __forceinline__ KvLine(const mtk_kv_attn_kargs &args, int lane_, int *words) : a(args), lane(lane_), sm(words) {}
+  __device__ __forceinline__ void lay() {
     const kv_seq s = load_seq(a, lane);
     const int len = len_of(lane);
     const kv_share h = share_of(s);

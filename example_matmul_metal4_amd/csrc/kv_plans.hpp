@@ -146,24 +146,28 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
   a.rows_most = INT32_MAX;
   const long long pairs = (long long)d.S_q * G;
   const int nr = pairs <= 16 ? 1 : pairs <= 32 || dp == 256 ? 2 : 4, rows = 16 * nr;
-  const KvShape shape = kv_kernel_shape(d.format, dp, nr);
+  // few pairs of short sequences: one workgroup of 16 wavefronts each, no second kernel
+  const long long positions = (long long)d.max_pages * d.page_size;
+  const bool wide = nr == 1 && dp <= 128 && positions <= 4096 && kv_max_blocks(d.B, d.T, d.S_q, G, rows) * d.H_kv <= cus;
+  const KvShape shape = wide ? KvShape{32, 16, 1} : kv_kernel_shape(d.format, dp, nr);
   a.units = cus * shape.per_cu;
-  a.least = 1024 / shape.step();
+  a.least = 2;
   const long long steps = std::max(1LL, ((long long)d.max_pages * d.page_size + shape.step() - 1) / shape.step());
   const long long each = ((pairs + rows - 1) / rows) * d.B * d.H_kv;  // blocks, whatever row_start holds
   if (each * (steps + a.least) > INT32_MAX)
     return fail(MTK_ERR_UNSUPPORTED, "a batch of %lld row blocks over %lld positions is not supported", each, (long long)d.max_pages * d.page_size);
-  a.whole = steps <= a.least ? 1 : 0;
+  a.whole = positions <= (wide ? 4096 : 1024) && each < (1 << 23) ? 1 : 0;
   a.part_ld = a.blocks * 32;
   const bool split = !a.whole;
-  const int grid = a.whole ? (int)(kv_max_blocks(d.B, d.T, d.S_q, G, rows) * d.H_kv) : a.units;
+  a.most_blocks = (int)((pairs + rows - 1) / rows);
+  const int grid = a.whole ? (int)each : a.units;
   mtk_plan *p = new mtk_plan();
   p->ctx = ctx;
   p->kind = PLAN_KV_ATTN;
   p->kv = d;
   char name[96];
   Launch g;
-  snprintf(name, sizeof name, "mtk_kv_attend_%s_d%d_r%d_%s", kv_format(d), dp, nr, kv_suffix(d).c_str());
+  snprintf(name, sizeof name, "mtk_kv_attend_%s_d%d_r%d_%s%s", kv_format(d), dp, nr, wide ? "w16_" : "", kv_suffix(d).c_str());
   g.name = name;
   g.grid = (unsigned)grid;
   g.block = 64u * (unsigned)shape.waves;
