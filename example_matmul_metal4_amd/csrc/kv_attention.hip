@@ -529,7 +529,7 @@ __device__ __forceinline__ void kv_combine(const mtk_kv_attn_kargs &a) {
   __shared__ int sm_line[kKvCombine / 64][kLineWords];
   KvLine<ROWS, STEP> line(a, lane, sm_line[tid >> 6]);
   line.lay();
-  int b = -1, base = 0, length = 1;
+  int b = -1, base = 0, length = 1, blocks = 0;
   KvSegment seq{};
   for (; it < end; ++it) {  // uniform: every wavefront takes the same items
     const int t = it / a.H, h = it - t * a.H;
@@ -543,14 +543,15 @@ __device__ __forceinline__ void kv_combine(const mtk_kv_attn_kargs &a) {
       int pairs;
       seq = line.sequence(at, length, base, pairs);
       if (pairs == 0) length = 0;
+      blocks = kv_div(pairs, a.H_kv);
     }
     if (length == 0 || t - seq.seq.first >= a.S_q || (line.cut.padded && length == line.cut.each)) {
       it = min((int64_t)end, (int64_t)(seq.seq.first + seq.seq.rows) * a.H) - 1;  // none of the sequence's, or none left
       continue;
     }
     const int hk = h / G, r = (t - seq.seq.first) * G + h - hk * G;
-    const int start = base + (r / ROWS * a.H_kv + hk) * length;
-    const int w0 = kv_div(start, line.cut.each), w1 = min(kv_div(start + seq.steps - 1, line.cut.each), a.units - 1);
+    const int start = base + ((a.by_pair ? blocks - 1 - r / ROWS : r / ROWS) * a.H_kv + hk) * length;
+    const int w0 = kv_div(start, line.cut.each), w1 = min(kv_div(start + seq.steps - 1, line.cut.each), a.places - 1);
     if (w0 >= w1) continue;  // one workgroup's
     const int first = start == w0 * line.cut.each ? 0 : 1;
     KvPart sum;
@@ -561,7 +562,7 @@ __device__ __forceinline__ void kv_combine(const mtk_kv_attn_kargs &a) {
       for (int i = 0; i < kAhead; ++i) {
         const int w = s0 + i * groups;
         if (w <= w1) {
-          const size_t at = ((size_t)w * 2 + (w == w0 ? first : 0)) * ROWS + r % ROWS;
+          const size_t at = (a.by_pair ? (size_t)w : (size_t)w * 2 + (w == w0 ? first : 0)) * ROWS + r % ROWS;
           const f32x2 ml = *(const f32x2 *)(a.part_ml + 2 * at);
           p[i] = KvPart{ml.x, ml.y, *(const f32x4 *)(a.part + at * a.part_ld + d)};
         }
@@ -580,6 +581,59 @@ __device__ __forceinline__ void kv_combine(const mtk_kv_attn_kargs &a) {
       }
       store_out<DT>(a, t, h, d, sum);
     }
+  }
+}
+
+// The same where rows are many and parts few (kv_prefill.hip's): each group of lanes has a query head of its own.
+template <int DT, int ROWS, int STEP>
+__device__ __forceinline__ void kv_combine_rows(const mtk_kv_attn_kargs &a) {
+  __shared__ int sm_line[kKvCombine / 64][kLineWords];
+  const int tid = threadIdx.x, lane = tid & 63, G = a.G;
+  const int chunks = a.part_ld / 4, groups = kKvCombine / chunks;
+  const int g = tid / chunks, d = 4 * (tid - g * chunks);
+  const int per = (a.T + gridDim.x - 1) / gridDim.x, end = min(a.T, ((int)blockIdx.x + 1) * per);
+  int t = blockIdx.x * per;
+  if (t >= end) return;
+  KvLine<ROWS, STEP> line(a, lane, sm_line[tid >> 6]);
+  line.lay();
+  while (t < end) {  // uniform
+    const int at = line.find_row(t);
+    if (at < 0) {
+      ++t;
+      continue;
+    }
+    int length, base, pairs;
+    const KvSegment seq = line.sequence(at, length, base, pairs);
+    const int past = min(end, seq.seq.first + seq.seq.rows);
+    const bool cut = pairs > 0 && length > line.cut.each;
+    const int blocks = kv_div(pairs, a.H_kv);
+    if (cut) {
+      for (; t < past; ++t) {
+        const int i = t - seq.seq.first;
+        if (i >= a.S_q) break;
+        for (int h = g; h < a.H && g < groups; h += groups) {
+          const int hk = kv_div(h, G), r = i * G + h - hk * G;
+          const int start = base + ((a.by_pair ? blocks - 1 - r / ROWS : r / ROWS) * a.H_kv + hk) * length;
+          const int w0 = kv_div(start, line.cut.each), w1 = min(kv_div(start + seq.steps - 1, line.cut.each), a.places - 1);
+          KvPart sum;
+          constexpr int kAhead = 4;
+          for (int s0 = w0; s0 <= w1; s0 += kAhead) {
+            KvPart p[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+              if (s0 + k <= w1) {
+                const size_t place = (size_t)(s0 + k) * ROWS + r % ROWS;
+                const f32x2 ml = *(const f32x2 *)(a.part_ml + 2 * place);
+                p[k] = KvPart{ml.x, ml.y, *(const f32x4 *)(a.part + place * a.part_ld + d)};
+              }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) add_part(sum, p[k]);
+          }
+          store_out<DT>(a, t, h, d, sum);
+        }
+      }
+    }
+    t = past;
   }
 }
 
@@ -635,3 +689,10 @@ MTK_KV_COMBINE(2, 512)
 MTK_KV_COMBINE(2, 256)
 MTK_KV_COMBINE(2, 128)
 MTK_KV_COMBINE(4, 128)
+
+extern "C" __global__ void __launch_bounds__(kKvCombine) mtk_kv_combine_rows_f16(const mtk_kv_attn_kargs a) {
+  kv_combine_rows<DT_F16, 128, 64>(a);
+}
+extern "C" __global__ void __launch_bounds__(kKvCombine) mtk_kv_combine_rows_bf16(const mtk_kv_attn_kargs a) {
+  kv_combine_rows<DT_BF16, 128, 64>(a);
+}

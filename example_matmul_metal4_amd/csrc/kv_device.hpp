@@ -138,6 +138,12 @@ struct KvLine {
       own += x.blocks * a.H_kv * kv_own(x, a.least);
     }
     work = __builtin_amdgcn_readlane(wave_scan(work), 63);
+    if (a.by_pair) {
+      cut.padded = 1;
+      cut.each = __builtin_amdgcn_readfirstlane(max(a.least, kv_div(work + a.units - 1, a.units)));
+      place(s, len, h);
+      return;
+    }
     own = __builtin_amdgcn_readlane(wave_scan(own), 63);
     cut = kv_cut_of(work, own, a.units, a.least, a.whole);
     cut.each = __builtin_amdgcn_readfirstlane(cut.each);
@@ -194,6 +200,7 @@ struct KvLine {
     g.to = min(g.steps, end - g.start);
     g.rb = __builtin_amdgcn_readfirstlane(kv_div(pair, a.H_kv));
     g.hk = pair - g.rb * a.H_kv;
+    if (a.by_pair) g.rb = kv_div(pairs, a.H_kv) - 1 - g.rb;
     return g;
   }
 };

@@ -142,57 +142,100 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
   a.max_pages = d.max_pages;
   a.causal = d.causal ? 1 : 0;
   a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)d.D));
-  a.rows_above = 0;
-  a.rows_most = INT32_MAX;
-  const long long pairs = (long long)d.S_q * G;
-  const int nr = pairs <= 16 ? 1 : pairs <= 32 || dp == 256 ? 2 : 4, rows = 16 * nr;
-  // few pairs of short sequences: one workgroup of 16 wavefronts each, no second kernel
-  const long long positions = (long long)d.max_pages * d.page_size;
-  const bool wide = nr == 1 && dp <= 128 && positions <= 4096 && kv_max_blocks(d.B, d.T, d.S_q, G, rows) * d.H_kv <= cus;
-  const KvShape shape = wide ? KvShape{32, 16, 1} : kv_kernel_shape(d.format, dp, nr);
-  a.units = cus * shape.per_cu;
-  a.least = 2;
-  const long long steps = std::max(1LL, ((long long)d.max_pages * d.page_size + shape.step() - 1) / shape.step());
-  const long long each = ((pairs + rows - 1) / rows) * d.B * d.H_kv;  // blocks, whatever row_start holds
-  if (each * (steps + a.least) > INT32_MAX)
-    return fail(MTK_ERR_UNSUPPORTED, "a batch of %lld row blocks over %lld positions is not supported", each, (long long)d.max_pages * d.page_size);
-  a.whole = positions <= (wide ? 4096 : 1024) && each < (1 << 23) ? 1 : 0;
   a.part_ld = a.blocks * 32;
-  const bool split = !a.whole;
-  a.most_blocks = (int)((pairs + rows - 1) / rows);
-  const int grid = a.whole ? (int)each : a.units;
+  const long long positions = (long long)d.max_pages * d.page_size;
+  const long long pairs = (long long)d.S_q * G;  // (row, query head) pairs of a sequence and K/V head, at most
+  // Sequences of up to 64 pairs: kernels whose wavefronts split the keys. Others: kernels whose wavefronts split the
+  // rows, and the former for the sequences that have one new row (or few) all the same.
+  const int most = dp == 256 ? 32 : 64;
+  const int few = pairs <= most ? (int)pairs : G <= most ? G : 0;
+  std::vector<Launch> launches;
+  size_t workspace = 0;
+  std::string how;
+  char name[96];
+  // The launches of one kernel; rows per block and keys per step as it has them.
+  auto add = [&](mtk_kv_attn_kargs k, const std::string &kernel, const std::string &joiner, int rows, int block, long long grid, bool split,
+                 long long places) {
+    Launch g;
+    g.name = kernel;
+    g.grid = (unsigned)grid;
+    g.block = (unsigned)block;
+    k.places = (int)places;
+    // run-time pointers: offsets in the workspace until then
+    const size_t part = workspace, ml = part + (size_t)places * (k.by_pair ? 1 : 2) * rows * k.part_ld * sizeof(float);
+    if (split) {
+      workspace = ml + (size_t)places * (k.by_pair ? 1 : 2) * rows * 2 * sizeof(float);
+      k.part = (float *)part;
+      k.part_ml = (float *)ml;
+    }
+    set_args(g, k);
+    launches.push_back(g);
+    char text[96];
+    snprintf(text, sizeof text, " rows/wg=%d grid=%lld%s", rows, grid, split ? " keys split" : "");
+    how += text;
+    if (split) {
+      Launch c = g;
+      c.name = joiner;
+      c.block = 256;
+      c.grid = (unsigned)std::min<long long>(k.by_pair ? (long long)d.T : (long long)d.T * d.H, 8LL * cus);
+      launches.push_back(c);
+    }
+  };
+  auto too_large = [&](long long blocks, long long steps) {
+    return blocks >= (1 << 23) || blocks * steps > INT32_MAX
+               ? fail(MTK_ERR_UNSUPPORTED, "a batch of %lld row blocks over %lld positions is not supported", blocks, positions)
+               : MTK_OK;
+  };
+  if (few) {
+    const int nr = few <= 16 ? 1 : few <= 32 || dp == 256 ? 2 : 4, rows = 16 * nr;
+    // few pairs of short sequences: one workgroup of 16 wavefronts each, no second kernel
+    const bool wide = nr == 1 && dp <= 128 && positions <= 4096 && (long long)d.B * d.H_kv <= cus;
+    const KvShape shape = wide ? KvShape{32, 16, 1} : kv_kernel_shape(d.format, dp, nr);
+    mtk_kv_attn_kargs k = a;
+    k.rows_above = 0;
+    k.rows_most = rows;
+    k.units = cus * shape.per_cu;
+    k.least = 2;
+    k.most_blocks = 1;
+    const long long blocks = (long long)d.B * d.H_kv, steps = (positions + shape.step() - 1) / shape.step();
+    if ((s = too_large(blocks, steps + k.least)) != MTK_OK) return s;
+    k.whole = positions <= (wide ? 4096 : 1024) ? 1 : 0;
+    snprintf(name, sizeof name, "mtk_kv_attend_%s_d%d_r%d_%s%s", kv_format(d), dp, nr, wide ? "w16_" : "", kv_suffix(d).c_str());
+    const std::string kernel = name;
+    snprintf(name, sizeof name, "mtk_kv_combine_r%d_k%d_%s", nr, shape.step(), kv_suffix(d).c_str());
+    add(k, kernel, name, rows, 64 * shape.waves, k.whole ? blocks : k.units, !k.whole, k.units);
+  }
+  if (pairs > most) {
+    const int rows = 128, step = 64;
+    mtk_kv_attn_kargs k = a;
+    k.rows_above = few ? 16 * (few <= 16 ? 1 : few <= 32 || dp == 256 ? 2 : 4) : 0;
+    k.rows_most = INT32_MAX;
+    k.by_pair = 1;
+    k.units = cus * (dp == 256 ? 1 : 2);
+    const long long each = (long long)d.B * ((pairs + rows - 1) / rows) * d.H_kv;  // blocks, whatever row_start holds
+    const long long blocks = kv_max_blocks(d.B, d.T, d.S_q, G, rows) * d.H_kv, steps = (positions + step - 1) / step;
+    // fewer blocks than workgroups: the keys are split, into 8 steps (512 keys) or more; else never
+    const bool split = blocks < k.units && steps > 8;
+    k.least = split ? 8 : (int)steps;
+    if ((s = too_large(each, 2 * steps + k.least)) != MTK_OK) return s;
+    const long long grid = split ? k.units + blocks : blocks;
+    snprintf(name, sizeof name, "mtk_kv_prefill_%s_d%d_%s", kv_format(d), dp, kv_suffix(d).c_str());
+    add(k, name, "mtk_kv_combine_rows_" + kv_suffix(d), rows, 256, grid, split, split ? grid : 0);
+  }
   mtk_plan *p = new mtk_plan();
   p->ctx = ctx;
   p->kind = PLAN_KV_ATTN;
   p->kv = d;
-  char name[96];
-  Launch g;
-  snprintf(name, sizeof name, "mtk_kv_attend_%s_d%d_r%d_%s%s", kv_format(d), dp, nr, wide ? "w16_" : "", kv_suffix(d).c_str());
-  g.name = name;
-  g.grid = (unsigned)grid;
-  g.block = 64u * (unsigned)shape.waves;
-  set_args(g, a);
-  p->launches.push_back(g);
-  if (split) {
-    Launch c = g;
-    snprintf(name, sizeof name, "mtk_kv_combine_r%d_k%d_%s", nr, shape.step(), kv_suffix(d).c_str());
-    c.name = name;
-    c.block = 256;
-    c.grid = (unsigned)std::min<long long>((long long)d.T * d.H, 8LL * cus);
-    p->launches.push_back(c);
-    p->part_ml_at = (size_t)a.units * 2 * rows * a.part_ld * sizeof(float);
-    p->workspace = p->part_ml_at + (size_t)a.units * 2 * rows * 2 * sizeof(float);
-  }
-  const double cap = (double)d.max_pages * d.page_size;
+  p->launches = launches;
+  p->workspace = workspace;
+  const double cap = (double)positions;
   p->flops = 4.0 * d.T * d.H * d.D * cap;
   p->bytes = d.B * cap * d.H_kv * 2.0 * (kv_row_bytes(d.format, a.blocks) + a.blocks) + 4.0 * d.T * d.H * d.D +
              4.0 * (2.0 * d.B + 1 + (double)d.B * d.max_pages);
   char desc[320];
-  snprintf(desc, sizeof desc,
-           "kv attention %s %s B=%d T=%d S_q=%d H=%d H_kv=%d D=%d pages=%dx%d max_pages=%d causal=%d rows/wg=%d grid=%d%s",
-           kv_format(d), kv_suffix(d).c_str(), d.B, d.T, d.S_q, d.H, d.H_kv, d.D, d.n_pages, d.page_size, d.max_pages, a.causal, rows,
-           grid, a.whole ? "" : ", equal shares of all keys");
-  p->description = desc;
+  snprintf(desc, sizeof desc, "kv attention %s %s B=%d T=%d S_q=%d H=%d H_kv=%d D=%d pages=%dx%d max_pages=%d causal=%d", kv_format(d),
+           kv_suffix(d).c_str(), d.B, d.T, d.S_q, d.H, d.H_kv, d.D, d.n_pages, d.page_size, d.max_pages, a.causal);
+  p->description = desc + how;
   return finish_kv(p, out);
 }
 
@@ -255,8 +298,8 @@ void patch_kv(const mtk_plan *p, const Launch &, char *block, const void *argset
     a.table = t->table;
     a.O = t->O;
     a.lse = t->lse;
-    a.part = p->workspace ? (float *)t->workspace : nullptr;
-    a.part_ml = p->workspace ? (float *)((char *)t->workspace + p->part_ml_at) : nullptr;
+    a.part = (float *)((uintptr_t)a.part + (uintptr_t)t->workspace);
+    a.part_ml = (float *)((uintptr_t)a.part_ml + (uintptr_t)t->workspace);
     return;
   }
   mtk_kv_move_kargs &a = *(mtk_kv_move_kargs *)block;
