@@ -176,6 +176,7 @@ typedef struct {
   /* the sequences of this launch: those with more than rows_above and at most rows_most (row, query head)
    * pairs per K/V head */
   int32_t rows_above, rows_most;
+  int32_t rows_shift, step_shift; /* log2 of the kernel's rows per block and keys per step */
   /* who does what (kv_cache.h): workgroups wanted (at most), least steps of one, or one for each pair */
   int32_t units, least, whole;
   int32_t most_blocks; /* whole: row blocks of a sequence, at most */

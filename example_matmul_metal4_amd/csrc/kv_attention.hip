@@ -512,128 +512,83 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
   }
 }
 
-// The partial sums of each (row, query head) of a pair that workgroups share, in an order that their number fixes: a group
-// of D / 4 lanes (4 dims each) adds every NGth part, a workgroup's NG groups are added in turn.
-constexpr int kKvCombine = 256;  // threads
-template <int DT, int ROWS, int STEP>
-__device__ __forceinline__ void kv_combine(const mtk_kv_attn_kargs &a) {
-  __shared__ f32x4 sm_x[kKvCombine];
-  __shared__ f32x2 sm_ml[kKvCombine];
-  const int tid = threadIdx.x, lane = tid & 63, G = a.G;
-  const int chunks = a.part_ld / 4, groups = kKvCombine / chunks;
+// The partial sums of each (row, query head) of a pair that workgroups share, in an order that their number fixes.
+// A group of D / 4 lanes (4 dims each) adds parts, kAhead of them in flight at once.
+//   PARTS: a workgroup has one (row, query head); group g of NG adds every NGth part, the groups are added in turn. For
+//   few pairs of long sequences, which have many parts.
+//   else: each group has a query head of its own, a workgroup NG heads of a row.
+constexpr int kKvJoin = 256;  // threads
+template <int DT, bool PARTS>
+__device__ __forceinline__ void kv_join(const mtk_kv_attn_kargs &a) {
+  __shared__ f32x4 sm_x[PARTS ? kKvJoin : 1];
+  __shared__ f32x2 sm_ml[PARTS ? kKvJoin : 1];
+  __shared__ int sm_line[kKvJoin / 64][kLineWords];
+  const int tid = threadIdx.x, lane = tid & 63, G = a.G, rows = 1 << a.rows_shift;
+  const int chunks = a.part_ld / 4, groups = kKvJoin / chunks;
   const int g = tid / chunks, d = 4 * (tid - g * chunks);
-  const int items = a.T * a.H, per = (items + gridDim.x - 1) / gridDim.x;
+  const int heads = PARTS ? 1 : groups, per_row = (a.H + heads - 1) / heads;  // items of a row
+  const int items = a.T * per_row, per = (items + gridDim.x - 1) / gridDim.x;
   const int end = min(items, ((int)blockIdx.x + 1) * per);
   int it = blockIdx.x * per;
   if (it >= end) return;
-  __shared__ int sm_line[kKvCombine / 64][kLineWords];
-  KvLine<ROWS, STEP> line(a, lane, sm_line[tid >> 6]);
+  KvLine<0, 0> line(a, lane, sm_line[tid >> 6]);
   line.lay();
-  int b = -1, base = 0, length = 1, blocks = 0;
-  KvSegment seq{};
-  for (; it < end; ++it) {  // uniform: every wavefront takes the same items
-    const int t = it / a.H, h = it - t * a.H;
-    if (b < 0 || t >= seq.seq.first + seq.seq.rows) {
-      const int at = line.find_row(t);
-      b = at;
-      if (at < 0) {
-        it = (t + 1) * a.H - 1;
-        continue;
-      }
-      int pairs;
-      seq = line.sequence(at, length, base, pairs);
-      if (pairs == 0) length = 0;
-      blocks = kv_div(pairs, a.H_kv);
-    }
-    if (length == 0 || t - seq.seq.first >= a.S_q || (line.cut.padded && length == line.cut.each)) {
-      it = min((int64_t)end, (int64_t)(seq.seq.first + seq.seq.rows) * a.H) - 1;  // none of the sequence's, or none left
-      continue;
-    }
-    const int hk = h / G, r = (t - seq.seq.first) * G + h - hk * G;
-    const int start = base + ((a.by_pair ? blocks - 1 - r / ROWS : r / ROWS) * a.H_kv + hk) * length;
-    const int w0 = kv_div(start, line.cut.each), w1 = min(kv_div(start + seq.steps - 1, line.cut.each), a.places - 1);
-    if (w0 >= w1) continue;  // one workgroup's
-    const int first = start == w0 * line.cut.each ? 0 : 1;
-    KvPart sum;
-    constexpr int kAhead = 8;  // parts in flight
-    for (int s0 = w0 + g; s0 <= w1; s0 += kAhead * groups) {
-      KvPart p[kAhead];
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int w = s0 + i * groups;
-        if (w <= w1) {
-          const size_t at = (a.by_pair ? (size_t)w : (size_t)w * 2 + (w == w0 ? first : 0)) * ROWS + r % ROWS;
-          const f32x2 ml = *(const f32x2 *)(a.part_ml + 2 * at);
-          p[i] = KvPart{ml.x, ml.y, *(const f32x4 *)(a.part + at * a.part_ld + d)};
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) add_part(sum, p[i]);
-    }
-    __syncthreads();
-    sm_x[tid] = sum.x;
-    sm_ml[tid] = f32x2{sum.m, sum.l};
-    __syncthreads();
-    if (tid < chunks) {
-      for (int i = 1; i < min(groups, w1 - w0 + 1); ++i) {
-        const int k = tid + i * chunks;
-        add_part(sum, KvPart{sm_ml[k].x, sm_ml[k].y, sm_x[k]});
-      }
-      store_out<DT>(a, t, h, d, sum);
-    }
-  }
-}
-
-// The same where rows are many and parts few (kv_prefill.hip's): each group of lanes has a query head of its own.
-template <int DT, int ROWS, int STEP>
-__device__ __forceinline__ void kv_combine_rows(const mtk_kv_attn_kargs &a) {
-  __shared__ int sm_line[kKvCombine / 64][kLineWords];
-  const int tid = threadIdx.x, lane = tid & 63, G = a.G;
-  const int chunks = a.part_ld / 4, groups = kKvCombine / chunks;
-  const int g = tid / chunks, d = 4 * (tid - g * chunks);
-  const int per = (a.T + gridDim.x - 1) / gridDim.x, end = min(a.T, ((int)blockIdx.x + 1) * per);
-  int t = blockIdx.x * per;
-  if (t >= end) return;
-  KvLine<ROWS, STEP> line(a, lane, sm_line[tid >> 6]);
-  line.lay();
-  while (t < end) {  // uniform
-    const int at = line.find_row(t);
-    if (at < 0) {
-      ++t;
+  while (it < end) {  // uniform: every wavefront takes the same items
+    int t = it / per_row;
+    const int l = line.find_row(t);
+    if (l < 0) {
+      it = (t + 1) * per_row;
       continue;
     }
     int length, base, pairs;
-    const KvSegment seq = line.sequence(at, length, base, pairs);
-    const int past = min(end, seq.seq.first + seq.seq.rows);
-    const bool cut = pairs > 0 && length > line.cut.each;
+    const KvSegment seq = line.sequence(l, length, base, pairs);
+    const int64_t past = (int64_t)(seq.seq.first + min(seq.seq.rows, a.S_q)) * per_row;
     const int blocks = kv_div(pairs, a.H_kv);
-    if (cut) {
-      for (; t < past; ++t) {
-        const int i = t - seq.seq.first;
-        if (i >= a.S_q) break;
-        for (int h = g; h < a.H && g < groups; h += groups) {
-          const int hk = kv_div(h, G), r = i * G + h - hk * G;
-          const int start = base + ((a.by_pair ? blocks - 1 - r / ROWS : r / ROWS) * a.H_kv + hk) * length;
-          const int w0 = kv_div(start, line.cut.each), w1 = min(kv_div(start + seq.steps - 1, line.cut.each), a.places - 1);
-          KvPart sum;
-          constexpr int kAhead = 4;
-          for (int s0 = w0; s0 <= w1; s0 += kAhead) {
-            KvPart p[kAhead];
+    const bool none = pairs == 0 || (line.cut.padded && length == line.cut.each);  // no pair is shared
+    for (; !none && it < min((int64_t)end, past); ++it) {
+      t = it / per_row;
+      const int h = (it - t * per_row) * heads + (PARTS ? 0 : g);
+      if (h >= a.H || g >= groups) continue;
+      const int hk = kv_div(h, G), r = (t - seq.seq.first) * G + h - hk * G, rb = r >> a.rows_shift;
+      const int start = base + ((a.by_pair ? blocks - 1 - rb : rb) * a.H_kv + hk) * length;
+      const int w0 = kv_div(start, line.cut.each), w1 = min(kv_div(start + seq.steps - 1, line.cut.each), a.places - 1);
+      if (w0 >= w1) continue;  // one workgroup's
+      const int first = start == w0 * line.cut.each ? 0 : 1;
+      KvPart sum;
+      constexpr int kAhead = 8;
+      const int step = PARTS ? groups : 1;
+      for (int s0 = w0 + (PARTS ? g : 0); s0 <= w1; s0 += kAhead * step) {
+        KvPart p[kAhead];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k)
-              if (s0 + k <= w1) {
-                const size_t place = (size_t)(s0 + k) * ROWS + r % ROWS;
-                const f32x2 ml = *(const f32x2 *)(a.part_ml + 2 * place);
-                p[k] = KvPart{ml.x, ml.y, *(const f32x4 *)(a.part + place * a.part_ld + d)};
-              }
+        for (int i = 0; i < kAhead; ++i) {
+          const int w = s0 + i * step;
+          if (w <= w1) {
+            const size_t place = a.by_pair ? (size_t)w : (size_t)w * 2 + (w == w0 ? first : 0);
+            const size_t at = (place << a.rows_shift) + (r & (rows - 1));
+            const f32x2 ml = *(const f32x2 *)(a.part_ml + 2 * at);
+            p[i] = KvPart{ml.x, ml.y, *(const f32x4 *)(a.part + at * a.part_ld + d)};
+          }
+        }
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) add_part(sum, p[k]);
+        for (int i = 0; i < kAhead; ++i) add_part(sum, p[i]);
+      }
+      if constexpr (PARTS) {
+        __syncthreads();
+        sm_x[tid] = sum.x;
+        sm_ml[tid] = f32x2{sum.m, sum.l};
+        __syncthreads();
+        if (tid < chunks) {
+          for (int i = 1; i < min(groups, w1 - w0 + 1); ++i) {
+            const int k = tid + i * chunks;
+            add_part(sum, KvPart{sm_ml[k].x, sm_ml[k].y, sm_x[k]});
           }
           store_out<DT>(a, t, h, d, sum);
         }
+      } else {
+        store_out<DT>(a, t, h, d, sum);
       }
     }
-    t = past;
+    if (none || it >= past) it = max((int64_t)it, (int64_t)(seq.seq.first + seq.seq.rows) * per_row);
   }
 }
 
@@ -675,24 +630,9 @@ MTK_KV_ATTEND_W16(fp4, KV_FP4, 128, 2)
 MTK_KV_ATTEND_W16(fp8, KV_FP8, 64, 2)
 MTK_KV_ATTEND_W16(fp8, KV_FP8, 128, 2)
 
-#define MTK_KV_COMBINE(NR, STEP)                                                                                                 \
-  extern "C" __global__ void __launch_bounds__(kKvCombine) mtk_kv_combine_r##NR##_k##STEP##_f16(const mtk_kv_attn_kargs a) {  \
-    kv_combine<DT_F16, 16 * NR, STEP>(a);                                                                                        \
-  }                                                                                                                              \
-  extern "C" __global__ void __launch_bounds__(kKvCombine) mtk_kv_combine_r##NR##_k##STEP##_bf16(const mtk_kv_attn_kargs a) { \
-    kv_combine<DT_BF16, 16 * NR, STEP>(a);                                                                                       \
-  }
-MTK_KV_COMBINE(1, 512)
-MTK_KV_COMBINE(1, 256)
-MTK_KV_COMBINE(1, 128)
-MTK_KV_COMBINE(2, 512)
-MTK_KV_COMBINE(2, 256)
-MTK_KV_COMBINE(2, 128)
-MTK_KV_COMBINE(4, 128)
-
-extern "C" __global__ void __launch_bounds__(kKvCombine) mtk_kv_combine_rows_f16(const mtk_kv_attn_kargs a) {
-  kv_combine_rows<DT_F16, 128, 64>(a);
-}
-extern "C" __global__ void __launch_bounds__(kKvCombine) mtk_kv_combine_rows_bf16(const mtk_kv_attn_kargs a) {
-  kv_combine_rows<DT_BF16, 128, 64>(a);
-}
+#define MTK_KV_JOIN(NAME, DT, PARTS) \
+  extern "C" __global__ void __launch_bounds__(kKvJoin) NAME(const mtk_kv_attn_kargs a) { kv_join<DT, PARTS>(a); }
+MTK_KV_JOIN(mtk_kv_join_rows_f16, DT_F16, false)
+MTK_KV_JOIN(mtk_kv_join_rows_bf16, DT_BF16, false)
+MTK_KV_JOIN(mtk_kv_join_parts_f16, DT_F16, true)
+MTK_KV_JOIN(mtk_kv_join_parts_bf16, DT_BF16, true)

@@ -70,8 +70,8 @@ MTK_KV_FN int kv_div(int x, int d) {
 #endif
 }
 
-// Who does what in attention. A sequence has `blocks` blocks of `rows` (row, query head) pairs for each K/V head, and
-// `steps` steps of keys (at least one). The (block, head) pairs of all sequences, sequence after sequence, lie on a
+// Who does what in attention. A sequence has `blocks` blocks of 2^rows_shift (row, query head) pairs for each K/V head,
+// and `steps` steps of 2^step_shift keys (at least one). The (block, head) pairs of all sequences, sequence after sequence, lie on a
 // line; workgroup w has the steps from w * each to (w + 1) * each of it, so that all of them have the same work, whatever
 // the lengths. A pair that a boundary cuts leaves partial sums.
 //   each = max(least, work / units), so that there are at most `units` workgroups.
@@ -81,12 +81,12 @@ typedef struct {
   int blocks, steps;
 } kv_share;
 
-MTK_KV_FN kv_share kv_blocks(kv_seq s, int S_q, int G, int rows, int step, int rows_above, int rows_most) {
+MTK_KV_FN kv_share kv_blocks(kv_seq s, int S_q, int G, int rows_shift, int step_shift, int rows_above, int rows_most) {
   kv_share r;
   const uint32_t pairs = (uint32_t)(s.rows < S_q ? s.rows : S_q) * (uint32_t)G;  // S_q * G < 2^31
   const int mine = pairs > (uint32_t)rows_above && pairs <= (uint32_t)rows_most;
-  r.blocks = mine ? (int)((pairs + (uint32_t)rows - 1) / (uint32_t)rows) : 0;
-  r.steps = (int)(((uint32_t)s.keys + (uint32_t)step - 1) / (uint32_t)step);
+  r.blocks = mine ? (int)((pairs + (1u << rows_shift) - 1) >> rows_shift) : 0;
+  r.steps = (int)(((uint32_t)s.keys + (1u << step_shift) - 1) >> step_shift);
   if (r.steps < 1) r.steps = 1;
   return r;
 }

@@ -102,7 +102,7 @@ struct KvSegment {
 };
 
 // A wavefront's view of the line: 64 sequences at a time, in LDS words of its own (registers are what the kernel is
-// short of). ROWS rows per block, STEP keys per step.
+// short of). ROWS rows per block, STEP keys per step (0: as the launch says).
 constexpr int kLineWords = 4 * 64;
 template <int ROWS, int STEP>
 struct KvLine {
@@ -114,7 +114,8 @@ struct KvLine {
   int b0 = 0, before = 0; // the first of the 64, and where its pairs start
 
   __device__ __forceinline__ kv_share share_of(const kv_seq &x) const {
-    return kv_blocks(x, a.S_q, a.G, ROWS, STEP, a.rows_above, a.rows_most);
+    return kv_blocks(x, a.S_q, a.G, ROWS ? __builtin_ctz(ROWS ? ROWS : 1) : a.rows_shift, STEP ? __builtin_ctz(STEP ? STEP : 1) : a.step_shift,
+                     a.rows_above, a.rows_most);
   }
   __device__ __forceinline__ int len_of(int b) const { return b < a.B ? a.kv_len[b] : 0; }
   __device__ __forceinline__ void place(const kv_seq &s, int len, const kv_share &h) {

@@ -154,17 +154,18 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
   std::string how;
   char name[96];
   // The launches of one kernel; rows per block and keys per step as it has them.
-  auto add = [&](mtk_kv_attn_kargs k, const std::string &kernel, const std::string &joiner, int rows, int block, long long grid, bool split,
-                 long long places) {
+  auto add = [&](mtk_kv_attn_kargs k, const std::string &kernel, int rows, int step, int block, long long grid, bool split) {
     Launch g;
     g.name = kernel;
     g.grid = (unsigned)grid;
     g.block = (unsigned)block;
-    k.places = (int)places;
-    // run-time pointers: offsets in the workspace until then
-    const size_t part = workspace, ml = part + (size_t)places * (k.by_pair ? 1 : 2) * rows * k.part_ld * sizeof(float);
-    if (split) {
-      workspace = ml + (size_t)places * (k.by_pair ? 1 : 2) * rows * 2 * sizeof(float);
+    k.rows_shift = __builtin_ctz((unsigned)rows);
+    k.step_shift = __builtin_ctz((unsigned)step);
+    k.places = split ? (int)grid : 0;
+    if (split) {  // run-time pointers: offsets in the workspace until then
+      const size_t held = (size_t)grid * (k.by_pair ? 1 : 2) * rows;
+      const size_t part = workspace, ml = part + held * k.part_ld * sizeof(float);
+      workspace = ml + held * 2 * sizeof(float);
       k.part = (float *)part;
       k.part_ml = (float *)ml;
     }
@@ -174,10 +175,15 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
     snprintf(text, sizeof text, " rows/wg=%d grid=%lld%s", rows, grid, split ? " keys split" : "");
     how += text;
     if (split) {
+      // fewer than 8 parts for each pair on average: a group of lanes for each; the rows that this kernel can have
+      const long long pairs_most = (long long)d.B * d.H_kv;
+      const bool parts = !k.by_pair && pairs_most * 8 < grid;
+      const int heads = parts ? 1 : 1024 / k.part_ld;
+      const long long mine = k.by_pair ? d.T : std::min<long long>(d.T, (long long)d.B * std::max(1, k.rows_most / G));
       Launch c = g;
-      c.name = joiner;
+      c.name = std::string(parts ? "mtk_kv_join_parts_" : "mtk_kv_join_rows_") + kv_suffix(d);
       c.block = 256;
-      c.grid = (unsigned)std::min<long long>(k.by_pair ? (long long)d.T : (long long)d.T * d.H, 8LL * cus);
+      c.grid = (unsigned)std::min<long long>(mine * ((d.H + heads - 1) / heads), 8LL * cus);
       launches.push_back(c);
     }
   };
@@ -201,9 +207,7 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
     if ((s = too_large(blocks, steps + k.least)) != MTK_OK) return s;
     k.whole = positions <= (wide ? 4096 : 1024) ? 1 : 0;
     snprintf(name, sizeof name, "mtk_kv_attend_%s_d%d_r%d_%s%s", kv_format(d), dp, nr, wide ? "w16_" : "", kv_suffix(d).c_str());
-    const std::string kernel = name;
-    snprintf(name, sizeof name, "mtk_kv_combine_r%d_k%d_%s", nr, shape.step(), kv_suffix(d).c_str());
-    add(k, kernel, name, rows, 64 * shape.waves, k.whole ? blocks : k.units, !k.whole, k.units);
+    add(k, name, rows, shape.step(), 64 * shape.waves, k.whole ? blocks : k.units, !k.whole);
   }
   if (pairs > most) {
     const int rows = 128, step = 64;
@@ -220,7 +224,7 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
     if ((s = too_large(each, 2 * steps + k.least)) != MTK_OK) return s;
     const long long grid = split ? k.units + blocks : blocks;
     snprintf(name, sizeof name, "mtk_kv_prefill_%s_d%d_%s", kv_format(d), dp, kv_suffix(d).c_str());
-    add(k, name, "mtk_kv_combine_rows_" + kv_suffix(d), rows, 256, grid, split, split ? grid : 0);
+    add(k, name, rows, step, 256, grid, split);
   }
   mtk_plan *p = new mtk_plan();
   p->ctx = ctx;
