@@ -119,12 +119,13 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
   const uint32_t k_scales = (2 * row_b) << a.page_shift, v_codes = row_b << a.page_shift;
   const uint32_t v_scales = k_scales + ((uint32_t)a.blocks << a.page_shift);
   constexpr uint32_t kHalf = FMT == KV_FP4 ? 8 : 16;  // bytes of half a block
-  uint32_t code_at[kSc], scale_at[kSc];
+  uint32_t code_at[kSc], scale_at[kSc], scale_bit[kSc];  // scales are loaded as whole words
 #pragma unroll
   for (int s = 0; s < kSc; ++s) {
     const int blk = min(DP == 64 ? j >> 1 : j + 4 * s, a.blocks - 1);
     code_at[s] = c * row_b + blk * 2 * kHalf + (DP == 64 ? (j & 1) * kHalf : 0u);
-    scale_at[s] = (uint32_t)(c * a.blocks + blk);
+    scale_at[s] = (uint32_t)(c * a.blocks + blk) & ~3u;
+    scale_bit[s] = 8 * ((uint32_t)(c * a.blocks + blk) & 3u);
   }
   struct Tile {
     uint32_t k[kKb][kRaw], v[kKb][kRaw], ks[kKb][kSc], vs[kKb][kSc];
@@ -188,8 +189,8 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
 #pragma unroll
       for (int s = 0; s < kSc; ++s) {
         const uint32_t at = p.at[kb] * (uint32_t)a.blocks;
-        t.ks[kb][s] = __builtin_amdgcn_raw_buffer_load_b8(p.r[kb], scale_at[s], k_scales + at, 0);
-        t.vs[kb][s] = __builtin_amdgcn_raw_buffer_load_b8(p.r[kb], scale_at[s], v_scales + at, 0);
+        t.ks[kb][s] = __builtin_amdgcn_raw_buffer_load_b32(p.r[kb], scale_at[s], k_scales + at, 0);
+        t.vs[kb][s] = __builtin_amdgcn_raw_buffer_load_b32(p.r[kb], scale_at[s], v_scales + at, 0);
       }
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -287,16 +288,19 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
     asm volatile("" : "+v"(v_put), "+v"(v_get));  // the flips are done in the loop: their results would fill registers
     // ---- NaN blocks and pages that are none: bit k of kn (vn[s][q]) is key k of the tile
     uint64_t kn = 0, vn[kSc][4] = {};
-    uint32_t vs[kKb][kSc];  // the next tile's are loaded before this one's have been used
+    uint32_t ks[kKb][kSc], vs[kKb][kSc];  // the next tile's are loaded before this one's have been used
 #pragma unroll
     for (int kb = 0; kb < kKb; ++kb)
 #pragma unroll
-      for (int s = 0; s < kSc; ++s) vs[kb][s] = t.vs[kb][s];
+      for (int s = 0; s < kSc; ++s) {
+        ks[kb][s] = __builtin_amdgcn_ubfe(t.ks[kb][s], scale_bit[s], 8);
+        vs[kb][s] = __builtin_amdgcn_ubfe(t.vs[kb][s], scale_bit[s], 8);
+      }
     uint32_t top = t.bad ? kNanScale : 0;
 #pragma unroll
     for (int kb = 0; kb < kKb; ++kb)
 #pragma unroll
-      for (int s = 0; s < kSc; ++s) top = max(top, max(t.ks[kb][s], vs[kb][s]));
+      for (int s = 0; s < kSc; ++s) top = max(top, max(ks[kb][s], vs[kb][s]));
     const bool rare = __any(top == kNanScale);
     if (rare) {
 #pragma unroll
@@ -304,11 +308,11 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
         const bool none = (t.bad >> kb) & 1;
 #pragma unroll
         for (int s = 0; s < kSc; ++s) {
-          const uint64_t x = none ? ~0ull : __ballot(t.ks[kb][s] == kNanScale), y = none ? ~0ull : __ballot(vs[kb][s] == kNanScale);
+          const uint64_t x = none ? ~0ull : __ballot(ks[kb][s] == kNanScale), y = none ? ~0ull : __ballot(vs[kb][s] == kNanScale);
           kn |= ((x | x >> 16 | x >> 32 | x >> 48) & 0xffff) << (16 * kb);
 #pragma unroll
           for (int q = 0; q < 4; ++q) vn[s][q] |= ((y >> (16 * q)) & 0xffff) << (16 * kb);
-          if (none || t.ks[kb][s] == kNanScale) t.ks[kb][s] = 127;
+          if (none || ks[kb][s] == kNanScale) ks[kb][s] = 127;
           if (none || vs[kb][s] == kNanScale) {
             vs[kb][s] = 127;
 #pragma unroll
@@ -336,7 +340,7 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
       for (int n = 0; n < NR; ++n) s[n][kb] = f32x4{};
 #pragma unroll
       for (int f = 0; f < kFr; ++f) {
-        const u32x4 kf = values8<DT, FMT>(t.k[kb] + f * kW8, scale_of(t.ks[kb][kSc == 2 ? f >> 2 : 0]));
+        const u32x4 kf = values8<DT, FMT>(t.k[kb] + f * kW8, scale_of(ks[kb][kSc == 2 ? f >> 2 : 0]));
 #pragma unroll
         for (int n = 0; n < NR; ++n) s[n][kb] = mfma16x16x32<DT>(kf, qf[n][f], s[n][kb]);
       }
