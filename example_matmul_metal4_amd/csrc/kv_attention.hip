@@ -85,6 +85,7 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
   const int c = lane & 15, j = lane >> 4;
   const int G = a.G;
 
+  __shared__ int sm_window[W == 16 ? 1 : W][128];
   __shared__ int sm_line[W == 16 ? 1 : W][kLineWords];  // 16 wavefronts: pairs are whole
   KvLine<kRows, kKvStep> line(a, lane, sm_line[W == 16 ? 0 : wave]);
   int wg = 0, line_from = 0, line_to = 0;
@@ -141,7 +142,7 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
     int last_block, e0, window, next_window;
     int key0, key_end, n_keys;  // this wavefront's first key, the segment's end, the keys that its rows see
   };
-  auto source = [&](const KvSegment &g) {
+  auto source = [&](const KvSegment &g, bool windows) {
     Source x;
     const int rows = min(g.seq.rows, a.S_q) * G, r_last = min(g.rb * kRows + kRows, rows) - 1;
     const int64_t p_last = a.causal ? g.seq.pos0 + kv_div(r_last, G) : (int64_t)g.seq.keys - 1;
@@ -153,8 +154,10 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
     x.pages = g.seq.bad ? 0u : (uint32_t)a.n_pages;
     x.last_block = (max(x.n_keys, 1) - 1) & ~15;
     x.e0 = x.key0 >> a.page_shift;
-    x.window = x.table[min(x.e0 + lane, a.max_pages - 1)];
-    x.next_window = x.table[min(x.e0 + kWindow + lane, a.max_pages - 1)];
+    if (windows) {
+      x.window = x.table[min(x.e0 + lane, a.max_pages - 1)];
+      x.next_window = x.table[min(x.e0 + kWindow + lane, a.max_pages - 1)];
+    }
     return x;
   };
   // Where the blocks of a tile are. The range of the loads is the page's region.
@@ -256,7 +259,7 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
     }
   };
 
-  Source src = source(seg);
+  Source src = source(seg, true);
   load_q(seg);
   Tile t;
   if (src.key0 < src.key_end) load_tile(t, src, src.key0);
@@ -264,11 +267,10 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
   for (;;) {
     // the next segment's table entries, ahead of their use
     const bool more = !whole && !line.cut.padded && seg.start + seg.to < line_to;
-    int window = 0, next_window = 0;
     if (more) {
-      const Source x = source(line.at(seg.start + seg.to, line_to));
-      window = x.window;
-      next_window = x.next_window;
+      const Source x = source(line.at(seg.start + seg.to, line_to), true);
+      sm_window[wave][lane] = x.window;  // in LDS until then, for want of registers
+      sm_window[wave][64 + lane] = x.next_window;
     }
     float m_off[NR], l_run[NR];
     f32x4 o[NR][kDb];
@@ -461,14 +463,16 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
     KvSegment next = seg;
     if (more) {
       next = line.at(seg.start + seg.to, line_to);
-      src = source(next);
-      src.window = window;
-      src.next_window = next_window;
+      src = source(next, false);
+      src.window = sm_window[wave][lane];
+      src.next_window = sm_window[wave][64 + lane];
       load_q(next);
       if (src.key0 < src.key_end) load_tile(t, src, src.key0);
     }
 
     // ---- the wavefronts' sums, 16 rows at a time, in wavefront order
+    // lane numbers taken anew: what follows from them is not kept in registers over the loop
+    const int lane2 = lane_id(), tid2 = 64 * wave + lane2, c2 = lane2 & 15, j2 = lane2 >> 4;
     const bool alone = seg.from == 0 && seg.to == seg.steps;
     const int rows = min(seg.seq.rows, a.S_q) * G;
     const size_t place = (size_t)wg * 2 + (seg.start + seg.from == line_from ? 0 : 1);
@@ -476,15 +480,15 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
     for (int n = 0; n < NR; ++n) {
       const float l_tot = quarters_sum(l_run[n]);
       __syncthreads();  // the staging tiles, or the last rows, have been read
-      if (j == 0) {
-        sm_m[wave][c] = m_off[n];
-        sm_l[wave][c] = l_tot;
+      if (j2 == 0) {
+        sm_m[wave][c2] = m_off[n];
+        sm_l[wave][c2] = l_tot;
       }
       float *park = (float *)smem + wave * (kParkB / 4);
 #pragma unroll
-      for (int d = 0; d < kDb; ++d) *(f32x4 *)(park + c * kPitch + 16 * d + 4 * j) = o[n][d];
+      for (int d = 0; d < kDb; ++d) *(f32x4 *)(park + c2 * kPitch + 16 * d + 4 * j2) = o[n][d];
       __syncthreads();
-      for (int it = tid; it < 16 * (DP / 4); it += 64 * W) {
+      for (int it = tid2; it < 16 * (DP / 4); it += 64 * W) {
         const int rr = it / (DP / 4), d0 = 4 * (it % (DP / 4));
         const int r = seg.rb * kRows + 16 * n + rr;
         if (r >= rows) continue;
