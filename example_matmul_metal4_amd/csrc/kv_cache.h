@@ -27,10 +27,10 @@ MTK_KV_FN uint64_t kv_region_bytes(int fmt, int blocks, int page_shift) {
 }
 
 // One sequence of the batch, from its entries of row_start and kv_len, whatever they hold. Its rows are
-// [first, first + rows) of the packed tensors, row i at position pos0 + i. keys: cached positions, at most the
-// table's; bad: kv_len is more than the table holds.
+// [first, first + rows) of the packed tensors, row i at position pos0 + i. len: kv_len; keys: cached positions, at most
+// the table's; bad: kv_len is more than the table holds.
 typedef struct {
-  int first, rows;
+  int first, rows, len;
   int64_t pos0;
   int keys, bad;
 } kv_seq;
@@ -41,6 +41,7 @@ MTK_KV_FN kv_seq kv_sequence(int start, int next, int len, int T, int max_pages,
   s.first = start < 0 ? 0 : start > T ? T : start;
   const int last = next < s.first ? s.first : next > T ? T : next;
   s.rows = last - s.first;
+  s.len = len;
   s.pos0 = (int64_t)len - s.rows;
   s.bad = len > cap;
   s.keys = len < 0 ? 0 : len > cap ? cap : len;

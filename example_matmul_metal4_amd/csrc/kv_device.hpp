@@ -55,40 +55,11 @@ __device__ __forceinline__ int wave_scan(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
   return x;
 }
-__device__ __forceinline__ float wave_sum(float v) {
-  auto step = [](float x, auto ctrl, auto mask) {
-    return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value,
-                                                                     decltype(mask)::value, 0xf, false));
-  };
-  using std::integral_constant;
-  v = step(v, integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});
-  v = step(v, integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
-  v = step(v, integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
-  v = step(v, integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
-  v = step(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
-  v = step(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
-}
 
 template <typename A>
 __device__ __forceinline__ kv_seq load_seq(const A &a, int b) {
   if (b >= a.B) return kv_sequence(0, 0, 0, 0, a.max_pages, a.page_shift);
   return kv_sequence(a.row_start[b], a.row_start[b + 1], a.kv_len[b], a.T, a.max_pages, a.page_shift);
-}
-
-// The sequence that holds packed row t (every lane gets it), or -1.
-template <typename A>
-__device__ __forceinline__ int seq_of_row(const A &a, int t, int lane) {
-  int found = -1;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int b = b0 + lane;
-    const uint64_t in = __ballot(b < a.B && a.row_start[min(b, a.B)] <= t && t < a.row_start[min(b, a.B - 1) + 1]);
-    if (in) {
-      found = b0 + __builtin_ctzll(in);
-      break;
-    }
-  }
-  return __builtin_amdgcn_readfirstlane(found);
 }
 
 // Some steps of one pair (kv_cache.h).

@@ -74,13 +74,15 @@ int plan_kv_move(mtk_ctx *ctx, const mtk_kv_desc *d_in, PlanKind kind, mtk_plan 
   a.max_pages = d.max_pages;
   const long long items = 8LL * d.H_kv * a.blocks;  // of 16 bytes of K or V, per row
   if (items > (1 << 28)) return fail(MTK_ERR_UNSUPPORTED, "rows of this size are not supported");
-  // wavefronts per row: enough to fill the device with few rows, at least one item per lane
+  // Up to 4 rows per wavefront, whose places it looks up once and whose lines in the cache it fills itself; fewer where
+  // that would leave less than 8 wavefronts per CU. 64 items of each.
   const int cus = ctx ? ctx->prop.multiProcessorCount : 256;
-  a.parts = (int)std::max(1LL, std::min((items + 63) / 64, (16LL * cus + d.T - 1) / d.T));
-  // rows per wavefront: as many (up to 8) as leave 16 wavefronts per CU
-  a.rows_per_wave = a.parts > 1 ? 1 : (int)std::max(1LL, std::min(8LL, d.T / (16LL * cus)));
+  a.parts = (int)((items + 63) / 64);
+  a.rows_per_wave = 1;
+  while (a.rows_per_wave < 4 && (d.T + 2LL * a.rows_per_wave - 1) / (2 * a.rows_per_wave) * a.parts >= 8LL * cus) a.rows_per_wave *= 2;
+  const long long groups = (d.T + a.rows_per_wave - 1) / a.rows_per_wave;
   a.mul_blocks = a.blocks == 1 ? 0u : (uint32_t)((0x100000000ull + a.blocks - 1) / a.blocks);
-  const long long waves = (long long)a.parts * ((d.T + a.rows_per_wave - 1) / a.rows_per_wave);
+  const long long waves = a.parts * groups;
   if ((waves + 3) / 4 > INT32_MAX / 256) return fail(MTK_ERR_UNSUPPORTED, "T of %d is not supported", d.T);
   mtk_plan *p = new mtk_plan();
   p->ctx = ctx;

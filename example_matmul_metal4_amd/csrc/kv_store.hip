@@ -43,38 +43,40 @@ struct KvItem {
   }
 };
 
-// The rows of this wavefront: [t0, t0 + n), part `part` of each; lane i has the page of row t0 + i (-1: no page, -2:
-// a row of no sequence) and its place in it. Rows of one sequence, the common case, are looked up at once.
+// The rows of this wavefront: [t0, t0 + n), items [64 * part, 64 * part + 64) of each; lane i has the page of row t0 + i
+// (-1: no page, -2: a row of no sequence) and its place in it.
 struct KvRows {
-  int t0, n = 0, part, page, off;
+  int t0, n = 0, part, page = -2, off = 0;
   __device__ __forceinline__ KvRows(const mtk_kv_move_kargs &a, int lane) {
-    const int64_t w = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t group = a.parts == 1 ? w : w / a.parts;
+    const int64_t w = (int64_t)xcd_remap(blockIdx.x, gridDim.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t group = w / a.parts;
     part = (int)(w - group * a.parts);
     if (group * a.rows_per_wave >= a.T) return;
     t0 = (int)(group * a.rows_per_wave);
     n = min(a.rows_per_wave, a.T - t0);
-    page = -2;
-    off = 0;
-    for (int i = 0; i < n;) {
-      const int b = seq_of_row(a, t0 + i, lane);
-      if (b < 0) {
-        ++i;
-        continue;
-      }
+    bool open = lane < n;  // this lane's row has no sequence yet
+    for (int b0 = 0; b0 < a.B && __ballot(open); b0 += 64) {
+      const int b = min(b0 + lane, a.B - 1);
       const kv_seq s = load_seq(a, b);
-      const int end = min(n, s.first + s.rows - t0);
-      if (lane >= i && lane < end) {
-        const int64_t pos = s.pos0 + (t0 + lane - s.first);
-        off = (int)(pos & ((1 << a.page_shift) - 1));
-        page = kv_page(a.table + (size_t)b * a.max_pages, pos, a.n_pages, a.max_pages, a.page_shift);
+      const int end = s.first + s.rows;
+      uint64_t meets = __ballot(b0 + lane < a.B && s.first < t0 + n && end > t0);
+      for (; meets; meets &= meets - 1) {
+        const int i = __builtin_ctzll(meets);
+        const int first = __builtin_amdgcn_readlane(s.first, i), last = __builtin_amdgcn_readlane(end, i);
+        const int len = __builtin_amdgcn_readlane(s.len, i);
+        const int t = t0 + lane;
+        if (open && t >= first && t < last) {
+          const int64_t pos = (int64_t)len - (last - t);
+          off = (int)(pos & ((1 << a.page_shift) - 1));
+          page = kv_page(a.table + (size_t)(b0 + i) * a.max_pages, pos, a.n_pages, a.max_pages, a.page_shift);
+          open = false;
+        }
       }
-      i = max(end, i + 1);
     }
   }
 };
 
-constexpr int kMoveAhead = 4;  // items of a lane whose loads are in flight at once
+constexpr int kMoveAhead = 4;  // rows of a lane whose loads are in flight at once
 
 template <int DT, int FMT>
 __device__ __forceinline__ void kv_write(const mtk_kv_move_kargs &a) {
@@ -140,27 +142,24 @@ __device__ __forceinline__ void kv_write(const mtk_kv_move_kargs &a) {
     }
     if (x.quarter == 0) *(uint8_t *)(at + x.scale + (uint32_t)off * (uint32_t)a.blocks) = (uint8_t)(bad ? kNanScale : byte);
   };
-  for (int it0 = rows.part * 64 + lane; it0 < items; it0 += 64 * a.parts * kMoveAhead) {  // 4 lanes are a whole block
-    for (int i = 0; i < rows.n; ++i) {
-      const int page = __builtin_amdgcn_readlane(rows.page, i), off = __builtin_amdgcn_readlane(rows.off, i);
-      if (page < 0) continue;
-      const size_t t = (size_t)(rows.t0 + i);
-      char *at = (char *)a.cache + (uint64_t)(uint32_t)page * page_b;
+  const int it = rows.part * 64 + lane;
+  if (it < items) {  // 4 lanes are a whole block
+    const KvItem<FMT> x(a, it);
+    const bool in = x.d < a.D;
+    const uint16_t *src = (const uint16_t *)(x.v ? a.V : a.K) + (size_t)x.head * a.D + x.d;
+    const int64_t ld = x.v ? a.ld_v : a.ld_k;
+    for (int i0 = 0; i0 < rows.n; i0 += kMoveAhead) {
       u32x4 v[kMoveAhead];
 #pragma unroll
       for (int k = 0; k < kMoveAhead; ++k) {
-        const int it = it0 + 64 * a.parts * k;
         v[k] = u32x4{0u, 0u, 0u, 0u};
-        if (it < items) {
-          const KvItem<FMT> x(a, it);
-          if (x.d < a.D)
-            v[k] = *(const u32x4 *)((const uint16_t *)(x.v ? a.V : a.K) + t * (x.v ? a.ld_v : a.ld_k) + (size_t)x.head * a.D + x.d);
-        }
+        if (in && i0 + k < rows.n) v[k] = __builtin_nontemporal_load((const u32x4 *)(src + (size_t)(rows.t0 + i0 + k) * ld));
       }
 #pragma unroll
       for (int k = 0; k < kMoveAhead; ++k) {
-        const int it = it0 + 64 * a.parts * k;
-        if (it < items) one(KvItem<FMT>(a, it), at, off, v[k]);
+        if (i0 + k >= rows.n) break;
+        const int page = __builtin_amdgcn_readlane(rows.page, i0 + k), off = __builtin_amdgcn_readlane(rows.off, i0 + k);
+        if (page >= 0) one(x, (char *)a.cache + (uint64_t)(uint32_t)page * page_b, off, v[k]);
       }
     }
   }
@@ -174,19 +173,19 @@ __device__ __forceinline__ void kv_read(const mtk_kv_move_kargs &a) {
   const uint64_t page_b = kv_region_bytes(FMT, a.blocks, a.page_shift) * (uint64_t)a.H_kv;
   const uint32_t row_b = (uint32_t)kv_row_bytes(FMT, a.blocks);
   constexpr uint32_t kNan = DT == DT_F16 ? 0x7E007E00u : 0x7FC07FC0u;
-  for (int it0 = rows.part * 64 + lane; it0 < items; it0 += 64 * a.parts * kMoveAhead) {
-    for (int i = 0; i < rows.n; ++i) {
-      const int page = __builtin_amdgcn_readlane(rows.page, i), off = __builtin_amdgcn_readlane(rows.off, i);
-      if (page == -2) continue;  // no sequence's row: left as it was
-      const size_t t = (size_t)(rows.t0 + i);
-      const char *at = (const char *)a.cache + (uint64_t)(uint32_t)max(page, 0) * page_b;  // page -1 is not looked at
+  const int it = rows.part * 64 + lane;
+  const KvItem<FMT> x(a, it);
+  if (it < items && x.d < a.D) {
+    uint16_t *dst = (uint16_t *)(x.v ? a.V : a.K) + (size_t)x.head * a.D + x.d;
+    const int64_t ld = x.v ? a.ld_v : a.ld_k;
+    for (int i0 = 0; i0 < rows.n; i0 += kMoveAhead) {
       uint32_t words[kMoveAhead][kWords8<FMT>], s[kMoveAhead];
 #pragma unroll
       for (int k = 0; k < kMoveAhead; ++k) {
-        const int it = it0 + 64 * a.parts * k;
+        const int page = __builtin_amdgcn_readlane(rows.page, i0 + k), off = __builtin_amdgcn_readlane(rows.off, i0 + k);
         s[k] = kNanScale;
-        if (it < items && page >= 0) {
-          const KvItem<FMT> x(a, it);
+        if (i0 + k < rows.n && page >= 0) {
+          const char *at = (const char *)a.cache + (uint64_t)(uint32_t)page * page_b;
           const char *code = at + x.code + (uint32_t)off * row_b;
           if constexpr (FMT == KV_FP4) {
             words[k][0] = *(const uint32_t *)code;
@@ -200,13 +199,11 @@ __device__ __forceinline__ void kv_read(const mtk_kv_move_kargs &a) {
       }
 #pragma unroll
       for (int k = 0; k < kMoveAhead; ++k) {
-        const int it = it0 + 64 * a.parts * k;
-        if (it >= items) continue;
-        const KvItem<FMT> x(a, it);
-        if (x.d >= a.D) continue;
+        if (i0 + k >= rows.n) break;
+        if (__builtin_amdgcn_readlane(rows.page, i0 + k) == -2) continue;  // no sequence's row: left as it was
         u32x4 v = u32x4{kNan, kNan, kNan, kNan};
         if (s[k] != kNanScale) v = values8<DT, FMT>(words[k], scale_of(s[k]));
-        *(u32x4 *)((uint16_t *)(x.v ? a.V : a.K) + t * (x.v ? a.ld_v : a.ld_k) + (size_t)x.head * a.D + x.d) = v;
+        *(u32x4 *)(dst + (size_t)(rows.t0 + i0 + k) * ld) = v;
       }
     }
   }
