@@ -55,7 +55,7 @@ MTK_KV_FN int kv_page(const int32_t *row_of_table, int64_t pos, int n_pages, int
   return page >= 0 && page < n_pages ? page : -1;
 }
 
-// x / d for 0 <= x < 2^31, 0 < d < 2^24.
+// x / d for 0 <= x < 2^31, 0 < d <= 2^24.
 MTK_KV_FN int kv_div(int x, int d) {
 #ifdef __HIP_DEVICE_COMPILE__
   // by a reciprocal in 32 bits: at most x 2^-22 / d + 1 off, so a second estimate of the rest is at most one off
@@ -110,6 +110,17 @@ MTK_KV_FN kv_cut kv_cut_of(int work, int own, int units, int least, int whole) {
     const int n = kv_div(work + units - 1, units);
     if (n > least) c.each = n;
   }
+  return c;
+}
+
+// Launches whose workgroups have one pair each (by_pair): shares of `each` steps of it, so that there are about `units` of
+// them; `least` or more, and no more than `most`, the steps of a full table.
+MTK_KV_FN kv_cut kv_cut_pairs(int work, int units, int least, int most) {
+  kv_cut c;
+  c.padded = 1;
+  c.each = kv_div(work + units - 1, units);
+  if (c.each > most) c.each = most;
+  if (c.each < least) c.each = least;
   return c;
 }
 

@@ -88,19 +88,17 @@ struct KvLine {
     return kv_blocks(x, a.S_q, a.G, ROWS ? __builtin_ctz(ROWS ? ROWS : 1) : a.rows_shift, STEP ? __builtin_ctz(STEP ? STEP : 1) : a.step_shift,
                      a.rows_above, a.rows_most);
   }
-  __device__ __forceinline__ int len_of(int b) const { return b < a.B ? a.kv_len[b] : 0; }
-  __device__ __forceinline__ void place(const kv_seq &s, int len, const kv_share &h) {
+  __device__ __forceinline__ void place(const kv_seq &s, const kv_share &h) {
     sm[lane] = before + wave_scan(h.blocks * a.H_kv * kv_length(h, cut));
     sm[64 + lane] = s.first;
     sm[128 + lane] = s.rows;
-    sm[192 + lane] = len;
+    sm[192 + lane] = s.len;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
   __device__ __forceinline__ KvLine(const mtk_kv_attn_kargs &args, int lane_, int *words) : a(args), lane(lane_), sm(words) {}
   __device__ __forceinline__ void lay() {
     const kv_seq s = load_seq(a, lane);
-    const int len = len_of(lane);
     const kv_share h = share_of(s);
     int work = h.blocks * a.H_kv * h.steps, own = h.blocks * a.H_kv * kv_own(h, a.least);
 #pragma unroll 1
@@ -111,22 +109,23 @@ struct KvLine {
     }
     work = __builtin_amdgcn_readlane(wave_scan(work), 63);
     if (a.by_pair) {
-      cut.padded = 1;
-      cut.each = __builtin_amdgcn_readfirstlane(max(a.least, kv_div(work + a.units - 1, a.units)));
-      place(s, len, h);
+      const int shift = STEP ? __builtin_ctz(STEP ? STEP : 1) : a.step_shift;
+      cut = kv_cut_pairs(work, a.units, a.least, (int)((((uint32_t)a.max_pages << a.page_shift) + (1u << shift) - 1) >> shift));
+      cut.each = __builtin_amdgcn_readfirstlane(cut.each);
+      place(s, h);
       return;
     }
     own = __builtin_amdgcn_readlane(wave_scan(own), 63);
     cut = kv_cut_of(work, own, a.units, a.least, a.whole);
     cut.each = __builtin_amdgcn_readfirstlane(cut.each);
     total = cut.padded ? own * a.least : work;
-    place(s, len, h);
+    place(s, h);
   }
   __device__ __forceinline__ void next() {  // the next 64
     before = __builtin_amdgcn_readfirstlane(sm[63]);
     b0 += 64;
     const kv_seq s = load_seq(a, b0 + lane);
-    place(s, len_of(b0 + lane), share_of(s));
+    place(s, share_of(s));
   }
   // The lane of the sequence that pos falls into, or -1. pos ascends from call to call.
   __device__ __forceinline__ int find(int pos) {

@@ -61,7 +61,6 @@ int plan_kv_move(mtk_ctx *ctx, const mtk_kv_desc *d_in, PlanKind kind, mtk_plan 
   const mtk_kv_desc d = *d_in;
   int s = check_kv_batch(d);
   if (s != MTK_OK) return s;
-  if ((long long)d.H_kv * d.D > INT32_MAX) return fail(MTK_ERR_UNSUPPORTED, "rows of more than 2^31 elements are not supported");
   mtk_kv_move_kargs a{};
   if ((s = kv_ld(d.ld_k, d.H_kv * d.D, "ld_k", &a.ld_k)) != MTK_OK || (s = kv_ld(d.ld_v, d.H_kv * d.D, "ld_v", &a.ld_v)) != MTK_OK) return s;
   a.B = d.B;
@@ -73,14 +72,13 @@ int plan_kv_move(mtk_ctx *ctx, const mtk_kv_desc *d_in, PlanKind kind, mtk_plan 
   a.n_pages = d.n_pages;
   a.max_pages = d.max_pages;
   const long long items = 8LL * d.H_kv * a.blocks;  // of 16 bytes of K or V, per row
-  if (items > (1 << 28)) return fail(MTK_ERR_UNSUPPORTED, "rows of this size are not supported");
   // Up to 4 rows per wavefront, whose places it looks up once and whose lines in the cache it fills itself; fewer where
   // that would leave less than 8 wavefronts per CU. 64 items of each.
   const int cus = ctx ? ctx->prop.multiProcessorCount : 256;
   a.parts = (int)((items + 63) / 64);
   a.rows_per_wave = 1;
   while (a.rows_per_wave < 4 && (d.T + 2LL * a.rows_per_wave - 1) / (2 * a.rows_per_wave) * a.parts >= 8LL * cus) a.rows_per_wave *= 2;
-  const long long groups = (d.T + a.rows_per_wave - 1) / a.rows_per_wave;
+  const long long groups = ((long long)d.T + a.rows_per_wave - 1) / a.rows_per_wave;
   a.mul_blocks = a.blocks == 1 ? 0u : (uint32_t)((0x100000000ull + a.blocks - 1) / a.blocks);
   const long long waves = a.parts * groups;
   if ((waves + 3) / 4 > INT32_MAX / 256) return fail(MTK_ERR_UNSUPPORTED, "T of %d is not supported", d.T);
@@ -206,7 +204,7 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
     k.least = 2;
     k.most_blocks = 1;
     const long long blocks = (long long)d.B * d.H_kv, steps = (positions + shape.step() - 1) / shape.step();
-    if ((s = too_large(blocks, steps + k.least)) != MTK_OK) return s;
+    if ((s = too_large(blocks, 2 * (steps + k.least))) != MTK_OK) return s;
     k.whole = positions <= (wide ? 4096 : 1024) ? 1 : 0;
     snprintf(name, sizeof name, "mtk_kv_attend_%s_d%d_r%d_%s%s", kv_format(d), dp, nr, wide ? "w16_" : "", kv_suffix(d).c_str());
     add(k, name, rows, shape.step(), 64 * shape.waves, k.whole ? blocks : k.units, !k.whole);
@@ -223,7 +221,7 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
     // fewer blocks than workgroups: the keys are split, into 8 steps (512 keys) or more; else never
     const bool split = blocks < k.units && steps > 8;
     k.least = split ? 8 : (int)steps;
-    if ((s = too_large(each, 2 * steps + k.least)) != MTK_OK) return s;
+    if ((s = too_large(each, 3 * steps + k.least)) != MTK_OK) return s;
     const long long grid = split ? k.units + blocks : blocks;
     snprintf(name, sizeof name, "mtk_kv_prefill_%s_d%d_%s", kv_format(d), dp, kv_suffix(d).c_str());
     add(k, name, rows, step, 256, grid, split);
@@ -270,8 +268,20 @@ int check_kv_args(const mtk_plan *p, const void *argset) {
     if (p->workspace && (!t->workspace || !aligned(t->workspace, 16)))
       return fail(MTK_ERR_INVALID, "this plan needs a 16-byte aligned workspace of %zu bytes", p->workspace);
     const int64_t width = (int64_t)d.H * d.D;
-    if (overlap(t->Q, kv_span(d.T, d.ld_q ? d.ld_q : width, width), t->O, kv_span(d.T, width, width)))
-      return fail(MTK_ERR_INVALID, "Q and O overlap");
+    struct {
+      const char *name;
+      const void *at;
+      uint64_t bytes;
+    } const in[] = {{"Q", t->Q, kv_span(d.T, d.ld_q ? d.ld_q : width, width)}, {"the cache", cache, kv_cache_size(d)}},
+      out[] = {{"O", t->O, kv_span(d.T, width, width)}, {"lse", t->lse, 4ull * d.T * d.H}, {"the workspace", t->workspace, p->workspace}};
+    for (int i = 0; i < 3; ++i) {
+      if (!out[i].at || !out[i].bytes) continue;
+      for (const auto &x : in)
+        if (x.at && overlap(out[i].at, out[i].bytes, x.at, x.bytes)) return fail(MTK_ERR_INVALID, "%s overlaps %s", out[i].name, x.name);
+      for (int k = 0; k < i; ++k)
+        if (out[k].at && overlap(out[i].at, out[i].bytes, out[k].at, out[k].bytes))
+          return fail(MTK_ERR_INVALID, "%s overlaps %s", out[i].name, out[k].name);
+    }
   } else {
     const bool write = p->kind == PLAN_KV_WRITE;
     const mtk_kv_write_args *w = (const mtk_kv_write_args *)argset;
