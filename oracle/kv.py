@@ -141,8 +141,9 @@ class Cache:
                 out[w][first:first + n] = bits_of(self.values(w, page, pos % self.page), self.dtype)
         return out
 
-    def attention(self, Q, row_start, kv_len, table, causal=True, S_q=0):
-        """(O, lse, bound) in 64 bits; rows of no sequence are NaN with bound -1 (not computed). `bound` is what O may
+    def attention(self, Q, row_start, kv_len, table, causal=True, S_q=0, only=None):
+        """(O, lse, bound) in 64 bits; rows of no sequence are NaN with bound -1 (not computed), and so are rows that are not
+        in `only`, if it is given. `bound` is what O may
         be off: half a step of the result; the weights' rounding, half a step of each; and the scores in 32 bits: D + 3
         roundings of 2^-24 of sum |q k| and of the scaled score and its offset, which move a weight by as much."""
         T, H, D = Q.shape
@@ -158,6 +159,8 @@ class Cache:
                 page[:] = -1
             k, v = (self.values(w, page, pos % self.page) for w in range(2))
             for i in range(min(n, S_q or T)):
+                if only is not None and first + i not in only:
+                    continue
                 m = max(0, min(keys, pos0 + i + 1)) if causal else keys
                 for h in range(H):
                     x = q[first + i, h]
