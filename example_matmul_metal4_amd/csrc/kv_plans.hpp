@@ -175,11 +175,12 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
     snprintf(text, sizeof text, " rows/wg=%d grid=%lld%s", rows, grid, split ? " keys split" : "");
     how += text;
     if (split) {
-      // fewer than 8 parts for each pair on average: a group of lanes for each; the rows that this kernel can have
-      const long long pairs_most = (long long)d.B * d.H_kv;
-      const bool parts = !k.by_pair && pairs_most * 8 < grid;
-      const int heads = parts ? 1 : 1024 / k.part_ld;
+      // The join's lanes: over the parts of each (row, head) where a pair has more than 8 parts and there are few (row, head)s
+      // to fill the device with, else over the heads. 1 x 131071 positions, 8 K/V heads: both kernels 35.5 us, over the heads
+      // 49.6; 4 x 8000: 17.6 and 20.1; but 4 x 2000 with 16 rows of 16 heads: 23.0 and 20.7, 16 x 8000: 35.9 and 34.6.
       const long long mine = k.by_pair ? d.T : std::min<long long>(d.T, (long long)d.B * std::max(1, k.rows_most / G));
+      const bool parts = !k.by_pair && (long long)d.B * d.H_kv * 8 < grid && mine * d.H < 2LL * cus;
+      const int heads = parts ? 1 : 1024 / k.part_ld;
       Launch c = g;
       c.name = std::string(parts ? "mtk_kv_join_parts_" : "mtk_kv_join_rows_") + kv_suffix(d);
       c.block = 256;
@@ -194,18 +195,22 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
   };
   if (few) {
     const int nr = few <= 16 ? 1 : few <= 32 || dp == 256 ? 2 : 4, rows = 16 * nr;
-    // few pairs of short sequences: one workgroup of 16 wavefronts each, no second kernel
-    const bool wide = nr == 1 && dp <= 128 && positions <= 4096 && (long long)d.B * d.H_kv <= cus;
+    // Few pairs of short sequences: one workgroup of 16 wavefronts each, no second kernel. 1000 positions, 8 pairs: 9.2 us
+    // against 13.2 with the keys split; 32 x 4000 (256 pairs): 26.8 and 32.5; but 4 x 4000 (32 pairs): 19.6 and 14.3. Longer
+    // tables would gain too where pairs fill the device and are equally long (32 x 8000: 53.6 and 62.3), not where one is long.
+    const long long blocks = (long long)d.B * d.H_kv;
+    const bool wide = nr == 1 && dp <= 128 && blocks <= cus && positions <= (2 * blocks >= cus ? 4096 : 2048);
     const KvShape shape = wide ? KvShape{32, 16, 1} : kv_kernel_shape(d.format, dp, nr);
     mtk_kv_attn_kargs k = a;
     k.rows_above = 0;
     k.rows_most = rows;
     k.units = cus * shape.per_cu;
-    k.least = 2;
+    k.least = 2;  // 1 x 16000: 14.7 us, least 1: 16.9; 4 x 2000 with 16 rows: 23.0, least 4: 25.1
     k.most_blocks = 1;
-    const long long blocks = (long long)d.B * d.H_kv, steps = (positions + shape.step() - 1) / shape.step();
+    const long long steps = (positions + shape.step() - 1) / shape.step();
     if ((s = too_large(blocks, 2 * (steps + k.least))) != MTK_OK) return s;
-    k.whole = positions <= (wide ? 4096 : 1024) ? 1 : 0;
+    // 64 x 1000: whole pairs 16.3 us, split 22.1; 64 x 2000 (512 pairs): 28.3 and 32.5; 8 x 4000 with 16 rows: 80 and 34
+    k.whole = wide || positions <= (blocks >= 2 * cus ? 2048 : 1024) ? 1 : 0;
     snprintf(name, sizeof name, "mtk_kv_attend_%s_d%d_r%d_%s%s", kv_format(d), dp, nr, wide ? "w16_" : "", kv_suffix(d).c_str());
     add(k, name, rows, shape.step(), 64 * shape.waves, k.whole ? blocks : k.units, !k.whole);
   }

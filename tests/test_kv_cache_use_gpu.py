@@ -210,8 +210,8 @@ def test_shared_pages_and_long_tables(dev):
     g = Given(dev, 49, lens, [1] * 40, 8, 8, 64, 16, "fp4", "f16", n_pages=60, width=300)
     g.check(1)
     g.free()
-    lens = [3900, 2000]
-    g = Given(dev, 50, lens, [1, 1], 2, 2, 128, 16, "fp8", "bf16", n_pages=30)
+    lens = [3900] + [100] * 14 + [2000]
+    g = Given(dev, 50, lens, [1] * 16, 8, 8, 128, 16, "fp8", "bf16", n_pages=30)
     assert "_w16_" in g.plan(1).describe()
     g.check(1)
     g.free()
