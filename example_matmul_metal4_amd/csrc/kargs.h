@@ -179,7 +179,6 @@ typedef struct {
   int32_t rows_shift, step_shift; /* log2 of the kernel's rows per block and keys per step */
   /* who does what (kv_cache.h): workgroups wanted (at most), least steps of one, or one for each pair */
   int32_t units, least, whole;
-  int32_t most_blocks; /* whole: row blocks of a sequence, at most */
   int32_t by_pair;     /* a workgroup has steps of one pair only, the sequence's last row blocks first */
   int32_t places;      /* workgroups that part has room for: two places each, by_pair: one */
   int32_t part_ld; /* floats per row of part */

@@ -4,9 +4,11 @@
 //   O[i][h] = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(q_i . k_j / sqrt(D)),  j <= position of row i (causal)
 //
 // with k_j, v_j the cached values. One pass over the keys with a running exponent offset and sum per row (fp32).
-//   * A workgroup has one (sequence, K/V head, 16 NR rows of (row, query head) pairs, split of the keys); its 4
-//     wavefronts take every 4th tile of 32 keys. Which split is found on the device from the lengths themselves
-//     (find_unit), so that a captured launch serves any lengths.
+//   * The wavefronts of a workgroup (4, 8 or 16) take tiles of 16 KB keys in turn for the same 16 NR (row, query head) pairs
+//     of a K/V head. Where a sequence's pairs are few enough for one workgroup each (runtime: plan_kv_attn), that is all;
+//     else the steps of all pairs lie on a line that persistent workgroups share evenly (kv_cache.h), found on the device
+//     from the lengths, so that a captured launch serves any lengths. fp8, 16 x 8192 ragged positions: equal splits of each
+//     sequence 68 us, of all of them 55.
 //   * K: a lane has the codes of one key and a quarter of the head's dims: exactly an operand of the 16x16x32
 //     MFMA (the dims may be summed in any order, Q is loaded in the same one). They go from the load through
 //     v_cvt_scalef32_pk (two codes and their scale per instruction, exact) into S^T = K Q^T without LDS.
@@ -17,11 +19,21 @@
 //     offsets and sums stay in fp32.
 //   * Keys past the length have their V codes zeroed (a page's unused rows may hold anything); a NaN block's V is
 //     zeroed too and its dims set to NaN only for the rows that see the key, so that nothing masked reaches O.
+//
+// Bound: HBM where there is much to read, else latency. A wavefront's loads of the next tile are issued as its registers
+// fall free (K and scales before the softmax, V after its codes are staged); nothing spills, for scratch traffic cost more
+// than a third wavefront per SIMD won (fp8, 128 dims: 3 per SIMD 49.7 us, 4 with spills 58.7). Loads of the head's last,
+// half-empty block behind a branch: without it 31.7 -> 33.0 us. Loads that bypass the caches: 5 % faster on one long
+// sequence, 12 to 18 % slower where sequences share pages. Scales as whole words: 64 dims 41.4 -> 36.5 us.
+// Measured, fp4, 8 K/V heads of 128 dims, 4 query heads each, first kernel and join: 1 x 131071 positions 31.7 + 7.0 us
+// (4.5 TB/s in the first), 64 x 6000 82 + 7 (5.1 TB/s), 32 x 4096 ragged 21.8, 1 x 1000 8.8 (0.8 to find its work, 1.6 for
+// the first bytes, 2 tiles of 1.1, 2.4 for the sum over 16 wavefronts, the launch); 64-dim heads without groups, 64 x 2048:
+// 28.2; fp8 16 x 8192: 49.7 + 4.7 (4.85 TB/s).
 #include "kv_device.hpp"
 
 namespace mtk {
 
-constexpr float kKvSlack = 8.0f;  // log2-domain headroom before O is rescaled
+constexpr float kKvSlack = 8.0f;  // log2-domain headroom before O is rescaled: weights up to 2^8, in range for f16 as well
 constexpr int kWindow = 56;       // table entries between the starts of two windows (below)
 
 // max over the lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -92,15 +104,14 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
   KvSegment seg;
   const bool whole = W == 16 || a.whole;
   if (whole) {  // a workgroup for each pair, by its number: nothing to look up
-    const int q = kv_div(blockIdx.x, a.H_kv);
-    seg.hk = blockIdx.x - q * a.H_kv;
-    seg.b = a.most_blocks == 1 ? q : kv_div(q, a.most_blocks);
-    seg.rb = q - seg.b * a.most_blocks;
+    seg.b = kv_div(blockIdx.x, a.H_kv);
+    seg.hk = blockIdx.x - seg.b * a.H_kv;
+    seg.rb = 0;
     seg.seq = load_seq(a, seg.b);
     const kv_share h = line.share_of(seg.seq);
     seg.from = seg.start = 0;
     seg.to = seg.steps = h.steps;
-    if (seg.rb >= h.blocks) return;
+    if (h.blocks == 0) return;
   } else {
     line.lay();
     const int wgs = kv_div(line.total + line.cut.each - 1, line.cut.each);
@@ -525,6 +536,8 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
 //   PARTS: a workgroup has one (row, query head); group g of NG adds every NGth part, the groups are added in turn. For
 //   few pairs of long sequences, which have many parts.
 //   else: each group has a query head of its own, a workgroup NG heads of a row.
+// Bound by latency (the lengths, the parts' statistics and the parts in turn): 4.6 us for 128 rows of heads, 7.0 for one row
+// of 32 heads in 128 parts each. runtime: plan_kv_attn has both sides of the choice.
 constexpr int kKvJoin = 256;  // threads
 template <int DT, bool PARTS>
 __device__ __forceinline__ void kv_join(const mtk_kv_attn_kargs &a) {

@@ -113,15 +113,13 @@ MTK_KV_FN kv_cut kv_cut_of(int work, int own, int units, int least, int whole) {
   return c;
 }
 
-// Launches whose workgroups have one pair each (by_pair): shares of `each` steps of it, so that there are about `units` of
-// them; `least` or more, and no more than `most`, the steps of a full table.
-MTK_KV_FN kv_cut kv_cut_pairs(int work, int units, int least, int most) {
-  kv_cut c;
-  c.padded = 1;
-  c.each = kv_div(work + units - 1, units);
-  if (c.each > most) c.each = most;
-  if (c.each < least) c.each = least;
-  return c;
+// Launches whose workgroups have one pair each (by_pair): shares of `each` steps of it, at least `least` and no more than
+// `most`, the steps of a full table. With `each` of this or more there are at most `units` workgroups: pairs ceil their
+// steps / each, which adds less than 1 for each. own: the pairs; where they are `units` or more, each has one workgroup.
+MTK_KV_FN int kv_each_of_pairs(int work, int own, int units, int least, int most) {
+  int each = own < units ? kv_div(work + (units - own) - 1, units - own) : most;
+  if (each > most) each = most;
+  return each < least ? least : each;
 }
 
 MTK_KV_FN int kv_length(kv_share r, kv_cut c) { return c.padded ? kv_div(r.steps + c.each - 1, c.each) * c.each : r.steps; }

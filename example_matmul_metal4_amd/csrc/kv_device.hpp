@@ -73,7 +73,8 @@ struct KvSegment {
 };
 
 // A wavefront's view of the line: 64 sequences at a time, in LDS words of its own (registers are what the kernel is
-// short of). ROWS rows per block, STEP keys per step (0: as the launch says).
+// short of). ROWS rows per block (128: the kernel whose workgroups have one pair each), STEP keys per step (0: as the
+// launch says).
 constexpr int kLineWords = 4 * 64;
 template <int ROWS, int STEP>
 struct KvLine {
@@ -84,6 +85,7 @@ struct KvLine {
   int total = 0;          // length of the line
   int b0 = 0, before = 0; // the first of the 64, and where its pairs start
 
+  __device__ __forceinline__ bool by_pair() const { return ROWS ? ROWS == 128 : a.by_pair != 0; }
   __device__ __forceinline__ kv_share share_of(const kv_seq &x) const {
     return kv_blocks(x, a.S_q, a.G, ROWS ? __builtin_ctz(ROWS ? ROWS : 1) : a.rows_shift, STEP ? __builtin_ctz(STEP ? STEP : 1) : a.step_shift,
                      a.rows_above, a.rows_most);
@@ -100,22 +102,36 @@ struct KvLine {
   __device__ __forceinline__ void lay() {
     const kv_seq s = load_seq(a, lane);
     const kv_share h = share_of(s);
-    int work = h.blocks * a.H_kv * h.steps, own = h.blocks * a.H_kv * kv_own(h, a.least);
+    auto own_of = [&](const kv_share &x) { return x.blocks * a.H_kv * (by_pair() ? 1 : kv_own(x, a.least)); };
+    int work = h.blocks * a.H_kv * h.steps, own = own_of(h);
 #pragma unroll 1
     for (int b = 64; b < a.B; b += 64) {
       const kv_share x = share_of(load_seq(a, b + lane));
       work += x.blocks * a.H_kv * x.steps;
-      own += x.blocks * a.H_kv * kv_own(x, a.least);
+      own += own_of(x);
     }
-    work = __builtin_amdgcn_readlane(wave_scan(work), 63);
-    if (a.by_pair) {
+    auto sum = [](int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); };
+    work = sum(work);
+    own = sum(own);
+    if (by_pair()) {
       const int shift = STEP ? __builtin_ctz(STEP ? STEP : 1) : a.step_shift;
-      cut = kv_cut_pairs(work, a.units, a.least, (int)((((uint32_t)a.max_pages << a.page_shift) + (1u << shift) - 1) >> shift));
-      cut.each = __builtin_amdgcn_readfirstlane(cut.each);
+      const int most = (int)((((uint32_t)a.max_pages << a.page_shift) + (1u << shift) - 1) >> shift);
+      int hi = kv_each_of_pairs(work, own, a.units, a.least, most);
+      if (a.B <= 64) {  // the least that makes no more workgroups than that
+        int lo = min(hi, max(a.least, kv_div(work + a.units - 1, a.units)));
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (sum(h.blocks * a.H_kv * kv_div(h.steps + mid - 1, mid)) <= a.units)
+            hi = mid;
+          else
+            lo = mid + 1;
+        }
+      }
+      cut.padded = 1;
+      cut.each = __builtin_amdgcn_readfirstlane(hi);
       place(s, h);
       return;
     }
-    own = __builtin_amdgcn_readlane(wave_scan(own), 63);
     cut = kv_cut_of(work, own, a.units, a.least, a.whole);
     cut.each = __builtin_amdgcn_readfirstlane(cut.each);
     total = cut.padded ? own * a.least : work;
@@ -152,6 +168,8 @@ struct KvLine {
     g.b = b0 + at;
     const int first = __builtin_amdgcn_readfirstlane(sm[64 + at]), rows = __builtin_amdgcn_readfirstlane(sm[128 + at]);
     g.seq = kv_sequence(first, first + rows, __builtin_amdgcn_readfirstlane(sm[192 + at]), a.T, a.max_pages, a.page_shift);
+    g.seq.keys = __builtin_amdgcn_readfirstlane(g.seq.keys);  // as they are in every lane: else what follows from them fills vector
+    g.seq.bad = __builtin_amdgcn_readfirstlane(g.seq.bad);    // registers, and the loads' descriptors need loops
     const kv_share h = share_of(g.seq);
     g.steps = h.steps;
     length = __builtin_amdgcn_readfirstlane(kv_length(h, cut));
@@ -171,7 +189,7 @@ struct KvLine {
     g.to = min(g.steps, end - g.start);
     g.rb = __builtin_amdgcn_readfirstlane(kv_div(pair, a.H_kv));
     g.hk = pair - g.rb * a.H_kv;
-    if (a.by_pair) g.rb = kv_div(pairs, a.H_kv) - 1 - g.rb;
+    if (by_pair()) g.rb = __builtin_amdgcn_readfirstlane(kv_div(pairs, a.H_kv)) - 1 - g.rb;
     return g;
   }
 };

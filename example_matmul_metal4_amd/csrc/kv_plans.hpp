@@ -100,7 +100,9 @@ int plan_kv_move(mtk_ctx *ctx, const mtk_kv_desc *d_in, PlanKind kind, mtk_plan 
   return finish_kv(p, out);
 }
 
-// Of the attention kernels (kv_attention.hip): keys per tile, wavefronts per workgroup, workgroups per CU.
+// Of the attention kernels (kv_attention.hip): keys per tile, wavefronts per workgroup, workgroups per CU as their registers
+// and LDS allow. Measured for 32 rows of (row, query head) pairs, fp4, 128 dims (8 x 3000 to 8000 positions, the first
+// kernel): 32 keys, 8 wavefronts, 1 workgroup 22.3 us; 4 and 2 22.8; 64 keys, 8 and 1 23.7; 64 keys, 4 and 2 24.1.
 struct KvShape {
   int tile, waves, per_cu;
   int step() const { return tile * waves; }
@@ -206,7 +208,6 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
     k.rows_most = rows;
     k.units = cus * shape.per_cu;
     k.least = 2;  // 1 x 16000: 14.7 us, least 1: 16.9; 4 x 2000 with 16 rows: 23.0, least 4: 25.1
-    k.most_blocks = 1;
     const long long steps = (positions + shape.step() - 1) / shape.step();
     if ((s = too_large(blocks, 2 * (steps + k.least))) != MTK_OK) return s;
     // 64 x 1000: whole pairs 16.3 us, split 22.1; 64 x 2000 (512 pairs): 28.3 and 32.5; 8 x 4000 with 16 rows: 80 and 34
@@ -223,11 +224,13 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
     k.units = cus * (dp == 256 ? 1 : 2);
     const long long each = (long long)d.B * ((pairs + rows - 1) / rows) * d.H_kv;  // blocks, whatever row_start holds
     const long long blocks = kv_max_blocks(d.B, d.T, d.S_q, G, rows) * d.H_kv, steps = (positions + step - 1) / step;
-    // fewer blocks than workgroups: the keys are split, into 8 steps (512 keys) or more; else never
-    const bool split = blocks < k.units && steps > 8;
-    k.least = split ? 8 : (int)steps;
+    // Fewer blocks than workgroups: the keys are split, into 4 steps (256 keys) or more, so that all workgroups are on the
+    // device at once; else never. 300 rows of 8 heads of 64 dims, 1000 positions: 17.8 us, 8 steps 22.6, 2 steps 16.8;
+    // 2 x 4000 positions, 100 rows, 256 dims: 47.4, 54.8 and 47.3, with shares of equal work (two rounds) 51.3, unsplit 215.
+    const bool split = blocks < k.units && steps > 4;
+    k.least = split ? 4 : (int)steps;
     if ((s = too_large(each, 3 * steps + k.least)) != MTK_OK) return s;
-    const long long grid = split ? k.units + blocks : blocks;
+    const long long grid = split ? k.units : blocks;
     snprintf(name, sizeof name, "mtk_kv_prefill_%s_d%d_%s", kv_format(d), dp, kv_suffix(d).c_str());
     add(k, name, rows, step, 256, grid, split);
   }

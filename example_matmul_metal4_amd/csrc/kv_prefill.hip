@@ -11,7 +11,13 @@
 //   * Grouped heads share a K/V head's tiles: 128 pairs are 128 / G queries.
 //   * Keys past the length have their V codes zeroed, NaN blocks are zeroed in V and set to NaN for the rows that see
 //     them, as in kv_attention.hip; bit masks of such keys lie in LDS beside the tiles.
-//   * Few row blocks: the keys are split over workgroups (kv_cache.h), whose partial sums kv_combine adds.
+//   * Few row blocks: the keys are split over workgroups (kv_cache.h), whose partial sums kv_join adds.
+//
+// Bound by the matrix units and the VALU beside them (the exponentials, and the conversions of a tile, shared by 128 pairs):
+// 2048 rows of 32 heads of 128 dims behind 6144 positions 274 us, 0.88 PFLOP/s, where the 16-bit kernel of attention.hpp
+// reaches 0.93 at such sizes. With the key-splitting kernels such a chunk took 644 us. Converting a tile during the
+// second product instead of the first made no difference. 500 rows of 24 heads, 8 K/V heads of 96 dims, 4000 positions, with a
+// join: 53.8 us, with shares of equal work, which need two rounds of workgroups, 68, unsplit 101.
 #include "kv_device.hpp"
 
 namespace mtk {
@@ -46,7 +52,9 @@ __device__ __forceinline__ void kv_prefill(const mtk_kv_attn_kargs &a) {
   KvLine<kPfRows, kPfKeys> line(a, lane, sm_line[wave]);
   line.lay();
   const int wg = blockIdx.x;
-  const KvSegment seg = line.at(wg * line.cut.each, (wg + 1) * line.cut.each);
+  const int64_t line_from = (int64_t)wg * line.cut.each;  // past the line's end, which 32 bits hold, for workgroups of no share
+  if (line_from > INT32_MAX - line.cut.each) return;
+  const KvSegment seg = line.at((int)line_from, (int)line_from + line.cut.each);
   if (seg.b < 0) return;
   const kv_seq seq = seg.seq;
   const int rows = min(seq.rows, a.S_q) * G;

@@ -336,10 +336,12 @@ int mtk_permute_run(const mtk_plan *plan, const mtk_permute_run_args *args);
  *   row_start [B + 1]         sequence b has rows row_start[b] .. row_start[b + 1] - 1 of the packed tensors (n of
  *                             them, none allowed); ascending, within [0, T]. Rows of no sequence are left as they were.
  *   kv_len [B]                its positions, those of its rows included: row i is position kv_len[b] - n + i
- *   table [B][max_pages]      its pages in order; entries past its length are not read
+ *   table [B][max_pages]      its pages in order; entries past its length are not used
  * The kernels check all of it: a position whose page is out of [0, n_pages), or past the table, or below 0 is not written,
- * reads as NaN, and makes the attention of the rows that see it NaN. Two sequences may share pages; where both are
- * written at one position of one page in one call, its bytes are some mix of the two.
+ * reads as NaN, and makes the attention of the rows that see it NaN; a kv_len of more than the table holds makes all of its
+ * sequence's rows that see a position NaN. row_start is limited to [0, T] and to ascend; rows that two sequences claim come out
+ * as one or the other's, or undefined in attention. Two sequences may share pages; where both are written at one position of
+ * one page in one call, its bytes are some mix of the two.
  *
  * One descriptor for the three plans. */
 #define MTK_KV_FP4 0
@@ -356,8 +358,9 @@ typedef struct {
                            fused projection) */
 } mtk_kv_desc;
 
-/* Bytes of a cache of n_pages pages (page_size, H_kv, D, format of the descriptor). Zeroed or not: no position is read
- * that kv_len does not cover. */
+/* Bytes of a cache of n_pages pages (page_size, H_kv, D, format of the descriptor). Zeroed or not: no position counts
+ * that kv_len does not cover. Those it covers hold what mtk_kv_write stored (e4m3's NaN codes, which it never stores, are
+ * not told from values). */
 int mtk_kv_cache_bytes(const mtk_kv_desc *desc, size_t *bytes);
 
 /* Rows of K and V ([T][H_kv][D]) into the cache. */
@@ -383,7 +386,9 @@ int mtk_kv_read_run(const mtk_plan *plan, const mtk_kv_read_args *args);
  * K/V head h / (H / H_kv). The new rows' own K and V are read from the cache: write them first. A row that sees no
  * position gives zeros and a log-sum-exp of -inf. The keys of long sequences are split over workgroups, whose partial
  * sums lie in the workspace until a second kernel adds them in a fixed order: the result does not vary from run to run,
- * and runs that may overlap need a workspace each. O may not overlap Q. */
+ * and runs that may overlap need a workspace each. O, lse and the workspace may not overlap Q, the cache or each other.
+ * A plan whose sequences may have more than 64 (row, query head) pairs per K/V head (32 above 128 dims) has kernels for those
+ * and, where S_q > 1, for the sequences with few rows beside them: give S_q = 1 for a batch of single tokens. */
 int mtk_kv_attn_plan(mtk_ctx *ctx, const mtk_kv_desc *desc, mtk_plan **out);
 typedef struct {
   const void *Q;

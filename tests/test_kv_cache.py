@@ -153,11 +153,28 @@ static void schedule(const mtk_kv_attn_kargs &k, const Launch &l, const std::vec
   }
   CHECK(work <= INT32_MAX && own * k.least <= INT32_MAX, "work %lld own %lld", (long long)work, (long long)own);
   kv_cut cut;
-  if (k.by_pair) cut = kv_cut_pairs((int)work, k.units, k.least, (int)((((int64_t)k.max_pages << k.page_shift) + (1 << k.step_shift) - 1) >> k.step_shift));
+  if (k.by_pair) {
+    int64_t pairs = 0;
+    for (auto &s : seqs) pairs += s.h.blocks * k.H_kv;
+    const int most = (int)((((int64_t)k.max_pages << k.page_shift) + (1 << k.step_shift) - 1) >> k.step_shift);
+    int hi = kv_each_of_pairs((int)work, (int)pairs, k.units, k.least, most);
+    auto wgs_of = [&](int each) {
+      int64_t n = 0;
+      for (auto &s : seqs) n += s.h.blocks * (int64_t)k.H_kv * ((s.h.steps + each - 1) / each);
+      return n;
+    };
+    CHECK(wgs_of(hi) <= std::max<int64_t>(k.units, pairs), "each %d", hi);
+    if (k.B <= 64)
+      for (int lo = std::min(hi, std::max<int>(k.least, (work + k.units - 1) / k.units)); lo < hi;) {
+        const int mid = (lo + hi) >> 1;
+        wgs_of(mid) <= k.units ? hi = mid : lo = mid + 1;
+      }
+    cut = {hi, 1};
+  }
   else cut = kv_cut_of((int)work, (int)own, k.units, k.least, k.whole);
   if (k.whole && !k.by_pair) {  // by the workgroup's number
     CHECK(l.grid == (unsigned)(k.B * k.H_kv), "grid %u", l.grid);
-    for (auto &s : seqs) CHECK(s.h.blocks <= k.most_blocks && s.h.steps * (1 << k.step_shift) >= 0, "blocks %d", s.h.blocks);
+    for (auto &s : seqs) CHECK(s.h.blocks <= 1, "blocks %d", s.h.blocks);
     return;
   }
   int64_t total = 0;
