@@ -154,7 +154,7 @@ typedef struct {
   int32_t blocks;     /* blocks of 32 dims of a head */
   int32_t page_shift; /* log2 of the positions per page */
   int32_t n_pages, max_pages;
-  int32_t parts, rows_per_wave; /* wavefronts that share a row; rows of a wavefront (1 with several parts) */
+  int32_t parts, rows_per_wave; /* wavefronts that share a row (64 items of 16 bytes each); rows of a wavefront */
   uint32_t mul_blocks;          /* n / blocks = umulhi(n, mul_blocks), 0: blocks is 1 */
 } mtk_kv_move_kargs;
 
@@ -166,7 +166,7 @@ typedef struct {
   void *O;
   float *lse; /* [T][H] or NULL */
   /* partial sums of the pairs that a workgroup has part of: [workgroup][2][rows of a block][part_ld], and the rows'
-   * (exponent offset in log2, sum of weights). Place 0: the part that the workgroup's range starts with, 1: any other. */
+   * (exponent offset in log2, sum of weights). Place 0: the part that the workgroup's range starts with, 1: any other (by_pair: one place). */
   float *part, *part_ml;
   int64_t ld_q; /* elements between rows of Q */
   int32_t B, T, S_q, H, H_kv, G, D; /* G: H / H_kv */
@@ -177,7 +177,7 @@ typedef struct {
    * pairs per K/V head */
   int32_t rows_above, rows_most;
   int32_t rows_shift, step_shift; /* log2 of the kernel's rows per block and keys per step */
-  /* who does what (kv_cache.h): workgroups wanted (at most), least steps of one, or one for each pair */
+  /* who does what (kv_cache.h): workgroups at most, least steps of one, or (whole) one for each pair */
   int32_t units, least, whole;
   int32_t by_pair;     /* a workgroup has steps of one pair only, the sequence's last row blocks first */
   int32_t places;      /* workgroups that part has room for: two places each, by_pair: one */

@@ -61,7 +61,7 @@ MTK_KV_FN int kv_div(int x, int d) {
   // by a reciprocal in 32 bits: at most x 2^-22 / d + 1 off, so a second estimate of the rest is at most one off
   const float inv = __builtin_amdgcn_rcpf((float)d);
   int q = (int)((float)x * inv);
-  int r = x - q * d;
+  int r = (int)((uint32_t)x - (uint32_t)q * (uint32_t)d);
   const int e = (int)((float)r * inv);
   q += e;
   r -= e * d;
@@ -100,11 +100,10 @@ typedef struct {
   int padded; /* a pair's length is a multiple of it */
 } kv_cut;
 
-// From the sums over all sequences of blocks * heads * steps and blocks * heads * kv_own. whole: every pair has one
-// workgroup (its steps are at most `least`), however many.
-MTK_KV_FN kv_cut kv_cut_of(int work, int own, int units, int least, int whole) {
+// From the sums over all sequences of blocks * heads * steps and blocks * heads * kv_own.
+MTK_KV_FN kv_cut kv_cut_of(int work, int own, int units, int least) {
   kv_cut c;
-  c.padded = whole || own <= units;
+  c.padded = own <= units;
   c.each = least;
   if (!c.padded) {
     const int n = kv_div(work + units - 1, units);

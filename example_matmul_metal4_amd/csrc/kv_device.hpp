@@ -132,7 +132,7 @@ struct KvLine {
       place(s, h);
       return;
     }
-    cut = kv_cut_of(work, own, a.units, a.least, a.whole);
+    cut = kv_cut_of(work, own, a.units, a.least);
     cut.each = __builtin_amdgcn_readfirstlane(cut.each);
     total = cut.padded ? own * a.least : work;
     place(s, h);
@@ -168,8 +168,6 @@ struct KvLine {
     g.b = b0 + at;
     const int first = __builtin_amdgcn_readfirstlane(sm[64 + at]), rows = __builtin_amdgcn_readfirstlane(sm[128 + at]);
     g.seq = kv_sequence(first, first + rows, __builtin_amdgcn_readfirstlane(sm[192 + at]), a.T, a.max_pages, a.page_shift);
-    g.seq.keys = __builtin_amdgcn_readfirstlane(g.seq.keys);  // as they are in every lane: else what follows from them fills vector
-    g.seq.bad = __builtin_amdgcn_readfirstlane(g.seq.bad);    // registers, and the loads' descriptors need loops
     const kv_share h = share_of(g.seq);
     g.steps = h.steps;
     length = __builtin_amdgcn_readfirstlane(kv_length(h, cut));

@@ -299,6 +299,7 @@ int check_kv_args(const mtk_plan *p, const void *argset) {
     ints[0] = write ? w->row_start : r->row_start, ints[1] = write ? w->kv_len : r->kv_len, ints[2] = write ? w->table : r->table;
     if (!K || !V) return fail(MTK_ERR_INVALID, "K and V must be non-null");
     if (!aligned(K, 16) || !aligned(V, 16)) return fail(MTK_ERR_INVALID, "K and V must be 16-byte aligned");
+    if (!write && K == V) return fail(MTK_ERR_INVALID, "K and V are the same rows");
     const int64_t width = (int64_t)d.H_kv * d.D;
     if (cache && (overlap(K, kv_span(d.T, d.ld_k ? d.ld_k : width, width), cache, kv_cache_size(d)) ||
                   overlap(V, kv_span(d.T, d.ld_v ? d.ld_v : width, width), cache, kv_cache_size(d))))

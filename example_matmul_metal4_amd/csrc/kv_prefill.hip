@@ -54,8 +54,12 @@ __device__ __forceinline__ void kv_prefill(const mtk_kv_attn_kargs &a) {
   const int wg = blockIdx.x;
   const int64_t line_from = (int64_t)wg * line.cut.each;  // past the line's end, which 32 bits hold, for workgroups of no share
   if (line_from > INT32_MAX - line.cut.each) return;
-  const KvSegment seg = line.at((int)line_from, (int)line_from + line.cut.each);
+  KvSegment seg = line.at((int)line_from, (int)line_from + line.cut.each);
   if (seg.b < 0) return;
+  // As they are in every lane: else what follows from them fills vector registers, and the loads' descriptors need loops
+  // (2048 rows at 8192 positions: 285 us, without 308).
+  seg.seq.keys = __builtin_amdgcn_readfirstlane(seg.seq.keys);
+  seg.seq.bad = __builtin_amdgcn_readfirstlane(seg.seq.bad);
   const kv_seq seq = seg.seq;
   const int rows = min(seq.rows, a.S_q) * G;
   const int r = seg.rb * kPfRows + wave * 32 + col, qi = kv_div(r, G), h = seg.hk * G + r - qi * G;

@@ -171,7 +171,7 @@ static void schedule(const mtk_kv_attn_kargs &k, const Launch &l, const std::vec
       }
     cut = {hi, 1};
   }
-  else cut = kv_cut_of((int)work, (int)own, k.units, k.least, k.whole);
+  else cut = kv_cut_of((int)work, (int)own, k.units, k.least);
   if (k.whole && !k.by_pair) {  // by the workgroup's number
     CHECK(l.grid == (unsigned)(k.B * k.H_kv), "grid %u", l.grid);
     for (auto &s : seqs) CHECK(s.h.blocks <= 1, "blocks %d", s.h.blocks);
@@ -307,6 +307,8 @@ int main() {
   mtk_kv_read_args rx = rd;
   rx.K = at;
   bad(r, &rx, "overlaps the cache");
+  rx = rd, rx.V = rd.K;
+  bad(r, &rx, "the same rows");
   CHECK(t->workspace > 0, " ");
   const mtk_kv_attn_args ta{at, at + q, ints, ints, ints, at + q + (1 << 24), nullptr, at + (1 << 26)};
   CHECK(check_kv_args(t, &ta) == MTK_OK, "%s", mtk_last_error());
