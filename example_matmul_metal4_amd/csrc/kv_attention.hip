@@ -29,7 +29,7 @@
 // (4.5 TB/s in the first), 64 x 6000 82 + 7 (5.1 TB/s), 32 x 4096 ragged 21.8, 1 x 1000 8.8 (0.8 to find its work, 1.6 for
 // the first bytes, 2 tiles of 1.1, 2.4 for the sum over 16 wavefronts, the launch); 64-dim heads without groups, 64 x 2048:
 // 28.2; fp8 16 x 8192: 49.7 + 4.7 (4.85 TB/s).
-#include "kv_device.hpp"
+#include "kv_join.hpp"
 
 namespace mtk {
 
@@ -48,32 +48,6 @@ __device__ __forceinline__ float quarters_sum(float x) {
   const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
   const uint32_t r0 = r[0], r1 = r[1];
   return __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
-}
-
-// Sums of some keys of a row (4 dims), unscaled, with their exponent offset (log2) and the sum of the weights.
-struct KvPart {
-  float m = -INFINITY, l = 0.0f;
-  f32x4 x = f32x4{};
-};
-__device__ __forceinline__ void add_part(KvPart &s, const KvPart &t) {
-  const float m = fmaxf(s.m, t.m);
-  const float m0 = m == -INFINITY ? 0.0f : m;
-  const float f = __builtin_amdgcn_exp2f(s.m - m0), g = __builtin_amdgcn_exp2f(t.m - m0);
-  // an offset of -inf has no keys, or only NaN scores: its sums count as they are
-  s.l = s.l * (s.m == -INFINITY ? 1.0f : f) + t.l * (t.m == -INFINITY ? 1.0f : g);
-  s.x = s.x * (s.m == -INFINITY ? 1.0f : f) + t.x * (t.m == -INFINITY ? 1.0f : g);
-  s.m = m;
-}
-
-// 4 dims of (packed row, query head) from d on; the row's log-sum-exp with d == 0.
-template <int DT>
-__device__ __forceinline__ void store_out(const mtk_kv_attn_kargs &a, int row, int h, int d, const KvPart &s) {
-  const float inv = s.l != 0.0f ? 1.0f / s.l : 0.0f;  // no key: 0; NaN stays
-  if (d < a.D)
-    *(u32x2 *)((uint16_t *)a.O + ((size_t)row * a.H + h) * a.D + d) =
-        u32x2{pack2<DT>(s.x.x * inv, s.x.y * inv), pack2<DT>(s.x.z * inv, s.x.w * inv)};
-  if (d == 0 && a.lse)
-    a.lse[(size_t)row * a.H + h] = s.l == 0.0f ? -INFINITY : (s.m == -INFINITY ? s.l : s.m + __builtin_amdgcn_logf(s.l)) * 0.6931471805599453f;
 }
 
 template <int DT, int FMT, int DP, int NR, int KB, int W>
@@ -531,88 +505,6 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
   }
 }
 
-// The partial sums of each (row, query head) of a pair that workgroups share, in an order that their number fixes.
-// A group of D / 4 lanes (4 dims each) adds parts, kAhead of them in flight at once.
-//   PARTS: a workgroup has one (row, query head); group g of NG adds every NGth part, the groups are added in turn. For
-//   few pairs of long sequences, which have many parts.
-//   else: each group has a query head of its own, a workgroup NG heads of a row.
-// Bound by latency (the lengths, the parts' statistics and the parts in turn): 4.6 us for 128 rows of heads, 7.0 for one row
-// of 32 heads in 128 parts each. runtime: plan_kv_attn has both sides of the choice.
-constexpr int kKvJoin = 256;  // threads
-template <int DT, bool PARTS>
-__device__ __forceinline__ void kv_join(const mtk_kv_attn_kargs &a) {
-  __shared__ f32x4 sm_x[PARTS ? kKvJoin : 1];
-  __shared__ f32x2 sm_ml[PARTS ? kKvJoin : 1];
-  __shared__ int sm_line[kKvJoin / 64][kLineWords];
-  const int tid = threadIdx.x, lane = tid & 63, G = a.G, rows = 1 << a.rows_shift;
-  const int chunks = a.part_ld / 4, groups = kKvJoin / chunks;
-  const int g = tid / chunks, d = 4 * (tid - g * chunks);
-  const int heads = PARTS ? 1 : groups, per_row = (a.H + heads - 1) / heads;  // items of a row
-  const int items = a.T * per_row, per = (items + gridDim.x - 1) / gridDim.x;
-  const int end = min(items, ((int)blockIdx.x + 1) * per);
-  int it = blockIdx.x * per;
-  if (it >= end) return;
-  KvLine<0, 0> line(a, lane, sm_line[tid >> 6]);
-  line.lay();
-  while (it < end) {  // uniform: every wavefront takes the same items
-    int t = it / per_row;
-    const int l = line.find_row(t);
-    if (l < 0) {
-      it = (t + 1) * per_row;
-      continue;
-    }
-    int length, base, pairs;
-    const KvSegment seq = line.sequence(l, length, base, pairs);
-    const int64_t past = (int64_t)(seq.seq.first + min(seq.seq.rows, a.S_q)) * per_row;
-    const int blocks = kv_div(pairs, a.H_kv);
-    const bool none = pairs == 0 || (line.cut.padded && length == line.cut.each);  // no pair is shared
-    for (; !none && it < min((int64_t)end, past); ++it) {
-      t = it / per_row;
-      const int h = (it - t * per_row) * heads + (PARTS ? 0 : g);
-      if (h >= a.H || g >= groups) continue;
-      const int hk = kv_div(h, G), r = (t - seq.seq.first) * G + h - hk * G, rb = r >> a.rows_shift;
-      const int start = base + ((a.by_pair ? blocks - 1 - rb : rb) * a.H_kv + hk) * length;
-      const int w0 = kv_div(start, line.cut.each), w1 = min(kv_div(start + seq.steps - 1, line.cut.each), a.places - 1);
-      if (w0 >= w1) continue;  // one workgroup's
-      const int first = start == w0 * line.cut.each ? 0 : 1;
-      KvPart sum;
-      constexpr int kAhead = 8;
-      const int step = PARTS ? groups : 1;
-      for (int s0 = w0 + (PARTS ? g : 0); s0 <= w1; s0 += kAhead * step) {
-        KvPart p[kAhead];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          const int w = s0 + i * step;
-          if (w <= w1) {
-            const size_t place = a.by_pair ? (size_t)w : (size_t)w * 2 + (w == w0 ? first : 0);
-            const size_t at = (place << a.rows_shift) + (r & (rows - 1));
-            const f32x2 ml = *(const f32x2 *)(a.part_ml + 2 * at);
-            p[i] = KvPart{ml.x, ml.y, *(const f32x4 *)(a.part + at * a.part_ld + d)};
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) add_part(sum, p[i]);
-      }
-      if constexpr (PARTS) {
-        __syncthreads();
-        sm_x[tid] = sum.x;
-        sm_ml[tid] = f32x2{sum.m, sum.l};
-        __syncthreads();
-        if (tid < chunks) {
-          for (int i = 1; i < min(groups, w1 - w0 + 1); ++i) {
-            const int k = tid + i * chunks;
-            add_part(sum, KvPart{sm_ml[k].x, sm_ml[k].y, sm_x[k]});
-          }
-          store_out<DT>(a, t, h, d, sum);
-        }
-      } else {
-        store_out<DT>(a, t, h, d, sum);
-      }
-    }
-    if (none || it >= past) it = max((int64_t)it, (int64_t)(seq.seq.first + seq.seq.rows) * per_row);
-  }
-}
-
 }  // namespace mtk
 
 using namespace mtk;
@@ -651,8 +543,11 @@ MTK_KV_ATTEND_W16(fp4, KV_FP4, 128, 2)
 MTK_KV_ATTEND_W16(fp8, KV_FP8, 64, 2)
 MTK_KV_ATTEND_W16(fp8, KV_FP8, 128, 2)
 
-#define MTK_KV_JOIN(NAME, DT, PARTS) \
-  extern "C" __global__ void __launch_bounds__(kKvJoin) NAME(const mtk_kv_attn_kargs a) { kv_join<DT, PARTS>(a); }
+#define MTK_KV_JOIN(NAME, DT, PARTS)                                                                   \
+  extern "C" __global__ void __launch_bounds__(kKvJoin) NAME(const mtk_kv_attn_kargs a) {             \
+    __shared__ int sm_line[kKvJoin / 64][kLineWords];                                                 \
+    kv_join<DT, PARTS>(a, blockIdx.x, gridDim.x, sm_line);                                            \
+  }
 MTK_KV_JOIN(mtk_kv_join_rows_f16, DT_F16, false)
 MTK_KV_JOIN(mtk_kv_join_rows_bf16, DT_BF16, false)
 MTK_KV_JOIN(mtk_kv_join_parts_f16, DT_F16, true)

@@ -155,46 +155,46 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
   size_t workspace = 0;
   std::string how;
   char name[96];
-  // The launches of one kernel; rows per block and keys per step as it has them.
-  auto add = [&](mtk_kv_attn_kargs k, const std::string &kernel, int rows, int step, int block, long long grid, bool split) {
+  // Partial sums of a launch with `grid` workgroups. Run-time pointers: offsets in the workspace until then.
+  auto partial_sums = [&](mtk_kv_attn_kargs &k, long long grid) {
+    k.places = (int)grid;
+    const size_t held = (size_t)grid * (k.by_pair ? 1 : 2) << k.rows_shift;
+    const size_t part = workspace, ml = part + held * k.part_ld * sizeof(float);
+    workspace = ml + held * 2 * sizeof(float);
+    k.part = (float *)part;
+    k.part_ml = (float *)ml;
+  };
+  // Workgroups that join them with the lanes over the heads, or in a launch of its own over the parts of each (row, head):
+  // where a pair has more than 8 parts and there are few (row, head)s to fill the device with. 1 x 131071 positions, 8 K/V heads:
+  // both kernels 35.5 us, over the heads 49.6; 4 x 8000: 17.6 and 20.1; but 4 x 2000 with 16 rows of 16 heads: 23.0 and 20.7,
+  // 16 x 8000: 35.9 and 34.6.
+  auto joins = [&](const mtk_kv_attn_kargs &k, bool parts, int most_wgs) {
+    const long long mine = k.by_pair ? d.T : std::min<long long>(d.T, (long long)d.B * std::max(1, k.rows_most / G));
+    const int heads = parts ? 1 : 1024 / k.part_ld;
+    return (int)std::min<long long>(mine * ((d.H + heads - 1) / heads), most_wgs);
+  };
+  auto add = [&](const std::string &kernel, long long grid, int block, const auto &args) {
     Launch g;
     g.name = kernel;
     g.grid = (unsigned)grid;
     g.block = (unsigned)block;
-    k.rows_shift = __builtin_ctz((unsigned)rows);
-    k.step_shift = __builtin_ctz((unsigned)step);
-    k.places = split ? (int)grid : 0;
-    if (split) {  // run-time pointers: offsets in the workspace until then
-      const size_t held = (size_t)grid * (k.by_pair ? 1 : 2) * rows;
-      const size_t part = workspace, ml = part + held * k.part_ld * sizeof(float);
-      workspace = ml + held * 2 * sizeof(float);
-      k.part = (float *)part;
-      k.part_ml = (float *)ml;
-    }
-    set_args(g, k);
+    set_args(g, args);
     launches.push_back(g);
+  };
+  auto add_join = [&](const mtk_kv_attn_kargs &k, bool parts) {
+    add(std::string(parts ? "mtk_kv_join_parts_" : "mtk_kv_join_rows_") + kv_suffix(d), joins(k, parts, 8 * cus), 256, k);
+  };
+  auto tell = [&](int rows, long long grid, bool split) {
     char text[96];
     snprintf(text, sizeof text, " rows/wg=%d grid=%lld%s", rows, grid, split ? " keys split" : "");
     how += text;
-    if (split) {
-      // The join's lanes: over the parts of each (row, head) where a pair has more than 8 parts and there are few (row, head)s
-      // to fill the device with, else over the heads. 1 x 131071 positions, 8 K/V heads: both kernels 35.5 us, over the heads
-      // 49.6; 4 x 8000: 17.6 and 20.1; but 4 x 2000 with 16 rows of 16 heads: 23.0 and 20.7, 16 x 8000: 35.9 and 34.6.
-      const long long mine = k.by_pair ? d.T : std::min<long long>(d.T, (long long)d.B * std::max(1, k.rows_most / G));
-      const bool parts = !k.by_pair && (long long)d.B * d.H_kv * 8 < grid && mine * d.H < 2LL * cus;
-      const int heads = parts ? 1 : 1024 / k.part_ld;
-      Launch c = g;
-      c.name = std::string(parts ? "mtk_kv_join_parts_" : "mtk_kv_join_rows_") + kv_suffix(d);
-      c.block = 256;
-      c.grid = (unsigned)std::min<long long>(mine * ((d.H + heads - 1) / heads), 8LL * cus);
-      launches.push_back(c);
-    }
   };
   auto too_large = [&](long long blocks, long long steps) {
     return blocks >= (1 << 23) || blocks * steps > INT32_MAX
                ? fail(MTK_ERR_UNSUPPORTED, "a batch of %lld row blocks over %lld positions is not supported", blocks, positions)
                : MTK_OK;
   };
+  mtk_kv_attn_kargs k = a;  // of the sequences with few rows
   if (few) {
     const int nr = few <= 16 ? 1 : few <= 32 || dp == 256 ? 2 : 4, rows = 16 * nr;
     // Few pairs of short sequences: one workgroup of 16 wavefronts each, no second kernel. 1000 positions, 8 pairs: 9.2 us
@@ -203,9 +203,10 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
     const long long blocks = (long long)d.B * d.H_kv;
     const bool wide = nr == 1 && dp <= 128 && blocks <= cus && positions <= (2 * blocks >= cus ? 4096 : 2048);
     const KvShape shape = wide ? KvShape{32, 16, 1} : kv_kernel_shape(d.format, dp, nr);
-    mtk_kv_attn_kargs k = a;
     k.rows_above = 0;
     k.rows_most = rows;
+    k.rows_shift = __builtin_ctz((unsigned)rows);
+    k.step_shift = __builtin_ctz((unsigned)shape.step());
     k.units = cus * shape.per_cu;
     k.least = 2;  // 1 x 16000: 14.7 us, least 1: 16.9; 4 x 2000 with 16 rows: 23.0, least 4: 25.1
     const long long steps = (positions + shape.step() - 1) / shape.step();
@@ -213,26 +214,43 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
     // 64 x 1000: whole pairs 16.3 us, split 22.1; 64 x 2000 (512 pairs): 28.3 and 32.5; 8 x 4000 with 16 rows: 80 and 34
     k.whole = wide || positions <= (blocks >= 2 * cus ? 2048 : 1024) ? 1 : 0;
     snprintf(name, sizeof name, "mtk_kv_attend_%s_d%d_r%d_%s%s", kv_format(d), dp, nr, wide ? "w16_" : "", kv_suffix(d).c_str());
-    add(k, name, rows, shape.step(), 64 * shape.waves, k.whole ? blocks : k.units, !k.whole);
+    const long long grid = k.whole ? blocks : k.units;
+    if (!k.whole) partial_sums(k, grid);
+    add(name, grid, 64 * shape.waves, k);
+    tell(rows, grid, !k.whole);
+    if (!k.whole && pairs <= most) add_join(k, blocks * 8 < grid && (long long)joins(k, true, INT32_MAX) < 2LL * cus);
   }
   if (pairs > most) {
     const int rows = 128, step = 64;
-    mtk_kv_attn_kargs k = a;
-    k.rows_above = few ? 16 * (few <= 16 ? 1 : few <= 32 || dp == 256 ? 2 : 4) : 0;
-    k.rows_most = INT32_MAX;
-    k.by_pair = 1;
-    k.units = cus * (dp == 256 ? 1 : 2);
+    mtk_kv_prefill_kargs both{};
+    mtk_kv_attn_kargs &r = both.rows;
+    r = a;
+    r.rows_above = few ? k.rows_most : 0;
+    r.rows_most = INT32_MAX;
+    r.by_pair = 1;
+    r.units = cus * (dp == 256 ? 1 : 2);
     const long long each = (long long)d.B * ((pairs + rows - 1) / rows) * d.H_kv;  // blocks, whatever row_start holds
     const long long blocks = kv_max_blocks(d.B, d.T, d.S_q, G, rows) * d.H_kv, steps = (positions + step - 1) / step;
     // Fewer blocks than workgroups: the keys are split, into 4 steps (256 keys) or more, so that all workgroups are on the
     // device at once; else never. 300 rows of 8 heads of 64 dims, 1000 positions: 17.8 us, 8 steps 22.6, 2 steps 16.8;
     // 2 x 4000 positions, 100 rows, 256 dims: 47.4, 54.8 and 47.3, with shares of equal work (two rounds) 51.3, unsplit 215.
-    const bool split = blocks < k.units && steps > 4;
-    k.least = split ? 4 : (int)steps;
-    if ((s = too_large(each, 3 * steps + k.least)) != MTK_OK) return s;
-    const long long grid = split ? k.units : blocks;
+    const bool split = blocks < r.units && steps > 4;
+    r.least = split ? 4 : (int)steps;
+    if ((s = too_large(each, 3 * steps + r.least)) != MTK_OK) return s;
+    r.rows_shift = __builtin_ctz((unsigned)rows);
+    r.step_shift = __builtin_ctz((unsigned)step);
+    const long long grid = split ? r.units : blocks;
+    if (split) partial_sums(r, grid);
+    // The sums that the launch before has left are joined by this one's first workgroups, at most one per CU: a launch
+    // less (5 to 6 us), and they run beside the others.
+    if (k.places) {
+      both.join = k;
+      both.joins = joins(k, false, cus);
+    }
     snprintf(name, sizeof name, "mtk_kv_prefill_%s_d%d_%s", kv_format(d), dp, kv_suffix(d).c_str());
-    add(k, name, rows, step, 256, grid, split);
+    add(name, grid + both.joins, 256, both);
+    tell(rows, grid, split);
+    if (split) add_join(r, false);
   }
   mtk_plan *p = new mtk_plan();
   p->ctx = ctx;
@@ -312,19 +330,22 @@ int check_kv_args(const mtk_plan *p, const void *argset) {
 }
 
 // Writes the run-time pointers of a launch into `block`, a copy of its argument block.
-void patch_kv(const mtk_plan *p, const Launch &, char *block, const void *argset) {
+void patch_kv(const mtk_plan *p, const Launch &l, char *block, const void *argset) {
   if (p->kind == PLAN_KV_ATTN) {
     const mtk_kv_attn_args *t = (const mtk_kv_attn_args *)argset;
-    mtk_kv_attn_kargs &a = *(mtk_kv_attn_kargs *)block;
-    a.Q = t->Q;
-    a.cache = t->cache;
-    a.row_start = t->row_start;
-    a.kv_len = t->kv_len;
-    a.table = t->table;
-    a.O = t->O;
-    a.lse = t->lse;
-    a.part = (float *)((uintptr_t)a.part + (uintptr_t)t->workspace);
-    a.part_ml = (float *)((uintptr_t)a.part_ml + (uintptr_t)t->workspace);
+    mtk_kv_attn_kargs *const all = (mtk_kv_attn_kargs *)block;  // two of them: mtk_kv_prefill_kargs
+    for (int i = 0; i < (l.args.size() == sizeof(mtk_kv_prefill_kargs) ? 2 : 1); ++i) {
+      mtk_kv_attn_kargs &a = all[i];
+      a.Q = t->Q;
+      a.cache = t->cache;
+      a.row_start = t->row_start;
+      a.kv_len = t->kv_len;
+      a.table = t->table;
+      a.O = t->O;
+      a.lse = t->lse;
+      a.part = (float *)((uintptr_t)a.part + (uintptr_t)t->workspace);
+      a.part_ml = (float *)((uintptr_t)a.part_ml + (uintptr_t)t->workspace);
+    }
     return;
   }
   mtk_kv_move_kargs &a = *(mtk_kv_move_kargs *)block;

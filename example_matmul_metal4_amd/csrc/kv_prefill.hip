@@ -18,7 +18,7 @@
 // reaches 0.93 at such sizes. With the key-splitting kernels such a chunk took 644 us. Converting a tile during the
 // second product instead of the first made no difference. 500 rows of 24 heads, 8 K/V heads of 96 dims, 4000 positions, with a
 // join: 53.8 us, with shares of equal work, which need two rounds of workgroups, 68, unsplit 101.
-#include "kv_device.hpp"
+#include "kv_join.hpp"
 
 namespace mtk {
 
@@ -28,7 +28,8 @@ constexpr int kPfRows = 128;
 __device__ __forceinline__ int pf_key_order(int m) { return (m & ~12) | ((m & 4) << 1) | ((m & 8) >> 1); }
 
 template <int DT, int FMT, int DP>
-__device__ __forceinline__ void kv_prefill(const mtk_kv_attn_kargs &a) {
+__device__ __forceinline__ void kv_prefill(const mtk_kv_prefill_kargs &args) {
+  const mtk_kv_attn_kargs &a = args.rows;
   constexpr int kRowB = DP * 2, kTile = kPfKeys * kRowB;
   constexpr int kKs = DP / 16, kDb = DP / 32;
   constexpr int kEl = DP == 64 ? 16 : 32;                 // dims of a thread's item
@@ -43,6 +44,11 @@ __device__ __forceinline__ void kv_prefill(const mtk_kv_attn_kargs &a) {
   __shared__ int sm_nan;                                  // there was one
   __shared__ int sm_line[4][kLineWords];
 
+  if ((int)blockIdx.x < args.joins) {
+    kv_join<DT, false>(args.join, blockIdx.x, args.joins, sm_line);
+    return;
+  }
+
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, col = lane & 31, G = a.G;
@@ -51,7 +57,7 @@ __device__ __forceinline__ void kv_prefill(const mtk_kv_attn_kargs &a) {
 
   KvLine<kPfRows, kPfKeys> line(a, lane, sm_line[wave]);
   line.lay();
-  const int wg = blockIdx.x;
+  const int wg = (int)blockIdx.x - args.joins;
   const int64_t line_from = (int64_t)wg * line.cut.each;  // past the line's end, which 32 bits hold, for workgroups of no share
   if (line_from > INT32_MAX - line.cut.each) return;
   KvSegment seg = line.at((int)line_from, (int)line_from + line.cut.each);
@@ -400,7 +406,7 @@ using namespace mtk;
 // mtk_kv_prefill_<format>_d<padded head dimension>_<type>: two workgroups per CU, or one (D above 128)
 #define MTK_KV_PREFILL(NAME, DT, FMT, DP, EU)                                                       \
   extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(EU, EU)))   \
-  NAME(const mtk_kv_attn_kargs a) { kv_prefill<DT, FMT, DP>(a); }
+  NAME(const mtk_kv_prefill_kargs a) { kv_prefill<DT, FMT, DP>(a); }
 #define MTK_KV_PREFILL_DP(DP, EU)                                          \
   MTK_KV_PREFILL(mtk_kv_prefill_fp4_d##DP##_f16, DT_F16, KV_FP4, DP, EU)   \
   MTK_KV_PREFILL(mtk_kv_prefill_fp4_d##DP##_bf16, DT_BF16, KV_FP4, DP, EU) \

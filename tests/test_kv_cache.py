@@ -138,7 +138,7 @@ static int failures = 0;
 
 // What the kernels of a launch do with a batch (kv_device.hpp: lay, at), with the functions that they share with the
 // host: how often each step of each pair is taken, and the places of partial sums.
-static void schedule(const mtk_kv_attn_kargs &k, const Launch &l, const std::vector<int> &start, const std::vector<int> &len,
+static void schedule(const mtk_kv_attn_kargs &k, unsigned grid, const std::vector<int> &start, const std::vector<int> &len,
                      bool sane) {
   struct Pairs { kv_share h; int base, length; };
   std::vector<Pairs> seqs;
@@ -173,7 +173,7 @@ static void schedule(const mtk_kv_attn_kargs &k, const Launch &l, const std::vec
   }
   else cut = kv_cut_of((int)work, (int)own, k.units, k.least);
   if (k.whole && !k.by_pair) {  // by the workgroup's number
-    CHECK(l.grid == (unsigned)(k.B * k.H_kv), "grid %u", l.grid);
+    CHECK(grid == (unsigned)(k.B * k.H_kv), "grid %u", grid);
     for (auto &s : seqs) CHECK(s.h.blocks <= 1, "blocks %d", s.h.blocks);
     return;
   }
@@ -186,7 +186,7 @@ static void schedule(const mtk_kv_attn_kargs &k, const Launch &l, const std::vec
   CHECK(total <= INT32_MAX, "line of %lld", (long long)total);
   const int64_t wgs = (total + cut.each - 1) / cut.each;
   if (!sane && k.by_pair) return;  // rows claimed twice: workgroups past the grid are not there, and write nothing
-  CHECK(wgs <= (int64_t)l.grid, "%lld workgroups, grid %u", (long long)wgs, l.grid);
+  CHECK(wgs <= (int64_t)grid, "%lld workgroups, grid %u", (long long)wgs, grid);
   if (k.places) CHECK(wgs <= k.places, "%lld workgroups, %d places", (long long)wgs, k.places);
   for (auto &s : seqs)
     for (int p = 0; p < s.h.blocks * k.H_kv; ++p) {
@@ -200,8 +200,8 @@ static void schedule(const mtk_kv_attn_kargs &k, const Launch &l, const std::vec
     }
 }
 
-static size_t part_bytes(const Launch &l, const mtk_kv_attn_kargs &k) {
-  return (size_t)l.grid * (k.by_pair ? 1 : 2) * (1u << k.rows_shift);
+static size_t part_rows(const mtk_kv_attn_kargs &k) {
+  return (size_t)k.places * (k.by_pair ? 1 : 2) * (1u << k.rows_shift);
 }
 
 int main() {
@@ -227,20 +227,37 @@ int main() {
     for (int b = 0; b <= d.B; ++b) start[b] = sane ? (int)(rng() % (d.T + 1)) : (int)rng();
     if (sane) std::sort(start.begin(), start.end());
     for (int b = 0; b < d.B; ++b) len[b] = rng() % 5 == 0 ? (sane ? 0 : (int)rng()) : log(1, (int)cap + 1);
+    const mtk_kv_attn_kargs *before = nullptr;  // whose partial sums are not joined yet
     for (Launch &l : p->launches) {
       names.insert(l.name);
       const mtk_kv_attn_kargs &k = args_of<mtk_kv_attn_kargs>(l);
-      if (l.name.find("join") != std::string::npos) continue;
+      if (l.name.find("join") != std::string::npos) {  // after its launch
+        CHECK(before && before->places > 0 && memcmp(&k, before, sizeof k) == 0, "%s", p->description.c_str());
+        before = nullptr;
+        continue;
+      }
+      unsigned grid = l.grid;
+      if (l.name.find("prefill") != std::string::npos) {  // joins the sums of the launch before it, if there are any
+        const mtk_kv_prefill_kargs &both = args_of<mtk_kv_prefill_kargs>(l);
+        CHECK((both.joins > 0) == (before && before->places > 0), "%d joins", both.joins);
+        if (both.joins) CHECK(memcmp(&both.join, before, sizeof k) == 0, "%s", p->description.c_str());
+        grid -= both.joins;
+        before = nullptr;
+      }
+      CHECK(!before || before->places == 0, "%s", p->description.c_str());
+      before = k.places ? &k : nullptr;
+      CHECK(!k.places || (unsigned)k.places == grid, "%d places", k.places);
       if (k.places) {  // partial sums, then their statistics, one launch's after another's
-        const size_t rows = part_bytes(l, k);
+        const size_t rows = part_rows(k);
         CHECK((size_t)k.part == used && used % 16 == 0 && (size_t)k.part_ml % 8 == 0, "%s", p->description.c_str());
         CHECK((size_t)k.part + rows * k.part_ld * 4 <= (size_t)k.part_ml, "%s", p->description.c_str());
         used = (size_t)k.part_ml + rows * 8;
         CHECK(k.part_ld >= d.D && k.part_ld % 4 == 0, "%d", k.part_ld);
         ++split;
       }
-      schedule(k, l, start, len, sane);
+      schedule(k, grid, start, len, sane);
     }
+    CHECK(!before, "%s", p->description.c_str());
     CHECK(used <= p->workspace, "%zu of %zu", used, p->workspace);
     mtk_plan_destroy(p);
   }
