@@ -112,11 +112,18 @@ MTK_KV_FN kv_cut kv_cut_of(int work, int own, int units, int least) {
   return c;
 }
 
-// Launches whose workgroups have one pair each (by_pair): shares of `each` steps of it, at least `least` and no more than
-// `most`, the steps of a full table. With `each` of this or more there are at most `units` workgroups: pairs ceil their
-// steps / each, which adds less than 1 for each. own: the pairs; where they are `units` or more, each has one workgroup.
+// Launches whose workgroups have one pair each (by_pair). own: the pairs. Whether they have more than one workgroup each: not
+// where they are `units` or more, nor where two shares of one, of KV_FEW_STEPS or less on average, gain less than the join costs
+// (2 x 500 rows of 32 heads, 8 K/V heads: 32 steps 73.9 us whole, 76.9 in two shares; 48 steps 90.5 and 88.7; 64 113.6 and 103.4).
+#define KV_FEW_STEPS 40
+MTK_KV_FN int kv_pairs_split(int work, int own, int units) {
+  return own < units && (own <= units / 3 || work > KV_FEW_STEPS * own);
+}
+
+// Steps of a share, at least `least` and no more than `most`, the steps of a full table. With this or more there are at most
+// `units` workgroups: pairs ceil their steps / each, which adds less than 1 for each.
 MTK_KV_FN int kv_each_of_pairs(int work, int own, int units, int least, int most) {
-  int each = own < units ? kv_div(work + (units - own) - 1, units - own) : most;
+  int each = kv_pairs_split(work, own, units) ? kv_div(work + (units - own) - 1, units - own) : most;
   if (each > most) each = most;
   return each < least ? least : each;
 }

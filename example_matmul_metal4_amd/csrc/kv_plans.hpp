@@ -181,8 +181,9 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
     set_args(g, args);
     launches.push_back(g);
   };
+  // At most 4 workgroups per CU, which are there at once: 2 x 500 rows of 32 heads in two parts 16.8 us, 8 per CU 19.6, 2 17.9.
   auto add_join = [&](const mtk_kv_attn_kargs &k, bool parts) {
-    add(std::string(parts ? "mtk_kv_join_parts_" : "mtk_kv_join_rows_") + kv_suffix(d), joins(k, parts, 8 * cus), 256, k);
+    add(std::string(parts ? "mtk_kv_join_parts_" : "mtk_kv_join_rows_") + kv_suffix(d), joins(k, parts, 4 * cus), 256, k);
   };
   auto tell = [&](int rows, long long grid, bool split) {
     char text[96];
@@ -234,15 +235,16 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
     // Fewer blocks than workgroups: the keys are split, into 4 steps (256 keys) or more, so that all workgroups are on the
     // device at once; else never. 300 rows of 8 heads of 64 dims, 1000 positions: 17.8 us, 8 steps 22.6, 2 steps 16.8;
     // 2 x 4000 positions, 100 rows, 256 dims: 47.4, 54.8 and 47.3, with shares of equal work (two rounds) 51.3, unsplit 215.
-    const bool split = blocks < r.units && steps > 4;
+    // Decided on the device; here only whether the blocks may be so few, each sequence's last one aside.
+    const bool split = std::min(blocks, (long long)d.T * G / rows * d.H_kv) < r.units && steps > 4;
     r.least = split ? 4 : (int)steps;
     if ((s = too_large(each, 3 * steps + r.least)) != MTK_OK) return s;
     r.rows_shift = __builtin_ctz((unsigned)rows);
     r.step_shift = __builtin_ctz((unsigned)step);
-    const long long grid = split ? r.units : blocks;
-    if (split) partial_sums(r, grid);
-    // The sums that the launch before has left are joined by this one's first workgroups, at most one per CU: a launch
-    // less (5 to 6 us), and they run beside the others.
+    const long long grid = split ? std::max<long long>(r.units, blocks) : blocks;
+    if (split) partial_sums(r, r.units);
+    // The sums that the launch before has left are joined by this one's first workgroups, at most one per CU, beside the
+    // others: 500 rows at 4000 positions and 31 tokens at 8000 106.6 us, with a launch of their own 112.8.
     if (k.places) {
       both.join = k;
       both.joins = joins(k, false, cus);

@@ -164,7 +164,7 @@ static void schedule(const mtk_kv_attn_kargs &k, unsigned grid, const std::vecto
       return n;
     };
     CHECK(wgs_of(hi) <= std::max<int64_t>(k.units, pairs), "each %d", hi);
-    if (k.B <= 64)
+    if (k.B <= 64 && kv_pairs_split((int)work, (int)pairs, k.units))
       for (int lo = std::min(hi, std::max<int>(k.least, (work + k.units - 1) / k.units)); lo < hi;) {
         const int mid = (lo + hi) >> 1;
         wgs_of(mid) <= k.units ? hi = mid : lo = mid + 1;
@@ -187,11 +187,12 @@ static void schedule(const mtk_kv_attn_kargs &k, unsigned grid, const std::vecto
   const int64_t wgs = (total + cut.each - 1) / cut.each;
   if (!sane && k.by_pair) return;  // rows claimed twice: workgroups past the grid are not there, and write nothing
   CHECK(wgs <= (int64_t)grid, "%lld workgroups, grid %u", (long long)wgs, grid);
-  if (k.places) CHECK(wgs <= k.places, "%lld workgroups, %d places", (long long)wgs, k.places);
+  if (k.places && !k.by_pair) CHECK(wgs <= k.places, "%lld workgroups, %d places", (long long)wgs, k.places);
   for (auto &s : seqs)
     for (int p = 0; p < s.h.blocks * k.H_kv; ++p) {
       const int64_t at = s.base + (int64_t)p * s.length;
       if (k.by_pair) CHECK(at % cut.each == 0 && s.length % cut.each == 0, "pair at %lld", (long long)at);
+      if (k.by_pair && s.h.steps > cut.each) CHECK((at + s.h.steps - 1) / cut.each < k.places, "place of %lld", (long long)at);
       if (!k.places) CHECK(at / cut.each == (at + s.h.steps - 1) / cut.each, "a pair of several workgroups without a workspace");
       CHECK(s.length >= s.h.steps && s.length < s.h.steps + cut.each, "length %d of %d", s.length, s.h.steps);
       // at most two pairs of a workgroup are shared: its first and its last
@@ -246,7 +247,7 @@ int main() {
       }
       CHECK(!before || before->places == 0, "%s", p->description.c_str());
       before = k.places ? &k : nullptr;
-      CHECK(!k.places || (unsigned)k.places == grid, "%d places", k.places);
+      CHECK(!k.places || (unsigned)k.places == grid || (k.by_pair && (unsigned)k.places < grid), "%d places", k.places);
       if (k.places) {  // partial sums, then their statistics, one launch's after another's
         const size_t rows = part_rows(k);
         CHECK((size_t)k.part == used && used % 16 == 0 && (size_t)k.part_ml % 8 == 0, "%s", p->description.c_str());
