@@ -184,7 +184,7 @@ typedef struct {
   int32_t part_ld; /* floats per row of part */
 } mtk_kv_attn_kargs;
 
-/* Attention of sequences with many rows; its first `joins` workgroups join the partial sums that the launch before it, of
+/* Attention of sequences with many rows; its last `joins` workgroups join the partial sums that the launch before it, of
  * the sequences with few rows (join), has left. */
 typedef struct {
   mtk_kv_attn_kargs rows, join;

@@ -114,8 +114,9 @@ MTK_KV_FN kv_cut kv_cut_of(int work, int own, int units, int least) {
 
 // Launches whose workgroups have one pair each (by_pair). own: the pairs. Whether they have more than one workgroup each: not
 // where they are `units` or more, nor where two shares of one, of KV_FEW_STEPS or less on average, gain less than the join costs
-// (2 x 500 rows of 32 heads, 8 K/V heads: 32 steps 73.9 us whole, 76.9 in two shares; 48 steps 90.5 and 88.7; 64 113.6 and 103.4).
-#define KV_FEW_STEPS 40
+// (32 heads, 8 K/V heads of 128 dims, 500 rows in 2 sequences each: 16 steps 38.1 us whole, 47.2 in two shares; 24 steps 49.7 and
+// 54.1; 32 steps 61.1 and 61.2; 200 rows in 4: 39.3 and 45.7, 51.1 and 52.6, 62.9 and 59.1).
+#define KV_FEW_STEPS 28
 MTK_KV_FN int kv_pairs_split(int work, int own, int units) {
   return own < units && (own <= units / 3 || work > KV_FEW_STEPS * own);
 }

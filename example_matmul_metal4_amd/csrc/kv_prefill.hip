@@ -14,8 +14,8 @@
 //   * Few row blocks: the keys are split over workgroups (kv_cache.h), whose partial sums kv_join adds.
 //
 // Bound by the matrix units and the VALU beside them (the exponentials, and the conversions of a tile, shared by 128 pairs):
-// 2048 rows of 32 heads of 128 dims behind 6144 positions 274 us, 0.88 PFLOP/s, where the 16-bit kernel of attention.hpp
-// reaches 0.93 at such sizes. With the key-splitting kernels such a chunk took 644 us. Converting a tile during the
+// 2048 rows of 32 heads of 128 dims behind 6144 positions 249 us, 0.97 PFLOP/s (274 to 290 under a profiler), where the 16-bit
+// kernel of attention.hpp reaches 0.93 at such sizes. With the key-splitting kernels such a chunk took 644 us. Converting a tile during the
 // second product instead of the first made no difference. 500 rows of 24 heads, 8 K/V heads of 96 dims, 4000 positions, with a
 // join: 53.8 us, with shares of equal work, which need two rounds of workgroups, 68, unsplit 101.
 #include "kv_join.hpp"
@@ -44,8 +44,9 @@ __device__ __forceinline__ void kv_prefill(const mtk_kv_prefill_kargs &args) {
   __shared__ int sm_nan;                                  // there was one
   __shared__ int sm_line[4][kLineWords];
 
-  if ((int)blockIdx.x < args.joins) {
-    kv_join<DT, false>(args.join, blockIdx.x, args.joins, sm_line);
+  const int wg = blockIdx.x, others = (int)gridDim.x - args.joins;
+  if (wg >= others) {
+    kv_join<DT, false>(args.join, wg - others, args.joins, sm_line);
     return;
   }
 
@@ -57,7 +58,6 @@ __device__ __forceinline__ void kv_prefill(const mtk_kv_prefill_kargs &args) {
 
   KvLine<kPfRows, kPfKeys> line(a, lane, sm_line[wave]);
   line.lay();
-  const int wg = (int)blockIdx.x - args.joins;
   const int64_t line_from = (int64_t)wg * line.cut.each;  // past the line's end, which 32 bits hold, for workgroups of no share
   if (line_from > INT32_MAX - line.cut.each) return;
   KvSegment seg = line.at((int)line_from, (int)line_from + line.cut.each);

@@ -223,6 +223,20 @@ def test_shared_pages_and_long_tables(dev):
     g.free()
 
 
+@pytest.mark.parametrize("tokens, D, fmt, dtype", [(3, 64, "fp4", "f16"), (70, 64, "fp8", "bf16"), (9, 256, "fp4", "bf16")])
+def test_tokens_beside_a_chunk(dev, tokens, D, fmt, dtype):
+    # single tokens whose keys are split, joined in the chunk's launch; a chunk whose keys are split; one in the middle of the
+    # batch, rows of no sequence between
+    rng = rng_of(54)
+    half = tokens // 2
+    lens = [int(x) for x in rng.integers(900, 1400, half)] + [1500] + [int(x) for x in rng.integers(1, 1400, tokens - half)]
+    g = Given(dev, 55, lens, [1] * half + [80] + [1] * (tokens - half), 8, 2, D, 16, fmt, dtype, n_pages=100, width=200)
+    d = g.plan().describe()
+    assert "prefill" in d and d.count("keys split") == 2 and d.count("join") == 1
+    g.check()
+    g.free()
+
+
 def test_offsets_past_32_bits(dev):
     # pages whose bytes lie past 2^32 in the cache: 280000 of 17408 bytes, 4.9 GB
     H_kv, D, page = 8, 128, 16
