@@ -4,7 +4,7 @@
 //   O[i][h] = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(q_i . k_j / sqrt(D)),  j <= position of row i (causal)
 //
 // with k_j, v_j the cached values. One pass over the keys with a running exponent offset and sum per row (fp32).
-//   * The wavefronts of a workgroup (4, 8 or 16) take tiles of 16 KB keys in turn for the same 16 NR (row, query head) pairs
+//   * The wavefronts of a workgroup (4, 8 or 16) take tiles of 32 or 64 keys in turn for the same 16 NR (row, query head) pairs
 //     of a K/V head. Where a sequence's pairs are few enough for one workgroup each (runtime: plan_kv_attn), that is all;
 //     else the steps of all pairs lie on a line that persistent workgroups share evenly (kv_cache.h), found on the device
 //     from the lengths, so that a captured launch serves any lengths. fp8, 16 x 8192 ragged positions: equal splits of each
@@ -15,15 +15,15 @@
 //   * S^T leaves each lane with 4 keys of one row per 16 keys, which is the operand layout of P^T in
 //     O^T = V^T P^T. V^T needs 8 keys of one dim per lane: V is converted the same way, written to the
 //     wavefront's own LDS tile and read back transposed (ds_read_b64_tr_b16).
-//   * P is rounded to the 16-bit type for the MFMA (2^-9 or 2^-12 of its value, averaged over the keys); scores,
+//   * P is rounded to the 16-bit type for the MFMA (off by up to 2^-8 or 2^-11 of its value, averaged over the keys); scores,
 //     offsets and sums stay in fp32.
 //   * Keys past the length have their V codes zeroed (a page's unused rows may hold anything); a NaN block's V is
 //     zeroed too and its dims set to NaN only for the rows that see the key, so that nothing masked reaches O.
 //
 // Bound: HBM where there is much to read, else latency. A wavefront's loads of the next tile are issued as its registers
 // fall free (K and scales before the softmax, V after its codes are staged); nothing spills, for scratch traffic cost more
-// than a third wavefront per SIMD won (fp8, 128 dims: 3 per SIMD 49.7 us, 4 with spills 58.7). Loads of the head's last,
-// half-empty block behind a branch: without it 31.7 -> 33.0 us. Loads that bypass the caches: 5 % faster on one long
+// than a third wavefront per SIMD won (fp8, 128 dims: 3 per SIMD 49.7 us, 4 with spills 58.7). The next tile's loads are
+// behind a branch: issued always, with an empty range past the last one, 33.0 us instead of 31.7. Loads that bypass the caches: 5 % faster on one long
 // sequence, 12 to 18 % slower where sequences share pages. Scales as whole words: 64 dims 41.4 -> 36.5 us.
 // Measured, fp4, 8 K/V heads of 128 dims, 4 query heads each, first kernel and join: 1 x 131071 positions 31.7 + 7.0 us
 // (4.5 TB/s in the first), 64 x 6000 82 + 7 (5.1 TB/s), 32 x 4096 ragged 21.8, 1 x 1000 8.8 (0.8 to find its work, 1.6 for

@@ -72,8 +72,8 @@ MTK_KV_FN int kv_div(int x, int d) {
 }
 
 // Who does what in attention. A sequence has `blocks` blocks of 2^rows_shift (row, query head) pairs for each K/V head,
-// and `steps` steps of 2^step_shift keys (at least one). The (block, head) pairs of all sequences, sequence after sequence, lie on a
-// line; workgroup w has the steps from w * each to (w + 1) * each of it, so that all of them have the same work, whatever
+// and `steps` steps of 2^step_shift keys (at least one). The (block, head) pairs of all sequences, one sequence after another,
+// lie on a line; workgroup w has the steps from w * each to (w + 1) * each of it, so that all of them have the same work, whatever
 // the lengths. A pair that a boundary cuts leaves partial sums.
 //   each = max(least, work / units), so that there are at most `units` workgroups.
 // Where so little work is left that pairs of their own workgroups (ceil(steps / least) each) are no more than `units`,

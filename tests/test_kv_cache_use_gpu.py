@@ -230,7 +230,7 @@ def test_tokens_beside_a_chunk(dev, tokens, D, fmt, dtype):
     rng = rng_of(54)
     half = tokens // 2
     lens = [int(x) for x in rng.integers(900, 1400, half)] + [1500] + [int(x) for x in rng.integers(1, 1400, tokens - half)]
-    g = Given(dev, 55, lens, [1] * half + [80] + [1] * (tokens - half), 8, 2, D, 16, fmt, dtype, n_pages=100, width=200)
+    g = Given(dev, 55, lens, [1] * half + [80] + [1] * (tokens - half), 8, 2, D, 16, fmt, dtype, n_pages=100, width=300)
     d = g.plan().describe()
     assert "prefill" in d and d.count("keys split") == 2 and d.count("join") == 1
     g.check()
