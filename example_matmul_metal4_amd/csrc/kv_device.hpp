@@ -4,6 +4,7 @@
 
 #include "device.hpp"
 #include "kv_cache.h"
+#include "kv_walk.hpp"
 
 namespace mtk {
 
@@ -54,6 +55,13 @@ __device__ __forceinline__ int wave_scan(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
   x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
   return x;
+}
+
+// Minimum over the lanes.
+__device__ __forceinline__ int wave_min(int x) {
+#pragma unroll
+  for (int i = 1; i < 64; i *= 2) x = min(x, __shfl_xor(x, i));
+  return __builtin_amdgcn_readfirstlane(x);
 }
 
 template <typename A>
@@ -137,12 +145,13 @@ struct KvLine {
     total = cut.padded ? own * a.least : work;
     place(s, h);
   }
-  __device__ __forceinline__ void next() {  // the next 64
-    before = __builtin_amdgcn_readfirstlane(sm[63]);
-    b0 += 64;
+  __device__ __forceinline__ void show(int first, int starts) {  // the 64 sequences from `first` on, whose pairs start there
+    b0 = first;
+    before = starts;
     const kv_seq s = load_seq(a, b0 + lane);
     place(s, share_of(s));
   }
+  __device__ __forceinline__ void next() { show(b0 + 64, __builtin_amdgcn_readfirstlane(sm[63])); }
   // The lane of the sequence that pos falls into, or -1. pos ascends from call to call.
   __device__ __forceinline__ int find(int pos) {
     for (;;) {
@@ -152,15 +161,25 @@ struct KvLine {
       next();
     }
   }
-  // The lane of the sequence that packed row t belongs to, or -1. t ascends from call to call.
-  __device__ __forceinline__ int find_row(int t) {
-    for (;;) {
-      const int first = sm[64 + lane];
-      const uint64_t in = __ballot(b0 + lane < a.B && first <= t && t < first + sm[128 + lane]);
-      if (in) return __builtin_amdgcn_readfirstlane(__builtin_ctzll(in));
-      if (b0 + 64 >= a.B) return -1;
+  // ---- as a view of kv_walk
+  __device__ __forceinline__ int windows() const { return (a.B + 63) >> 6; }
+  __device__ __forceinline__ int hit(int t) const {
+    const int first = sm[64 + lane];
+    const uint64_t in = __ballot(b0 + lane < a.B && first <= t && t < first + sm[128 + lane]);
+    return in ? __builtin_amdgcn_readfirstlane(__builtin_ctzll(in)) : -1;
+  }
+  __device__ __forceinline__ int later(int t) const {
+    const int first = sm[64 + lane];
+    return wave_min(b0 + lane < a.B && first > t && sm[128 + lane] > 0 ? first : INT32_MAX);
+  }
+  __device__ __forceinline__ void step() {
+    if (b0 + 64 < a.B)
       next();
-    }
+    else if (b0 > 0)
+      show(0, 0);
+  }
+  __device__ __forceinline__ kv_rows rows_of(int l) const {
+    return kv_rows{__builtin_amdgcn_readfirstlane(sm[64 + l]), __builtin_amdgcn_readfirstlane(sm[128 + l])};
   }
   // That sequence; the length of its pairs and where they start.
   __device__ __forceinline__ KvSegment sequence(int at, int &length, int &base, int &pairs) const {

@@ -47,68 +47,60 @@ __device__ __forceinline__ void kv_join(const mtk_kv_attn_kargs &a, int block, i
   const int chunks = a.part_ld / 4, groups = kKvJoin / chunks;
   const int g = tid / chunks, d = 4 * (tid - g * chunks);
   const int heads = PARTS ? 1 : groups, per_row = (a.H + heads - 1) / heads;  // items of a row
-  const int items = a.T * per_row;  // taken in turn by the workgroups, as the rows that are shared may lie together
-  if (block >= items) return;
+  if (block >= a.T * per_row) return;
   KvLine<0, 0> line(a, lane, sm_line[tid >> 6]);
   line.lay();
-  for (int it = block; it < items;) {  // uniform: every wavefront takes the same items
-    int t = it / per_row;
-    const int l = line.find_row(t);
-    if (l < 0) {
-      it += n_blocks;
-      continue;
-    }
-    int length, base, pairs;
-    const KvSegment seq = line.sequence(l, length, base, pairs);
-    const int64_t past = (int64_t)(seq.seq.first + min(seq.seq.rows, a.S_q)) * per_row;
-    const int blocks = kv_div(pairs, a.H_kv);
-    const bool none = pairs == 0 || (line.cut.padded && length == line.cut.each);  // no pair is shared
-    for (; !none && it < min((int64_t)items, past); it += n_blocks) {
-      t = it / per_row;
-      const int h = (it - t * per_row) * heads + (PARTS ? 0 : g);
-      if (h >= a.H || g >= groups) continue;
-      const int hk = kv_div(h, G), r = (t - seq.seq.first) * G + h - hk * G, rb = r >> a.rows_shift;
-      const int start = base + ((a.by_pair ? blocks - 1 - rb : rb) * a.H_kv + hk) * length;
-      const int w0 = kv_div(start, line.cut.each), w1 = min(kv_div(start + seq.steps - 1, line.cut.each), a.places - 1);
-      if (w0 >= w1) continue;  // one workgroup's
-      const int first = start == w0 * line.cut.each ? 0 : 1;
-      KvPart sum;
-      constexpr int kAhead = 8;
-      const int step = PARTS ? groups : 1;
-      for (int s0 = w0 + (PARTS ? g : 0); s0 <= w1; s0 += kAhead * step) {
-        KvPart p[kAhead];
+  int length, base, pairs, blocks;
+  KvSegment seq;
+  auto open = [&](int l) {
+    seq = line.sequence(l, length, base, pairs);
+    blocks = kv_div(pairs, a.H_kv);
+    return !(pairs == 0 || (line.cut.padded && length == line.cut.each));  // none of its pairs is shared
+  };
+  // Items are taken in turn by the workgroups, as the rows that are shared may lie together; uniform: every wavefront of a
+  // workgroup takes the same ones.
+  kv_walk(line, a.T, per_row, a.S_q, block, n_blocks, open, [&](int it) {
+    const int t = it / per_row, h = (it - t * per_row) * heads + (PARTS ? 0 : g);
+    if (h >= a.H || g >= groups) return;
+    const int hk = kv_div(h, G), r = (t - seq.seq.first) * G + h - hk * G, rb = r >> a.rows_shift;
+    const int start = base + ((a.by_pair ? blocks - 1 - rb : rb) * a.H_kv + hk) * length;
+    const int w0 = kv_div(start, line.cut.each), w1 = min(kv_div(start + seq.steps - 1, line.cut.each), a.places - 1);
+    if (w0 >= w1) return;  // one workgroup's
+    const int first = start == w0 * line.cut.each ? 0 : 1;
+    KvPart sum;
+    constexpr int kAhead = 8;
+    const int step = PARTS ? groups : 1;
+    for (int s0 = w0 + (PARTS ? g : 0); s0 <= w1; s0 += kAhead * step) {
+      KvPart p[kAhead];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          const int w = s0 + i * step;
-          if (w <= w1) {
-            const size_t place = a.by_pair ? (size_t)w : (size_t)w * 2 + (w == w0 ? first : 0);
-            const size_t at = (place << a.rows_shift) + (r & (rows - 1));
-            const f32x2 ml = *(const f32x2 *)(a.part_ml + 2 * at);
-            p[i] = KvPart{ml.x, ml.y, *(const f32x4 *)(a.part + at * a.part_ld + d)};
-          }
+      for (int i = 0; i < kAhead; ++i) {
+        const int w = s0 + i * step;
+        if (w <= w1) {
+          const size_t place = a.by_pair ? (size_t)w : (size_t)w * 2 + (w == w0 ? first : 0);
+          const size_t at = (place << a.rows_shift) + (r & (rows - 1));
+          const f32x2 ml = *(const f32x2 *)(a.part_ml + 2 * at);
+          p[i] = KvPart{ml.x, ml.y, *(const f32x4 *)(a.part + at * a.part_ld + d)};
         }
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) add_part(sum, p[i]);
       }
-      if constexpr (PARTS) {
-        __syncthreads();
-        sm_x[tid] = sum.x;
-        sm_ml[tid] = f32x2{sum.m, sum.l};
-        __syncthreads();
-        if (tid < chunks) {
-          for (int i = 1; i < min(groups, w1 - w0 + 1); ++i) {
-            const int k = tid + i * chunks;
-            add_part(sum, KvPart{sm_ml[k].x, sm_ml[k].y, sm_x[k]});
-          }
-          store_out<DT>(a, t, h, d, sum);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) add_part(sum, p[i]);
+    }
+    if constexpr (PARTS) {
+      __syncthreads();
+      sm_x[tid] = sum.x;
+      sm_ml[tid] = f32x2{sum.m, sum.l};
+      __syncthreads();
+      if (tid < chunks) {
+        for (int i = 1; i < min(groups, w1 - w0 + 1); ++i) {
+          const int k = tid + i * chunks;
+          add_part(sum, KvPart{sm_ml[k].x, sm_ml[k].y, sm_x[k]});
         }
-      } else {
         store_out<DT>(a, t, h, d, sum);
       }
+    } else {
+      store_out<DT>(a, t, h, d, sum);
     }
-    const int64_t rest = (int64_t)(seq.seq.first + seq.seq.rows) * per_row - it;  // of the sequence: nothing to do
-    if (rest > 0 && it < items) it += (int)((rest + n_blocks - 1) / n_blocks) * n_blocks;
-  }
+  });
 }
 
 }  // namespace mtk
