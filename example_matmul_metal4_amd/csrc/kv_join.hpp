@@ -61,7 +61,8 @@ __device__ __forceinline__ void kv_join(const mtk_kv_attn_kargs &a, int block, i
   // workgroup takes the same ones.
   kv_walk(line, a.T, per_row, a.S_q, block, n_blocks, open, [&](int it) {
     const int t = it / per_row, h = (it - t * per_row) * heads + (PARTS ? 0 : g);
-    if (h >= a.H || g >= groups) return;
+    const bool mine = g < groups && h < a.H;  // lanes behind the last group, or behind the last head, add nothing
+    if (!PARTS && !mine) return;  // PARTS: they reach the barriers below with the others
     const int hk = kv_div(h, G), r = (t - seq.seq.first) * G + h - hk * G, rb = r >> a.rows_shift;
     const int start = base + ((a.by_pair ? blocks - 1 - rb : rb) * a.H_kv + hk) * length;
     const int w0 = kv_div(start, line.cut.each), w1 = min(kv_div(start + seq.steps - 1, line.cut.each), a.places - 1);
@@ -70,7 +71,7 @@ __device__ __forceinline__ void kv_join(const mtk_kv_attn_kargs &a, int block, i
     KvPart sum;
     constexpr int kAhead = 8;
     const int step = PARTS ? groups : 1;
-    for (int s0 = w0 + (PARTS ? g : 0); s0 <= w1; s0 += kAhead * step) {
+    for (int s0 = w0 + (PARTS ? g : 0); mine && s0 <= w1; s0 += kAhead * step) {
       KvPart p[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import example_matmul_metal4_amd as mtk  # noqa: F401
-from test_kv_cache_use_gpu import Given, rng_of
+from test_kv_cache_use_gpu import Given, agree, rng_of
 
 pytestmark = pytest.mark.gpu
 
@@ -29,6 +29,15 @@ def test_rows_before_the_first_sequence(dev, n, dead, chunk, fmt, dtype):
     got, lse = g.attend(S_q)
     want, ref, bound = g.cache.attention(g.Q, g.start, g.lens, g.table, True, S_q, some)
     assert (got[:dead] == 0x1234).all() and (lse[:dead] == 77.0).all()
-    from test_kv_cache_use_gpu import agree
     agree(got, lse, want, ref, bound, dtype, untouched=False)
+    g.free()
+
+
+@pytest.mark.parametrize("D", [72, 96, 136, 160, 192, 224])
+@pytest.mark.parametrize("fmt, dtype", [("fp4", "f16"), ("fp8", "bf16")])
+def test_joins_over_the_parts_with_lanes_left_over(dev, D, fmt, dtype):
+    # head dimensions whose D / 4 lanes do not divide the 256 threads of a join
+    g = Given(dev, 85, [9000, 2000, 40], [1, 0, 1], 6, 2, D, 16, fmt, dtype, n_pages=200)
+    assert "mtk_kv_join_parts" in g.plan(1).describe()
+    g.check(1)
     g.free()
