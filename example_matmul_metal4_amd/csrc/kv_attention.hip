@@ -15,8 +15,8 @@
 //   * S^T leaves each lane with 4 keys of one row per 16 keys, which is the operand layout of P^T in
 //     O^T = V^T P^T. V^T needs 8 keys of one dim per lane: V is converted the same way, written to the
 //     wavefront's own LDS tile and read back transposed (ds_read_b64_tr_b16).
-//   * P is rounded to the 16-bit type for the MFMA (off by up to 2^-8 or 2^-11 of its value, averaged over the keys); scores,
-//     offsets and sums stay in fp32.
+//   * P is rounded to the 16-bit type for the MFMA (off by up to 2^-8 or 2^-11 of its value, averaged over the keys; f16: or by
+//     2^-32 of the row's largest weight, kv_join.hpp); scores, offsets and sums stay in fp32.
 //   * Keys past the length have their V codes zeroed (a page's unused rows may hold anything); a NaN block's V is
 //     zeroed too and its dims set to NaN only for the rows that see the key, so that nothing masked reaches O.
 //
@@ -33,7 +33,6 @@
 
 namespace mtk {
 
-constexpr float kKvSlack = 8.0f;  // log2-domain headroom before O is rescaled: weights up to 2^8, in range for f16 as well
 constexpr int kWindow = 56;       // table entries between the starts of two windows (below)
 
 // max over the lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -381,9 +380,9 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
       for (int kb = 0; kb < kKb; ++kb) mx = vmax3(vmax3(mx, s[n][kb][0], s[n][kb][1]), s[n][kb][2], s[n][kb][3]);
       const float m_tile = quarters_max(mx) * cl;
       float alpha = 1.0f;
-      if (m_tile > m_off[n] + kKvSlack) {
-        alpha = __builtin_amdgcn_exp2f(m_off[n] - m_tile);
-        m_off[n] = m_tile;
+      if (m_tile - m_off[n] > kKvLift<DT> + kKvSlack) {  // a difference: exact where scores are far from zero
+        alpha = __builtin_amdgcn_exp2f(m_off[n] - (m_tile - kKvLift<DT>));
+        m_off[n] = m_tile - kKvLift<DT>;
       }
       const float moff = m_off[n] == -INFINITY ? 0.0f : m_off[n];
       if (__any(alpha != 1.0f)) {

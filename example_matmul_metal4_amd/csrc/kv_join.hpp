@@ -5,6 +5,14 @@
 
 namespace mtk {
 
+// Weights are exp2(score - offset). An offset is raised to the scores' maximum less kKvLift<DT> once that is more than kKvSlack
+// above it, so that sums are rarely rescaled: the largest weight lies in 2^lift to 2^(lift + slack). They go to the second
+// product in 16 bits; f16 holds none below 2^-25, which with a lift of 7 is 2^-32 of the row's largest (without, 2^-25: of 131072
+// positions 0.4 % of the sum could be lost), while 2^15 and the rounding above stay in its range. bf16 has the range of fp32.
+template <int DT>
+constexpr float kKvLift = DT == DT_F16 ? 7.0f : 0.0f;
+constexpr float kKvSlack = 8.0f;
+
 // Sums of some keys of a row (4 dims), unscaled, with their exponent offset (log2) and the sum of the weights.
 struct KvPart {
   float m = -INFINITY, l = 0.0f;

@@ -292,9 +292,9 @@ __device__ __forceinline__ void kv_prefill(const mtk_kv_prefill_kargs &args) {
       mx = half_max(mx);
       const float m_tile = mx * c;
       float alpha = 1.0f;
-      if (m_tile > m_off + 8.0f) {
-        alpha = __builtin_amdgcn_exp2f(m_off - m_tile);
-        m_off = m_tile;
+      if (m_tile - m_off > kKvLift<DT> + kKvSlack) {  // a difference: exact where scores are far from zero
+        alpha = __builtin_amdgcn_exp2f(m_off - (m_tile - kKvLift<DT>));
+        m_off = m_tile - kKvLift<DT>;
       }
       const float moff = m_off == -INFINITY ? 0.0f : m_off;
       l_run *= alpha;

@@ -145,7 +145,10 @@ class Cache:
         """(O, lse, bound) in 64 bits; rows of no sequence are NaN with bound -1 (not computed), and so are rows that are not
         in `only`, if it is given. `bound` is what O may
         be off: half a step of the result; the weights' rounding, half a step of each; and the scores in 32 bits: D + 3
-        roundings of 2^-24 of sum |q k| and of the scaled score and its offset, which move a weight by as much."""
+        roundings of 2^-24 of sum |q k| and of the scaled score and its offset, which move a weight by as much.
+        f16 weights below 2^-14 have steps of 2^-24 whatever their value, so that half a step is 2^-25. Of some keys of a row the
+        largest weight is held as 2^7 or more, so that this is at most 2^-25 / 2^7 = 2^-32 of the row's largest weight
+        (of w below, whose largest is 1)."""
         T, H, D = Q.shape
         G, u = H // self.H_kv, HALF_STEP[self.dtype]
         q = to_f64(Q, self.dtype)
@@ -179,5 +182,6 @@ class Cache:
                     lse[first + i, h] = top + np.log(total)
                     # 32-bit sums over m keys: pairwise in the matrix unit and over tiles, at most m / 32 + 8 steps
                     sums = 2.0 ** -24 * (m / 32 + 8)
-                    bound[first + i, h] = u * np.abs(o) + (u + 2 * slip + 2 * sums) * spread * (1 + u) + 2.0 ** -24
+                    small = 2.0 ** -32 * np.abs(vv).sum(0) / total if self.dtype == "f16" else 0.0
+                    bound[first + i, h] = u * np.abs(o) + ((u + 2 * slip + 2 * sums) * spread + small) * (1 + u) + 2.0 ** -24
         return O, lse, bound

@@ -1,5 +1,5 @@
 """Attention over the paged cache where its weights are far apart: one key far above thousands of others, whose small weights
-together still count, and scores that are infinite. Against numpy in 64 bits."""
+together still count. Against numpy in 64 bits."""
 import numpy as np
 import pytest
 
@@ -64,28 +64,4 @@ def test_one_key_far_above_the_others(dev, case, first, dtype):
     live = bound[..., 1] >= 0
     assert (np.abs(want[..., 1][live]) > 0).all() and (bound[..., 1][live] < 0.1 * want[..., 1][live]).all()  # the small weights show
     agree(got, lse, want, ref, bound, dtype)
-    g.free()
-
-
-@pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("case", KERNELS, ids=str)
-def test_infinite_queries(dev, case, dtype):
-    # a row whose scores are all -inf gives NaN, with a log-sum-exp of -inf; one of them +inf: NaN
-    lens, rows, H, H_kv, D, page, fmt, width, kernel = case
-    g = Given(dev, 84, lens, rows, H, H_kv, D, page, fmt, dtype, width=width)
-    set_dim(g, 0, range(max(lens)), 2, 1.0)
-    set_dim(g, 0, [0, lens[0] - 2, lens[0] - 1], 3, -0.5)
-    x = kv.to_f64(g.Q, dtype).copy()
-    for t in range(g.T):
-        for h in range(H):
-            x[t, h, 2] = (-np.inf, np.inf, x[t, h, 2], x[t, h, 2])[(t + h) % 4]
-    x[0, 0, 2], x[0, 0, 3] = 0.5, np.nan
-    g.Q = kv.bits_of(x, dtype)
-    got, lse = g.attend(max(rows))
-    with np.errstate(all="ignore"):
-        want, ref, bound = g.cache.attention(g.Q, g.start, g.lens, g.table, True, max(rows))
-    row, low = ~(bound[..., 0] < 0), np.isneginf(x[..., 2])
-    assert np.isnan(want[row & np.isinf(x[..., 2])]).all() and (row & low).any()
-    ref = np.where(row & low, -np.inf, ref)
-    agree(got, lse, want, ref, np.where(np.isnan(bound), 0.0, bound), dtype)
     g.free()
