@@ -260,7 +260,7 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
     f32x4 o[NR][kDb];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
-      m_off[n] = -INFINITY;
+      m_off[n] = first_offset(lim[n] >= 0);
       l_run[n] = 0.0f;
 #pragma unroll
       for (int d = 0; d < kDb; ++d) o[n][d] = f32x4{};
@@ -482,7 +482,7 @@ __device__ __forceinline__ void kv_attend(const mtk_kv_attn_kargs &a) {
         const float m0 = sum.m == -INFINITY ? 0.0f : sum.m;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          const float m = sm_m[w][rr], f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m0);  // no keys, or NaN scores
+          const float m = sm_m[w][rr], f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - m0);  // no keys
           sum.l = __builtin_fmaf(f, sm_l[w][rr], sum.l);
           const f32x4 x = *(const f32x4 *)((const float *)smem + w * (kParkB / 4) + rr * kPitch + d0);
           sum.x = f32x4{__builtin_fmaf(f, x.x, sum.x.x), __builtin_fmaf(f, x.y, sum.x.y), __builtin_fmaf(f, x.z, sum.x.z),

@@ -22,16 +22,25 @@ __device__ __forceinline__ void add_part(KvPart &s, const KvPart &t) {
   const float m = fmaxf(s.m, t.m);
   const float m0 = m == -INFINITY ? 0.0f : m;
   const float f = __builtin_amdgcn_exp2f(s.m - m0), g = __builtin_amdgcn_exp2f(t.m - m0);
-  // an offset of -inf has no keys, or only NaN scores: its sums count as they are
+  // an offset of -inf has no keys: its sums count as they are
   s.l = s.l * (s.m == -INFINITY ? 1.0f : f) + t.l * (t.m == -INFINITY ? 1.0f : g);
   s.x = s.x * (s.m == -INFINITY ? 1.0f : f) + t.x * (t.m == -INFINITY ? 1.0f : g);
   s.m = m;
 }
 
+// The offset that a row's sums start with: rows that see a key are told from those that see none by it, also where all their
+// scores are -inf.
+__device__ __forceinline__ float first_offset(bool sees) { return sees ? -3.402823466e38f : -INFINITY; }
+// What a row's sums are divided by its weights' sum with. No weights: zeros where it sees no key, NaN where all its scores
+// are -inf.
+__device__ __forceinline__ float inverse_of(float l, float m) {
+  return l != 0.0f ? 1.0f / l : m == -INFINITY ? 0.0f : __builtin_nanf("");
+}
+
 // 4 dims of (packed row, query head) from d on; the row's log-sum-exp with d == 0.
 template <int DT>
 __device__ __forceinline__ void store_out(const mtk_kv_attn_kargs &a, int row, int h, int d, const KvPart &s) {
-  const float inv = s.l != 0.0f ? 1.0f / s.l : 0.0f;  // no key: 0; NaN stays
+  const float inv = inverse_of(s.l, s.m);
   if (d < a.D)
     *(u32x2 *)((uint16_t *)a.O + ((size_t)row * a.H + h) * a.D + d) =
         u32x2{pack2<DT>(s.x.x * inv, s.x.y * inv), pack2<DT>(s.x.z * inv, s.x.w * inv)};

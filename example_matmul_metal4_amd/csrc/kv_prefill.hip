@@ -227,7 +227,7 @@ __device__ __forceinline__ void kv_prefill(const mtk_kv_prefill_kargs &args) {
     });
   };
 
-  float m_off = -INFINITY, l_run = 0.0f;
+  float m_off = first_offset(lim >= 0), l_run = 0.0f;
   f32x16 o[kDb];
 #pragma unroll
   for (int i = 0; i < kDb; ++i) o[i] = f32x16{};
@@ -373,7 +373,7 @@ __device__ __forceinline__ void kv_prefill(const mtk_kv_prefill_kargs &args) {
   const float l_tot = half_sum(l_run);
   if (!live) return;
   if (seg.from == 0 && seg.to == seg.steps) {
-    const float inv = l_tot != 0.0f ? 1.0f / l_tot : 0.0f;
+    const float inv = inverse_of(l_tot, m_off);
     uint16_t *O = (uint16_t *)a.O + ((size_t)(seq.first + qi) * a.H + h) * a.D;
 #pragma unroll
     for (int db = 0; db < kDb; ++db)

@@ -384,7 +384,9 @@ int mtk_kv_read_run(const mtk_plan *plan, const mtk_kv_read_args *args);
 
 /* O = softmax(Q K^T / sqrt(D)) V over the cached positions, Q [T][H][D] (ld_q), O [T][H][D] packed, query head h on
  * K/V head h / (H / H_kv). The new rows' own K and V are read from the cache: write them first. A row that sees no
- * position gives zeros and a log-sum-exp of -inf. The keys of long sequences are split over workgroups, whose partial
+ * position gives zeros and a log-sum-exp of -inf; one whose scores are all -inf (infinities in Q) gives NaN and -inf, and one
+ * with a score of +inf or NaN gives NaN in both. Scores are held in 32 bits: beyond 2^27 in magnitude they are too coarse for
+ * weights. The keys of long sequences are split over workgroups, whose partial
  * sums lie in the workspace until a second kernel adds them in a fixed order: the result does not vary from run to run,
  * and runs that may overlap need a workspace each. O, lse and the workspace may not overlap Q, the cache or each other.
  * A plan whose sequences may have more than 64 (row, query head) pairs per K/V head (32 above 128 dims) has kernels for those

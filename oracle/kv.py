@@ -179,7 +179,7 @@ class Cache:
                     spread = np.abs(w) @ np.abs(vv) / total
                     slip = 2.0 ** -24 * ((D + 3) * (np.abs(kk) @ np.abs(x)).max() / np.sqrt(D) + 4 * np.abs(s).max() + 8)
                     O[first + i, h] = o
-                    lse[first + i, h] = top + np.log(total)
+                    lse[first + i, h] = top + np.log(total) if top > -np.inf else top
                     # 32-bit sums over m keys: pairwise in the matrix unit and over tiles, at most m / 32 + 8 steps
                     sums = 2.0 ** -24 * (m / 32 + 8)
                     small = 2.0 ** -32 * np.abs(vv).sum(0) / total if self.dtype == "f16" else 0.0
