@@ -113,20 +113,40 @@ MTK_KV_FN kv_cut kv_cut_of(int work, int own, int units, int least) {
 }
 
 // Launches whose workgroups have one pair each (by_pair). own: the pairs. Whether they have more than one workgroup each: not
-// where they are `units` or more, nor where two shares of one, of KV_FEW_STEPS or less on average, gain less than the join costs
-// (32 heads, 8 K/V heads of 128 dims, 500 rows in 2 sequences each: 16 steps 38.1 us whole, 47.2 in two shares; 24 steps 49.7 and
-// 54.1; 32 steps 61.1 and 61.2; 200 rows in 4: 39.3 and 45.7, 51.1 and 52.6, 62.9 and 59.1).
-#define KV_FEW_STEPS 28
-MTK_KV_FN int kv_pairs_split(int work, int own, int units) {
-  return own < units && (own <= units / 3 || work > KV_FEW_STEPS * own);
+// where they are `units` or more, nor where two shares of one, of `few` steps or less on average, gain less than the join costs
+// (32 heads, 8 K/V heads of 128 dims, 500 rows in 2 sequences each: 16 steps of 64 keys 38.1 us whole, 47.2 in two shares; 24 steps
+// 49.7 and 54.1; 32 steps 61.1 and 61.2; 200 rows in 4: 39.3 and 45.7, 51.1 and 52.6, 62.9 and 59.1).
+#define KV_FEW_STEPS 28 /* of 64 keys */
+MTK_KV_FN int kv_few_steps(int step_shift) { return (KV_FEW_STEPS << 6) >> step_shift; }
+MTK_KV_FN int kv_pairs_split(int work, int own, int units, int few = KV_FEW_STEPS) {
+  return own < units && (own <= units / 3 || work > few * own);
 }
 
 // Steps of a share, at least `least` and no more than `most`, the steps of a full table. With this or more there are at most
 // `units` workgroups: pairs ceil their steps / each, which adds less than 1 for each.
-MTK_KV_FN int kv_each_of_pairs(int work, int own, int units, int least, int most) {
-  int each = kv_pairs_split(work, own, units) ? kv_div(work + (units - own) - 1, units - own) : most;
+MTK_KV_FN int kv_each_of_pairs(int work, int own, int units, int least, int most, int few = KV_FEW_STEPS) {
+  int each = kv_pairs_split(work, own, units, few) ? kv_div(work + (units - own) - 1, units - own) : most;
   if (each > most) each = most;
   return each < least ? least : each;
+}
+
+// The steps of such a launch, 2^shift keys each: 64, but more where the sums over `pairs` pairs of full tables would not fit 32
+// bits (a pair's padded length and a share past it). `pairs` counts S_q rows of every sequence, as no less is sure whatever
+// row_start holds; starts that ascend make far fewer, whose shares are then just longer. least: shares of 256 keys or more where
+// pairs may be split, else whole ones.
+typedef struct {
+  int shift; /* -1: none fits */
+  int steps, least;
+} kv_pair_steps;
+MTK_KV_FN kv_pair_steps kv_steps_of_pairs(int64_t pairs, int64_t positions, int split) {
+  kv_pair_steps s;
+  for (s.shift = 6; s.shift <= 30; ++s.shift) {
+    s.steps = (int)((positions + ((int64_t)1 << s.shift) - 1) >> s.shift);
+    s.least = split ? (s.shift < 8 ? 256 >> s.shift : 1) : s.steps;
+    if (pairs <= INT32_MAX / (3 * (int64_t)s.steps + s.least)) return s;
+  }
+  s.shift = -1;
+  return s;
 }
 
 MTK_KV_FN int kv_length(kv_share r, kv_cut c) { return c.padded ? kv_div(r.steps + c.each - 1, c.each) * c.each : r.steps; }

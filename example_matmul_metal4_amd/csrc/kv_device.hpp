@@ -124,8 +124,9 @@ struct KvLine {
     if (by_pair()) {
       const int shift = STEP ? __builtin_ctz(STEP ? STEP : 1) : a.step_shift;
       const int most = (int)((((uint32_t)a.max_pages << a.page_shift) + (1u << shift) - 1) >> shift);
-      int hi = kv_each_of_pairs(work, own, a.units, a.least, most);
-      if (a.B <= 64 && kv_pairs_split(work, own, a.units)) {  // the least that makes no more workgroups than that
+      const int few = kv_few_steps(shift);
+      int hi = kv_each_of_pairs(work, own, a.units, a.least, most, few);
+      if (a.B <= 64 && kv_pairs_split(work, own, a.units, few)) {  // the least that makes no more workgroups than that
         int lo = min(hi, max(a.least, kv_div(work + a.units - 1, a.units)));
         while (lo < hi) {
           const int mid = (lo + hi) >> 1;

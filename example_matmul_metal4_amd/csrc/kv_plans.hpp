@@ -222,7 +222,7 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
     if (!k.whole && pairs <= most) add_join(k, blocks * 8 < grid && (long long)joins(k, true, INT32_MAX) < 2LL * cus);
   }
   if (pairs > most) {
-    const int rows = 128, step = 64;
+    const int rows = 128;
     mtk_kv_prefill_kargs both{};
     mtk_kv_attn_kargs &r = both.rows;
     r = a;
@@ -231,16 +231,18 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
     r.by_pair = 1;
     r.units = cus * (dp == 256 ? 1 : 2);
     const long long each = (long long)d.B * ((pairs + rows - 1) / rows) * d.H_kv;  // blocks, whatever row_start holds
-    const long long blocks = kv_max_blocks(d.B, d.T, d.S_q, G, rows) * d.H_kv, steps = (positions + step - 1) / step;
+    const long long blocks = kv_max_blocks(d.B, d.T, d.S_q, G, rows) * d.H_kv;
     // Fewer blocks than workgroups: the keys are split, into 4 steps (256 keys) or more, so that all workgroups are on the
     // device at once; else never. 300 rows of 8 heads of 64 dims, 1000 positions: 17.8 us, 8 steps 22.6, 2 steps 16.8;
     // 2 x 4000 positions, 100 rows, 256 dims: 47.4, 54.8 and 47.3, with shares of equal work (two rounds) 51.3, unsplit 215.
     // Decided on the device; here only whether the blocks may be so few, each sequence's last one aside.
-    const bool split = std::min(blocks, (long long)d.T * G / rows * d.H_kv) < r.units && steps > 4;
-    r.least = split ? 4 : (int)steps;
-    if ((s = too_large(each, 3 * steps + r.least)) != MTK_OK) return s;
+    const bool split = std::min(blocks, (long long)d.T * G / rows * d.H_kv) < r.units && positions > 256;
+    const kv_pair_steps steps = kv_steps_of_pairs(each, positions, split);
+    if (steps.shift < 0 || blocks >= (1 << 23))
+      return fail(MTK_ERR_UNSUPPORTED, "a batch of %lld row blocks is not supported", steps.shift < 0 ? each : blocks);
+    r.least = steps.least;
+    r.step_shift = steps.shift;
     r.rows_shift = __builtin_ctz((unsigned)rows);
-    r.step_shift = __builtin_ctz((unsigned)step);
     const long long grid = split ? std::max<long long>(r.units, blocks) : blocks;
     if (split) partial_sums(r, r.units);
     // The sums that the launch before has left are joined by this one's last workgroups, at most one per CU, beside the

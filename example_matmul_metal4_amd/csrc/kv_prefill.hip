@@ -57,7 +57,7 @@ __device__ __forceinline__ void kv_prefill(const mtk_kv_prefill_kargs &args) {
   if (tid == 0) sm_nan = 0;
   for (int i = tid; i < 2 * 4 * 4 * kIt; i += 256) (&sm_bad[0][0][0][0])[i] = 0;
 
-  KvLine<kPfRows, kPfKeys> line(a, lane, sm_line[wave]);
+  KvLine<kPfRows, 0> line(a, lane, sm_line[wave]);
   line.lay();
   const int64_t line_from = (int64_t)wg * line.cut.each;  // past the line's end, which 32 bits hold, for workgroups of no share
   if (line_from > INT32_MAX - line.cut.each) return;
@@ -76,7 +76,7 @@ __device__ __forceinline__ void kv_prefill(const mtk_kv_prefill_kargs &args) {
   const int r_last = min(seg.rb * kPfRows + kPfRows, rows) - 1;
   const int64_t p_last = a.causal ? seq.pos0 + kv_div(r_last, G) : (int64_t)seq.keys - 1;
   const int n_keys = (int)max((int64_t)0, min((int64_t)seq.keys, p_last + 1));
-  const int key_from = seg.from * kPfKeys, key_end = min(n_keys, seg.to * kPfKeys);
+  const int key_from = seg.from << a.step_shift, key_end = min(n_keys, seg.to << a.step_shift);
   const int n_tiles = key_end > key_from ? (key_end - key_from + kPfKeys - 1) / kPfKeys : 0;
   const int64_t pos = a.causal ? seq.pos0 + qi : (int64_t)seq.keys - 1;
   const int lim = live && pos >= 0 ? (int)min(pos, (int64_t)seq.keys - 1) : -1;
