@@ -283,8 +283,31 @@ bool overlap(const void *a, uint64_t a_bytes, const void *b, uint64_t b_bytes) {
 // Bytes that `rows` rows of `width` elements with `ld` between them span.
 uint64_t kv_span(int rows, int64_t ld, int64_t width) { return 2 * ((uint64_t)(rows - 1) * (uint64_t)ld + (uint64_t)width); }
 
+// Whether one of n rows of `width` elements from a on, `ld_a` apart, meets one of as many from b on: slices of one buffer lie
+// between each other.
+bool rows_meet(const void *a, int64_t ld_a, const void *b, int64_t ld_b, int n, int64_t width) {
+  if (!overlap(a, kv_span(n, ld_a, width), b, kv_span(n, ld_b, width))) return false;
+  const uint64_t x = (uintptr_t)a, y = (uintptr_t)b, bytes = 2 * (uint64_t)width, step_a = 2 * (uint64_t)ld_a, step_b = 2 * (uint64_t)ld_b;
+  if (ld_a == ld_b) {  // the distances of their rows: |x - y| less so many strides
+    const uint64_t apart = x < y ? y - x : x - y, rows = apart / step_a, rest = apart % step_a;
+    return (rest < bytes && rows < (uint64_t)n) || (step_a - rest < bytes && rows + 1 < (uint64_t)n);
+  }
+  for (int i = 0, j = 0; i < n && j < n;) {
+    const uint64_t s = x + (uint64_t)i * step_a, t = y + (uint64_t)j * step_b;
+    if (s < t ? t - s < bytes : s - t < bytes) return true;
+    s < t ? ++i : ++j;
+  }
+  return false;
+}
+
 int check_kv_args(const mtk_plan *p, const void *argset) {
   const mtk_kv_desc &d = p->kv;
+  struct Buffer {
+    const char *name;
+    const void *at;
+    uint64_t bytes;
+  };
+  Buffer in[5] = {}, out[3] = {};  // what the operator reads and writes
   const int32_t *ints[3];
   const void *cache;
   if (!argset) return fail(MTK_ERR_INVALID, "null arguments");
@@ -298,20 +321,11 @@ int check_kv_args(const mtk_plan *p, const void *argset) {
     if (p->workspace && (!t->workspace || !aligned(t->workspace, 16)))
       return fail(MTK_ERR_INVALID, "this plan needs a 16-byte aligned workspace of %zu bytes", p->workspace);
     const int64_t width = (int64_t)d.H * d.D;
-    struct {
-      const char *name;
-      const void *at;
-      uint64_t bytes;
-    } const in[] = {{"Q", t->Q, kv_span(d.T, d.ld_q ? d.ld_q : width, width)}, {"the cache", cache, kv_cache_size(d)}},
-      out[] = {{"O", t->O, kv_span(d.T, width, width)}, {"lse", t->lse, 4ull * d.T * d.H}, {"the workspace", t->workspace, p->workspace}};
-    for (int i = 0; i < 3; ++i) {
-      if (!out[i].at || !out[i].bytes) continue;
-      for (const auto &x : in)
-        if (x.at && overlap(out[i].at, out[i].bytes, x.at, x.bytes)) return fail(MTK_ERR_INVALID, "%s overlaps %s", out[i].name, x.name);
-      for (int k = 0; k < i; ++k)
-        if (out[k].at && overlap(out[i].at, out[i].bytes, out[k].at, out[k].bytes))
-          return fail(MTK_ERR_INVALID, "%s overlaps %s", out[i].name, out[k].name);
-    }
+    in[0] = {"Q", t->Q, kv_span(d.T, d.ld_q ? d.ld_q : width, width)};
+    in[1] = {"the cache", cache, kv_cache_size(d)};
+    out[0] = {"O", t->O, kv_span(d.T, width, width)};
+    out[1] = {"lse", t->lse, 4ull * d.T * d.H};
+    out[2] = {"the workspace", t->workspace, p->workspace};
   } else {
     const bool write = p->kind == PLAN_KV_WRITE;
     const mtk_kv_write_args *w = (const mtk_kv_write_args *)argset;
@@ -321,15 +335,30 @@ int check_kv_args(const mtk_plan *p, const void *argset) {
     ints[0] = write ? w->row_start : r->row_start, ints[1] = write ? w->kv_len : r->kv_len, ints[2] = write ? w->table : r->table;
     if (!K || !V) return fail(MTK_ERR_INVALID, "K and V must be non-null");
     if (!aligned(K, 16) || !aligned(V, 16)) return fail(MTK_ERR_INVALID, "K and V must be 16-byte aligned");
+    const int64_t width = (int64_t)d.H_kv * d.D, ld_k = d.ld_k ? d.ld_k : width, ld_v = d.ld_v ? d.ld_v : width;
     if (!write && K == V) return fail(MTK_ERR_INVALID, "K and V are the same rows");
-    const int64_t width = (int64_t)d.H_kv * d.D;
-    if (cache && (overlap(K, kv_span(d.T, d.ld_k ? d.ld_k : width, width), cache, kv_cache_size(d)) ||
-                  overlap(V, kv_span(d.T, d.ld_v ? d.ld_v : width, width), cache, kv_cache_size(d))))
-      return fail(MTK_ERR_INVALID, "K or V overlaps the cache");
+    if (!write && rows_meet(K, ld_k, V, ld_v, d.T, width)) return fail(MTK_ERR_INVALID, "K overlaps V");
+    const Buffer rows[2] = {{"K", K, kv_span(d.T, ld_k, width)}, {"V", V, kv_span(d.T, ld_v, width)}}, held = {"the cache", cache, kv_cache_size(d)};
+    (write ? in : out)[0] = rows[0];
+    (write ? in : out)[1] = rows[1];
+    (write ? out : in)[2] = held;
   }
   if (!cache || !aligned(cache, 16)) return fail(MTK_ERR_INVALID, "the cache must be non-null and 16-byte aligned");
   for (const int32_t *x : ints)
     if (!x || !aligned(x, 4)) return fail(MTK_ERR_INVALID, "row_start, kv_len and table must be non-null and 4-byte aligned");
+  const Buffer arrays[3] = {{"row_start", ints[0], 4 * ((uint64_t)d.B + 1)}, {"kv_len", ints[1], 4 * (uint64_t)d.B},
+                            {"the table", ints[2], 4 * (uint64_t)d.B * (uint64_t)d.max_pages}};
+  for (int i = 0; i < 3; ++i) {
+    const Buffer &o = out[i];
+    if (!o.at || !o.bytes) continue;
+    auto meets = [&](const Buffer &x) { return x.at && overlap(o.at, o.bytes, x.at, x.bytes); };
+    for (const Buffer &x : in)
+      if (meets(x)) return fail(MTK_ERR_INVALID, "%s overlaps %s", p->kind == PLAN_KV_WRITE ? x.name : o.name, p->kind == PLAN_KV_WRITE ? o.name : x.name);
+    for (const Buffer &x : arrays)
+      if (meets(x)) return fail(MTK_ERR_INVALID, "%s overlaps %s", o.name, x.name);
+    for (int k = 0; p->kind == PLAN_KV_ATTN && k < i; ++k)
+      if (meets(out[k])) return fail(MTK_ERR_INVALID, "%s overlaps %s", o.name, out[k].name);
+  }
   return MTK_OK;
 }
 

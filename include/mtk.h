@@ -342,6 +342,8 @@ int mtk_permute_run(const mtk_plan *plan, const mtk_permute_run_args *args);
  * sequence's rows that see a position NaN. row_start is limited to [0, T] and to ascend; rows that two sequences claim come out
  * as one or the other's, or undefined in attention. Two sequences may share pages; where both are written at one position of
  * one page in one call, its bytes are some mix of the two.
+ * What an operator writes (the cache, the rows read back, O, lse, the workspace) may not overlap what it reads, these arrays among
+ * it, or its other outputs; slices of one buffer whose rows lie between each other do not.
  *
  * One descriptor for the three plans. */
 #define MTK_KV_FP4 0
@@ -388,7 +390,7 @@ int mtk_kv_read_run(const mtk_plan *plan, const mtk_kv_read_args *args);
  * with a score of +inf or NaN gives NaN in both. Scores are held in 32 bits: beyond 2^27 in magnitude they are too coarse for
  * weights. The keys of long sequences are split over workgroups, whose partial
  * sums lie in the workspace until a second kernel adds them in a fixed order: the result does not vary from run to run,
- * and runs that may overlap need a workspace each. O, lse and the workspace may not overlap Q, the cache or each other.
+ * and runs that may overlap need a workspace each.
  * A plan whose sequences may have more than 64 (row, query head) pairs per K/V head (32 above 128 dims) has kernels for those
  * and, where S_q > 1, for the sequences with few rows beside them: give S_q = 1 for a batch of single tokens. */
 int mtk_kv_attn_plan(mtk_ctx *ctx, const mtk_kv_desc *desc, mtk_plan **out);
