@@ -26,6 +26,9 @@ MTK_KV_FN uint64_t kv_region_bytes(int fmt, int blocks, int page_shift) {
   return ((uint64_t)2 * (uint64_t)(kv_row_bytes(fmt, blocks) + blocks)) << page_shift;
 }
 
+/* Rows of a wavefront that writes or reads rows, at most: the loads of all of them are in flight at once. */
+enum { KV_MOVE_ROWS = 4 };
+
 // One sequence of the batch, from its entries of row_start and kv_len, whatever they hold. Its rows are
 // [first, first + rows) of the packed tensors, row i at position pos0 + i. len: kv_len; keys: cached positions, at most
 // the table's; bad: kv_len is more than the table holds.

@@ -72,12 +72,12 @@ int plan_kv_move(mtk_ctx *ctx, const mtk_kv_desc *d_in, PlanKind kind, mtk_plan 
   a.n_pages = d.n_pages;
   a.max_pages = d.max_pages;
   const long long items = 8LL * d.H_kv * a.blocks;  // of 16 bytes of K or V, per row
-  // Up to 4 rows per wavefront, whose places it looks up once and whose lines in the cache it fills itself; fewer where
+  // Up to KV_MOVE_ROWS rows per wavefront, whose places it looks up once and whose lines in the cache it fills itself; fewer where
   // that would leave less than 8 wavefronts per CU. 64 items of each.
   const int cus = ctx ? ctx->prop.multiProcessorCount : 256;
   a.parts = (int)((items + 63) / 64);
   a.rows_per_wave = 1;
-  while (a.rows_per_wave < 4 && (d.T + 2LL * a.rows_per_wave - 1) / (2 * a.rows_per_wave) * a.parts >= 8LL * cus) a.rows_per_wave *= 2;
+  while (a.rows_per_wave < KV_MOVE_ROWS && (d.T + 2LL * a.rows_per_wave - 1) / (2 * a.rows_per_wave) * a.parts >= 8LL * cus) a.rows_per_wave *= 2;
   const long long groups = ((long long)d.T + a.rows_per_wave - 1) / a.rows_per_wave;
   a.mul_blocks = a.blocks == 1 ? 0u : (uint32_t)((0x100000000ull + a.blocks - 1) / a.blocks);
   const long long waves = a.parts * groups;

@@ -84,12 +84,24 @@ struct KvRows {
   }
 };
 
-constexpr int kMoveAhead = 4;  // rows of a lane whose loads are in flight at once: all that it has
+// The pages and places of a wavefront's rows, as every lane has them: taken from the lanes that looked them up while all lanes
+// run, as lanes without an item leave the code below.
+struct KvPlaces {
+  int page[KV_MOVE_ROWS], off[KV_MOVE_ROWS];
+  __device__ __forceinline__ explicit KvPlaces(const KvRows &rows) {
+#pragma unroll
+    for (int k = 0; k < KV_MOVE_ROWS; ++k) {
+      page[k] = __builtin_amdgcn_readlane(rows.page, k);
+      off[k] = __builtin_amdgcn_readlane(rows.off, k);
+    }
+  }
+};
 
 template <int DT, int FMT>
 __device__ __forceinline__ void kv_write(const mtk_kv_move_kargs &a) {
   const int lane = threadIdx.x & 63;
   const KvRows rows(a, lane);
+  const KvPlaces of(rows);
   const int items = 8 * a.H_kv * a.blocks;
   const uint64_t page_b = kv_region_bytes(FMT, a.blocks, a.page_shift) * (uint64_t)a.H_kv;
   const uint32_t row_b = (uint32_t)kv_row_bytes(FMT, a.blocks);
@@ -156,20 +168,15 @@ __device__ __forceinline__ void kv_write(const mtk_kv_move_kargs &a) {
     const bool in = x.d < a.D;
     const uint16_t *src = (const uint16_t *)(x.v ? a.V : a.K) + (size_t)x.head * a.D + x.d;
     const int64_t ld = x.v ? a.ld_v : a.ld_k;
-    for (int i0 = 0; i0 < rows.n; i0 += kMoveAhead) {
-      u32x4 v[kMoveAhead];
+    u32x4 v[KV_MOVE_ROWS];
 #pragma unroll
-      for (int k = 0; k < kMoveAhead; ++k) {
-        v[k] = u32x4{0u, 0u, 0u, 0u};
-        if (in && i0 + k < rows.n) v[k] = __builtin_nontemporal_load((const u32x4 *)(src + (size_t)(rows.t0 + i0 + k) * ld));
-      }
-#pragma unroll
-      for (int k = 0; k < kMoveAhead; ++k) {
-        if (i0 + k >= rows.n) break;
-        const int page = __builtin_amdgcn_readlane(rows.page, i0 + k), off = __builtin_amdgcn_readlane(rows.off, i0 + k);
-        if (page >= 0) one(x, (char *)a.cache + (uint64_t)(uint32_t)page * page_b, off, v[k]);
-      }
+    for (int k = 0; k < KV_MOVE_ROWS; ++k) {
+      v[k] = u32x4{0u, 0u, 0u, 0u};
+      if (in && k < rows.n) v[k] = __builtin_nontemporal_load((const u32x4 *)(src + (size_t)(rows.t0 + k) * ld));
     }
+#pragma unroll
+    for (int k = 0; k < KV_MOVE_ROWS; ++k)
+      if (k < rows.n && of.page[k] >= 0) one(x, (char *)a.cache + (uint64_t)(uint32_t)of.page[k] * page_b, of.off[k], v[k]);
   }
 }
 
@@ -177,6 +184,7 @@ template <int DT, int FMT>
 __device__ __forceinline__ void kv_read(const mtk_kv_move_kargs &a) {
   const int lane = threadIdx.x & 63;
   const KvRows rows(a, lane);
+  const KvPlaces of(rows);
   const int items = 8 * a.H_kv * a.blocks;
   const uint64_t page_b = kv_region_bytes(FMT, a.blocks, a.page_shift) * (uint64_t)a.H_kv;
   const uint32_t row_b = (uint32_t)kv_row_bytes(FMT, a.blocks);
@@ -186,33 +194,29 @@ __device__ __forceinline__ void kv_read(const mtk_kv_move_kargs &a) {
   if (it < items && x.d < a.D) {
     uint16_t *dst = (uint16_t *)(x.v ? a.V : a.K) + (size_t)x.head * a.D + x.d;
     const int64_t ld = x.v ? a.ld_v : a.ld_k;
-    for (int i0 = 0; i0 < rows.n; i0 += kMoveAhead) {
-      uint32_t words[kMoveAhead][kWords8<FMT>], s[kMoveAhead];
+    uint32_t words[KV_MOVE_ROWS][kWords8<FMT>], s[KV_MOVE_ROWS];
 #pragma unroll
-      for (int k = 0; k < kMoveAhead; ++k) {
-        const int page = __builtin_amdgcn_readlane(rows.page, i0 + k), off = __builtin_amdgcn_readlane(rows.off, i0 + k);
-        s[k] = kNanScale;
-        if (i0 + k < rows.n && page >= 0) {
-          const char *at = (const char *)a.cache + (uint64_t)(uint32_t)page * page_b;
-          const char *code = at + x.code + (uint32_t)off * row_b;
-          if constexpr (FMT == KV_FP4) {
-            words[k][0] = *(const uint32_t *)code;
-          } else {
-            const u32x2 y = *(const u32x2 *)code;
-            words[k][0] = y.x;
-            words[k][1] = y.y;
-          }
-          s[k] = *(const uint8_t *)(at + x.scale + (uint32_t)off * (uint32_t)a.blocks);
+    for (int k = 0; k < KV_MOVE_ROWS; ++k) {
+      s[k] = kNanScale;
+      if (k < rows.n && of.page[k] >= 0) {
+        const char *at = (const char *)a.cache + (uint64_t)(uint32_t)of.page[k] * page_b;
+        const char *code = at + x.code + (uint32_t)of.off[k] * row_b;
+        if constexpr (FMT == KV_FP4) {
+          words[k][0] = *(const uint32_t *)code;
+        } else {
+          const u32x2 y = *(const u32x2 *)code;
+          words[k][0] = y.x;
+          words[k][1] = y.y;
         }
+        s[k] = *(const uint8_t *)(at + x.scale + (uint32_t)of.off[k] * (uint32_t)a.blocks);
       }
+    }
 #pragma unroll
-      for (int k = 0; k < kMoveAhead; ++k) {
-        if (i0 + k >= rows.n) break;
-        if (__builtin_amdgcn_readlane(rows.page, i0 + k) == -2) continue;  // no sequence's row: left as it was
-        u32x4 v = u32x4{kNan, kNan, kNan, kNan};
-        if (s[k] != kNanScale) v = values8<DT, FMT>(words[k], scale_of(s[k]));
-        *(u32x4 *)(dst + (size_t)(rows.t0 + i0 + k) * ld) = v;
-      }
+    for (int k = 0; k < KV_MOVE_ROWS; ++k) {
+      if (k >= rows.n || of.page[k] == -2) continue;  // no sequence's row: left as it was
+      u32x4 v = u32x4{kNan, kNan, kNan, kNan};
+      if (s[k] != kNanScale) v = values8<DT, FMT>(words[k], scale_of(s[k]));
+      *(u32x4 *)(dst + (size_t)(rows.t0 + k) * ld) = v;
     }
   }
 }
