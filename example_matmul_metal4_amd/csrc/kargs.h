@@ -9,7 +9,7 @@
 
 #include <stdint.h>
 
-#define MTK_KARGS_VERSION 17
+#define MTK_KARGS_VERSION 18
 
 /* In-workgroup split-K: bytes of workspace slot per output tile of BM x BM (256 or 128). Each
  * wavefront keeps these accumulator blocks (32 x 32 fp32, 4 KB) of its running sum in the slot,
@@ -176,7 +176,7 @@ typedef struct {
   /* the sequences of this launch: those with more than rows_above and at most rows_most (row, query head)
    * pairs per K/V head */
   int32_t rows_above, rows_most;
-  int32_t rows_shift, step_shift; /* log2 of the kernel's rows per block and keys per step */
+  int32_t rows_shift, step_shift; /* log2 of the kernel's rows per block; of the keys per step (chunks: 64 or more) */
   /* who does what (kv_cache.h): workgroups at most, least steps of one, or (whole) one for each pair */
   int32_t units, least, whole;
   int32_t by_pair;     /* a workgroup has steps of one pair only, the sequence's last row blocks first */
