@@ -25,10 +25,12 @@
 // than a third wavefront per SIMD won (fp8, 128 dims: 3 per SIMD 49.7 us, 4 with spills 58.7). The next tile's loads are
 // behind a branch: issued always, with an empty range past the last one, 33.0 us instead of 31.7. Loads that bypass the caches: 5 % faster on one long
 // sequence, 12 to 18 % slower where sequences share pages. Scales as whole words: 64 dims 41.4 -> 36.5 us.
-// Measured, fp4, 8 K/V heads of 128 dims, 4 query heads each, first kernel and join: 1 x 131071 positions 31.7 + 7.0 us
-// (4.5 TB/s in the first), 64 x 6000 82 + 7 (5.1 TB/s), 32 x 4096 ragged 21.8, 1 x 1000 8.8 (0.8 to find its work, 1.6 for
+// Measured, three sets of operands in turn, tables that end with the longest sequence (figures of a profiler's trace, 1 to 3 % above
+// those of a stream of calls; sets of 900 MB in turn, past the last-level cache: 1 to 10 % more): fp4, 8 K/V heads of 128 dims, 4
+// query heads each, first kernel and join: 1 x 131071 positions 32.2 + 7.2 us
+// (4.5 TB/s in the first), 64 x 6000 82 + 7 (5.1 TB/s), 32 x 4096 ragged 22.4, 1 x 1000 9.0 (0.8 to find its work, 1.6 for
 // the first bytes, 2 tiles of 1.1, 2.4 for the sum over 16 wavefronts, the launch); 64-dim heads without groups, 64 x 2048:
-// 28.2; fp8 16 x 8192: 49.7 + 4.7 (4.85 TB/s).
+// 29.4; fp8 16 x 8192: 50.4 + 4.9 (4.8 TB/s).
 #include "kv_join.hpp"
 
 namespace mtk {

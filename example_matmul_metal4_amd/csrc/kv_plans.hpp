@@ -198,9 +198,11 @@ int plan_kv_attn(mtk_ctx *ctx, const mtk_kv_desc *d_in, mtk_plan **out) {
   mtk_kv_attn_kargs k = a;  // of the sequences with few rows
   if (few) {
     const int nr = few <= 16 ? 1 : few <= 32 || dp == 256 ? 2 : 4, rows = 16 * nr;
-    // Few pairs of short sequences: one workgroup of 16 wavefronts each, no second kernel. 1000 positions, 8 pairs: 9.2 us
-    // against 13.2 with the keys split; 32 x 4000 (256 pairs): 26.8 and 32.5; but 4 x 4000 (32 pairs): 19.6 and 14.3. Longer
+    // Few pairs of short sequences: one workgroup of 16 wavefronts each, no second kernel. 1000 positions, 8 pairs: 9.0 us
+    // against 12.0 with the keys split; 32 x 4000 (256 pairs): 26.8 and 32.5; but 4 x 4000 (32 pairs): 19.6 and 14.3. Longer
     // tables would gain too where pairs fill the device and are equally long (32 x 8000: 53.6 and 62.3), not where one is long.
+    // The lengths lie on the device, so that the table's capacity stands for them here: short sequences behind a long table
+    // take the split kernels.
     const long long blocks = (long long)d.B * d.H_kv;
     const bool wide = nr == 1 && dp <= 128 && blocks <= cus && positions <= (2 * blocks >= cus ? 4096 : 2048);
     const KvShape shape = wide ? KvShape{32, 16, 1} : kv_kernel_shape(d.format, dp, nr);

@@ -14,8 +14,8 @@
 //   * Few row blocks: the keys are split over workgroups (kv_cache.h), whose partial sums kv_join adds.
 //
 // Bound by the matrix units and the VALU beside them (the exponentials, and the conversions of a tile, shared by 128 pairs):
-// 2048 rows of 32 heads of 128 dims behind 6144 positions 254 us with the launch before it, 0.95 PFLOP/s (274 to 290 under a
-// profiler), where the 16-bit kernel of attention.hpp reaches 0.93 at such sizes. With the key-splitting kernels such a
+// 2048 rows of 32 heads of 128 dims behind 6144 positions 247 us with the launch before it, 0.97 PFLOP/s (262 where the card
+// clocks lower, 269 to 300 under a profiler; fp8 257; 1024 rows of 256 dims 418, at half the rate with one workgroup per CU), where the 16-bit kernel of attention.hpp reaches 0.93 at such sizes. With the key-splitting kernels such a
 // chunk took 644 us. Converting a tile during the second product instead of the first made no difference. 500 rows of 24
 // heads, 8 K/V heads of 96 dims, 4000 positions, with a join: 50 us, with shares of equal work, which need two rounds of
 // workgroups, 68, unsplit 101.

@@ -339,8 +339,8 @@ int mtk_permute_run(const mtk_plan *plan, const mtk_permute_run_args *args);
  *   table [B][max_pages]      its pages in order; entries past its length are not used
  * The kernels check all of it: a position whose page is out of [0, n_pages), or past the table, or below 0 is not written,
  * reads as NaN, and makes the attention of the rows that see it NaN; a kv_len of more than the table holds makes all of its
- * sequence's rows that see a position NaN. row_start is limited to [0, T] and to ascend; rows that two sequences claim come out
- * as one or the other's, or undefined in attention. Two sequences may share pages; where both are written at one position of
+ * sequence's rows that see a position NaN. row_start is limited to [0, T], and a sequence whose end lies before its start has no
+ * rows; rows that two sequences claim come out as one or the other's, but attention's outputs of such a batch are undefined. Two sequences may share pages; where both are written at one position of
  * one page in one call, its bytes are some mix of the two.
  * What an operator writes (the cache, the rows read back, O, lse, the workspace) may not overlap what it reads, these arrays among
  * it, or its other outputs; slices of one buffer whose rows lie between each other do not.
@@ -388,9 +388,11 @@ int mtk_kv_read_run(const mtk_plan *plan, const mtk_kv_read_args *args);
  * K/V head h / (H / H_kv). The new rows' own K and V are read from the cache: write them first. A row that sees no
  * position gives zeros and a log-sum-exp of -inf; one whose scores are all -inf (infinities in Q) gives NaN and -inf, and one
  * with a score of +inf or NaN gives NaN in both. Scores are held in 32 bits: beyond 2^27 in magnitude they are too coarse for
- * weights. The keys of long sequences are split over workgroups, whose partial
- * sums lie in the workspace until a second kernel adds them in a fixed order: the result does not vary from run to run,
- * and runs that may overlap need a workspace each.
+ * weights. So are the sums of weights times values, the weights up to 2^8 in bf16: values of more than 2^120 / positions may
+ * overflow there. The keys of long sequences are split over workgroups, whose partial sums lie in the workspace until a second
+ * kernel adds them in a fixed order: the result does not vary from run to run, and runs that may overlap need a workspace each.
+ * max_pages x page_size, the table's capacity, decides whether keys may be split: never up to 1024 positions, up to 2048 or 4096 by
+ * the sequences and heads (mtk_plan_describe tells). Short sequences behind a longer table take 3 to 5 us more.
  * A plan whose sequences may have more than 64 (row, query head) pairs per K/V head (32 above 128 dims) has kernels for those
  * and, where S_q > 1, for the sequences with few rows beside them: give S_q = 1 for a batch of single tokens. */
 int mtk_kv_attn_plan(mtk_ctx *ctx, const mtk_kv_desc *desc, mtk_plan **out);
