@@ -8,7 +8,7 @@ import pytest
 
 import example_matmul_metal4_amd as mtk
 
-DRIVER = r"""
+PROGRAM = r"""
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
@@ -87,7 +87,7 @@ def test_every_row_of_a_sequence_is_joined_once(tmp_path):
     if shutil.which("g++") is None:
         pytest.skip("needs g++")
     src, exe = tmp_path / "walk.cpp", tmp_path / "walk"
-    src.write_text(DRIVER)
+    src.write_text(PROGRAM)
     r = subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover=all",
                         f"-I{os.path.join(mtk.PKG, 'csrc')}", str(src), "-o", str(exe)], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr[-3000:]

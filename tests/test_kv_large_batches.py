@@ -39,7 +39,7 @@ def test_batches_past_the_sums_are_refused():
         assert e.value.status == mtk.MTK_ERR_UNSUPPORTED and e.value.message
 
 
-DRIVER = r"""
+PROGRAM = r"""
 #include "runtime.cpp"
 #include <random>
 
@@ -117,7 +117,7 @@ def test_schedule(tmp_path):
     if shutil.which("g++") is None or not os.path.exists(scratch_obj):
         pytest.skip("needs g++ and a built library (python -m example_matmul_metal4_amd.build)")
     src, exe = tmp_path / "large.cpp", tmp_path / "large"
-    src.write_text(DRIVER)
+    src.write_text(PROGRAM)
     r = subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-D__HIP_PLATFORM_AMD__",
                         f"-I{ROCM}/include", f"-I{os.path.join(mtk.PKG, 'csrc')}", str(src), scratch_obj, f"-L{ROCM}/lib",
                         "-lamdhip64", f"-Wl,-rpath,{ROCM}/lib", "-ldl", "-o", str(exe)], capture_output=True, text=True)

@@ -10,7 +10,7 @@ import example_matmul_metal4_amd as mtk
 
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
-DRIVER = r"""
+PROGRAM = r"""
 #include "runtime.cpp"
 #include <random>
 
@@ -110,7 +110,7 @@ def test_overlaps(tmp_path):
     if shutil.which("g++") is None or not os.path.exists(scratch_obj):
         pytest.skip("needs g++ and a built library (python -m example_matmul_metal4_amd.build)")
     src, exe = tmp_path / "overlaps.cpp", tmp_path / "overlaps"
-    src.write_text(DRIVER)
+    src.write_text(PROGRAM)
     r = subprocess.run(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-D__HIP_PLATFORM_AMD__",
                         f"-I{ROCM}/include", f"-I{os.path.join(mtk.PKG, 'csrc')}", str(src), scratch_obj, f"-L{ROCM}/lib",
                         "-lamdhip64", f"-Wl,-rpath,{ROCM}/lib", "-ldl", "-o", str(exe)], capture_output=True, text=True)
