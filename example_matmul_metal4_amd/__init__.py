@@ -132,6 +132,38 @@ class KvAttnArgs(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("Q", "cache", "row_start", "kv_len", "table", "O", "lse", "workspace")]
 
 
+class GroupedDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("E", "T", "N", "K", "lda", "ldb", "ldc", "trans_b", "dtype", "has_bias", "out_f32")]
+
+
+class GroupedGemmArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("A", "B", "bias", "row_start", "C", "workspace")]
+
+
+class GroupedGradArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("A", "dC", "row_start", "dB", "dbias", "workspace")]
+
+
+class MxRowsDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("R", "K", "ld", "dtype")]
+
+
+class MxQuantizeArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("src", "codes", "scales")]
+
+
+class MxDequantizeArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("codes", "scales", "dst")]
+
+
+class MxGemmDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("E", "T", "N", "K", "lda", "ldc", "dtype", "has_bias", "quantize_a")]
+
+
+class MxGemmArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("A", "a_scales", "B", "b_scales", "bias", "row_start", "C", "workspace")]
+
+
 class Timing(ctypes.Structure):
     _fields_ = [("total_ms", ctypes.c_double), ("kernel_ms", ctypes.c_double * 4), ("n_kernels", ctypes.c_int),
                 ("kernel_names", (ctypes.c_char * 64) * 4)]
@@ -182,6 +214,17 @@ SIGNATURES = {
     "mtk_kv_read_run": (ctypes.c_int, [_VP, ctypes.POINTER(KvReadArgs)]),
     "mtk_kv_attn_plan": (ctypes.c_int, [_VP, ctypes.POINTER(KvDesc), _PP]),
     "mtk_kv_attn_run": (ctypes.c_int, [_VP, ctypes.POINTER(KvAttnArgs)]),
+    "mtk_grouped_gemm_plan": (ctypes.c_int, [_VP, ctypes.POINTER(GroupedDesc), _PP]),
+    "mtk_grouped_gemm_run": (ctypes.c_int, [_VP, ctypes.POINTER(GroupedGemmArgs)]),
+    "mtk_grouped_grad_plan": (ctypes.c_int, [_VP, ctypes.POINTER(GroupedDesc), _PP]),
+    "mtk_grouped_grad_run": (ctypes.c_int, [_VP, ctypes.POINTER(GroupedGradArgs)]),
+    "mtk_mx_bytes": (ctypes.c_int, [ctypes.c_int, ctypes.c_int] + [ctypes.POINTER(ctypes.c_size_t)] * 2),
+    "mtk_mx_quantize_plan": (ctypes.c_int, [_VP, ctypes.POINTER(MxRowsDesc), _PP]),
+    "mtk_mx_quantize_run": (ctypes.c_int, [_VP, ctypes.POINTER(MxQuantizeArgs)]),
+    "mtk_mx_dequantize_plan": (ctypes.c_int, [_VP, ctypes.POINTER(MxRowsDesc), _PP]),
+    "mtk_mx_dequantize_run": (ctypes.c_int, [_VP, ctypes.POINTER(MxDequantizeArgs)]),
+    "mtk_mx_gemm_plan": (ctypes.c_int, [_VP, ctypes.POINTER(MxGemmDesc), _PP]),
+    "mtk_mx_gemm_run": (ctypes.c_int, [_VP, ctypes.POINTER(MxGemmArgs)]),
     "mtk_plan_workspace_bytes": (ctypes.c_size_t, [_VP]),
     "mtk_plan_describe": (ctypes.c_int, [_VP, ctypes.c_char_p, ctypes.c_size_t]),
     "mtk_plan_work": (ctypes.c_int, [_VP, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]),
@@ -651,6 +694,126 @@ class KvAttentionPlan(_KvPlan):
         self._run(self.args(Q, cache, row_start, kv_len, table, O, lse, workspace))
 
 
+# ------------------------------------------------------------------ products grouped by expert
+
+class _DescPlan(_Plan):
+    _plan_fn = None
+
+    def __init__(self, device: Device | None, desc):
+        self.desc = desc
+        h = ctypes.c_void_p()
+        _check(getattr(lib(), self._plan_fn)(device.handle if device else None, ctypes.byref(desc), ctypes.byref(h)))
+        super().__init__(h)
+
+
+class GroupedGemmPlan(_DescPlan):
+    """C[t] = A[t] op(B_e) + bias_e for the rows t of group e: A [T][K], B [E][N][K] (trans_b) or [E][K][N], bias [E][N],
+    C [T][N]; row_start [E + 1], int32 on the device: group e has the rows row_start[e] .. row_start[e + 1] - 1. With N and K
+    exchanged and trans_b inverted it is the input gradient over the same weights."""
+
+    _args_type = GroupedGemmArgs
+    _run_fn = "mtk_grouped_gemm_run"
+    _plan_fn = "mtk_grouped_gemm_plan"
+
+    def __init__(self, device: Device | None, E, T, N, K, *, trans_b=True, dtype="f16", has_bias=False, lda=0, ldb=0, ldc=0):
+        super().__init__(device, GroupedDesc(E=E, T=T, N=N, K=K, lda=lda, ldb=ldb, ldc=ldc, trans_b=1 if trans_b else 0,
+                                             dtype=_DT[dtype], has_bias=1 if has_bias else 0))
+
+    @staticmethod
+    def args(A, B, bias, row_start, C, workspace=None) -> GroupedGemmArgs:
+        return GroupedGemmArgs(A=_ptr(A), B=_ptr(B), bias=_ptr(bias), row_start=_ptr(row_start), C=_ptr(C), workspace=_ptr(workspace))
+
+    def run(self, A, B, bias, row_start, C, workspace=None):
+        self._run(self.args(A, B, bias, row_start, C, workspace))
+
+
+class GroupedGradPlan(_DescPlan):
+    """The gradients of a grouped product's weights and bias: dB_e = dC_e^T A_e ([E][N][K] with trans_b, else [E][K][N]) and
+    dbias_e, the column sums of dC_e; in 16 bits, or fp32 with out_f32. Groups without a row get zeros."""
+
+    _args_type = GroupedGradArgs
+    _run_fn = "mtk_grouped_grad_run"
+    _plan_fn = "mtk_grouped_grad_plan"
+
+    def __init__(self, device: Device | None, E, T, N, K, *, trans_b=True, dtype="f16", has_bias=False, out_f32=False, lda=0, ldc=0):
+        super().__init__(device, GroupedDesc(E=E, T=T, N=N, K=K, lda=lda, ldc=ldc, trans_b=1 if trans_b else 0, dtype=_DT[dtype],
+                                             has_bias=1 if has_bias else 0, out_f32=1 if out_f32 else 0))
+
+    @staticmethod
+    def args(A, dC, row_start, dB, dbias=None, workspace=None) -> GroupedGradArgs:
+        return GroupedGradArgs(A=_ptr(A), dC=_ptr(dC), row_start=_ptr(row_start), dB=_ptr(dB), dbias=_ptr(dbias),
+                               workspace=_ptr(workspace))
+
+    def run(self, A, dC, row_start, dB, dbias=None, workspace=None):
+        self._run(self.args(A, dC, row_start, dB, dbias, workspace))
+
+
+# ------------------------------------------------------------------ rows and products in 4 bits
+
+def mx_bytes(R, K) -> tuple[int, int]:
+    """Bytes of the codes and of the scales of R rows of K values (mtk_mx_bytes)."""
+    c, s = ctypes.c_size_t(), ctypes.c_size_t()
+    _check(lib().mtk_mx_bytes(R, K, ctypes.byref(c), ctypes.byref(s)))
+    return int(c.value), int(s.value)
+
+
+class MxQuantizePlan(_DescPlan):
+    """16-bit rows [R][ld] into blocks of 32 e2m1 values with one power-of-two scale; include/mtk.h has the layout."""
+
+    _args_type = MxQuantizeArgs
+    _run_fn = "mtk_mx_quantize_run"
+    _plan_fn = "mtk_mx_quantize_plan"
+
+    def __init__(self, device: Device | None, R, K, *, dtype="f16", ld=0):
+        super().__init__(device, MxRowsDesc(R=R, K=K, ld=ld, dtype=_DT[dtype]))
+
+    @staticmethod
+    def args(src, codes, scales) -> MxQuantizeArgs:
+        return MxQuantizeArgs(src=_ptr(src), codes=_ptr(codes), scales=_ptr(scales))
+
+    def run(self, src, codes, scales):
+        self._run(self.args(src, codes, scales))
+
+
+class MxDequantizePlan(_DescPlan):
+    """Rows of MxQuantizePlan back in 16 bits, exactly."""
+
+    _args_type = MxDequantizeArgs
+    _run_fn = "mtk_mx_dequantize_run"
+    _plan_fn = "mtk_mx_dequantize_plan"
+
+    def __init__(self, device: Device | None, R, K, *, dtype="f16", ld=0):
+        super().__init__(device, MxRowsDesc(R=R, K=K, ld=ld, dtype=_DT[dtype]))
+
+    @staticmethod
+    def args(codes, scales, dst) -> MxDequantizeArgs:
+        return MxDequantizeArgs(codes=_ptr(codes), scales=_ptr(scales), dst=_ptr(dst))
+
+    def run(self, codes, scales, dst):
+        self._run(self.args(codes, scales, dst))
+
+
+class MxGemmPlan(_DescPlan):
+    """C[t] = A[t] B_e^T + bias_e with A and B held in 4 bits: A T rows, B E x N rows (E 0: one product, B N rows, no
+    row_start). quantize_a: A are 16-bit rows that the run brings into the format first (a_scales None)."""
+
+    _args_type = MxGemmArgs
+    _run_fn = "mtk_mx_gemm_run"
+    _plan_fn = "mtk_mx_gemm_plan"
+
+    def __init__(self, device: Device | None, T, N, K, *, E=0, dtype="f16", has_bias=False, quantize_a=False, lda=0, ldc=0):
+        super().__init__(device, MxGemmDesc(E=E, T=T, N=N, K=K, lda=lda, ldc=ldc, dtype=_DT[dtype], has_bias=1 if has_bias else 0,
+                                            quantize_a=1 if quantize_a else 0))
+
+    @staticmethod
+    def args(A, a_scales, B, b_scales, bias, row_start, C, workspace=None) -> MxGemmArgs:
+        return MxGemmArgs(A=_ptr(A), a_scales=_ptr(a_scales), B=_ptr(B), b_scales=_ptr(b_scales), bias=_ptr(bias),
+                          row_start=_ptr(row_start), C=_ptr(C), workspace=_ptr(workspace))
+
+    def run(self, A, a_scales, B, b_scales, bias, row_start, C, workspace=None):
+        self._run(self.args(A, a_scales, B, b_scales, bias, row_start, C, workspace))
+
+
 # ------------------------------------------------------------------ harness-level calls
 
 def gemm(dev: Device, A, B, bias=None, *, trans_b=True, dtype="f16", split_k=1, tile=0,
@@ -743,4 +906,5 @@ def validate(actual, expected, abs_tol: float, dtype="f16") -> dict:
 
 
 __all__ = ["Device", "DeviceBuffer", "GemmPlan", "AttentionPlan", "ConvPlan", "KvWritePlan", "KvReadPlan",
-           "KvAttentionPlan", "kv_cache_bytes", "conv_desc", "gemm", "attention", "conv", "validate", "MtkError", "lib", "SIGNATURES"]
+           "KvAttentionPlan", "kv_cache_bytes", "GroupedGemmPlan", "GroupedGradPlan", "MxQuantizePlan",
+           "MxDequantizePlan", "MxGemmPlan", "mx_bytes", "conv_desc", "gemm", "attention", "conv", "validate", "MtkError", "lib", "SIGNATURES"]

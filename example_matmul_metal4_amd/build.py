@@ -25,7 +25,7 @@ LIB = os.path.join(PKG, "lib")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 HIP_UNITS = ["gemm_f16", "gemm_bf16", "conv", "attention", "attention_hd", "attention_bwd", "attention_bwd256", "attention_wide", "attention_kv",
-             "kv_store", "kv_attention", "kv_prefill", "skinny", "permute", "util"]
+             "grouped_f16", "grouped_bf16", "mx_rows", "mx_gemm", "kv_store", "kv_attention", "kv_prefill", "skinny", "permute", "util"]
 
 HIPCC_FLAGS = [
     "--genco", "--offload-arch=gfx950", "-O3", "-std=c++17",

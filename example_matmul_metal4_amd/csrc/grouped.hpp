@@ -1,0 +1,219 @@
+// Products grouped by expert: C[t] = A[t] op(B_e) + bias_e for the rows t of group e, and the weights' gradients
+// dB_e = sum over its rows of dC[t] x A[t]. The tiles are the GEMM's (tile_direct.hpp, quarter.hpp); here a workgroup
+// finds its group and tile, and narrows operands and buffer ranges to them.
+//
+// Where the groups start lies on the device, so a launch's grid is what ascending groups need at most, and workgroups past
+// what they do need end at once. Every wavefront looks its tile up by itself: the groups' block counts, 64 groups to a
+// window of lanes, summed over the lanes; the tiles of all groups, one group after another, are dealt to the XCDs in
+// contiguous runs of the count that there is (not of the grid's), so that neighbours share an L2 and no XCD goes idle.
+// Rows behind a group's end are out of the tile's buffer range: they read as zeros, whatever the next group holds.
+#pragma once
+
+#include "groups.h"
+#include "quarter.hpp"
+#include "tile_direct.hpp"
+
+namespace mtk {
+
+// Inclusive sum over the lanes up to this one.
+__device__ __forceinline__ int lanes_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return x;
+}
+
+// A window of 64 groups in the lanes.
+struct GroupWindow {
+  group_rows g;
+  int end;  // blocks of the window's groups up to this lane's
+  __device__ __forceinline__ GroupWindow(const int32_t *row_start, int E, int T, int block, int e0) {
+    const int e = e0 + (threadIdx.x & 63);
+    g = e < E ? group_of(row_start[e], row_start[e + 1], T) : group_rows{0, 0};
+    end = lanes_scan((g.rows + block - 1) / block);
+  }
+  __device__ __forceinline__ int blocks() const { return __builtin_amdgcn_readlane(end, 63); }
+};
+
+// A workgroup's group, and which of the group's blocks x tiles_n tiles it has.
+struct GroupTile {
+  int e = -1;  // none
+  int first, rows, blocks, t;
+};
+
+template <int BLOCK>
+__device__ __forceinline__ GroupTile group_tile(const int32_t *row_start, int E, int T, int tiles_n) {
+  GroupTile r;
+  GroupWindow w(row_start, E, T, BLOCK, 0);
+  int total = w.blocks();
+#pragma unroll 1
+  for (int e0 = 64; e0 < E; e0 += 64) total += GroupWindow(row_start, E, T, BLOCK, e0).blocks();
+  total *= tiles_n;
+  if ((int)blockIdx.x >= total) return r;
+  int id = xcd_remap(blockIdx.x, total);
+#pragma unroll 1
+  for (int e0 = 0;;) {
+    const uint64_t in = __ballot(w.end * tiles_n > id);
+    if (in) {
+      const int i = __builtin_ctzll(in);
+      const int end = __builtin_amdgcn_readlane(w.end, i);
+      r.e = e0 + i;
+      r.first = __builtin_amdgcn_readlane(w.g.first, i);
+      r.rows = __builtin_amdgcn_readlane(w.g.rows, i);
+      r.blocks = (r.rows + BLOCK - 1) / BLOCK;
+      r.t = id - (end - r.blocks) * tiles_n;
+      return r;
+    }
+    id -= w.blocks() * tiles_n;
+    e0 += 64;
+    if (e0 >= E) return r;  // never: id < total
+    w = GroupWindow(row_start, E, T, BLOCK, e0);
+  }
+}
+
+// Bytes from the dword in which an operand starts to the end of its last element's dword.
+__device__ __forceinline__ uint32_t range_of(const void *p, uint32_t exact, bool any) {
+  return (exact + (any ? (uint32_t)(uintptr_t)p & 2u : 0u) + 3u) & ~3u;
+}
+
+// The part of the GEMM's arguments that a tile of group e takes: `rows` rows of A from `row` on, one block at most.
+template <int BLOCK, bool ANY>
+__device__ __forceinline__ mtk_tile_args group_args(const mtk_grouped_kargs &g, int e, int row, int rows) {
+  mtk_tile_args a{};
+  rows = min(rows, BLOCK);
+  a.A = (const uint16_t *)g.A + (size_t)row * (size_t)g.lda;
+  a.B = (const uint16_t *)g.B + (size_t)e * (size_t)g.b_stride;
+  a.bias = (const uint16_t *)g.bias + (size_t)e * (size_t)g.N;
+  a.C = (uint16_t *)g.C + (size_t)row * (size_t)g.ldc;
+  a.M = rows;
+  a.N = g.N;
+  a.K = g.K;
+  a.lda = g.lda;
+  a.ldb = g.ldb;
+  a.ldc = g.ldc;
+  a.a_bytes = range_of(a.A, ((uint32_t)(rows - 1) * (uint32_t)g.lda + (uint32_t)g.K) * 2u, ANY);
+  a.b_bytes = range_of(a.B, g.b_exact, ANY);
+  a.k_tiles = a.k_tiles_per_split = g.k_tiles;
+  a.split_k = 1;
+  a.has_bias = g.has_bias;
+  return a;
+}
+
+// Row block and column of tile t of a group, groups of 4 row blocks at a time as in the GEMM.
+template <int BM, int BN>
+__device__ __forceinline__ TileAt tile_at(int t, int blocks, int tiles_n) {
+  const int group = kGroupM * tiles_n;
+  const int first = (t / group) * kGroupM;
+  const int gm = min(blocks - first, kGroupM);
+  return TileAt{(first + (t % group) % gm) * BM, (t % group) / gm * BN};
+}
+
+template <int DT, int BM, int WAVES_M, int WAVES_N, typename AOP, typename BOP>
+__device__ __forceinline__ void grouped_direct(const mtk_grouped_kargs &g) {
+  const GroupTile gt = group_tile<BM>(g.row_start, g.E, g.T, g.tiles_n);
+  if (gt.e < 0) return;
+  const TileAt at = tile_at<BM, BM>(gt.t, gt.blocks, g.tiles_n);
+  const mtk_tile_args a = group_args<BM, false>(g, gt.e, gt.first + at.m0, gt.rows - at.m0);
+  tile_direct<DT, BM, BM, WAVES_M, WAVES_N, AOP, BOP, false, true>(a, TileAt{0, at.n0});
+}
+
+template <int DT, bool BN, bool ANY, int W>
+__device__ __forceinline__ void grouped_quarter(const mtk_grouped_kargs &g) {
+  const GroupTile gt = group_tile<64>(g.row_start, g.E, g.T, g.tiles_n);
+  if (gt.e < 0) return;
+  const TileAt at = tile_at<64, 64>(gt.t, gt.blocks, g.tiles_n);
+  const mtk_tile_args a = group_args<64, ANY>(g, gt.e, gt.first + at.m0, gt.rows - at.m0);
+  using A = QuarterOp<false, ANY>;
+  quarter_tile<DT, A, BN, ANY, W, true>(a, A{}, TileAt{0, at.n0});
+}
+
+// Gradients: K runs over the group's rows, of which both operands hold K rows of M and of N columns. A group without a row has
+// zeros.
+template <bool ANY>
+__device__ __forceinline__ mtk_tile_args grad_args(const mtk_grouped_kargs &g, int e) {
+  mtk_tile_args a{};
+  const int start = __builtin_amdgcn_readfirstlane(g.row_start[e]), next = __builtin_amdgcn_readfirstlane(g.row_start[e + 1]);
+  const group_rows r = group_of(start, next, g.T);
+  a.A = (const uint16_t *)g.A + (size_t)r.first * (size_t)g.lda;
+  a.B = (const uint16_t *)g.B + (size_t)r.first * (size_t)g.ldb;
+  const size_t out = (size_t)e * (size_t)g.M * (size_t)g.N;
+  a.C = (uint16_t *)g.C + out;
+  a.partial = g.C32 ? g.C32 + out : nullptr;
+  a.M = g.M;
+  a.N = g.N;
+  a.K = r.rows;
+  a.lda = g.lda;
+  a.ldb = g.ldb;
+  a.ldc = g.N;
+  a.a_bytes = r.rows ? range_of(a.A, ((uint32_t)(r.rows - 1) * (uint32_t)g.lda + (uint32_t)g.M) * 2u, ANY) : 0u;
+  a.b_bytes = r.rows ? range_of(a.B, ((uint32_t)(r.rows - 1) * (uint32_t)g.ldb + (uint32_t)g.N) * 2u, ANY) : 0u;
+  a.k_tiles = a.k_tiles_per_split = (r.rows + kBK - 1) / kBK;
+  a.split_k = 1;
+  return a;
+}
+
+template <int DT, int BM, int WAVES_M, int WAVES_N, typename AOP, typename BOP>
+__device__ __forceinline__ void grouped_grad_direct(const mtk_grouped_kargs &g) {
+  const int tiles = g.tiles_m * g.tiles_n, id = xcd_remap(blockIdx.x, gridDim.x), e = id / tiles;
+  const mtk_tile_args a = grad_args<false>(g, e);
+  tile_direct<DT, BM, BM, WAVES_M, WAVES_N, AOP, BOP, false, true>(a, tile_at<BM, BM>(id - e * tiles, g.tiles_m, g.tiles_n));
+}
+
+template <int DT, bool ANY, int W>
+__device__ __forceinline__ void grouped_grad_quarter(const mtk_grouped_kargs &g) {
+  const int tiles = g.tiles_m * g.tiles_n, id = xcd_remap(blockIdx.x, gridDim.x), e = id / tiles;
+  const mtk_tile_args a = grad_args<ANY>(g, e);
+  using A = QuarterOp<true, ANY>;
+  quarter_tile<DT, A, true, ANY, W, true>(a, A{}, tile_at<64, 64>(id - e * tiles, g.tiles_m, g.tiles_n));
+}
+
+// dbias_e[n] = sum over the group's rows of dC[t][n]: 128 columns per workgroup, two per lane; its 8 wavefronts take every
+// 8th row, and their sums in 32 bits are added in wavefront order.
+constexpr int kBiasWaves = 8, kBiasCols = 128;
+template <int DT>
+__device__ __forceinline__ void grouped_bias_grad(const mtk_grouped_kargs &g) {
+  __shared__ float sums[kBiasWaves][kBiasCols];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int e = blockIdx.x / g.tiles_n, n0 = (blockIdx.x - e * g.tiles_n) * kBiasCols;
+  const int start = __builtin_amdgcn_readfirstlane(g.row_start[e]), next = __builtin_amdgcn_readfirstlane(g.row_start[e + 1]);
+  const group_rows r = group_of(start, next, g.T);
+  float s0 = 0.0f, s1 = 0.0f;
+  const int n = n0 + 2 * lane;
+  const uint16_t *at = (const uint16_t *)g.A + (size_t)r.first * (size_t)g.lda + n;
+  const bool pair = ((g.lda & 1) == 0) && (((uintptr_t)g.A & 3) == 0);  // whole dwords
+  if (pair && n + 1 < g.N) {
+#pragma unroll 8
+    for (int i = wave; i < r.rows; i += kBiasWaves) {
+      const uint32_t v = *(const uint32_t *)(at + (size_t)i * (size_t)g.lda);
+      s0 += from_bits<DT>(v & 0xffffu);
+      s1 += from_bits<DT>(v >> 16);
+    }
+  } else if (n < g.N) {
+    const bool two = n + 1 < g.N;
+#pragma unroll 4
+    for (int i = wave; i < r.rows; i += kBiasWaves) {
+      const uint16_t *p = at + (size_t)i * (size_t)g.lda;
+      s0 += from_bits<DT>(p[0]);
+      if (two) s1 += from_bits<DT>(p[1]);
+    }
+  }
+  sums[wave][2 * lane] = s0;
+  sums[wave][2 * lane + 1] = s1;
+  __syncthreads();
+  const int c = threadIdx.x;
+  if (c < kBiasCols && n0 + c < g.N) {
+    float s = sums[0][c];
+#pragma unroll
+    for (int w = 1; w < kBiasWaves; ++w) s += sums[w][c];
+    const size_t out = (size_t)e * (size_t)g.N + n0 + c;
+    if (g.C32)
+      g.C32[out] = s;
+    else
+      ((uint16_t *)g.C)[out] = to_bits<DT>(s);
+  }
+}
+
+}  // namespace mtk

@@ -1,0 +1,437 @@
+// Plans of products grouped by expert and of rows and products in few bits (include/mtk.h, groups.h, mx.h): checks, kernel
+// choice and argument blocks. Part of runtime.cpp's translation unit, inside its unnamed namespace.
+
+constexpr int kMaxWidth = 1 << 22;  // N, K and leading dimensions: 256 rows of a tile, and 64 past an operand's end, stay in 32 bits
+
+bool is_grouped(const mtk_plan *p) { return p->kind >= PLAN_GROUPED && p->kind <= PLAN_MX_GEMM; }
+
+int check_ld(int ld, int width, const char *name, int *out) {
+  *out = ld ? ld : width;
+  if (ld != 0 && ld < width) return fail(MTK_ERR_INVALID, "%s must be 0 or at least %d (got %d)", name, width, ld);
+  if (*out > kMaxWidth) return fail(MTK_ERR_UNSUPPORTED, "%s of more than 2^22 (%d) is not supported", name, *out);
+  return MTK_OK;
+}
+
+int finish_plan(mtk_plan *p, mtk_plan **out) {
+  const int s = resolve(p);
+  if (s != MTK_OK) {
+    delete p;
+    return s;
+  }
+  *out = p;
+  return MTK_OK;
+}
+
+template <typename T>
+void add_launch(mtk_plan *p, const std::string &name, long long grid, int block, const T &args) {
+  Launch l;
+  l.name = name;
+  l.grid = (unsigned)grid;
+  l.block = (unsigned)block;
+  set_args(l, args);
+  p->launches.push_back(l);
+}
+
+int check_grouped(const mtk_grouped_desc &d) {
+  if (d.E <= 0 || d.T <= 0 || d.N <= 0 || d.K <= 0)
+    return fail(MTK_ERR_INVALID, "E, T, N and K must be positive (got %d, %d, %d, %d)", d.E, d.T, d.N, d.K);
+  if (d.N > kMaxWidth || d.K > kMaxWidth) return fail(MTK_ERR_UNSUPPORTED, "N and K above 2^22 are not supported (got %d, %d)", d.N, d.K);
+  if (d.E > (1 << 20)) return fail(MTK_ERR_UNSUPPORTED, "E above 2^20 is not supported (got %d)", d.E);
+  if (d.dtype != MTK_F16 && d.dtype != MTK_BF16) return fail(MTK_ERR_INVALID, "dtype must be MTK_F16 or MTK_BF16");
+  return MTK_OK;
+}
+
+// The blocks of a launch that finds its tiles from row_start: at most `blocks` of them if the groups ascend, and no count
+// passes 32 bits whatever row_start holds.
+int check_tiles(int E, int T, int block, long long tiles_n, long long *grid) {
+  *grid = group_max_blocks(E, T, block) * tiles_n;
+  if ((long long)E * ((T + block - 1) / block) * tiles_n > INT32_MAX || *grid > INT32_MAX / 512)
+    return fail(MTK_ERR_UNSUPPORTED, "%d groups of up to %d rows with this N are not supported", E, T);
+  return MTK_OK;
+}
+
+const char *dtype_name(int dtype) { return dtype == MTK_F16 ? "f16" : "bf16"; }
+
+int plan_grouped(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
+  if (!d_in || !out) return fail(MTK_ERR_INVALID, "null descriptor or output");
+  mtk_grouped_desc d = *d_in;
+  int s = check_grouped(d);
+  if (s != MTK_OK) return s;
+  if (d.out_f32) return fail(MTK_ERR_INVALID, "out_f32 is for gradients");
+  if ((s = check_ld(d.lda, d.K, "lda", &d.lda)) != MTK_OK || (s = check_ld(d.ldb, d.trans_b ? d.K : d.N, "ldb", &d.ldb)) != MTK_OK ||
+      (s = check_ld(d.ldc, d.N, "ldc", &d.ldc)) != MTK_OK)
+    return s;
+  const long long b_rows = d.trans_b ? d.N : d.K, b_width = d.trans_b ? d.K : d.N;
+  const uint64_t b_exact = 2 * ((uint64_t)(b_rows - 1) * (uint64_t)d.ldb + (uint64_t)b_width);
+  if (b_exact > kMaxOperandBytes) return fail(MTK_ERR_UNSUPPORTED, "the weights of a group must be below 2 GiB");
+  const int cus = ctx ? ctx->prop.multiProcessorCount : 256;
+  const bool even = d.lda % 2 == 0 && d.ldb % 2 == 0;
+  auto wgs = [&](int tile) { return group_max_blocks(d.E, d.T, tile) * ((d.N + tile - 1) / tile); };
+  int tile = 64;
+  if (even && wgs(256) >= cus * 5 / 8 && d.T >= 64LL * d.E) tile = 256;
+  else if (even && wgs(128) >= cus && d.T >= 32LL * d.E) tile = 128;
+  mtk_grouped_kargs a{};
+  a.E = d.E;
+  a.T = d.T;
+  a.N = d.N;
+  a.K = d.K;
+  a.lda = d.lda;
+  a.ldb = d.ldb;
+  a.ldc = d.ldc;
+  a.b_stride = b_rows * d.ldb;
+  a.b_exact = (uint32_t)b_exact;
+  a.tiles_n = (d.N + tile - 1) / tile;
+  a.k_tiles = (d.K + 63) / 64;
+  a.has_bias = d.has_bias ? 1 : 0;
+  long long grid;
+  if ((s = check_tiles(d.E, d.T, tile, a.tiles_n, &grid)) != MTK_OK) return s;
+  mtk_plan *p = new mtk_plan();
+  p->ctx = ctx;
+  p->kind = PLAN_GROUPED;
+  p->grouped = d;
+  p->align_a = p->align_b = even ? 4 : 2;
+  const std::string name = std::string("mtk_grouped_") + dtype_name(d.dtype) + (d.trans_b ? "_nt_" : "_nn_") + std::to_string(tile) +
+                           (even ? "" : "_any");
+  add_launch(p, name, grid, tile == 128 ? 256 : 512, a);
+  p->flops = 2.0 * d.T * d.N * d.K;
+  p->bytes = 2.0 * ((double)d.T * (d.N + d.K) + (double)std::min(d.E, d.T) * d.N * d.K);
+  char desc[256];
+  snprintf(desc, sizeof desc, "grouped gemm %s E=%d T=%d N=%d K=%d b=%s bias=%d tile=%d grid=%lld kernel=%s", dtype_name(d.dtype), d.E, d.T,
+           d.N, d.K, d.trans_b ? "nk" : "kn", a.has_bias, tile, grid, name.c_str());
+  p->description = desc;
+  return finish_plan(p, out);
+}
+
+int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
+  if (!d_in || !out) return fail(MTK_ERR_INVALID, "null descriptor or output");
+  mtk_grouped_desc d = *d_in;
+  int s = check_grouped(d);
+  if (s != MTK_OK) return s;
+  if (d.ldb) return fail(MTK_ERR_INVALID, "gradients of the weights are packed: ldb must be 0 (got %d)", d.ldb);
+  if ((s = check_ld(d.lda, d.K, "lda", &d.lda)) != MTK_OK || (s = check_ld(d.ldc, d.N, "ldc", &d.ldc)) != MTK_OK) return s;
+  for (int ld : {d.lda, d.ldc})
+    if (2ull * (uint64_t)d.T * (uint64_t)ld > kMaxOperandBytes) return fail(MTK_ERR_UNSUPPORTED, "A and dC must be below 2 GiB");
+  const int cus = ctx ? ctx->prop.multiProcessorCount : 256;
+  const bool even = d.lda % 2 == 0 && d.ldc % 2 == 0;
+  mtk_grouped_kargs a{};
+  a.E = d.E;
+  a.T = d.T;
+  a.M = d.trans_b ? d.N : d.K;
+  a.N = d.trans_b ? d.K : d.N;
+  a.lda = d.trans_b ? d.ldc : d.lda;
+  a.ldb = d.trans_b ? d.lda : d.ldc;
+  auto tiles = [&](int tile, int n) { return (long long)((n + tile - 1) / tile); };
+  auto wgs = [&](int tile) { return d.E * tiles(tile, a.M) * tiles(tile, a.N); };
+  int tile = 64;
+  if (even && wgs(256) >= cus * 5 / 8) tile = 256;
+  else if (even && wgs(128) >= cus) tile = 128;
+  a.tiles_m = (int)tiles(tile, a.M);
+  a.tiles_n = (int)tiles(tile, a.N);
+  const long long grid = wgs(tile);
+  const long long bias_tiles = tiles(128, d.N);
+  if (grid > INT32_MAX / 512 || d.E * bias_tiles > INT32_MAX / 512)
+    return fail(MTK_ERR_UNSUPPORTED, "%d groups with these N and K are not supported", d.E);
+  mtk_plan *p = new mtk_plan();
+  p->ctx = ctx;
+  p->kind = PLAN_GROUPED_GRAD;
+  p->grouped = d;
+  p->align_a = p->align_b = even ? 4 : 2;
+  const std::string head = std::string("mtk_grouped_") + dtype_name(d.dtype);
+  const std::string name = head + "_grad_" + std::to_string(tile) + (even ? "" : "_any");
+  add_launch(p, name, grid, tile == 128 ? 256 : 512, a);
+  if (d.has_bias) {
+    mtk_grouped_kargs b{};
+    b.E = d.E;
+    b.T = d.T;
+    b.N = d.N;
+    b.lda = d.ldc;
+    b.tiles_n = (int)bias_tiles;
+    add_launch(p, head + "_bias_grad", d.E * bias_tiles, 512, b);
+    p->launches.back().role = ROLE_REDUCE;
+  }
+  p->flops = 2.0 * d.T * d.N * d.K;
+  p->bytes = 2.0 * d.T * (d.N + d.K) + (d.out_f32 ? 4.0 : 2.0) * d.E * d.N * d.K;
+  char desc[256];
+  snprintf(desc, sizeof desc, "grouped gradient %s E=%d T=%d N=%d K=%d b=%s bias=%d out=%s tile=%d grid=%lld kernel=%s", dtype_name(d.dtype),
+           d.E, d.T, d.N, d.K, d.trans_b ? "nk" : "kn", d.has_bias ? 1 : 0, d.out_f32 ? "f32" : "16", tile, grid, name.c_str());
+  p->description = desc;
+  return finish_plan(p, out);
+}
+
+// ------------------------------------------------------------------ rows in few bits
+
+int check_mx_rows(long long R, long long K) {
+  if (R <= 0 || K <= 0) return fail(MTK_ERR_INVALID, "R and K must be positive (got %lld, %lld)", R, K);
+  if (K > kMaxWidth) return fail(MTK_ERR_UNSUPPORTED, "K above 2^22 is not supported (got %lld)", K);
+  return MTK_OK;
+}
+
+// The launch that brings R rows into the format or back.
+Launch mx_rows_launch(bool quantize, int R, int K, int ld, int dtype) {
+  mtk_mx_rows_kargs a{};
+  a.R = R;
+  a.K = K;
+  a.ld = ld;
+  a.k_tiles = mx_k_tiles(K);
+  const long long waves = ((long long)R + 3) / 4 * ((a.k_tiles + 1) / 2);  // 4 rows x 2 K-tiles each
+  Launch l;
+  l.name = std::string(quantize ? "mtk_mx_quantize_" : "mtk_mx_dequantize_") + dtype_name(dtype);
+  l.grid = (unsigned)((waves + 3) / 4);
+  set_args(l, a);
+  return l;
+}
+
+int plan_mx_rows(mtk_ctx *ctx, const mtk_mx_rows_desc *d_in, bool quantize, mtk_plan **out) {
+  if (!d_in || !out) return fail(MTK_ERR_INVALID, "null descriptor or output");
+  mtk_mx_rows_desc d = *d_in;
+  int s = check_mx_rows(d.R, d.K);
+  if (s != MTK_OK) return s;
+  if (d.dtype != MTK_F16 && d.dtype != MTK_BF16) return fail(MTK_ERR_INVALID, "dtype must be MTK_F16 or MTK_BF16");
+  if ((s = check_ld(d.ld, d.K, "ld", &d.ld)) != MTK_OK) return s;
+  if (((long long)d.R + 15) / 16 * ((mx_k_tiles(d.K) + 1) / 2) > INT32_MAX / 256)
+    return fail(MTK_ERR_UNSUPPORTED, "%d rows of %d are not supported", d.R, d.K);
+  mtk_plan *p = new mtk_plan();
+  p->ctx = ctx;
+  p->kind = quantize ? PLAN_MX_QUANT : PLAN_MX_DEQUANT;
+  p->mx_rows = d;
+  p->launches.push_back(mx_rows_launch(quantize, d.R, d.K, d.ld, d.dtype));
+  p->bytes = (double)d.R * (2.0 * d.K + 136.0 * mx_k_tiles(d.K));
+  char desc[160];
+  snprintf(desc, sizeof desc, "mx %s %s R=%d K=%d ld=%d grid=%u", quantize ? "quantize" : "dequantize", dtype_name(d.dtype), d.R, d.K, d.ld,
+           p->launches[0].grid);
+  p->description = desc;
+  return finish_plan(p, out);
+}
+
+int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
+  if (!d_in || !out) return fail(MTK_ERR_INVALID, "null descriptor or output");
+  mtk_mx_gemm_desc d = *d_in;
+  if (d.E < 0 || d.T <= 0 || d.N <= 0 || d.K <= 0)
+    return fail(MTK_ERR_INVALID, "E must be 0 or more, T, N and K positive (got %d, %d, %d, %d)", d.E, d.T, d.N, d.K);
+  if (d.N > kMaxWidth || d.K > kMaxWidth) return fail(MTK_ERR_UNSUPPORTED, "N and K above 2^22 are not supported (got %d, %d)", d.N, d.K);
+  if (d.E > (1 << 20)) return fail(MTK_ERR_UNSUPPORTED, "E above 2^20 is not supported (got %d)", d.E);
+  if (d.dtype != MTK_F16 && d.dtype != MTK_BF16) return fail(MTK_ERR_INVALID, "dtype must be MTK_F16 or MTK_BF16");
+  if (!d.quantize_a && d.lda) return fail(MTK_ERR_INVALID, "lda is for 16-bit rows (quantize_a)");
+  int s;
+  if ((s = check_ld(d.lda, d.K, "lda", &d.lda)) != MTK_OK || (s = check_ld(d.ldc, d.N, "ldc", &d.ldc)) != MTK_OK) return s;
+  const long long groups = d.E ? d.E : 1;
+  const int k_tiles = mx_k_tiles(d.K);
+  // scales of an operand are read with 32-bit offsets: 2^31 bytes
+  if ((double)d.T * k_tiles * 8 > 2147483392.0 || (double)groups * d.N * k_tiles * 8 > 2147483392.0)
+    return fail(MTK_ERR_UNSUPPORTED, "T x K and E x N x K up to 2^36 are supported");
+  mtk_mx_gemm_kargs a{};
+  a.E = (int)groups;
+  a.T = d.T;
+  a.N = d.N;
+  a.k_tiles = k_tiles;
+  a.ldc = d.ldc;
+  a.has_bias = d.has_bias ? 1 : 0;
+  const int tile = 64;
+  a.tiles_n = (d.N + tile - 1) / tile;
+  long long grid;
+  if ((s = check_tiles((int)groups, d.T, tile, a.tiles_n, &grid)) != MTK_OK) return s;
+  if (!d.E) grid = (long long)((d.T + tile - 1) / tile) * a.tiles_n;
+  mtk_plan *p = new mtk_plan();
+  p->ctx = ctx;
+  p->kind = PLAN_MX_GEMM;
+  p->mx_gemm = d;
+  if (d.quantize_a) {
+    p->launches.push_back(mx_rows_launch(true, d.T, d.K, d.lda, d.dtype));
+    p->launches.back().role = ROLE_PERMUTE;
+    p->scales_at = (mx_code_bytes(d.T, k_tiles) + 255) & ~(size_t)255;  // the scales
+    p->workspace = p->scales_at + mx_scale_bytes(d.T, k_tiles);
+  }
+  const std::string name = std::string("mtk_mx_gemm_") + dtype_name(d.dtype) + "_" + std::to_string(tile);
+  add_launch(p, name, grid, 512, a);
+  p->flops = 2.0 * d.T * d.N * d.K;
+  p->bytes = 136.0 * k_tiles * ((d.quantize_a ? 0.0 : d.T) + (double)std::min<long long>(groups, d.T) * d.N) + 2.0 * d.T * d.N +
+             (d.quantize_a ? 2.0 * d.T * d.K : 0.0);
+  char desc[256];
+  snprintf(desc, sizeof desc, "mx gemm %s E=%d T=%d N=%d K=%d bias=%d quantize_a=%d tile=%d grid=%lld kernel=%s", dtype_name(d.dtype), d.E, d.T,
+           d.N, d.K, a.has_bias, d.quantize_a ? 1 : 0, tile, grid, name.c_str());
+  p->description = desc;
+  return finish_plan(p, out);
+}
+
+// ------------------------------------------------------------------ run-time arguments
+
+// What an operator reads or writes: n rows of `width` bytes, `step` bytes apart.
+struct Rows {
+  const char *name;
+  const void *at;
+  uint64_t n, width, step;
+  uint64_t bytes() const { return (n - 1) * step + width; }
+};
+Rows flat(const char *name, const void *at, uint64_t bytes) { return {name, at, 1, bytes, bytes}; }
+
+bool meet(const Rows &a, const Rows &b) {
+  if (!a.at || !b.at || !a.width || !b.width || !overlap(a.at, a.bytes(), b.at, b.bytes())) return false;
+  if (a.step != b.step || a.n < 2 || b.n < 2) return true;
+  const Rows &x = (uintptr_t)a.at <= (uintptr_t)b.at ? a : b, &y = &x == &a ? b : a;
+  const uint64_t apart = (uintptr_t)y.at - (uintptr_t)x.at, rows = apart / x.step, rest = apart % x.step;
+  // a row of y starts `rest` bytes behind one of x, and ends before or behind the start of x's next
+  return (rows < x.n && rest < x.width) || (rows + 1 < x.n && rest + y.width > x.step);
+}
+
+int check_overlaps(std::initializer_list<Rows> in, std::initializer_list<Rows> out) {
+  for (const Rows *o = out.begin(); o != out.end(); ++o) {
+    for (const Rows &x : in)
+      if (meet(*o, x)) return fail(MTK_ERR_INVALID, "%s overlaps %s", o->name, x.name);
+    for (const Rows *q = out.begin(); q != o; ++q)
+      if (meet(*o, *q)) return fail(MTK_ERR_INVALID, "%s overlaps %s", o->name, q->name);
+  }
+  return MTK_OK;
+}
+
+Rows rows16(const char *name, const void *at, int n, int width, int ld) {
+  return {name, at, (uint64_t)n, 2 * (uint64_t)width, 2 * (uint64_t)ld};
+}
+
+int check_grouped_args(const mtk_plan *p, const void *argset) {
+  if (!argset) return fail(MTK_ERR_INVALID, "null arguments");
+  auto workspace = [&](const void *ws) {
+    return p->workspace && (!ws || !aligned(ws, 16))
+               ? fail(MTK_ERR_INVALID, "this plan needs a 16-byte aligned workspace of %zu bytes", p->workspace)
+               : MTK_OK;
+  };
+  int s;
+  if (p->kind == PLAN_GROUPED) {
+    const mtk_grouped_gemm_args *t = (const mtk_grouped_gemm_args *)argset;
+    const mtk_grouped_desc &d = p->grouped;
+    if (!t->A || !t->B || !t->C || !t->row_start) return fail(MTK_ERR_INVALID, "A, B, C and row_start must be non-null");
+    if (d.has_bias && !t->bias) return fail(MTK_ERR_INVALID, "plan has a bias but bias is null");
+    if (!aligned(t->A, p->align_a) || !aligned(t->B, p->align_b))
+      return fail(MTK_ERR_INVALID, "A and B must be %u-byte aligned for this plan", p->align_a);
+    if (!aligned(t->C, 2) || !aligned(t->bias, 2) || !aligned(t->row_start, 4))
+      return fail(MTK_ERR_INVALID, "C and bias must be 2-byte, row_start 4-byte aligned");
+    if ((s = workspace(t->workspace)) != MTK_OK) return s;
+    const uint64_t b = 2 * (uint64_t)d.E * (uint64_t)(d.trans_b ? d.N : d.K) * (uint64_t)d.ldb;
+    return check_overlaps({rows16("A", t->A, d.T, d.K, d.lda), flat("B", t->B, b - 2 * (uint64_t)(d.ldb - (d.trans_b ? d.K : d.N))),
+                           flat("bias", d.has_bias ? t->bias : nullptr, 2 * (uint64_t)d.E * (uint64_t)d.N),
+                           flat("row_start", t->row_start, 4 * ((uint64_t)d.E + 1))},
+                          {rows16("C", t->C, d.T, d.N, d.ldc), flat("the workspace", t->workspace, p->workspace)});
+  }
+  if (p->kind == PLAN_GROUPED_GRAD) {
+    const mtk_grouped_grad_args *t = (const mtk_grouped_grad_args *)argset;
+    const mtk_grouped_desc &d = p->grouped;
+    if (!t->A || !t->dC || !t->dB || !t->row_start) return fail(MTK_ERR_INVALID, "A, dC, dB and row_start must be non-null");
+    if (d.has_bias && !t->dbias) return fail(MTK_ERR_INVALID, "plan has a bias but dbias is null");
+    if (!aligned(t->A, p->align_a) || !aligned(t->dC, p->align_b))
+      return fail(MTK_ERR_INVALID, "A and dC must be %u-byte aligned for this plan", p->align_a);
+    if (!aligned(t->dB, 16) || !aligned(t->dbias, 4) || !aligned(t->row_start, 4))
+      return fail(MTK_ERR_INVALID, "dB must be 16-byte, dbias and row_start 4-byte aligned");
+    if ((s = workspace(t->workspace)) != MTK_OK) return s;
+    const uint64_t size = d.out_f32 ? 4 : 2, groups = (uint64_t)d.E * (uint64_t)d.N;
+    return check_overlaps({rows16("A", t->A, d.T, d.K, d.lda), rows16("dC", t->dC, d.T, d.N, d.ldc),
+                           flat("row_start", t->row_start, 4 * ((uint64_t)d.E + 1))},
+                          {flat("dB", t->dB, size * groups * (uint64_t)d.K), flat("dbias", d.has_bias ? t->dbias : nullptr, size * groups),
+                           flat("the workspace", t->workspace, p->workspace)});
+  }
+  if (p->kind == PLAN_MX_QUANT || p->kind == PLAN_MX_DEQUANT) {
+    const bool q = p->kind == PLAN_MX_QUANT;
+    const mtk_mx_quantize_args *w = (const mtk_mx_quantize_args *)argset;
+    const mtk_mx_dequantize_args *r = (const mtk_mx_dequantize_args *)argset;
+    const void *rows = q ? w->src : r->dst, *codes = q ? w->codes : r->codes, *scales = q ? w->scales : r->scales;
+    const mtk_mx_rows_desc &d = p->mx_rows;
+    if (!rows || !codes || !scales) return fail(MTK_ERR_INVALID, "%s, codes and scales must be non-null", q ? "src" : "dst");
+    if (!aligned(rows, 2)) return fail(MTK_ERR_INVALID, "%s must be 2-byte aligned", q ? "src" : "dst");
+    if (!aligned(codes, 16) || !aligned(scales, 16)) return fail(MTK_ERR_INVALID, "codes and scales must be 16-byte aligned");
+    const int kt = mx_k_tiles(d.K);
+    const Rows x = rows16(q ? "src" : "dst", rows, d.R, d.K, d.ld), c = flat("codes", codes, mx_code_bytes(d.R, kt)),
+               y = flat("scales", scales, mx_scale_bytes(d.R, kt));
+    return q ? check_overlaps({x}, {c, y}) : check_overlaps({c, y}, {x});
+  }
+  const mtk_mx_gemm_args *t = (const mtk_mx_gemm_args *)argset;
+  const mtk_mx_gemm_desc &d = p->mx_gemm;
+  const int kt = mx_k_tiles(d.K);
+  const int64_t b_rows = (int64_t)(d.E ? d.E : 1) * d.N;
+  if (!t->A || !t->B || !t->b_scales || !t->C) return fail(MTK_ERR_INVALID, "A, B, b_scales and C must be non-null");
+  if (d.quantize_a ? t->a_scales != nullptr : !t->a_scales)
+    return fail(MTK_ERR_INVALID, d.quantize_a ? "a_scales must be NULL where the run quantises A" : "a_scales must be non-null");
+  if (d.E ? !t->row_start : t->row_start != nullptr)
+    return fail(MTK_ERR_INVALID, d.E ? "row_start must be non-null" : "row_start must be NULL without groups");
+  if (d.has_bias && !t->bias) return fail(MTK_ERR_INVALID, "plan has a bias but bias is null");
+  if (!aligned(t->A, d.quantize_a ? 2 : 16) || !aligned(t->a_scales, 16) || !aligned(t->B, 16) || !aligned(t->b_scales, 16))
+    return fail(MTK_ERR_INVALID, "codes and scales must be 16-byte aligned (16-bit rows 2-byte)");
+  if (!aligned(t->C, 2) || !aligned(t->bias, 2) || !aligned(t->row_start, 4))
+    return fail(MTK_ERR_INVALID, "C and bias must be 2-byte, row_start 4-byte aligned");
+  if ((s = workspace(t->workspace)) != MTK_OK) return s;
+  return check_overlaps({d.quantize_a ? rows16("A", t->A, d.T, d.K, d.lda) : flat("A", t->A, mx_code_bytes(d.T, kt)),
+                         flat("a_scales", t->a_scales, mx_scale_bytes(d.T, kt)), flat("B", t->B, mx_code_bytes(b_rows, kt)),
+                         flat("b_scales", t->b_scales, mx_scale_bytes(b_rows, kt)),
+                         flat("bias", d.has_bias ? t->bias : nullptr, 2 * (uint64_t)b_rows),
+                         flat("row_start", t->row_start, 4 * ((uint64_t)d.E + 1))},
+                        {rows16("C", t->C, d.T, d.N, d.ldc), flat("the workspace", t->workspace, p->workspace)});
+}
+
+// Writes the run-time pointers of a launch into `block`, a copy of its argument block.
+void patch_grouped(const mtk_plan *p, const Launch &l, char *block, const void *argset) {
+  if (p->kind == PLAN_GROUPED) {
+    const mtk_grouped_gemm_args *t = (const mtk_grouped_gemm_args *)argset;
+    mtk_grouped_kargs &a = *(mtk_grouped_kargs *)block;
+    a.A = t->A;
+    a.B = t->B;
+    a.bias = t->bias;
+    a.row_start = t->row_start;
+    a.C = t->C;
+  } else if (p->kind == PLAN_GROUPED_GRAD) {
+    const mtk_grouped_grad_args *t = (const mtk_grouped_grad_args *)argset;
+    mtk_grouped_kargs &a = *(mtk_grouped_kargs *)block;
+    const bool bias = l.role == ROLE_REDUCE;
+    a.A = bias || p->grouped.trans_b ? t->dC : t->A;
+    a.B = bias ? nullptr : p->grouped.trans_b ? t->A : t->dC;
+    a.row_start = t->row_start;
+    void *out = bias ? t->dbias : t->dB;
+    a.C = p->grouped.out_f32 ? nullptr : out;
+    a.C32 = p->grouped.out_f32 ? (float *)out : nullptr;
+  } else if (p->kind == PLAN_MX_GEMM && l.role == ROLE_MAIN) {
+    const mtk_mx_gemm_args *t = (const mtk_mx_gemm_args *)argset;
+    mtk_mx_gemm_kargs &a = *(mtk_mx_gemm_kargs *)block;
+    a.A = p->mx_gemm.quantize_a ? t->workspace : t->A;
+    a.a_scales = p->mx_gemm.quantize_a ? (char *)t->workspace + p->scales_at : t->a_scales;
+    a.B = t->B;
+    a.b_scales = t->b_scales;
+    a.bias = t->bias;
+    a.row_start = t->row_start;
+    a.C = t->C;
+  } else {
+    mtk_mx_rows_kargs &a = *(mtk_mx_rows_kargs *)block;
+    if (p->kind == PLAN_MX_DEQUANT) {
+      const mtk_mx_dequantize_args *t = (const mtk_mx_dequantize_args *)argset;
+      a.codes = const_cast<void *>(t->codes);
+      a.scales = const_cast<void *>(t->scales);
+      a.dst = t->dst;
+    } else if (p->kind == PLAN_MX_QUANT) {
+      const mtk_mx_quantize_args *t = (const mtk_mx_quantize_args *)argset;
+      a.src = t->src;
+      a.codes = t->codes;
+      a.scales = t->scales;
+    } else {
+      const mtk_mx_gemm_args *t = (const mtk_mx_gemm_args *)argset;
+      a.src = t->A;
+      a.codes = t->workspace;
+      a.scales = (char *)t->workspace + p->scales_at;
+    }
+    a.wide = a.ld % 8 == 0 && aligned(p->kind == PLAN_MX_DEQUANT ? a.dst : a.src, 16);
+  }
+}
+
+// A run: argument blocks on the stack, nothing is allocated.
+int run_grouped(const mtk_plan *p, PlanKind kind, const void *argset) {
+  if (!p) return fail(MTK_ERR_INVALID, "null plan");
+  if (p->kind != kind) return fail(MTK_ERR_INVALID, "the plan is of another operator");
+  if (!p->ctx) return fail(MTK_ERR_INVALID, "plan was created without a context (dry plan)");
+  const int s = check_grouped_args(p, argset);
+  if (s != MTK_OK) return s;
+  alignas(16) char block[256];
+  HIP_TRY(hipSetDevice(p->ctx->device));
+  for (const Launch &l : p->launches) {
+    if (l.args.size() > sizeof block) return fail(MTK_ERR_INVALID, "argument block of %s too large", l.name.c_str());
+    memcpy(block, l.args.data(), l.args.size());
+    patch_grouped(p, l, block, argset);
+    void *params[] = {block};
+    const hipError_t e = hipModuleLaunchKernel(l.fn, l.grid, 1, 1, l.block, 1, 1, 0, p->ctx->stream, params, nullptr);
+    if (e != hipSuccess) return fail(MTK_ERR_LAUNCH, "launch of %s failed: %s", l.name.c_str(), hipGetErrorString(e));
+  }
+  return MTK_OK;
+}

@@ -9,7 +9,7 @@
 
 #include <stdint.h>
 
-#define MTK_KARGS_VERSION 18
+#define MTK_KARGS_VERSION 19
 
 /* In-workgroup split-K: bytes of workspace slot per output tile of BM x BM (256 or 128). Each
  * wavefront keeps these accumulator blocks (32 x 32 fp32, 4 KB) of its running sum in the slot,
@@ -190,5 +190,42 @@ typedef struct {
   mtk_kv_attn_kargs rows, join;
   int32_t joins;
 } mtk_kv_prefill_kargs;
+
+/* Products grouped by expert (groups.h). Forward: C [T][ldc] = A [T][lda] op(B_e) + bias_e. Gradient of the weights: C or C32
+ * [E][M][N] = sum over the group's rows of A[t][m] B[t][n]; of the bias: C or C32 [E][N] = sum of A[t][n]. */
+typedef struct {
+  const void *A, *B, *bias;
+  const int32_t *row_start; /* [E + 1] */
+  void *C;
+  float *C32;       /* gradients in 32 bits, or NULL */
+  int64_t b_stride; /* elements between the weights of two groups */
+  int32_t E, T, M, N, K;
+  int32_t lda, ldb, ldc;
+  uint32_t b_exact; /* bytes of the weights of a group */
+  int32_t tiles_m, tiles_n, k_tiles;
+  int32_t has_bias;
+} mtk_grouped_kargs;
+
+/* Rows into blocks of 32 four-bit values with one scale, and back (mx.h has the layout). */
+typedef struct {
+  const void *src; /* rows in 16 bits (quantise) */
+  void *dst;       /* rows in 16 bits (dequantise) */
+  void *codes, *scales;
+  int64_t ld;      /* elements between 16-bit rows */
+  int32_t R, K;
+  int32_t k_tiles; /* ceil(K / 256) */
+  int32_t wide;    /* 16-bit rows are read or written 16 bytes at a time */
+} mtk_mx_rows_kargs;
+
+/* Products of rows in that format: C [T][ldc] = A B_e^T + bias_e. */
+typedef struct {
+  const void *A, *a_scales; /* codes [T][k_tiles * 128], scales [k_tiles][T][8] */
+  const void *B, *b_scales; /* codes [E * N][k_tiles * 128], scales [k_tiles][E * N][8] */
+  const void *bias;
+  const int32_t *row_start; /* [E + 1]; NULL: one group of T rows */
+  void *C;
+  int32_t E, T, N, k_tiles;
+  int32_t ldc, tiles_n, has_bias;
+} mtk_mx_gemm_kargs;
 
 #endif

@@ -147,8 +147,9 @@ struct QuarterConv {
   }
 };
 
-template <int DT, class AOp, bool BN, bool ANY, int W>
-__device__ __forceinline__ void quarter_tile(const mtk_tile_args &a, AOp oa) {
+// PLACED: the output tile's first row and column are given (at).
+template <int DT, class AOp, bool BN, bool ANY, int W, bool PLACED = false>
+__device__ __forceinline__ void quarter_tile(const mtk_tile_args &a, AOp oa, const TileAt at = {}) {
   constexpr int MB = AOp::kRows / 32;                   // 32-row blocks
   constexpr int kWaveB = (AOp::kRows + 64) * 128;
   constexpr int kPasses = MB * 8192 <= kWaveB ? 1 : 2;  // of the final sum: both column blocks at once, or one each
@@ -157,14 +158,18 @@ __device__ __forceinline__ void quarter_tile(const mtk_tile_args &a, AOp oa) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  const int tiles = a.tiles_m * a.tiles_n;
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int split = id / tiles;
-  const int t = id - split * tiles;
-  const int group = kGroupM * a.tiles_n;
-  const int first_m = (t / group) * kGroupM;
-  const int gm = min(a.tiles_m - first_m, kGroupM);
-  const int m0 = (first_m + (t % group) % gm) * AOp::kRows, n0 = (t % group) / gm * 64;
+  int split = 0, t = 0, m0 = at.m0, n0 = at.n0;
+  if constexpr (!PLACED) {
+    const int tiles = a.tiles_m * a.tiles_n;
+    const int id = xcd_remap(blockIdx.x, gridDim.x);
+    split = id / tiles;
+    t = id - split * tiles;
+    const int group = kGroupM * a.tiles_n;
+    const int first_m = (t / group) * kGroupM;
+    const int gm = min(a.tiles_m - first_m, kGroupM);
+    m0 = (first_m + (t % group) % gm) * AOp::kRows;
+    n0 = (t % group) / gm * 64;
+  }
   const int kt0 = split_first_tile(a, split, t);
   const int kt1 = split_first_tile(a, split + 1, t);
 

@@ -26,8 +26,10 @@
 #include <vector>
 
 #include "../../include/mtk.h"
+#include "groups.h"
 #include "kargs.h"
 #include "kv_cache.h"
+#include "mx.h"
 #include "scratch.h"
 
 namespace {
@@ -170,7 +172,8 @@ struct mtk_ctx {
 namespace {
 
 enum PlanKind { PLAN_GEMM = 1, PLAN_ATTN = 2, PLAN_CONV = 3, PLAN_ATTN_BWD = 4, PLAN_PERMUTE = 5,
-                PLAN_KV_WRITE = 6, PLAN_KV_READ = 7, PLAN_KV_ATTN = 8 };
+                PLAN_KV_WRITE = 6, PLAN_KV_READ = 7, PLAN_KV_ATTN = 8, PLAN_GROUPED = 9, PLAN_GROUPED_GRAD = 10,
+                PLAN_MX_QUANT = 11, PLAN_MX_DEQUANT = 12, PLAN_MX_GEMM = 13 };
 
 enum LaunchRole { ROLE_MAIN = 0, ROLE_REDUCE = 1, ROLE_PERMUTE = 2 };
 
@@ -192,6 +195,9 @@ struct mtk_plan {
   mtk_conv_desc conv{};
   mtk_permute_desc perm{};
   mtk_kv_desc kv{};
+  mtk_grouped_desc grouped{};  // leading dimensions filled in, as in the two below
+  mtk_mx_rows_desc mx_rows{};
+  mtk_mx_gemm_desc mx_gemm{};
   std::vector<Launch> launches;
   // attention with the keys split over workgroups: `launches` need a partial-sum buffer of the
   // library's; `plain` is the plan without one (one kernel that walks the splits in turn, the same bits),
@@ -200,6 +206,7 @@ struct mtk_plan {
   std::vector<Launch> plain;
   size_t workspace = 0;
   size_t lt_at = 0, part_kv_at = 0, part_q_at = 0;  // attention backward: byte offsets in the workspace
+  size_t scales_at = 0;                             // products in few bits: of the quantised rows' scales
   size_t part_ml_at = 0, part_bytes = 0;  // the per-row pairs' offset in the partial-sum buffer, its size
   // kernels that read rows at any 2-byte alignment: the operands' exact sizes, from which their buffer
   // ranges are made when the pointers are known (operand_range)
@@ -1317,6 +1324,7 @@ int plan_attn(mtk_ctx *ctx, const mtk_attn_desc *d_in, mtk_plan **out) {
 }
 
 #include "kv_plans.hpp"
+#include "grouped_plans.hpp"
 
 // ------------------------------------------------------------------ binding run-time pointers
 
@@ -1417,6 +1425,10 @@ int bind_args(const mtk_plan *p, const void *argset, std::vector<Launch> &ls, vo
     const int s = check_kv_args(p, argset);
     if (s != MTK_OK) return s;
     for (Launch &l : ls) patch_kv(p, l, l.args.data(), argset);
+  } else if (is_grouped(p)) {
+    const int s = check_grouped_args(p, argset);
+    if (s != MTK_OK) return s;
+    for (Launch &l : ls) patch_grouped(p, l, l.args.data(), argset);
   } else if (p->kind == PLAN_ATTN_BWD) {
     const mtk_attn_bwd_args *t = (const mtk_attn_bwd_args *)argset;
     if (!t || !t->Q || !t->K || !t->V || !t->O || !t->dO || !t->lse || !t->dQ || !t->dK || !t->dV)
@@ -1479,6 +1491,16 @@ size_t argset_size(const mtk_plan *p) {
       return sizeof(mtk_kv_read_args);
     case PLAN_KV_ATTN:
       return sizeof(mtk_kv_attn_args);
+    case PLAN_GROUPED:
+      return sizeof(mtk_grouped_gemm_args);
+    case PLAN_GROUPED_GRAD:
+      return sizeof(mtk_grouped_grad_args);
+    case PLAN_MX_QUANT:
+      return sizeof(mtk_mx_quantize_args);
+    case PLAN_MX_DEQUANT:
+      return sizeof(mtk_mx_dequantize_args);
+    case PLAN_MX_GEMM:
+      return sizeof(mtk_mx_gemm_args);
     default:
       return sizeof(mtk_attn_args);
   }
@@ -1820,6 +1842,26 @@ int mtk_kv_attn_plan(mtk_ctx *ctx, const mtk_kv_desc *desc, mtk_plan **out) { re
 int mtk_kv_write_run(const mtk_plan *plan, const mtk_kv_write_args *args) { return run_kv(plan, PLAN_KV_WRITE, args); }
 int mtk_kv_read_run(const mtk_plan *plan, const mtk_kv_read_args *args) { return run_kv(plan, PLAN_KV_READ, args); }
 int mtk_kv_attn_run(const mtk_plan *plan, const mtk_kv_attn_args *args) { return run_kv(plan, PLAN_KV_ATTN, args); }
+
+int mtk_grouped_gemm_plan(mtk_ctx *ctx, const mtk_grouped_desc *desc, mtk_plan **out) { return plan_grouped(ctx, desc, out); }
+int mtk_grouped_gemm_run(const mtk_plan *plan, const mtk_grouped_gemm_args *args) { return run_grouped(plan, PLAN_GROUPED, args); }
+int mtk_grouped_grad_plan(mtk_ctx *ctx, const mtk_grouped_desc *desc, mtk_plan **out) { return plan_grouped_grad(ctx, desc, out); }
+int mtk_grouped_grad_run(const mtk_plan *plan, const mtk_grouped_grad_args *args) { return run_grouped(plan, PLAN_GROUPED_GRAD, args); }
+
+int mtk_mx_bytes(int R, int K, size_t *code_bytes, size_t *scale_bytes) {
+  if (!code_bytes || !scale_bytes) return fail(MTK_ERR_INVALID, "null output");
+  const int s = check_mx_rows(R, K);
+  if (s != MTK_OK) return s;
+  *code_bytes = mx_code_bytes(R, mx_k_tiles(K));
+  *scale_bytes = mx_scale_bytes(R, mx_k_tiles(K));
+  return MTK_OK;
+}
+int mtk_mx_quantize_plan(mtk_ctx *ctx, const mtk_mx_rows_desc *desc, mtk_plan **out) { return plan_mx_rows(ctx, desc, true, out); }
+int mtk_mx_quantize_run(const mtk_plan *plan, const mtk_mx_quantize_args *args) { return run_grouped(plan, PLAN_MX_QUANT, args); }
+int mtk_mx_dequantize_plan(mtk_ctx *ctx, const mtk_mx_rows_desc *desc, mtk_plan **out) { return plan_mx_rows(ctx, desc, false, out); }
+int mtk_mx_dequantize_run(const mtk_plan *plan, const mtk_mx_dequantize_args *args) { return run_grouped(plan, PLAN_MX_DEQUANT, args); }
+int mtk_mx_gemm_plan(mtk_ctx *ctx, const mtk_mx_gemm_desc *desc, mtk_plan **out) { return plan_mx_gemm(ctx, desc, out); }
+int mtk_mx_gemm_run(const mtk_plan *plan, const mtk_mx_gemm_args *args) { return run_grouped(plan, PLAN_MX_GEMM, args); }
 
 size_t mtk_plan_workspace_bytes(const mtk_plan *plan) { return plan ? plan->workspace : 0; }
 

@@ -38,6 +38,11 @@ constexpr int kBK = 64;
 constexpr int kThreads = 256;
 constexpr int kGroupM = 4;
 
+// The first row and column of an output tile.
+struct TileAt {
+  int m0, n0;
+};
+
 __device__ __forceinline__ uint32_t lds_off(int row, int chunk) {
   return (uint32_t)(row * 128 + ((chunk ^ (row & 7) ^ ((row >> 3) & 7)) << 4));
 }

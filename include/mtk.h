@@ -406,6 +406,118 @@ typedef struct {
 } mtk_kv_attn_args;
 int mtk_kv_attn_run(const mtk_plan *plan, const mtk_kv_attn_args *args);
 
+/* ------------------------------------------------------------------ products grouped by expert */
+
+/* The products of a layer whose rows each belong to one of E groups (experts), sorted by group. No counterpart in the
+ * reference, whose GEMM has one B (Sources/matmul/matmul.swift:239-296).
+ *
+ *   C[t][n] = bias[e][n] + sum_k A[t][k] op(B_e)[k][n]      for the rows t of group e
+ *   A [T][lda], C [T][ldc], bias [E][N]; B [E][N][ldb] (trans_b, as the GEMM's default) or [E][K][ldb]
+ *   row_start [E + 1], int32 on the device, so that one plan (or graph) serves any routing: group e has the rows
+ *   row_start[e] .. row_start[e + 1] - 1 (none allowed), ascending, within [0, T].
+ * The kernels limit what row_start holds to [0, T]; a group whose end lies before its start has no rows. Rows of no group
+ * are left as they were. Where the groups do not ascend, which of the rows are computed, and by which group, is undefined;
+ * nothing outside of C is written. A row depends on its own values and its group's weights only.
+ * Sums in fp32, the bias added to them, one rounding.
+ *
+ * The input gradient of such a layer is the same product: dA = dC op(B_e)^T is a plan with N and K exchanged and trans_b
+ * inverted, over the same weights.
+ *
+ * Operands may be of any size but: 2 GiB for the weights of one group (forward), 2 GiB for A and dC (gradients of the weights),
+ * leading dimensions, N and K up to 2^22. Even leading dimensions run the GEMM's kernels (A, B 4-byte aligned), odd ones
+ * slower kernels that take rows at any 2-byte alignment. */
+typedef struct {
+  int E, T, N, K;
+  int lda, ldb, ldc; /* elements between rows; 0 = packed */
+  int trans_b;
+  int dtype;         /* MTK_F16 or MTK_BF16 */
+  int has_bias;
+  int out_f32;       /* gradients only: dB and dbias in fp32 */
+} mtk_grouped_desc;
+
+int mtk_grouped_gemm_plan(mtk_ctx *ctx, const mtk_grouped_desc *desc, mtk_plan **out);
+typedef struct {
+  const void *A, *B, *bias;
+  const int32_t *row_start;
+  void *C;         /* overlaps nothing that is read; slices of one buffer whose rows lie between each other do not */
+  void *workspace; /* >= mtk_plan_workspace_bytes(plan) bytes, 16-byte aligned, or NULL if 0 */
+} mtk_grouped_gemm_args;
+int mtk_grouped_gemm_run(const mtk_plan *plan, const mtk_grouped_gemm_args *args);
+
+/* The gradients of the weights and of the bias, for the descriptor of the forward product (ldc: of dC; dB is packed, so ldb
+ * must be 0):
+ *   dB_e[n][k] = sum over the rows t of group e of dC[t][n] A[t][k]  (trans_b; else [k][n]),  dbias[e][n] = sum of dC[t][n]
+ * Every group is written; one without a row gets zeros. Sums in fp32 in a fixed order, no atomics. */
+int mtk_grouped_grad_plan(mtk_ctx *ctx, const mtk_grouped_desc *desc, mtk_plan **out);
+typedef struct {
+  const void *A, *dC;
+  const int32_t *row_start;
+  void *dB;        /* [E][N][K] or [E][K][N], 16-byte aligned; 16 bits, or fp32 with out_f32 */
+  void *dbias;     /* [E][N], the same type, with has_bias */
+  void *workspace;
+} mtk_grouped_grad_args;
+int mtk_grouped_grad_run(const mtk_plan *plan, const mtk_grouped_grad_args *args);
+
+/* ------------------------------------------------------------------ rows and products in 4 bits */
+
+/* Rows held in few bits, for products on the scaled matrix instructions. No counterpart in the reference.
+ *
+ * Format: a block is 32 values of a row, held as e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6) times a power of two 2^e, the block format of
+ * the paged cache's MTK_KV_FP4: the smallest that brings the block's largest magnitude to at most 6 (and at least 2^-126), each
+ * value rounded to nearest, ties to the even code. Magnitudes above the largest such value that the 16-bit type holds (f16:
+ * 49152) are limited to it. A block with a NaN or an infinity is NaN, all of it, and so is every product with it.
+ * Layout, K padded with zeros to a multiple of 256: codes [R][ceil(K / 256)][128], two a byte with the even place in the low
+ * half; scales [ceil(K / 256)][R][8], a byte e + 127, 255 for a NaN block. mtk_mx_bytes has both sizes. Whoever fills them
+ * otherwise than by mtk_mx_quantize writes the padding too. */
+int mtk_mx_bytes(int R, int K, size_t *code_bytes, size_t *scale_bytes);
+
+typedef struct {
+  int R, K;
+  int ld;    /* elements between 16-bit rows, 0 = K */
+  int dtype; /* MTK_F16 or MTK_BF16 */
+} mtk_mx_rows_desc;
+
+/* 16-bit rows [R][ld] into codes and scales. The weights [E][N][K] of a grouped product are E x N rows. */
+int mtk_mx_quantize_plan(mtk_ctx *ctx, const mtk_mx_rows_desc *desc, mtk_plan **out);
+typedef struct {
+  const void *src;      /* 2-byte aligned; 16-byte aligned rows (ld a multiple of 8) are read faster */
+  void *codes, *scales; /* 16-byte aligned */
+} mtk_mx_quantize_args;
+int mtk_mx_quantize_run(const mtk_plan *plan, const mtk_mx_quantize_args *args);
+
+/* And back, each value exactly (f16 values below 2^-14 to the nearest subnormal). Places between K and ld are left. */
+int mtk_mx_dequantize_plan(mtk_ctx *ctx, const mtk_mx_rows_desc *desc, mtk_plan **out);
+typedef struct {
+  const void *codes, *scales;
+  void *dst;
+} mtk_mx_dequantize_args;
+int mtk_mx_dequantize_run(const mtk_plan *plan, const mtk_mx_dequantize_args *args);
+
+/* C[t][n] = bias[e][n] + sum_k A[t][k] B_e[n][k], both held in few bits: A T rows, B E x N rows. E 0: one product of all rows
+ * (B N rows, no row_start). With E, row_start and what holds for it as in mtk_grouped_gemm. The values' products are exact,
+ * their sums fp32; C is in 16 bits, rounded once.
+ * quantize_a: A are 16-bit rows [T][lda] that the run brings into the format first (in the workspace, or on chip), with the
+ * result of mtk_mx_quantize; else codes and scales of T rows.
+ * T x K and E x N x K up to 2^36, K, N and leading dimensions up to 2^22. */
+typedef struct {
+  int E, T, N, K;
+  int lda, ldc; /* 0 = packed; lda: with quantize_a only */
+  int dtype;    /* of C and bias, and of A with quantize_a */
+  int has_bias;
+  int quantize_a;
+} mtk_mx_gemm_desc;
+
+int mtk_mx_gemm_plan(mtk_ctx *ctx, const mtk_mx_gemm_desc *desc, mtk_plan **out);
+typedef struct {
+  const void *A, *a_scales; /* 16-bit rows and NULL with quantize_a */
+  const void *B, *b_scales; /* codes and scales: 16-byte aligned */
+  const void *bias;
+  const int32_t *row_start; /* [E + 1]; NULL where E is 0 */
+  void *C;
+  void *workspace;          /* runs that may overlap need one each */
+} mtk_mx_gemm_args;
+int mtk_mx_gemm_run(const mtk_plan *plan, const mtk_mx_gemm_args *args);
+
 /* ------------------------------------------------------------------ plans, validate, profile */
 
 size_t mtk_plan_workspace_bytes(const mtk_plan *plan);
@@ -422,7 +534,7 @@ int mtk_plan_destroy(mtk_plan *plan);
  * Runs `warmup` untimed iterations, then `iters` timed ones, cycling through `nsets` argument sets
  * (so a large operand can be rotated to defeat the 256 MB Infinity Cache). Each set is the op's
  * args struct (mtk_gemm_args / mtk_attn_args / mtk_attn_bwd_args / mtk_conv_args /
- * mtk_permute_run_args / mtk_kv_write_args / mtk_kv_read_args / mtk_kv_attn_args). HIP events on the plan's stream
+ * mtk_permute_run_args / mtk_kv_*_args / mtk_grouped_*_args / mtk_mx_*_args). HIP events on the plan's stream
  * bracket each kernel; results are averages per iteration, in milliseconds. */
 typedef struct {
   double total_ms;      /* per iteration, first launch start to last launch end */
