@@ -226,7 +226,11 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
   a.k_tiles = k_tiles;
   a.ldc = d.ldc;
   a.has_bias = d.has_bias ? 1 : 0;
-  const int tile = 64;
+  const int cus = ctx ? ctx->prop.multiProcessorCount : 256;
+  auto wgs = [&](int tile) { return group_max_blocks((int)groups, d.T, tile) * ((d.N + tile - 1) / tile); };
+  int tile = 64;
+  if (wgs(256) >= cus * 5 / 8 && d.T >= 64LL * groups) tile = 256;
+  else if (wgs(128) >= cus && d.T >= 32LL * groups) tile = 128;
   a.tiles_n = (d.N + tile - 1) / tile;
   long long grid;
   if ((s = check_tiles((int)groups, d.T, tile, a.tiles_n, &grid)) != MTK_OK) return s;
@@ -242,7 +246,7 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
     p->workspace = p->scales_at + mx_scale_bytes(d.T, k_tiles);
   }
   const std::string name = std::string("mtk_mx_gemm_") + dtype_name(d.dtype) + "_" + std::to_string(tile);
-  add_launch(p, name, grid, 512, a);
+  add_launch(p, name, grid, tile == 128 ? 256 : 512, a);
   p->flops = 2.0 * d.T * d.N * d.K;
   p->bytes = 136.0 * k_tiles * ((d.quantize_a ? 0.0 : d.T) + (double)std::min<long long>(groups, d.T) * d.N) + 2.0 * d.T * d.N +
              (d.quantize_a ? 2.0 * d.T * d.K : 0.0);

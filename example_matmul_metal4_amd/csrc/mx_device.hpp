@@ -22,6 +22,15 @@ __device__ __forceinline__ f32x4 mfma_mx16(u32x4 a, u32x4 b, f32x4 c, uint32_t s
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, SEL, (int)sa, SEL, (int)sb);
 }
 
+// ds_read_b32 as inline asm, for code with direct-to-LDS loads in flight (device.hpp): the caller waits for it.
+template <int OFF>
+__device__ __forceinline__ uint32_t ds_read_b32_at(uint32_t addr) {
+  static_assert(OFF >= 0 && OFF < 65536, "ds offset field");
+  uint32_t w;
+  asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(w) : "v"(addr), "i"(OFF));
+  return w;
+}
+
 // Buffers of `rows` rows of an operand, the first of them row `row` of `all`: codes, and scales with offsets
 // kt * all * 8 + r * 8 from that row.
 struct MxOperand {
