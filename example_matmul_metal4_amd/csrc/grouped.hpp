@@ -111,15 +111,6 @@ __device__ __forceinline__ TileAt tile_at(int t, int blocks, int tiles_n) {
   return TileAt{(first + (t % group) % gm) * BM, (t % group) / gm * BN};
 }
 
-template <int DT, int BM, int WAVES_M, int WAVES_N, typename AOP, typename BOP>
-__device__ __forceinline__ void grouped_direct(const mtk_grouped_kargs &g) {
-  const GroupTile gt = group_tile<BM>(g.row_start, g.E, g.T, g.tiles_n);
-  if (gt.e < 0) return;
-  const TileAt at = tile_at<BM, BM>(gt.t, gt.blocks, g.tiles_n);
-  const mtk_tile_args a = group_args<BM, false>(g, gt.e, gt.first + at.m0, gt.rows - at.m0);
-  tile_direct<DT, BM, BM, WAVES_M, WAVES_N, AOP, BOP, false, true>(a, TileAt{0, at.n0});
-}
-
 template <int DT, bool BN, bool ANY, int W>
 __device__ __forceinline__ void grouped_quarter(const mtk_grouped_kargs &g) {
   const GroupTile gt = group_tile<64>(g.row_start, g.E, g.T, g.tiles_n);
@@ -153,13 +144,6 @@ __device__ __forceinline__ mtk_tile_args grad_args(const mtk_grouped_kargs &g, i
   a.k_tiles = a.k_tiles_per_split = (r.rows + kBK - 1) / kBK;
   a.split_k = 1;
   return a;
-}
-
-template <int DT, int BM, int WAVES_M, int WAVES_N, typename AOP, typename BOP>
-__device__ __forceinline__ void grouped_grad_direct(const mtk_grouped_kargs &g) {
-  const int tiles = g.tiles_m * g.tiles_n, id = xcd_remap(blockIdx.x, gridDim.x), e = id / tiles;
-  const mtk_tile_args a = grad_args<false>(g, e);
-  tile_direct<DT, BM, BM, WAVES_M, WAVES_N, AOP, BOP, false, true>(a, tile_at<BM, BM>(id - e * tiles, g.tiles_m, g.tiles_n));
 }
 
 template <int DT, bool ANY, int W>

@@ -7,18 +7,35 @@
 //   *_any        rows at any 2-byte alignment (odd leading dimensions)
 #pragma once
 
-#include "grouped.hpp"
+#include "expert_tiles.hpp"
 
 namespace mtk_grouped_ops {
-using R256 = mtk::OpRows<256, 8>;
-using C256 = mtk::OpColsT<256, 8>;
-using R128 = mtk::OpRows<128, 4>;
-using C128 = mtk::OpColsT<128, 4>;
+using namespace mtk;
+using El = Half<MTK_GROUPED_DT>;
+// 256x256 tiles: 8 wavefronts (2 x 4, 128 x 64 each, two per SIMD); 128x128: 4 (2 x 2), two workgroups per CU
+__device__ __forceinline__ void nt_256(const mtk_grouped_kargs &g) {
+  expert_tiles<El, 256, 256, 2, 4, TileRows<256, 8>, TileRows<256, 8>>(ForwardTiles<256, 256, false>(g));
+}
+__device__ __forceinline__ void nn_256(const mtk_grouped_kargs &g) {
+  expert_tiles<El, 256, 256, 2, 4, TileRows<256, 8>, TileCols<256, 8>>(ForwardTiles<256, 256, true>(g));
+}
+__device__ __forceinline__ void nt_128(const mtk_grouped_kargs &g) {
+  expert_tiles<El, 128, 128, 2, 2, TileRows<128, 4>, TileRows<128, 4>>(ForwardTiles<128, 128, false>(g));
+}
+__device__ __forceinline__ void nn_128(const mtk_grouped_kargs &g) {
+  expert_tiles<El, 128, 128, 2, 2, TileRows<128, 4>, TileCols<128, 4>>(ForwardTiles<128, 128, true>(g));
+}
+__device__ __forceinline__ void grad_256(const mtk_grouped_kargs &g) {
+  expert_tiles<El, 256, 256, 2, 4, TileCols<256, 8>, TileCols<256, 8>>(GradTiles<256, 256>(g));
+}
+__device__ __forceinline__ void grad_128(const mtk_grouped_kargs &g) {
+  expert_tiles<El, 128, 128, 2, 2, TileCols<128, 4>, TileCols<128, 4>>(GradTiles<128, 128>(g));
+}
 }  // namespace mtk_grouped_ops
 
 #define MTK_GROUPED(NAME, THREADS, ...)                                                                     \
   extern "C" __global__ void __launch_bounds__(THREADS) MTK_GROUPED_NAME(NAME)(const mtk_grouped_kargs g) { \
-    mtk::__VA_ARGS__(g);                                                                                     \
+    __VA_ARGS__(g);                                                                                          \
   }
 // quarter tiles: one workgroup of 8 wavefronts per CU, whose registers they may all have
 #define MTK_GROUPED_QUARTER(NAME, ...)                                                              \
@@ -27,16 +44,16 @@ using C128 = mtk::OpColsT<128, 4>;
     mtk::__VA_ARGS__(g);                                                                             \
   }
 
-MTK_GROUPED(nt_256, 512, grouped_direct<MTK_GROUPED_DT, 256, 2, 4, mtk_grouped_ops::R256, mtk_grouped_ops::R256>)
-MTK_GROUPED(nn_256, 512, grouped_direct<MTK_GROUPED_DT, 256, 2, 4, mtk_grouped_ops::R256, mtk_grouped_ops::C256>)
-MTK_GROUPED(nt_128, 256, grouped_direct<MTK_GROUPED_DT, 128, 2, 2, mtk_grouped_ops::R128, mtk_grouped_ops::R128>)
-MTK_GROUPED(nn_128, 256, grouped_direct<MTK_GROUPED_DT, 128, 2, 2, mtk_grouped_ops::R128, mtk_grouped_ops::C128>)
+MTK_GROUPED(nt_256, 512, mtk_grouped_ops::nt_256)
+MTK_GROUPED(nn_256, 512, mtk_grouped_ops::nn_256)
+MTK_GROUPED(nt_128, 256, mtk_grouped_ops::nt_128)
+MTK_GROUPED(nn_128, 256, mtk_grouped_ops::nn_128)
 MTK_GROUPED_QUARTER(nt_64, grouped_quarter<MTK_GROUPED_DT, false, false, 8>)
 MTK_GROUPED_QUARTER(nn_64, grouped_quarter<MTK_GROUPED_DT, true, false, 8>)
 MTK_GROUPED_QUARTER(nt_64_any, grouped_quarter<MTK_GROUPED_DT, false, true, 8>)
 MTK_GROUPED_QUARTER(nn_64_any, grouped_quarter<MTK_GROUPED_DT, true, true, 8>)
-MTK_GROUPED(grad_256, 512, grouped_grad_direct<MTK_GROUPED_DT, 256, 2, 4, mtk_grouped_ops::C256, mtk_grouped_ops::C256>)
-MTK_GROUPED(grad_128, 256, grouped_grad_direct<MTK_GROUPED_DT, 128, 2, 2, mtk_grouped_ops::C128, mtk_grouped_ops::C128>)
+MTK_GROUPED(grad_256, 512, mtk_grouped_ops::grad_256)
+MTK_GROUPED(grad_128, 256, mtk_grouped_ops::grad_128)
 MTK_GROUPED_QUARTER(grad_64, grouped_grad_quarter<MTK_GROUPED_DT, false, 8>)
 MTK_GROUPED_QUARTER(grad_64_any, grouped_grad_quarter<MTK_GROUPED_DT, true, 8>)
-MTK_GROUPED(bias_grad, 512, grouped_bias_grad<MTK_GROUPED_DT>)
+MTK_GROUPED(bias_grad, 512, mtk::grouped_bias_grad<MTK_GROUPED_DT>)

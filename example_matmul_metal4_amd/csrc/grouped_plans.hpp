@@ -50,6 +50,11 @@ int check_tiles(int E, int T, int block, long long tiles_n, long long *grid) {
   return MTK_OK;
 }
 
+// Workgroups of the tiles that expert_tiles.hpp runs: as many as are on the device at once, each with one tile after another.
+long long tile_grid(int tile, int cus, long long tiles) {
+  return tile == 64 ? tiles : std::min<long long>(tiles, (tile == 128 ? 2LL : 1LL) * cus);
+}
+
 const char *dtype_name(int dtype) { return dtype == MTK_F16 ? "f16" : "bf16"; }
 
 int plan_grouped(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
@@ -85,6 +90,7 @@ int plan_grouped(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
   a.has_bias = d.has_bias ? 1 : 0;
   long long grid;
   if ((s = check_tiles(d.E, d.T, tile, a.tiles_n, &grid)) != MTK_OK) return s;
+  grid = tile_grid(tile, cus, grid);
   mtk_plan *p = new mtk_plan();
   p->ctx = ctx;
   p->kind = PLAN_GROUPED;
@@ -127,10 +133,11 @@ int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out
   else if (even && wgs(128) >= cus) tile = 128;
   a.tiles_m = (int)tiles(tile, a.M);
   a.tiles_n = (int)tiles(tile, a.N);
-  const long long grid = wgs(tile);
+  long long grid = wgs(tile);
   const long long bias_tiles = tiles(128, d.N);
   if (grid > INT32_MAX / 512 || d.E * bias_tiles > INT32_MAX / 512)
     return fail(MTK_ERR_UNSUPPORTED, "%d groups with these N and K are not supported", d.E);
+  grid = tile_grid(tile, cus, grid);
   mtk_plan *p = new mtk_plan();
   p->ctx = ctx;
   p->kind = PLAN_GROUPED_GRAD;
@@ -235,6 +242,7 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
   long long grid;
   if ((s = check_tiles((int)groups, d.T, tile, a.tiles_n, &grid)) != MTK_OK) return s;
   if (!d.E) grid = (long long)((d.T + tile - 1) / tile) * a.tiles_n;
+  grid = tile_grid(tile, cus, grid);
   mtk_plan *p = new mtk_plan();
   p->ctx = ctx;
   p->kind = PLAN_MX_GEMM;
@@ -416,7 +424,6 @@ void patch_grouped(const mtk_plan *p, const Launch &l, char *block, const void *
       a.codes = t->workspace;
       a.scales = (char *)t->workspace + p->scales_at;
     }
-    a.wide = a.ld % 8 == 0 && aligned(p->kind == PLAN_MX_DEQUANT ? a.dst : a.src, 16);
   }
 }
 

@@ -214,7 +214,6 @@ typedef struct {
   int64_t ld;      /* elements between 16-bit rows */
   int32_t R, K;
   int32_t k_tiles; /* ceil(K / 256) */
-  int32_t wide;    /* 16-bit rows are read or written 16 bytes at a time */
 } mtk_mx_rows_kargs;
 
 /* Products of rows in that format: C [T][ldc] = A B_e^T + bias_e. */

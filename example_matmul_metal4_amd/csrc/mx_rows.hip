@@ -75,6 +75,11 @@ struct MxPlace {
   }
 };
 
+// 16 bytes at any 2-byte alignment (the hardware splits what crosses a line).
+struct __attribute__((packed, aligned(2))) Chunk {
+  u32x4 v;
+};
+
 template <int DT>
 __device__ __forceinline__ void mx_quantise(const mtk_mx_rows_kargs &a) {
   const MxPlace p(a);
@@ -83,31 +88,38 @@ __device__ __forceinline__ void mx_quantise(const mtk_mx_rows_kargs &a) {
   const uint16_t *src = (const uint16_t *)a.src + p.r0 * a.ld + p.k;
   u32x4 v[kMxRows];
 #pragma unroll
-  for (int i = 0; i < kMxRows; ++i) {
-    v[i] = u32x4{0u, 0u, 0u, 0u};
-    if (i >= n || p.k >= a.K) continue;
-    const uint16_t *at = src + (int64_t)i * a.ld;
-    if (a.wide && p.k + 8 <= a.K) {
-      v[i] = __builtin_nontemporal_load((const u32x4 *)at);
-    } else {
+  for (int i = 0; i < kMxRows; ++i) v[i] = u32x4{0u, 0u, 0u, 0u};
+  if (p.k + 8 <= a.K) {
+#pragma unroll
+    for (int i = 0; i < kMxRows; ++i)
+      if (i < n) v[i] = ((const Chunk *)(src + (int64_t)i * a.ld))->v;
+  } else if (p.k < a.K) {
+#pragma unroll
+    for (int i = 0; i < kMxRows; ++i) {
+      if (i >= n) break;
       uint32_t h[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) h[j] = p.k + j < a.K ? at[j] : 0u;
+      for (int j = 0; j < 8; ++j) h[j] = p.k + j < a.K ? src[(int64_t)i * a.ld + j] : 0u;
       v[i] = u32x4{h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16)};
     }
   }
-  if (p.kt >= a.k_tiles) return;  // whole blocks: 32 lanes
-  uint32_t *codes = (uint32_t *)((char *)a.codes + p.r0 * mx_row_bytes(a.k_tiles) + p.kt * 128) + (threadIdx.x & 31);
-  uint8_t *scales = (uint8_t *)a.scales + ((int64_t)p.kt * a.R + p.r0) * 8 + p.block;
+  const int lane = threadIdx.x & 63;
+  char *codes = (char *)a.codes + p.r0 * mx_row_bytes(a.k_tiles) + (int64_t)p.kt * 128 + 4 * (lane & 31);
+  uint32_t bytes = 0;  // of the block's scales, row by row
 #pragma unroll
   for (int i = 0; i < kMxRows; ++i) {
-    if (i >= n) break;
     uint32_t c;
     int byte;
     mx_quantise8<DT>(v[i], c, byte);
-    *(uint32_t *)((char *)codes + i * mx_row_bytes(a.k_tiles)) = c;
-    if ((threadIdx.x & 3) == 0) scales[8 * i] = (uint8_t)byte;
+    bytes |= (uint32_t)byte << (8 * i);
+    if (i < n && p.kt < a.k_tiles) *(uint32_t *)(codes + i * mx_row_bytes(a.k_tiles)) = c;
   }
+  // A K-tile's scales of the four rows are 32 bytes in a row: lane 8 * row + block of each half stores one, all in one instruction.
+  static_assert(kMxRows == 4, "32 bytes for 32 lanes");
+  bytes = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * ((lane & 32) + 4 * (lane & 7)), (int)bytes);
+  const int row = (lane >> 3) & 3;
+  if (row < n && p.kt < a.k_tiles)
+    ((uint8_t *)a.scales)[((int64_t)p.kt * a.R + p.r0 + row) * 8 + (lane & 7)] = (uint8_t)(bytes >> (8 * row));
 }
 
 template <int DT>
@@ -115,7 +127,7 @@ __device__ __forceinline__ void mx_dequantise(const mtk_mx_rows_kargs &a) {
   const MxPlace p(a);
   if (p.r0 >= a.R || p.k >= a.K) return;
   const int n = (int)min((int64_t)kMxRows, a.R - p.r0);
-  const char *codes = (const char *)a.codes + p.r0 * mx_row_bytes(a.k_tiles) + p.kt * 128 + 4 * (threadIdx.x & 31);
+  const char *codes = (const char *)a.codes + p.r0 * mx_row_bytes(a.k_tiles) + (int64_t)p.kt * 128 + 4 * (threadIdx.x & 31);
   const uint8_t *scales = (const uint8_t *)a.scales + ((int64_t)p.kt * a.R + p.r0) * 8 + p.block;
   uint32_t c[kMxRows], s[kMxRows];
 #pragma unroll
@@ -128,14 +140,15 @@ __device__ __forceinline__ void mx_dequantise(const mtk_mx_rows_kargs &a) {
   }
   constexpr uint32_t kNan = DT == DT_F16 ? 0x7E007E00u : 0x7FC07FC0u;
   uint16_t *dst = (uint16_t *)a.dst + p.r0 * a.ld + p.k;
+  const bool whole = p.k + 8 <= a.K;
 #pragma unroll
   for (int i = 0; i < kMxRows; ++i) {
     if (i >= n) break;
     u32x4 v = u32x4{kNan, kNan, kNan, kNan};
     if (s[i] != kNanScale) v = values8<DT, KV_FP4>(&c[i], scale_of(s[i]));
     uint16_t *at = dst + (int64_t)i * a.ld;
-    if (a.wide && p.k + 8 <= a.K) {
-      *(u32x4 *)at = v;
+    if (whole) {
+      ((Chunk *)at)->v = v;
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {

@@ -296,11 +296,8 @@ __device__ __forceinline__ void frag_wait(u32x4 (&fa)[TA], u32x4 (&fb)[TB]) {
 // the accumulators restart from zero; the epilogue adds the running sum and the last partition,
 // then the bias. The arithmetic is the two-pass split-K's: every partition accumulates from zero
 // over the same K-tiles, partition sums are added in partition order, the bias last.
-//
-// PLACED: the output tile's first row and column are given (at); otherwise the workgroup's number says which tile of the grid
-// it has.
-template <int DT, int BM, int BN, int WAVES_M, int WAVES_N, typename AOP, typename BOP, bool SERIAL = false, bool PLACED = false>
-__device__ __forceinline__ void tile_direct(const mtk_tile_args &a, const TileAt at = {}) {
+template <int DT, int BM, int BN, int WAVES_M, int WAVES_N, typename AOP, typename BOP, bool SERIAL = false>
+__device__ __forceinline__ void tile_direct(const mtk_tile_args &a) {
   constexpr int NW = WAVES_M * WAVES_N;
   static_assert(NW == 4 || NW == 8, "4 or 8 wavefronts per workgroup");
   static_assert(AOP::kWaves == NW && BOP::kWaves == NW, "operand policies staged by the same wavefronts");
@@ -336,20 +333,16 @@ __device__ __forceinline__ void tile_direct(const mtk_tile_args &a, const TileAt
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wave_m = wave / WAVES_N, wave_n = wave % WAVES_N;
 
-  int split = 0, t = 0, m0 = at.m0, n0 = at.n0;
-  if constexpr (!PLACED) {
-    const int tiles = a.tiles_m * a.tiles_n;
-    const int id = xcd_remap(blockIdx.x, gridDim.x);
-    split = SERIAL ? 0 : id / tiles;
-    t = id - split * tiles;
-    const int group = kGroupM * a.tiles_n;
-    const int first_m = (t / group) * kGroupM;
-    const int gm = min(a.tiles_m - first_m, kGroupM);
-    const int tm = first_m + (t % group) % gm;
-    const int tn = (t % group) / gm;
-    m0 = tm * BM;
-    n0 = tn * BN;
-  }
+  const int tiles = a.tiles_m * a.tiles_n;
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int split = SERIAL ? 0 : id / tiles;
+  const int t = id - split * tiles;
+  const int group = kGroupM * a.tiles_n;
+  const int first_m = (t / group) * kGroupM;
+  const int gm = min(a.tiles_m - first_m, kGroupM);
+  const int tm = first_m + (t % group) % gm;
+  const int tn = (t % group) / gm;
+  const int m0 = tm * BM, n0 = tn * BN;
   const int kt0 = SERIAL ? 0 : split_first_tile(a, split, t);
   const int kt1 = SERIAL ? a.k_tiles : split_first_tile(a, split + 1, t);
   constexpr bool kAnyTail = AOP::kNeedsTail || BOP::kNeedsTail;

@@ -480,7 +480,7 @@ typedef struct {
 /* 16-bit rows [R][ld] into codes and scales. The weights [E][N][K] of a grouped product are E x N rows. */
 int mtk_mx_quantize_plan(mtk_ctx *ctx, const mtk_mx_rows_desc *desc, mtk_plan **out);
 typedef struct {
-  const void *src;      /* 2-byte aligned; 16-byte aligned rows (ld a multiple of 8) are read faster */
+  const void *src;      /* 2-byte aligned; rows of 16-byte alignment (ld a multiple of 8) are read fastest */
   void *codes, *scales; /* 16-byte aligned */
 } mtk_mx_quantize_args;
 int mtk_mx_quantize_run(const mtk_plan *plan, const mtk_mx_quantize_args *args);
