@@ -171,6 +171,7 @@ struct ForwardTiles {
   __device__ __forceinline__ int ldb() const { return g.ldb; }
   __device__ __forceinline__ int ldc() const { return g.ldc; }
   __device__ __forceinline__ bool f32() const { return false; }
+  __device__ __forceinline__ bool streamed() const { return false; }
   __device__ __forceinline__ ExpertTile get(int i) const {
     ExpertTile t{};
     const GroupTile gt = search.get(i);
@@ -207,6 +208,7 @@ struct GradTiles {
   __device__ __forceinline__ int ldb() const { return g.ldb; }
   __device__ __forceinline__ int ldc() const { return g.N; }
   __device__ __forceinline__ bool f32() const { return g.C32 != nullptr; }
+  __device__ __forceinline__ bool streamed() const { return true; }  // gradients: nothing reads them soon
   __device__ __forceinline__ ExpertTile get(int i) const {
     ExpertTile t{};
     const int tiles = g.tiles_m * g.tiles_n, id = nth_tile(i, g.E * tiles);
@@ -244,6 +246,7 @@ struct MxTiles {
   __device__ __forceinline__ int ldb() const { return (int)(row_b >> 1); }
   __device__ __forceinline__ int ldc() const { return g.ldc; }
   __device__ __forceinline__ bool f32() const { return false; }
+  __device__ __forceinline__ bool streamed() const { return false; }
   __device__ __forceinline__ size_t a_step() const { return (size_t)g.T * 8; }
   __device__ __forceinline__ size_t b_step() const { return (size_t)g.E * (size_t)g.N * 8; }
   __device__ __forceinline__ ExpertTile get(int i) const {
@@ -434,7 +437,9 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
     const size_t at = (size_t)(wave_m * WTM) * (size_t)ldc + (size_t)(wave_n * WTN);
     if (tiles.f32()) {
       float *C = (float *)t.c + at;
-      const bool two = (ldc & 1) == 0;  // 8-byte aligned pairs
+      // Past the caches where rows are whole halves of lines: 7183 rows, 128 groups of 6640 x 128 206 -> 117 us; rows of other lengths
+      // leave parts of lines for the L2 to join: 471 rows, 128 of 256 x 2616 199 -> 104 through it.
+      const bool streamed = (ldc & 15) == 0 && ((uintptr_t)C & 63) == 0;
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         const int col = col_l + 32 * j;
@@ -447,11 +452,13 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
             const int row = row_l + 32 * i + 8 * (r >> 2) + (r & 3);
             if (row >= rows) continue;
             float *p = C + (size_t)row * (size_t)ldc + col;
-            if (two && col + 1 < cols) {
-              __builtin_nontemporal_store(f32x2{lo, hi}, (f32x2 *)p);
-            } else {
-              if (col < cols) __builtin_nontemporal_store(lo, p);
-              if (col + 1 < cols) __builtin_nontemporal_store(hi, p + 1);
+            if (col + 1 < cols) {
+              if (streamed)
+                __builtin_nontemporal_store(f32x2{lo, hi}, (f32x2 *)p);
+              else
+                ((Pair *)p)->v = f32x2{lo, hi};
+            } else if (col < cols) {
+              *p = lo;
             }
           }
       }
@@ -464,7 +471,7 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
       bv[j] = t.bias && own < cols ? from_bits<DT>(t.bias[wave_n * WTN + own]) : 0.0f;
     }
     uint16_t *C = (uint16_t *)t.c + at;
-    const bool v16 = (ldc & 7) == 0 && ((uintptr_t)C & 15) == 0;
+    const bool streamed = tiles.streamed() && (ldc & 31) == 0 && ((uintptr_t)C & 63) == 0;
     const uint32_t park = lds + (uint32_t)(kPark + wave * 2048);
     // The chunk swizzle puts the four rows that one write touches on different banks. Reads and writes of a wavefront are done in
     // order; inline asm, as the compiler would make them wait for the loads in flight.
@@ -497,8 +504,11 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
         const int row = 16 * p + 8 * it + (le >> 3), c8 = 8 * (le & 7);
         if (row < rows) {
           uint16_t *dst = C + (size_t)row * (size_t)ldc + c8;
-          if (v16 && c8 + 8 <= cols) {
-            *(u32x4 *)dst = v[it];
+          if (c8 + 8 <= cols) {
+            if (streamed)
+              __builtin_nontemporal_store(v[it], (u32x4 *)dst);
+            else
+              ((Chunk *)dst)->v = v[it];
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {

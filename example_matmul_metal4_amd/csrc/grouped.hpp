@@ -15,6 +15,14 @@
 
 namespace mtk {
 
+// 16 and 8 bytes at any alignment that their elements have: one access, which the hardware splits where it crosses a line.
+struct __attribute__((packed, aligned(2))) Chunk {
+  u32x4 v;
+};
+struct __attribute__((packed, aligned(4))) Pair {
+  f32x2 v;
+};
+
 // Inclusive sum over the lanes up to this one.
 __device__ __forceinline__ int lanes_scan(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1

@@ -37,23 +37,27 @@ __device__ __forceinline__ void grad_128(const mtk_grouped_kargs &g) {
   extern "C" __global__ void __launch_bounds__(THREADS) MTK_GROUPED_NAME(NAME)(const mtk_grouped_kargs g) { \
     __VA_ARGS__(g);                                                                                          \
   }
-// quarter tiles: one workgroup of 8 wavefronts per CU, whose registers they may all have
-#define MTK_GROUPED_QUARTER(NAME, ...)                                                              \
-  extern "C" __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))      \
-  MTK_GROUPED_NAME(NAME)(const mtk_grouped_kargs g) {                                               \
-    mtk::__VA_ARGS__(g);                                                                             \
+// quarter tiles, K-tiles over W wavefronts: 8, or 4 in two workgroups per CU, or 1 in eight
+#define MTK_GROUPED_QUARTER(NAME, W, ...)                                                           \
+  extern "C" __global__ void __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2)))   \
+  MTK_GROUPED_NAME(NAME##_w##W)(const mtk_grouped_kargs g) {                                        \
+    mtk::__VA_ARGS__, W>(g);                                                                         \
   }
+#define MTK_GROUPED_QUARTERS(W)                                                      \
+  MTK_GROUPED_QUARTER(nt_64, W, grouped_quarter<MTK_GROUPED_DT, false, false)         \
+  MTK_GROUPED_QUARTER(nn_64, W, grouped_quarter<MTK_GROUPED_DT, true, false)          \
+  MTK_GROUPED_QUARTER(nt_64_any, W, grouped_quarter<MTK_GROUPED_DT, false, true)      \
+  MTK_GROUPED_QUARTER(nn_64_any, W, grouped_quarter<MTK_GROUPED_DT, true, true)       \
+  MTK_GROUPED_QUARTER(grad_64, W, grouped_grad_quarter<MTK_GROUPED_DT, false)         \
+  MTK_GROUPED_QUARTER(grad_64_any, W, grouped_grad_quarter<MTK_GROUPED_DT, true)
+MTK_GROUPED_QUARTERS(8)
+MTK_GROUPED_QUARTERS(4)
+MTK_GROUPED_QUARTERS(1)
 
 MTK_GROUPED(nt_256, 512, mtk_grouped_ops::nt_256)
 MTK_GROUPED(nn_256, 512, mtk_grouped_ops::nn_256)
 MTK_GROUPED(nt_128, 256, mtk_grouped_ops::nt_128)
 MTK_GROUPED(nn_128, 256, mtk_grouped_ops::nn_128)
-MTK_GROUPED_QUARTER(nt_64, grouped_quarter<MTK_GROUPED_DT, false, false, 8>)
-MTK_GROUPED_QUARTER(nn_64, grouped_quarter<MTK_GROUPED_DT, true, false, 8>)
-MTK_GROUPED_QUARTER(nt_64_any, grouped_quarter<MTK_GROUPED_DT, false, true, 8>)
-MTK_GROUPED_QUARTER(nn_64_any, grouped_quarter<MTK_GROUPED_DT, true, true, 8>)
 MTK_GROUPED(grad_256, 512, mtk_grouped_ops::grad_256)
 MTK_GROUPED(grad_128, 256, mtk_grouped_ops::grad_128)
-MTK_GROUPED_QUARTER(grad_64, grouped_grad_quarter<MTK_GROUPED_DT, false, 8>)
-MTK_GROUPED_QUARTER(grad_64_any, grouped_grad_quarter<MTK_GROUPED_DT, true, 8>)
 MTK_GROUPED(bias_grad, 512, mtk::grouped_bias_grad<MTK_GROUPED_DT>)

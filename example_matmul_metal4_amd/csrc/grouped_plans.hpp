@@ -55,6 +55,11 @@ long long tile_grid(int tile, int cus, long long tiles) {
   return tile == 64 ? tiles : std::min<long long>(tiles, (tile == 128 ? 2LL : 1LL) * cus);
 }
 
+int tile_waves(int tile) { return tile == 128 ? 4 : 8; }
+std::string tile_name(int tile, bool even, int waves) {
+  return std::to_string(tile) + (even ? "" : "_any") + (tile == 64 ? "_w" + std::to_string(waves) : "");
+}
+
 const char *dtype_name(int dtype) { return dtype == MTK_F16 ? "f16" : "bf16"; }
 
 int plan_grouped(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
@@ -96,9 +101,9 @@ int plan_grouped(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
   p->kind = PLAN_GROUPED;
   p->grouped = d;
   p->align_a = p->align_b = even ? 4 : 2;
-  const std::string name = std::string("mtk_grouped_") + dtype_name(d.dtype) + (d.trans_b ? "_nt_" : "_nn_") + std::to_string(tile) +
-                           (even ? "" : "_any");
-  add_launch(p, name, grid, tile == 128 ? 256 : 512, a);
+  const int waves = tile_waves(tile);
+  const std::string name = std::string("mtk_grouped_") + dtype_name(d.dtype) + (d.trans_b ? "_nt_" : "_nn_") + tile_name(tile, even, waves);
+  add_launch(p, name, grid, 64 * waves, a);
   p->flops = 2.0 * d.T * d.N * d.K;
   p->bytes = 2.0 * ((double)d.T * (d.N + d.K) + (double)std::min(d.E, d.T) * d.N * d.K);
   char desc[256];
@@ -144,8 +149,9 @@ int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out
   p->grouped = d;
   p->align_a = p->align_b = even ? 4 : 2;
   const std::string head = std::string("mtk_grouped_") + dtype_name(d.dtype);
-  const std::string name = head + "_grad_" + std::to_string(tile) + (even ? "" : "_any");
-  add_launch(p, name, grid, tile == 128 ? 256 : 512, a);
+  const int waves = tile_waves(tile);
+  const std::string name = head + "_grad_" + tile_name(tile, even, waves);
+  add_launch(p, name, grid, 64 * waves, a);
   if (d.has_bias) {
     mtk_grouped_kargs b{};
     b.E = d.E;

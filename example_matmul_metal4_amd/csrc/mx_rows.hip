@@ -9,6 +9,7 @@
 //
 // A lane has 8 places of a row (16 bytes in 16 bits, 4 in codes), 4 neighbours a block, 32 a K-tile; a wavefront two K-tiles
 // of MX_ROWS rows, whose loads are all in flight at once.
+#include "grouped.hpp"
 #include "kv_device.hpp"
 #include "mx.h"
 
@@ -73,11 +74,6 @@ struct MxPlace {
     k = kt * 256 + 8 * (lane & 31);
     block = (lane & 31) >> 2;
   }
-};
-
-// 16 bytes at any 2-byte alignment (the hardware splits what crosses a line).
-struct __attribute__((packed, aligned(2))) Chunk {
-  u32x4 v;
 };
 
 template <int DT>

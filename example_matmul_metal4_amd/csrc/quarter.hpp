@@ -215,6 +215,27 @@ __device__ __forceinline__ void quarter_tile(const mtk_tile_args &a, AOp oa, con
     __builtin_amdgcn_wave_barrier();
   }
 
+  if constexpr (W == 1) {  // one wavefront has the whole sum (of grouped products: never partials and a bias)
+    const uint16_t *bias1 = (const uint16_t *)a.bias;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int col = n0 + 32 * j + (lane & 31);
+      if (col >= a.N) continue;
+      const float bv = a.has_bias ? from_bits<DT>(bias1[col]) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int row = m0 + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+          if (row >= a.M) continue;
+          if (a.partial != nullptr)
+            a.partial[(size_t)row * (size_t)a.N + col] = acc[i][j][r];
+          else
+            ((uint16_t *)a.C)[(size_t)row * (size_t)a.ldc + col] = to_bits<DT>(acc[i][j][r] + bv);
+        }
+    }
+    return;
+  }
   // ---- add the wavefronts' sums: accumulator quads parked as [block][quad][lane], 16 bytes each
   constexpr int kCols = 2 / kPasses;  // column blocks per pass
   const uint16_t *bias = (const uint16_t *)a.bias;
