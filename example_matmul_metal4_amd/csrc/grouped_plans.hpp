@@ -52,12 +52,61 @@ int check_tiles(int E, int T, int block, long long tiles_n, long long *grid) {
 
 // Workgroups of the tiles that expert_tiles.hpp runs: as many as are on the device at once, each with one tile after another.
 long long tile_grid(int tile, int cus, long long tiles) {
-  return tile == 64 ? tiles : std::min<long long>(tiles, (tile == 128 ? 2LL : 1LL) * cus);
+  return tile <= 64 ? tiles : std::min<long long>(tiles, (tile == 128 ? 2LL : 1LL) * cus);
 }
 
-int tile_waves(int tile) { return tile == 128 ? 4 : 8; }
-std::string tile_name(int tile, bool even, int waves) {
-  return std::to_string(tile) + (even ? "" : "_any") + (tile == 64 ? "_w" + std::to_string(waves) : "");
+// Which kernel runs a product, by the time that it is expected to take, in us: `start` and the larger of
+//   rounds * (round + (step + full * part) * K-tiles of a wavefront)   and   bytes * byte (us per MB),
+// with 0.15 of the other. rounds: workgroups over those that are on the device at once, at least 1; part: that share, at most 1 (a full
+// device's K-tiles take longer). The groups' sizes lie on the device: of E groups, E (1 - exp(-T / E)) are taken to have rows, as if
+// each row chose one of E, and each to have half a block that is not full. Fitted to launches of 290 forward products, 170
+// gradients and 200 products in few bits, each by every kernel (random sizes, T to 16384, N and K 64 to 14336): the kernel chosen takes
+// 1.03, 1.03 and 1.01 times (geometric mean) the time of the fastest.
+// Examples, us (tiles of 256, of 128, of 64 with 8, 4, 1 wavefronts): 256 rows over 8 groups of 14336 x 4096: 199, 168, 175, 171, 168;
+// 8192 over 16 of 4096 x 4096: 316, 351, 634, 559, 535; 16 over 32 of 2048 x 2048: 40, 31, 23, 21, 31. Gradients: 4 over 7 of 7448 x
+// 7296: 226, 224, 1033, 580, 282; 1000 over 24 of 1023 x 520: -, -, 72, 51, 43.
+struct TileCost {
+  int tile, waves, per_cu;  // rows and columns of a tile (32: 64 columns); wavefronts and workgroups per CU
+  double start, round, step, full, byte;
+  double any;  // odd leading dimensions: K-tiles take longer by this share; below 0: not for these
+};
+constexpr TileCost kForward[] = {{256, 8, 1, 4.4, 0.26, 0.75, 1.13, 0.24, -1},
+                                 {128, 4, 2, 4.4, 0.0, 0.47, 0.85, 0.18, -1},
+                                 {64, 8, 1, 2.3, 1.03, 1.29, 0.99, 0.18, 0.36},
+                                 {64, 4, 2, 2.3, 1.78, 0.80, 1.23, 0.16, 0.34},
+                                 {64, 1, 8, 0.0, 4.57, 0.71, 1.16, 0.16, 0.29}};
+constexpr TileCost kGradient[] = {{256, 8, 1, 7.5, 2.10, 0.93, 2.17, 0.23, -1},
+                                  {128, 4, 2, 5.7, 0.96, 0.48, 1.40, 0.22, -1},
+                                  {64, 8, 1, 3.5, 0.0, 1.70, 1.01, 0.48, 0.14},
+                                  {64, 4, 2, 4.4, 0.0, 0.82, 2.06, 0.35, 0.16},
+                                  {64, 1, 8, 4.6, 2.05, 0.84, 2.65, 0.23, 0.43}};
+constexpr TileCost kFewBits[] = {{256, 8, 1, 8.8, 0.05, 0.82, 1.74, 0.33, 0},
+                                 {128, 4, 2, 6.9, 0.81, 0.47, 1.28, 0.27, 0},
+                                 {64, 8, 1, 5.0, 0.07, 1.77, 1.73, 0.22, 0},
+                                 {32, 8, 1, 4.8, 0.53, 1.01, 1.05, 0.20, 0}};
+
+double busy_groups(int E, int T) { return E > 1 ? E * -std::expm1(-(double)T / E) : 1.0; }
+double tiles_across(int tile, int n) { return (double)(((long long)n + std::max(tile, 64) - 1) / std::max(tile, 64)); }
+
+// wgs: workgroups with a tile of `tile`; k_tiles: of a tile
+template <int N, typename WGS>
+TileCost choose_tile(const TileCost (&costs)[N], bool even, int cus, double k_tiles, double mbytes, WGS wgs) {
+  const TileCost *best = nullptr;
+  double least = 0;
+  for (const TileCost &c : costs) {
+    if (!even && c.any < 0) continue;
+    const double there = wgs(c.tile) / ((double)cus * c.per_cu), rounds = std::max(1.0, there);
+    const double steps = c.tile > 64 || c.waves == 1 ? k_tiles : std::ceil(k_tiles / c.waves);
+    const double step = (c.step + c.full * std::min(1.0, there)) * (even ? 1.0 : 1.0 + c.any);
+    const double x = rounds * (c.round + step * steps), y = mbytes * c.byte;
+    const double t = c.start + std::max(x, y) + 0.15 * std::min(x, y);
+    if (!best || t < least) best = &c, least = t;
+  }
+  return *best;
+}
+
+std::string tile_name(const TileCost &c, bool even) {
+  return std::to_string(c.tile) + (even ? "" : "_any") + (c.tile == 64 ? "_w" + std::to_string(c.waves) : "");
 }
 
 const char *dtype_name(int dtype) { return dtype == MTK_F16 ? "f16" : "bf16"; }
@@ -76,10 +125,11 @@ int plan_grouped(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
   if (b_exact > kMaxOperandBytes) return fail(MTK_ERR_UNSUPPORTED, "the weights of a group must be below 2 GiB");
   const int cus = ctx ? ctx->prop.multiProcessorCount : 256;
   const bool even = d.lda % 2 == 0 && d.ldb % 2 == 0;
-  auto wgs = [&](int tile) { return group_max_blocks(d.E, d.T, tile) * ((d.N + tile - 1) / tile); };
-  int tile = 64;
-  if (even && wgs(256) >= cus * 5 / 8 && d.T >= 64LL * d.E) tile = 256;
-  else if (even && wgs(128) >= cus && d.T >= 32LL * d.E) tile = 128;
+  const double busy = busy_groups(d.E, d.T);
+  const TileCost kind = choose_tile(kForward, even, cus, (d.K + 63) / 64, 2e-6 * (busy * d.N * d.K + (double)d.T * ((double)d.N + d.K)), [&](int t) {
+    return std::max(busy, (double)d.T / t + 0.5 * busy) * tiles_across(t, d.N);
+  });
+  const int tile = kind.tile;
   mtk_grouped_kargs a{};
   a.E = d.E;
   a.T = d.T;
@@ -101,9 +151,8 @@ int plan_grouped(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
   p->kind = PLAN_GROUPED;
   p->grouped = d;
   p->align_a = p->align_b = even ? 4 : 2;
-  const int waves = tile_waves(tile);
-  const std::string name = std::string("mtk_grouped_") + dtype_name(d.dtype) + (d.trans_b ? "_nt_" : "_nn_") + tile_name(tile, even, waves);
-  add_launch(p, name, grid, 64 * waves, a);
+  const std::string name = std::string("mtk_grouped_") + dtype_name(d.dtype) + (d.trans_b ? "_nt_" : "_nn_") + tile_name(kind, even);
+  add_launch(p, name, grid, 64 * kind.waves, a);
   p->flops = 2.0 * d.T * d.N * d.K;
   p->bytes = 2.0 * ((double)d.T * (d.N + d.K) + (double)std::min(d.E, d.T) * d.N * d.K);
   char desc[256];
@@ -133,9 +182,10 @@ int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out
   a.ldb = d.trans_b ? d.lda : d.ldc;
   auto tiles = [&](int tile, int n) { return (long long)((n + tile - 1) / tile); };
   auto wgs = [&](int tile) { return d.E * tiles(tile, a.M) * tiles(tile, a.N); };
-  int tile = 64;
-  if (even && wgs(256) >= cus * 5 / 8) tile = 256;
-  else if (even && wgs(128) >= cus) tile = 128;
+  const double k_tiles = std::max(1.0, d.T / busy_groups(d.E, d.T) / 64);
+  const TileCost kind = choose_tile(kGradient, even, cus, k_tiles, 1e-6 * ((d.out_f32 ? 4.0 : 2.0) * d.E * d.N * d.K + 2.0 * d.T * ((double)d.N + d.K)),
+                                    [&](int t) { return (double)wgs(t); });
+  const int tile = kind.tile;
   a.tiles_m = (int)tiles(tile, a.M);
   a.tiles_n = (int)tiles(tile, a.N);
   long long grid = wgs(tile);
@@ -149,9 +199,8 @@ int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out
   p->grouped = d;
   p->align_a = p->align_b = even ? 4 : 2;
   const std::string head = std::string("mtk_grouped_") + dtype_name(d.dtype);
-  const int waves = tile_waves(tile);
-  const std::string name = head + "_grad_" + tile_name(tile, even, waves);
-  add_launch(p, name, grid, 64 * waves, a);
+  const std::string name = head + "_grad_" + tile_name(kind, even);
+  add_launch(p, name, grid, 64 * kind.waves, a);
   if (d.has_bias) {
     mtk_grouped_kargs b{};
     b.E = d.E;
@@ -236,15 +285,25 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
   a.E = (int)groups;
   a.T = d.T;
   a.N = d.N;
+  a.lda = d.lda;
+  a.K = d.K;
   a.k_tiles = k_tiles;
   a.ldc = d.ldc;
   a.has_bias = d.has_bias ? 1 : 0;
   const int cus = ctx ? ctx->prop.multiProcessorCount : 256;
-  auto wgs = [&](int tile) { return group_max_blocks((int)groups, d.T, tile) * ((d.N + tile - 1) / tile); };
-  int tile = 64;
-  if (wgs(256) >= cus * 5 / 8 && d.T >= 64LL * groups) tile = 256;
-  else if (wgs(128) >= cus && d.T >= 32LL * groups) tile = 128;
-  a.tiles_n = (d.N + tile - 1) / tile;
+  const double busy = busy_groups((int)groups, d.T);
+  TileCost kind = choose_tile(kFewBits, true, cus, k_tiles, 1e-6 * (0.53 * (busy * d.N * d.K + (double)d.T * d.K) + 2.0 * d.T * d.N), [&](int t) {
+    return (d.E ? std::max(busy, (double)d.T / t + 0.5 * busy) : (double)((d.T + t - 1) / t)) * tiles_across(t, d.N);
+  });
+  // Few rows are brought into the format by the product's own workgroups, each of them all that it needs: 0.2 us for two rows and a
+  // K-tile of a wavefront, against 2.4 for the launch. 14336 x 4096: 1 row 6.6 us (with the launch 8.3), 8 rows 8.5 (8.3), 16 10.2
+  // (8.6); 2048 x 2048: 16 rows 7.0 (7.3); 4096 x 14336: 1 row 12.6 (12.1).
+  const TileCost &few = kFewBits[3];
+  const double per = d.E ? std::max(1.0, d.T / busy) : d.T, rounds = std::ceil(busy * tiles_across(32, d.N) / cus);
+  const bool inside = d.quantize_a && d.T <= 32.0 * busy && std::ceil(per / 2) * std::ceil(k_tiles / 8.0) * rounds <= 8;
+  if (inside) kind = few;
+  const int tile = kind.tile;
+  a.tiles_n = (d.N + std::max(tile, 64) - 1) / std::max(tile, 64);
   long long grid;
   if ((s = check_tiles((int)groups, d.T, tile, a.tiles_n, &grid)) != MTK_OK) return s;
   if (!d.E) grid = (long long)((d.T + tile - 1) / tile) * a.tiles_n;
@@ -253,14 +312,14 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
   p->ctx = ctx;
   p->kind = PLAN_MX_GEMM;
   p->mx_gemm = d;
-  if (d.quantize_a) {
+  if (d.quantize_a && !inside) {
     p->launches.push_back(mx_rows_launch(true, d.T, d.K, d.lda, d.dtype));
     p->launches.back().role = ROLE_PERMUTE;
     p->scales_at = (mx_code_bytes(d.T, k_tiles) + 255) & ~(size_t)255;  // the scales
     p->workspace = p->scales_at + mx_scale_bytes(d.T, k_tiles);
   }
-  const std::string name = std::string("mtk_mx_gemm_") + dtype_name(d.dtype) + "_" + std::to_string(tile);
-  add_launch(p, name, grid, tile == 128 ? 256 : 512, a);
+  const std::string name = std::string("mtk_mx_gemm_") + dtype_name(d.dtype) + "_" + std::to_string(tile) + (inside ? "q" : "");
+  add_launch(p, name, grid, 64 * kind.waves, a);
   p->flops = 2.0 * d.T * d.N * d.K;
   p->bytes = 136.0 * k_tiles * ((d.quantize_a ? 0.0 : d.T) + (double)std::min<long long>(groups, d.T) * d.N) + 2.0 * d.T * d.N +
              (d.quantize_a ? 2.0 * d.T * d.K : 0.0);
@@ -405,8 +464,9 @@ void patch_grouped(const mtk_plan *p, const Launch &l, char *block, const void *
   } else if (p->kind == PLAN_MX_GEMM && l.role == ROLE_MAIN) {
     const mtk_mx_gemm_args *t = (const mtk_mx_gemm_args *)argset;
     mtk_mx_gemm_kargs &a = *(mtk_mx_gemm_kargs *)block;
-    a.A = p->mx_gemm.quantize_a ? t->workspace : t->A;
-    a.a_scales = p->mx_gemm.quantize_a ? (char *)t->workspace + p->scales_at : t->a_scales;
+    const bool held = p->mx_gemm.quantize_a && p->workspace;  // the launch before has brought the rows into the format
+    a.A = held ? t->workspace : t->A;
+    a.a_scales = held ? (char *)t->workspace + p->scales_at : t->a_scales;
     a.B = t->B;
     a.b_scales = t->b_scales;
     a.bias = t->bias;

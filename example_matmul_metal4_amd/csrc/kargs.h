@@ -218,12 +218,13 @@ typedef struct {
 
 /* Products of rows in that format: C [T][ldc] = A B_e^T + bias_e. */
 typedef struct {
-  const void *A, *a_scales; /* codes [T][k_tiles * 128], scales [k_tiles][T][8] */
+  const void *A, *a_scales; /* codes [T][k_tiles * 128], scales [k_tiles][T][8]; or 16-bit rows [T][lda] */
   const void *B, *b_scales; /* codes [E * N][k_tiles * 128], scales [k_tiles][E * N][8] */
   const void *bias;
   const int32_t *row_start; /* [E + 1]; NULL: one group of T rows */
   void *C;
-  int32_t E, T, N, k_tiles;
+  int64_t lda;
+  int32_t E, T, N, K, k_tiles;
   int32_t ldc, tiles_n, has_bias;
 } mtk_mx_gemm_kargs;
 
