@@ -162,9 +162,10 @@ __device__ __forceinline__ void grouped_grad_quarter(const mtk_grouped_kargs &g)
   quarter_tile<DT, A, true, ANY, W, true>(a, A{}, tile_at<64, 64>(id - e * tiles, g.tiles_m, g.tiles_n));
 }
 
-// dbias_e[n] = sum over the group's rows of dC[t][n]: 128 columns per workgroup, two per lane; its 8 wavefronts take every
-// 8th row, and their sums in 32 bits are added in wavefront order.
-constexpr int kBiasWaves = 8, kBiasCols = 128;
+// dbias_e[n] = sum over the group's rows of dC[t][n]: 64 columns per workgroup, one per lane; its 16 wavefronts take every 16th
+// row, 8 of them in flight at a time, and their sums in 32 bits are added in wavefront order. Latency bounds it: 343 rows of the
+// largest of 24 groups, 1023 columns: 8 wavefronts with two columns per lane 15.3 us.
+constexpr int kBiasWaves = 16, kBiasCols = 64;
 template <int DT>
 __device__ __forceinline__ void grouped_bias_grad(const mtk_grouped_kargs &g) {
   __shared__ float sums[kBiasWaves][kBiasCols];
@@ -172,39 +173,37 @@ __device__ __forceinline__ void grouped_bias_grad(const mtk_grouped_kargs &g) {
   const int e = blockIdx.x / g.tiles_n, n0 = (blockIdx.x - e * g.tiles_n) * kBiasCols;
   const int start = __builtin_amdgcn_readfirstlane(g.row_start[e]), next = __builtin_amdgcn_readfirstlane(g.row_start[e + 1]);
   const group_rows r = group_of(start, next, g.T);
-  float s0 = 0.0f, s1 = 0.0f;
-  const int n = n0 + 2 * lane;
-  const uint16_t *at = (const uint16_t *)g.A + (size_t)r.first * (size_t)g.lda + n;
-  const bool pair = ((g.lda & 1) == 0) && (((uintptr_t)g.A & 3) == 0);  // whole dwords
-  if (pair && n + 1 < g.N) {
-#pragma unroll 8
-    for (int i = wave; i < r.rows; i += kBiasWaves) {
-      const uint32_t v = *(const uint32_t *)(at + (size_t)i * (size_t)g.lda);
-      s0 += from_bits<DT>(v & 0xffffu);
-      s1 += from_bits<DT>(v >> 16);
-    }
-  } else if (n < g.N) {
-    const bool two = n + 1 < g.N;
-#pragma unroll 4
-    for (int i = wave; i < r.rows; i += kBiasWaves) {
-      const uint16_t *p = at + (size_t)i * (size_t)g.lda;
-      s0 += from_bits<DT>(p[0]);
-      if (two) s1 += from_bits<DT>(p[1]);
-    }
-  }
-  sums[wave][2 * lane] = s0;
-  sums[wave][2 * lane + 1] = s1;
-  __syncthreads();
-  const int c = threadIdx.x;
-  if (c < kBiasCols && n0 + c < g.N) {
-    float s = sums[0][c];
+  const uint16_t *at = (const uint16_t *)g.A + (size_t)(r.first + wave) * (size_t)g.lda + min(n0 + lane, g.N - 1);
+  const size_t step = (size_t)kBiasWaves * (size_t)g.lda;
+  float s = 0.0f;
+  int i = wave;
+  constexpr int kAhead = 8;
+  for (; i + (kAhead - 1) * kBiasWaves < r.rows; i += kAhead * kBiasWaves, at += kAhead * step) {
+    uint16_t v[kAhead];
 #pragma unroll
-    for (int w = 1; w < kBiasWaves; ++w) s += sums[w][c];
-    const size_t out = (size_t)e * (size_t)g.N + n0 + c;
+    for (int j = 0; j < kAhead; ++j) v[j] = at[j * step];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) s += from_bits<DT>(v[j]);
+  }
+  if (i < r.rows) {  // the rest, rows past the last read again and not added
+    uint16_t v[kAhead];
+    const int n = (r.rows - i + kBiasWaves - 1) / kBiasWaves;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) v[j] = at[min(j, n - 1) * step];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) s += j < n ? from_bits<DT>(v[j]) : 0.0f;
+  }
+  sums[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && n0 + lane < g.N) {
+    float t = sums[0][lane];
+#pragma unroll
+    for (int w = 1; w < kBiasWaves; ++w) t += sums[w][lane];
+    const size_t out = (size_t)e * (size_t)g.N + (size_t)(n0 + lane);
     if (g.C32)
-      g.C32[out] = s;
+      g.C32[out] = t;
     else
-      ((uint16_t *)g.C)[out] = to_bits<DT>(s);
+      ((uint16_t *)g.C)[out] = to_bits<DT>(t);
   }
 }
 

@@ -189,8 +189,8 @@ int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out
   a.tiles_m = (int)tiles(tile, a.M);
   a.tiles_n = (int)tiles(tile, a.N);
   long long grid = wgs(tile);
-  const long long bias_tiles = tiles(128, d.N);
-  if (grid > INT32_MAX / 512 || d.E * bias_tiles > INT32_MAX / 512)
+  const long long bias_tiles = tiles(64, d.N);
+  if (grid > INT32_MAX / 512 || d.E * bias_tiles > INT32_MAX / 1024)
     return fail(MTK_ERR_UNSUPPORTED, "%d groups with these N and K are not supported", d.E);
   grid = tile_grid(tile, cus, grid);
   mtk_plan *p = new mtk_plan();
@@ -208,7 +208,7 @@ int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out
     b.N = d.N;
     b.lda = d.ldc;
     b.tiles_n = (int)bias_tiles;
-    add_launch(p, head + "_bias_grad", d.E * bias_tiles, 512, b);
+    add_launch(p, head + "_bias_grad", d.E * bias_tiles, 1024, b);
     p->launches.back().role = ROLE_REDUCE;
   }
   p->flops = 2.0 * d.T * d.N * d.K;

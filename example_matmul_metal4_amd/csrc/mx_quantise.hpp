@@ -27,9 +27,11 @@ struct MxSource {
   }
   __device__ __forceinline__ uint32_t at(int row, int k) const { return (uint32_t)row * step + (uint32_t)k * 2u + mis; }
   // The 8 places of a row from k on, in two steps, so that many loads are in flight: the dwords that hold them ...
+  // (POLICY 2: past the caches)
+  template <int POLICY = 0>
   __device__ __forceinline__ void load(int row, int k, u32x4 &v, uint32_t &e) const {
     const uint32_t off = k < K ? at(row, k) : kOOBAny;
-    v = buf_load16(buf, off & ~3u);
+    v = __builtin_amdgcn_raw_buffer_load_b128(buf, off & ~3u, 0, POLICY);
     if (odd) e = buf_load4(buf, (off & ~3u) + 16u);
   }
   // ... and the places themselves, zeros from K on.

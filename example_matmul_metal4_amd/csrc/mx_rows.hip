@@ -39,7 +39,7 @@ __device__ __forceinline__ void mx_quantise(const mtk_mx_rows_kargs &a) {
   u32x4 v[kMxRows];
   uint32_t e[kMxRows] = {};
 #pragma unroll
-  for (int i = 0; i < kMxRows; ++i) src.load(i, p.k, v[i], e[i]);
+  for (int i = 0; i < kMxRows; ++i) src.load<2>(i, p.k, v[i], e[i]);
   const int lane = threadIdx.x & 63;
   char *codes = (char *)a.codes + p.r0 * mx_row_bytes(a.k_tiles) + (int64_t)p.kt * 128 + 4 * (lane & 31);
   uint32_t bytes = 0;  // of the block's scales, row by row
