@@ -85,6 +85,11 @@ constexpr TileCost kFewBits[] = {{256, 8, 1, 8.8, 0.05, 0.82, 1.74, 0.33, 0},
                                  {64, 8, 1, 5.0, 0.07, 1.77, 1.73, 0.22, 0},
                                  {32, 8, 1, 4.8, 0.53, 1.01, 1.05, 0.20, 0}};
 
+// Weights that one row block reads are loaded past the caches where all groups' are more than the last-level cache holds, so that the
+// next call finds none of them: 256 rows over 8 groups of 14336 x 4096 165 -> 150 us (6.3 TB/s), 16 over 32 of 2048 x 2048 32.3 ->
+// 30.3. Smaller ones may be there still: 14336 x 4096 in 4 bits, 16 rows, call after call 8.6 us, past the caches 9.5.
+constexpr double kLastLevelCache = 256e6;
+
 double busy_groups(int E, int T) { return E > 1 ? E * -std::expm1(-(double)T / E) : 1.0; }
 double tiles_across(int tile, int n) { return (double)(((long long)n + std::max(tile, 64) - 1) / std::max(tile, 64)); }
 
@@ -143,6 +148,7 @@ int plan_grouped(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
   a.tiles_n = (d.N + tile - 1) / tile;
   a.k_tiles = (d.K + 63) / 64;
   a.has_bias = d.has_bias ? 1 : 0;
+  a.b_once = 2.0 * d.E * d.N * d.K > kLastLevelCache ? 1 : 0;
   long long grid;
   if ((s = check_tiles(d.E, d.T, tile, a.tiles_n, &grid)) != MTK_OK) return s;
   grid = tile_grid(tile, cus, grid);
@@ -290,6 +296,7 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
   a.k_tiles = k_tiles;
   a.ldc = d.ldc;
   a.has_bias = d.has_bias ? 1 : 0;
+  a.b_once = 136.0 * k_tiles * groups * d.N > kLastLevelCache ? 1 : 0;
   const int cus = ctx ? ctx->prop.multiProcessorCount : 256;
   const double busy = busy_groups((int)groups, d.T);
   TileCost kind = choose_tile(kFewBits, true, cus, k_tiles, 1e-6 * (0.53 * (busy * d.N * d.K + (double)d.T * d.K) + 2.0 * d.T * d.N), [&](int t) {

@@ -204,6 +204,7 @@ typedef struct {
   uint32_t b_exact; /* bytes of the weights of a group */
   int32_t tiles_m, tiles_n, k_tiles;
   int32_t has_bias;
+  int32_t b_once; /* weights that one row block reads are loaded past the caches */
 } mtk_grouped_kargs;
 
 /* Rows into blocks of 32 four-bit values with one scale, and back (mx.h has the layout). */
@@ -226,6 +227,7 @@ typedef struct {
   int64_t lda;
   int32_t E, T, N, K, k_tiles;
   int32_t ldc, tiles_n, has_bias;
+  int32_t b_once; /* weights that one row block reads are loaded past the caches */
 } mtk_mx_gemm_kargs;
 
 #endif

@@ -33,6 +33,7 @@ __device__ __forceinline__ void mx_few(const mtk_mx_gemm_kargs &g) {
   const TileAt at = tile_at<ROWS, 64>(gt.t, gt.blocks, g.tiles_n);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rows = min(gt.rows - at.m0, ROWS), cols = min(g.N - at.n0, 64);
+  const bool b_once = !QUANT && g.b_once && gt.blocks == 1;
   const int64_t first = gt.first + at.m0;
   const MxOperand A(QUANT ? nullptr : g.A, QUANT ? nullptr : g.a_scales, first, QUANT ? 0 : rows, g.T, g.k_tiles);
   const MxOperand B(g.B, g.b_scales, (int64_t)gt.e * g.N + at.n0, cols, (int64_t)g.E * g.N, g.k_tiles);
@@ -49,7 +50,10 @@ __device__ __forceinline__ void mx_few(const mtk_mx_gemm_kargs &g) {
   uint32_t na[MB], nb[2];
   auto load = [&](int kt) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) vb[i] = buf_load16(B.codes, lane_b + (uint32_t)i * 8u * B.row_b + (uint32_t)kt * 128u);
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t off = lane_b + (uint32_t)i * 8u * B.row_b + (uint32_t)kt * 128u;
+      vb[i] = b_once ? __builtin_amdgcn_raw_buffer_load_b128(B.codes, off, 0, 2) : buf_load16(B.codes, off);
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) nb[i] = buf_load4(B.scales, lane_s + 256u * (uint32_t)i + (uint32_t)kt * B.tile_s);
     if constexpr (QUANT) {

@@ -34,15 +34,17 @@ struct QuarterOp {
     step_i = 16u * (uint32_t)ld;
     step_k = KMAJOR ? 128u * (uint32_t)ld : 128u;
   }
+  // (POLICY 2: past the caches, for an operand that is read once)
+  template <int POLICY = 0>
   __device__ __forceinline__ void load(rsrc_t r, int kt, int, u32x4 (&v)[kLoads], uint32_t (&e)[kLoads]) const {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const uint32_t off = lane_off + ((uint32_t)i * step_i + (uint32_t)kt * step_k);
       if constexpr (ANY) {
-        v[i] = buf_load16(r, off & ~3u);
+        v[i] = __builtin_amdgcn_raw_buffer_load_b128(r, off & ~3u, 0, POLICY);
         e[i] = buf_load4(r, (off & ~3u) + 16u);
       } else {
-        v[i] = buf_load16(r, off);
+        v[i] = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, POLICY);
       }
     }
   }
@@ -187,14 +189,28 @@ __device__ __forceinline__ void quarter_tile(const mtk_tile_args &a, AOp oa, con
   int kt = kt0 + wave;
   if (kt < kt1) {
     oa.load(ra, kt, lane, sa, ea);
-    ob.load(rb, kt, lane, sb, eb);
+    if constexpr (PLACED) {
+      if (at.b_once)
+        ob.template load<2>(rb, kt, lane, sb, eb);
+      else
+        ob.load(rb, kt, lane, sb, eb);
+    } else {
+      ob.load(rb, kt, lane, sb, eb);
+    }
   }
   for (; kt < kt1; kt += W) {
     oa.store(la, lane, kt, a.K - kt * kBK, sa, ea);
     ob.store(lb, lane, kt, a.K - kt * kBK, sb, eb);
     if (kt + W < kt1) {
       oa.load(ra, kt + W, lane, sa, ea);
-      ob.load(rb, kt + W, lane, sb, eb);
+      if constexpr (PLACED) {
+        if (at.b_once)
+          ob.template load<2>(rb, kt + W, lane, sb, eb);
+        else
+          ob.load(rb, kt + W, lane, sb, eb);
+      } else {
+        ob.load(rb, kt + W, lane, sb, eb);
+      }
     }
     // this wavefront's own region: LDS accesses of a wavefront complete in order, the compiler has to
     // keep the reads of other lanes' chunks behind the writes
