@@ -45,7 +45,7 @@ int check_grouped(const mtk_grouped_desc &d) {
 // passes 32 bits whatever row_start holds.
 int check_tiles(int E, int T, int block, long long tiles_n, long long *grid) {
   *grid = group_max_blocks(E, T, block) * tiles_n;
-  if ((long long)E * ((T + block - 1) / block) * tiles_n > INT32_MAX || *grid > INT32_MAX / 512)
+  if ((long long)E * (((long long)T + block - 1) / block) * tiles_n > INT32_MAX || *grid > INT32_MAX / 512)
     return fail(MTK_ERR_UNSUPPORTED, "%d groups of up to %d rows with this N are not supported", E, T);
   return MTK_OK;
 }
@@ -162,8 +162,8 @@ int plan_grouped(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
   p->flops = 2.0 * d.T * d.N * d.K;
   p->bytes = 2.0 * ((double)d.T * (d.N + d.K) + (double)std::min(d.E, d.T) * d.N * d.K);
   char desc[256];
-  snprintf(desc, sizeof desc, "grouped gemm %s E=%d T=%d N=%d K=%d b=%s bias=%d tile=%d grid=%lld kernel=%s", dtype_name(d.dtype), d.E, d.T,
-           d.N, d.K, d.trans_b ? "nk" : "kn", a.has_bias, tile, grid, name.c_str());
+  snprintf(desc, sizeof desc, "grouped gemm %s E=%d T=%d N=%d K=%d b=%s bias=%d tile=%d grid=%lld", dtype_name(d.dtype), d.E, d.T,
+           d.N, d.K, d.trans_b ? "nk" : "kn", a.has_bias, tile, grid);
   p->description = desc;
   return finish_plan(p, out);
 }
@@ -220,8 +220,8 @@ int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out
   p->flops = 2.0 * d.T * d.N * d.K;
   p->bytes = 2.0 * d.T * (d.N + d.K) + (d.out_f32 ? 4.0 : 2.0) * d.E * d.N * d.K;
   char desc[256];
-  snprintf(desc, sizeof desc, "grouped gradient %s E=%d T=%d N=%d K=%d b=%s bias=%d out=%s tile=%d grid=%lld kernel=%s", dtype_name(d.dtype),
-           d.E, d.T, d.N, d.K, d.trans_b ? "nk" : "kn", d.has_bias ? 1 : 0, d.out_f32 ? "f32" : "16", tile, grid, name.c_str());
+  snprintf(desc, sizeof desc, "grouped gradient %s E=%d T=%d N=%d K=%d b=%s bias=%d out=%s tile=%d grid=%lld", dtype_name(d.dtype),
+           d.E, d.T, d.N, d.K, d.trans_b ? "nk" : "kn", d.has_bias ? 1 : 0, d.out_f32 ? "f32" : "16", tile, grid);
   p->description = desc;
   return finish_plan(p, out);
 }
@@ -331,8 +331,8 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
   p->bytes = 136.0 * k_tiles * ((d.quantize_a ? 0.0 : d.T) + (double)std::min<long long>(groups, d.T) * d.N) + 2.0 * d.T * d.N +
              (d.quantize_a ? 2.0 * d.T * d.K : 0.0);
   char desc[256];
-  snprintf(desc, sizeof desc, "mx gemm %s E=%d T=%d N=%d K=%d bias=%d quantize_a=%d tile=%d grid=%lld kernel=%s", dtype_name(d.dtype), d.E, d.T,
-           d.N, d.K, a.has_bias, d.quantize_a ? 1 : 0, tile, grid, name.c_str());
+  snprintf(desc, sizeof desc, "mx gemm %s E=%d T=%d N=%d K=%d bias=%d quantize_a=%d tile=%d grid=%lld", dtype_name(d.dtype), d.E, d.T,
+           d.N, d.K, a.has_bias, d.quantize_a ? 1 : 0, tile, grid);
   p->description = desc;
   return finish_plan(p, out);
 }

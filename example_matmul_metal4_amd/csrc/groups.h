@@ -31,4 +31,13 @@ MTK_GROUP_FN group_rows group_of(int start, int next, int T) {
 // full.
 MTK_GROUP_FN int64_t group_max_blocks(int E, int T, int block) { return (int64_t)T / block + (E < T ? E : T); }
 
+// Where the i-th tile of workgroup `block` of a grid of `grid` is among all `total`, or -1: the XCDs have contiguous runs of them (a
+// workgroup is on XCD block % 8), through which the workgroups of each go in step.
+MTK_GROUP_FN int group_nth_tile(int block, int grid, int i, int total) {
+  const int x = block & 7, each = (grid - x + 7) >> 3;
+  const int q = total >> 3, r = total & 7;
+  const int at = (block >> 3) + i * each;
+  return at < q + (x < r ? 1 : 0) ? (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + at : -1;
+}
+
 #endif

@@ -15,12 +15,6 @@ __device__ __forceinline__ f32x16 mfma_mx32(u32x4 a, u32x4 b, f32x16 c, uint32_t
   const i32x8 x = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}, y = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, c, 4, 4, SEL, (int)sa, SEL, (int)sb);
 }
-// 16x16x128: row lane % 16, one of four blocks lane / 16.
-template <int SEL>
-__device__ __forceinline__ f32x4 mfma_mx16(u32x4 a, u32x4 b, f32x4 c, uint32_t sa, uint32_t sb) {
-  const i32x8 x = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0}, y = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, SEL, (int)sa, SEL, (int)sb);
-}
 
 // ds_read_b32 as inline asm, for code with direct-to-LDS loads in flight (device.hpp): the caller waits for it.
 template <int OFF>
