@@ -104,7 +104,17 @@ struct Mx {
 
 // ---------------------------------------------------------------- a workgroup's tiles
 
-__device__ __forceinline__ int nth_tile(int i, int total) { return group_nth_tile((int)blockIdx.x, (int)gridDim.x, i, total); }
+// Tiles of 256 rows are halved in the last round, as their wavefronts of the lower half share the SIMDs with those of the upper one;
+// of 128, each SIMD has one wavefront of a tile, and half of them would have nothing to do.
+template <int BM>
+__device__ __forceinline__ group_place nth_tile(int i, int total) {
+  return group_nth_tile((int)blockIdx.x, (int)gridDim.x, i, total, BM == 256);
+}
+// What a tile of BM rows of which `left` are left starts at and has, by halves.
+template <int BM>
+__device__ __forceinline__ int half_first(int half) { return half == 2 ? BM / 2 : 0; }
+template <int BM>
+__device__ __forceinline__ int half_rows(int half, int left) { return min(left, half ? BM / 2 : BM); }
 
 struct ExpertTile {
   const char *a, *b;         // its first row (column) of the operands
@@ -129,9 +139,11 @@ struct GroupSearch {
     for (int e0 = 64; e0 < E; e0 += 64) total += GroupWindow(row_start, E, T, BM, e0).blocks();
     total *= tiles_n;
   }
-  __device__ __forceinline__ GroupTile get(int i) const {
+  __device__ __forceinline__ GroupTile get(int i, int &half) const {
     GroupTile r;
-    int id = nth_tile(i, total);
+    const group_place place = nth_tile<BM>(i, total);
+    int id = place.tile;
+    half = place.half;
     if (id < 0) return r;
     GroupWindow v = w;
 #pragma unroll 1
@@ -169,12 +181,14 @@ struct ForwardTiles {
   __device__ __forceinline__ bool streamed() const { return false; }
   __device__ __forceinline__ ExpertTile get(int i) const {
     ExpertTile t{};
-    const GroupTile gt = search.get(i);
-    t.there = gt.e >= 0;
-    if (!t.there) return t;
+    int half;
+    const GroupTile gt = search.get(i, half);
+    if (gt.e < 0) return t;
     const TileAt at = tile_at<BM, BN>(gt.t, gt.blocks, g.tiles_n);
-    const int row = gt.first + at.m0;
-    t.rows = min(gt.rows - at.m0, BM);
+    const int m0 = at.m0 + half_first<BM>(half), row = gt.first + m0;
+    t.rows = half_rows<BM>(half, gt.rows - m0);
+    t.there = t.rows > 0;
+    if (!t.there) return t;
     t.cols = min(g.N - at.n0, BN);
     t.K = g.K;
     t.k_tiles = g.k_tiles;
@@ -206,14 +220,17 @@ struct GradTiles {
   __device__ __forceinline__ bool streamed() const { return true; }  // gradients: nothing reads them soon
   __device__ __forceinline__ ExpertTile get(int i) const {
     ExpertTile t{};
-    const int tiles = g.tiles_m * g.tiles_n, id = nth_tile(i, g.E * tiles);
-    t.there = id >= 0;
+    const int tiles = g.tiles_m * g.tiles_n;
+    const group_place place = nth_tile<BM>(i, g.E * tiles);
+    if (place.tile < 0) return t;
+    const int e = place.tile / tiles;
+    TileAt at = tile_at<BM, BN>(place.tile - e * tiles, g.tiles_m, g.tiles_n);
+    at.m0 += half_first<BM>(place.half);
+    t.rows = half_rows<BM>(place.half, g.M - at.m0);
+    t.there = t.rows > 0;
     if (!t.there) return t;
-    const int e = id / tiles;
-    const TileAt at = tile_at<BM, BN>(id - e * tiles, g.tiles_m, g.tiles_n);
     const int start = __builtin_amdgcn_readfirstlane(g.row_start[e]), next = __builtin_amdgcn_readfirstlane(g.row_start[e + 1]);
     const group_rows r = group_of(start, next, g.T);
-    t.rows = min(g.M - at.m0, BM);
     t.cols = min(g.N - at.n0, BN);
     t.K = r.rows;
     t.k_tiles = (r.rows + 63) / 64;
@@ -247,20 +264,25 @@ struct MxTiles {
   __device__ __forceinline__ ExpertTile get(int i) const {
     ExpertTile t{};
     GroupTile gt;
+    int half;
     if (g.row_start) {
-      gt = search.get(i);
+      gt = search.get(i, half);
     } else {
-      gt.t = nth_tile(i, search.total);
+      const group_place place = nth_tile<BM>(i, search.total);
+      half = place.half;
+      gt.t = place.tile;
       gt.e = gt.t < 0 ? -1 : 0;
       gt.first = 0;
       gt.rows = g.T;
       gt.blocks = (g.T + BM - 1) / BM;
     }
-    t.there = gt.e >= 0;
-    if (!t.there) return t;
+    if (gt.e < 0) return t;
     const TileAt at = tile_at<BM, BN>(gt.t, gt.blocks, g.tiles_n);
-    const int64_t row = gt.first + at.m0, col = (int64_t)gt.e * g.N + at.n0;
-    t.rows = min(gt.rows - at.m0, BM);
+    const int m0 = at.m0 + half_first<BM>(half);
+    const int64_t row = gt.first + m0, col = (int64_t)gt.e * g.N + at.n0;
+    t.rows = half_rows<BM>(half, gt.rows - m0);
+    t.there = t.rows > 0;
+    if (!t.there) return t;
     t.cols = min(g.N - at.n0, BN);
     t.k_tiles = g.k_tiles;
     t.a = (const char *)g.A + row * (int64_t)row_b;

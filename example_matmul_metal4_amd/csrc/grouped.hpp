@@ -125,7 +125,7 @@ __device__ __forceinline__ void grouped_quarter(const mtk_grouped_kargs &g) {
   if (gt.e < 0) return;
   const TileAt at = tile_at<64, 64>(gt.t, gt.blocks, g.tiles_n);
   const mtk_tile_args a = group_args<64, ANY>(g, gt.e, gt.first + at.m0, gt.rows - at.m0);
-  using A = QuarterOp<false, ANY>;
+  using A = std::conditional_t<ANY, QuarterAny<false>, QuarterOp<false, false>>;
   quarter_tile<DT, A, BN, ANY, W, true>(a, A{}, TileAt{0, at.n0, g.b_once && gt.blocks == 1});
 }
 
@@ -156,9 +156,11 @@ __device__ __forceinline__ mtk_tile_args grad_args(const mtk_grouped_kargs &g, i
 
 template <int DT, bool ANY, int W>
 __device__ __forceinline__ void grouped_grad_quarter(const mtk_grouped_kargs &g) {
-  const int tiles = g.tiles_m * g.tiles_n, id = xcd_remap(blockIdx.x, gridDim.x), e = id / tiles;
+  // an XCD has 16 neighbours of every 128 tiles: those of a large group are spread over all of them
+  const int tiles = g.tiles_m * g.tiles_n;
+  const int id = group_nth_tile((int)blockIdx.x & 127, 128, (int)blockIdx.x >> 7, (int)gridDim.x, 0).tile, e = id / tiles;
   const mtk_tile_args a = grad_args<ANY>(g, e);
-  using A = QuarterOp<true, ANY>;
+  using A = std::conditional_t<ANY, QuarterAny<true>, QuarterOp<true, false>>;
   quarter_tile<DT, A, true, ANY, W, true>(a, A{}, tile_at<64, 64>(id - e * tiles, g.tiles_m, g.tiles_n));
 }
 

@@ -31,13 +31,26 @@ MTK_GROUP_FN group_rows group_of(int start, int next, int T) {
 // full.
 MTK_GROUP_FN int64_t group_max_blocks(int E, int T, int block) { return (int64_t)T / block + (E < T ? E : T); }
 
-// Where the i-th tile of workgroup `block` of a grid of `grid` is among all `total`, or -1: the XCDs have contiguous runs of them (a
-// workgroup is on XCD block % 8), through which the workgroups of each go in step.
-MTK_GROUP_FN int group_nth_tile(int block, int grid, int i, int total) {
-  const int x = block & 7, each = (grid - x + 7) >> 3;
-  const int q = total >> 3, r = total & 7;
-  const int at = (block >> 3) + i * each;
-  return at < q + (x < r ? 1 : 0) ? (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + at : -1;
+// A workgroup's i-th tile among `total`: -1 none; half 0: all of it, 1 and 2: its upper and lower half.
+//
+// All workgroups of a persistent grid go through the tiles in step, `grid` of them at a time, so that tiles that take longer (a large
+// group's gradients) are everybody's; of each `grid` tiles an XCD has neighbours (a workgroup is on XCD block % 8). The last round's
+// tiles are spread over the XCDs, and where they are half of the grid or fewer two workgroups share each, if the tile can be halved.
+typedef struct {
+  int tile, half;
+} group_place;
+
+MTK_GROUP_FN group_place group_nth_tile(int block, int grid, int i, int total, int halves) {
+  group_place p = {-1, 0};
+  const int64_t done = (int64_t)i * grid, left = total - done;
+  const int two = halves && 2 * left <= grid;
+  const int n = left >= grid ? grid : left > 0 ? (int)left << two : 0;  // of this round
+  const int x = block & 7, j = block >> 3, q = n >> 3, r = n & 7;
+  if (j >= q + (x < r ? 1 : 0)) return p;
+  const int at = x * q + (x < r ? x : r) + j;
+  p.tile = (int)done + (two ? at >> 1 : at);
+  p.half = two ? 1 + (at & 1) : 0;
+  return p;
 }
 
 #endif

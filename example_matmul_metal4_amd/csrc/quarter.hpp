@@ -83,6 +83,49 @@ struct QuarterOp {
   }
 };
 
+// QuarterOp with rows at any 2-byte alignment, for operands of which every row has its own: the dword behind a lane's chunk is the
+// first of its neighbour's, and a row's last lane has it from one load more, of the dwords behind all 64 rows (lane 8 r + i: of row
+// 8 i + r). A dword more for every chunk, as above, doubles the loads: 1023 rows over 7 groups of 1001 x 1023 17.0 us.
+template <bool KMAJOR>
+struct QuarterAny {
+  static constexpr int kRows = 64, kLoads = 8;
+  uint32_t lane_off, lane_end, step_i, step_k;  // as above; lane_end: the chunk behind row 8 (lane % 8) + lane / 8
+
+  __device__ void init(int lane, int first, int ld, uint32_t mis) {
+    const int r = lane >> 3, c = lane & 7;
+    const uint32_t row0 = KMAJOR ? 0u : (uint32_t)first, col0 = KMAJOR ? (uint32_t)first : 0u;
+    lane_off = ((row0 + (uint32_t)r) * (uint32_t)ld + col0 + 8u * (uint32_t)c) * 2u + mis;
+    lane_end = ((row0 + (uint32_t)(8 * c + r)) * (uint32_t)ld + col0) * 2u + mis + 128u;
+    step_i = 16u * (uint32_t)ld;
+    step_k = KMAJOR ? 128u * (uint32_t)ld : 128u;
+  }
+  template <int POLICY = 0>
+  __device__ __forceinline__ void load(rsrc_t r, int kt, int, u32x4 (&v)[8], uint32_t (&e)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = __builtin_amdgcn_raw_buffer_load_b128(r, (lane_off + ((uint32_t)i * step_i + (uint32_t)kt * step_k)) & ~3u, 0, POLICY);
+    e[0] = buf_load4(r, (lane_end + (uint32_t)kt * step_k) & ~3u);
+  }
+  __device__ __forceinline__ void store(char *lds, int lane, int kt, int k, u32x4 (&v)[8], const uint32_t (&e)[8]) const {
+    const int r0 = lane >> 3, c = lane & 7;
+    static_for<0, 8>([&](auto i_c) {
+      constexpr int i = decltype(i_c)::value;
+      const u32x4 x = v[i];
+      const uint32_t beside = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x.x, 0x101, 0xf, 0xf, false);  // row_shl:1
+      const uint32_t behind = i == 7 ? e[0] : (uint32_t)__builtin_amdgcn_update_dpp(0, (int)e[0], i == 7 ? 0x111 : 0x110 + 7 - i, 0xf, 0xf, false);  // row_shr
+      const uint32_t sh = ((lane_off + ((uint32_t)i * step_i + (uint32_t)kt * step_k)) & 2u) << 3;
+      u32x4 w = u32x4{__builtin_amdgcn_alignbit(x.y, x.x, sh), __builtin_amdgcn_alignbit(x.z, x.y, sh),
+                      __builtin_amdgcn_alignbit(x.w, x.z, sh), __builtin_amdgcn_alignbit(c == 7 ? behind : beside, x.w, sh)};
+      const int r = 8 * i + r0;
+      if (k < kBK) w = keep_halves(w, KMAJOR ? (r < k ? 8 : 0) : k - 8 * c);
+      *(u32x4 *)(lds + (KMAJOR ? (uint32_t)(r * 128 + ((c ^ (4 * ((r >> 1) & 1))) << 4)) : lds_off(r, c))) = w;
+    });
+  }
+  __device__ __forceinline__ u32x4 frag(const char *lds, int lane, int b, int ks) const {
+    return QuarterOp<KMAJOR, false>{}.frag(lds, lane, b, ks);
+  }
+};
+
 // The activation of an implicit-GEMM convolution as the row operand: row m is output pixel (n, oz, oh,
 // ow), K element ((kd * KH + kh) * KW + kw) * C + c. With C a multiple of 8 a chunk of 8 lies in one
 // filter tap: every lane decodes its chunk's tap once per K-tile and adds it to its 8 rows' window
@@ -178,7 +221,7 @@ __device__ __forceinline__ void quarter_tile(const mtk_tile_args &a, AOp oa, con
   uint32_t mis_a = 0, mis_b = 0;
   const rsrc_t ra = ANY ? make_rsrc_any(a.A, a.a_bytes, mis_a) : make_rsrc(a.A, a.a_bytes);
   const rsrc_t rb = ANY ? make_rsrc_any(a.B, a.b_bytes, mis_b) : make_rsrc(a.B, a.b_bytes);
-  QuarterOp<BN, ANY> ob;
+  std::conditional_t<PLACED && ANY, QuarterAny<BN>, QuarterOp<BN, ANY>> ob;
   oa.init(lane, m0, a.lda, mis_a);
   ob.init(lane, n0, a.ldb, mis_b);
   char *la = smem + wave * kWaveB, *lb = la + AOp::kRows * 128;

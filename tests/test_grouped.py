@@ -164,21 +164,30 @@ static void groups() {
   }
 }
 
-// ---- every tile once, each by one workgroup, and every workgroup comes to an end
+// ---- every tile once, or its two halves once each, by one workgroup, and every workgroup comes to an end
 static void tiles() {
   for (int n = 0; n < 20000; ++n) {
-    const int total = upto(n % 3 ? 40 : 3000), grid = 1 + upto(n % 2 ? 600 : std::max(total, 1));
-    std::vector<int> times(total, 0);
+    const int total = upto(n % 3 ? 40 : 3000), grid = 1 + upto(n % 2 ? 600 : std::max(total, 1)), halves = upto(2);
+    std::vector<int> had(2 * total, 0);
+    int rounds = 0;
     for (int b = 0; b < grid; ++b)
       for (int i = 0;; ++i) {
-        const int t = group_nth_tile(b, grid, i, total);
-        if (t < 0) break;
-        CHECK(t < total, "tile %d of %d", t, total);
-        ++times[t];
+        const group_place p = group_nth_tile(b, grid, i, total, halves);
+        if (p.tile < 0) {
+          CHECK(group_nth_tile(b, grid, i + 1, total, halves).tile < 0, "none, and one behind it");
+          break;
+        }
+        CHECK(p.tile < total && p.half >= 0 && p.half <= 2 * halves, "tile %d of %d, half %d", p.tile, total, p.half);
+        if (p.half != 2) ++had[2 * p.tile];
+        if (p.half != 1) ++had[2 * p.tile + 1];
+        rounds = std::max(rounds, i + 1);
       }
-    // a grid has as many workgroups as are on the device at once, or as there are tiles: 8 at least where there are 8 tiles
-    for (int t = 0; t < total; ++t) CHECK(times[t] == 1 || (grid < 8 && grid < total && times[t] == 0), "tile %d of %d, grid %d: %d times", t, total, grid, times[t]);
-    CHECK(group_nth_tile(grid - 1, grid, INT32_MAX / 1024, total) == -1, " ");
+    for (int t = 0; t < 2 * total; ++t) CHECK(had[t] == 1, "half %d of %d, grid %d: %d times", t, 2 * total, grid, had[t]);
+    CHECK(rounds == (total + grid - 1) / grid, "%d rounds", rounds);
+  }
+  for (int b = 0; b < 256; ++b) {  // no count passes 32 bits
+    CHECK(group_nth_tile(b, 256, INT32_MAX / 256 - 1, INT32_MAX, 1).tile >= 0, " ");
+    CHECK(group_nth_tile(b, 256, INT32_MAX / 256 + 1, INT32_MAX, 1).tile == -1, " ");
   }
 }
 
