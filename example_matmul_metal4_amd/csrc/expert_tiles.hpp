@@ -123,6 +123,7 @@ struct ExpertTile {
   int rows, cols, K, k_tiles;
   char *c;                   // its first output
   const uint16_t *bias;      // of its first column, or null
+  int e, first, m, n;        // gradients: its group, the group's first row, and its block of rows and of columns
   bool there;
 };
 
@@ -169,6 +170,7 @@ struct GroupSearch {
 // C = A op(B_e) + bias_e
 template <int BM, int BN, bool KMAJOR>
 struct ForwardTiles {
+  static constexpr bool kWarm = false;
   const mtk_grouped_kargs &g;
   GroupSearch<BM> search;
   __device__ __forceinline__ explicit ForwardTiles(const mtk_grouped_kargs &g_) : g(g_), search(g_.row_start, g_.E, g_.T, g_.tiles_n) {}
@@ -209,8 +211,14 @@ struct ForwardTiles {
 };
 
 // Gradients of the weights: K runs over the group's rows, of which both operands hold K rows of M and of N columns.
+//
+// A round's workgroups have one group or few, with few K-tiles each, and write as much as they read: the first K-tiles of a new group
+// would come from HBM behind the last round's outputs. So the workgroups ask for the group's rows while they are busy with the one
+// before it (warm), each for its part of the columns that its tile has: rows i * tiles_n + n of A's, i * tiles_m + m of B's, a lane
+// for a line of 128 bytes. 8192 rows over 16 groups of 4096 x 4096, inputs not in the caches: 339 us without.
 template <int BM, int BN>
 struct GradTiles {
+  static constexpr bool kWarm = BM == 256;
   const mtk_grouped_kargs &g;
   __device__ __forceinline__ explicit GradTiles(const mtk_grouped_kargs &g_) : g(g_) {}
   __device__ __forceinline__ int lda() const { return g.lda; }
@@ -240,13 +248,29 @@ struct GradTiles {
     t.b_bytes = (uint32_t)(g.N - at.n0) * 2u;
     const size_t out = (size_t)e * (size_t)g.M * (size_t)g.N + (size_t)at.m0 * (size_t)g.N + (size_t)at.n0;
     t.c = g.C32 ? (char *)g.C32 + out * 4 : (char *)g.C + out * 2;
+    t.e = e;
+    t.first = r.first;
+    t.m = at.m0 / BM;
+    t.n = at.n0 / BN;
     return t;
+  }
+  // Where a wavefront asks (4 of them in A, 4 in B), and its lanes' offsets for tile t.
+  __device__ __forceinline__ rsrc_t warm(int wave) const {
+    const uint32_t ld = (uint32_t)(wave < 4 ? g.lda : g.ldb), width = (uint32_t)(wave < 4 ? g.M : g.N);
+    return make_rsrc(wave < 4 ? g.A : g.B, (((uint32_t)(g.T - 1) * ld + width) * 2u) & ~3u);
+  }
+  __device__ __forceinline__ uint32_t warm_off(const ExpertTile &t, int wave, int lane) const {
+    const bool a = wave < 4;
+    const int i = 16 * (wave & 3) + (lane >> 2), row = a ? i * g.tiles_n + t.n : i * g.tiles_m + t.m, col = 64 * (lane & 3);
+    if (row >= t.K || col >= (a ? t.rows : t.cols)) return kOOBAny;
+    return ((uint32_t)(t.first + row) * (uint32_t)(a ? g.lda : g.ldb) + (uint32_t)((a ? t.m * BM : t.n * BN) + col)) * 2u;
   }
 };
 
 // C = A B_e^T + bias_e, both in few bits; one group of all rows where there is no row_start.
 template <int BM, int BN>
 struct MxTiles {
+  static constexpr bool kWarm = false;
   const mtk_mx_gemm_kargs &g;
   GroupSearch<BM> search;
   uint32_t row_b;
@@ -314,7 +338,8 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
   constexpr int kScaleLoads = (BM + BN) / 128;  // of all wavefronts
   static_assert(!EL::kScales || (kScaleLoads <= NW && BM % 128 == 0 && BN % 128 == 0), "a wavefront has one load of scales at most");
   static_assert(WTN == 64 && TM % 2 == 0, "epilogue rows of 128 bytes, halves of a wavefront's rows");
-  constexpr int kSpare = EL::kScales ? 1024 : 0, kPark = 2 * kStage + kSpare;  // behind the stages: [wave][16 rows][128 bytes]
+  constexpr bool kWarm = TILES::kWarm;
+  constexpr int kSpare = EL::kScales || kWarm ? 1024 : 0, kPark = 2 * kStage + kSpare;  // behind the stages: [wave][16 rows][128 bytes]
   static_assert(kPark + NW * 2048 <= 160 * 1024, "LDS");
   __shared__ __attribute__((aligned(1024))) char smem[kPark + NW * 2048];
 
@@ -362,6 +387,12 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
       lds_direct16(r.s, smem + at_s + st * next_s, off_s);
   };
 
+  const rsrc_t rw = [&]() {
+    if constexpr (kWarm)
+      return tiles.warm(wave);
+    else
+      return make_rsrc(smem, 0u);
+  }();
   f32x16 acc[TM][TN];
   u32x4 fa[2][TM] = {}, fb[2][TN] = {};
   uint32_t sa[TM] = {}, sb[TN] = {}, na[TM] = {}, nb[TN] = {};  // this K-tile's scales, and the next one's
@@ -405,14 +436,14 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
   };
 
   // One K-tile of stage st, whose row blocks from NI on are not multiplied, and the loads of `next` into that stage.
-  auto ktile = [&](auto ni_c, int st, const Source &next) {
+  auto ktile = [&](auto ni_c, int st, const Source &next, uint32_t warm) {
     constexpr int NI = decltype(ni_c)::value;
     constexpr int kReads = (TM + TN + 1) / 2, kLoadsPer = (kLoads + TM - 1) / TM;
     static_for<0, 4>([&](auto k_c) {
       constexpr int ks = decltype(k_c)::value;
       if constexpr (ks > 0) frag_wait<0>(fa[ks & 1], fb[ks & 1]);
       if constexpr (ks == 3) {
-        vm_wait<0>();
+        vm_wait<kWarm ? 1 : 0>();  // the load behind the next K-tile's may be in flight
         __builtin_amdgcn_s_barrier();
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -432,6 +463,10 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
         __builtin_amdgcn_sched_barrier(0);
       });
     });
+    if constexpr (kWarm) {  // one load whether there is something to ask for or not, so that the count above holds
+      lds_direct16(rw, smem + 2 * kStage, warm);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     landed();  // nothing is in flight at the loop's back edge
   };
 
@@ -561,7 +596,9 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
     const Source s0 = source(cur, cur, 2, 0), s1 = source(cur, cur, 2, 1);
     static_for<0, kLoads>([&](auto q) { issue(q, s0, 0); });
     static_for<0, kLoads>([&](auto q) { issue(q, s1, 1); });
-    vm_wait<kLoads>();  // the first K-tile's
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (kWarm) lds_direct16(rw, smem + 2 * kStage, kOOBAny);
+    vm_wait<kLoads + (kWarm ? 1 : 0)>();  // the first K-tile's
     __builtin_amdgcn_s_barrier();
   }
   int st = 0;
@@ -569,6 +606,8 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
   for (int i = 0;; ++i) {
     const ExpertTile next = tiles.get(i + 1);
     const int n = max(cur.k_tiles, 2);
+    uint32_t warm = kOOBAny;
+    if constexpr (kWarm) warm = next.there && next.e != cur.e ? tiles.warm_off(next, wave, lane) : kOOBAny;
     clear();
     const int blocks = cur.cols > wave_n * WTN ? (cur.rows - wave_m * WTM + 31) >> 5 : 0;
     auto run = [&](auto ni_c) {
@@ -586,7 +625,7 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
 #pragma unroll 1
         for (; k < stop; ++k) {
           const Source s = source(cur, next, n, k + 2);
-          ktile(ni_c, st, s);
+          ktile(ni_c, st, s, k == n - 2 ? warm : kOOBAny);
           st ^= 1;
         }
       };
