@@ -57,33 +57,33 @@ long long tile_grid(int tile, int cus, long long tiles) {
 
 // Which kernel runs a product, by the time that it is expected to take, in us: `start` and the larger of
 //   rounds * (round + (step + full * part) * K-tiles of a wavefront)   and   bytes * byte (us per MB),
-// with 0.15 of the other. rounds: workgroups over those that are on the device at once, at least 1; part: that share, at most 1 (a full
-// device's K-tiles take longer). The groups' sizes lie on the device: of E groups, E (1 - exp(-T / E)) are taken to have rows, as if
-// each row chose one of E, and each to have half a block that is not full. Fitted to launches of 290 forward products, 170
-// gradients and 200 products in few bits, each by every kernel (random sizes, T to 16384, N and K 64 to 14336): the kernel chosen takes
-// 1.03, 1.03 and 1.01 times (geometric mean) the time of the fastest.
-// Examples, us (tiles of 256, of 128, of 64 with 8, 4, 1 wavefronts): 256 rows over 8 groups of 14336 x 4096: 199, 168, 175, 171, 168;
-// 8192 over 16 of 4096 x 4096: 316, 351, 634, 559, 535; 16 over 32 of 2048 x 2048: 40, 31, 23, 21, 31. Gradients: 4 over 7 of 7448 x
-// 7296: 226, 224, 1033, 580, 282; 1000 over 24 of 1023 x 520: -, -, 72, 51, 43.
+// with 0.15 of the other. rounds: workgroups over those that are on the device at once, between that and the next whole number, at
+// least 1; part: that share, at most 1 (a full device's K-tiles take longer). The groups' sizes lie on the device: of E groups,
+// E (1 - exp(-T / E)) are taken to have rows, as if each row chose one of E, and each to have half a block that is not full. Fitted
+// to launches of 400 forward products, 400 gradients and 350 products in few bits, each by every kernel (random sizes, T to 16384,
+// N and K 64 to 14336): the kernel chosen takes 1.02, 1.02 and 1.01 times (geometric mean) the time of the fastest.
+// Examples, us (tiles of 256, of 128, of 64 with 8, 4, 1 wavefronts): 256 rows over 8 groups of 14336 x 4096: 222, 207, 162, 156, 152;
+// 8192 over 16 of 4096 x 4096: 303, 345, 626, 563, 537; 16 over 32 of 2048 x 2048: 40, 31, 25, 22, 40. Gradients: 8192 over 16 of 4096
+// x 4096: 297, 357, 1294, 777, 601; 1000 over 24 of 1023 x 520 with the bias': -, -, 54, 35, 27.
 struct TileCost {
   int tile, waves, per_cu;  // rows and columns of a tile (32: 64 columns); wavefronts and workgroups per CU
   double start, round, step, full, byte;
   double any;  // odd leading dimensions: K-tiles take longer by this share; below 0: not for these
 };
-constexpr TileCost kForward[] = {{256, 8, 1, 4.4, 0.26, 0.75, 1.13, 0.24, -1},
-                                 {128, 4, 2, 4.4, 0.0, 0.47, 0.85, 0.18, -1},
-                                 {64, 8, 1, 2.3, 1.03, 1.29, 0.99, 0.18, 0.36},
-                                 {64, 4, 2, 2.3, 1.78, 0.80, 1.23, 0.16, 0.34},
-                                 {64, 1, 8, 0.0, 4.57, 0.71, 1.16, 0.16, 0.29}};
-constexpr TileCost kGradient[] = {{256, 8, 1, 7.5, 2.10, 0.93, 2.17, 0.23, -1},
-                                  {128, 4, 2, 5.7, 0.96, 0.48, 1.40, 0.22, -1},
-                                  {64, 8, 1, 3.5, 0.0, 1.70, 1.01, 0.48, 0.14},
-                                  {64, 4, 2, 4.4, 0.0, 0.82, 2.06, 0.35, 0.16},
-                                  {64, 1, 8, 4.6, 2.05, 0.84, 2.65, 0.23, 0.43}};
-constexpr TileCost kFewBits[] = {{256, 8, 1, 8.8, 0.05, 0.82, 1.74, 0.33, 0},
-                                 {128, 4, 2, 6.9, 0.81, 0.47, 1.28, 0.27, 0},
-                                 {64, 8, 1, 5.0, 0.07, 1.77, 1.73, 0.22, 0},
-                                 {32, 8, 1, 4.8, 0.53, 1.01, 1.05, 0.20, 0}};
+constexpr TileCost kForward[] = {{256, 8, 1, 4.9, 0.0, 0.75, 1.06, 0.24, -1},
+                                 {128, 4, 2, 1.1, 3.31, 0.51, 0.66, 0.17, -1},
+                                 {64, 8, 1, 1.7, 1.40, 1.35, 0.87, 0.17, 0.18},
+                                 {64, 4, 2, 1.7, 2.18, 0.83, 1.06, 0.17, 0.27},
+                                 {64, 1, 8, 0.0, 4.38, 0.77, 1.03, 0.17, 0.26}};
+constexpr TileCost kGradient[] = {{256, 8, 1, 5.3, 4.36, 1.13, 1.46, 0.22, -1},
+                                  {128, 4, 2, 3.9, 2.80, 0.62, 0.90, 0.21, -1},
+                                  {64, 8, 1, 3.2, 0.0, 1.96, 0.72, 0.36, 0.21},
+                                  {64, 4, 2, 3.8, 0.22, 1.22, 1.27, 0.34, 0.22},
+                                  {64, 1, 8, 3.1, 3.60, 0.92, 1.57, 0.23, 0.33}};
+constexpr TileCost kFewBits[] = {{256, 8, 1, 10.3, 0.43, 0.83, 1.50, 0.27, 0},
+                                 {128, 4, 2, 7.0, 1.69, 0.48, 0.91, 0.26, 0},
+                                 {64, 8, 1, 5.7, 0.29, 1.60, 1.34, 0.21, 0},
+                                 {32, 8, 1, 5.3, 0.49, 1.04, 0.82, 0.18, 0}};
 
 // Weights that one row block reads are loaded past the caches where all groups' are more than the last-level cache holds, so that the
 // next call finds none of them: 256 rows over 8 groups of 14336 x 4096 165 -> 150 us (6.3 TB/s), 16 over 32 of 2048 x 2048 32.3 ->
@@ -100,7 +100,7 @@ TileCost choose_tile(const TileCost (&costs)[N], bool even, int cus, double k_ti
   double least = 0;
   for (const TileCost &c : costs) {
     if (!even && c.any < 0) continue;
-    const double there = wgs(c.tile) / ((double)cus * c.per_cu), rounds = std::max(1.0, there);
+    const double there = wgs(c.tile) / ((double)cus * c.per_cu), rounds = std::max(1.0, 0.5 * (there + std::ceil(there)));
     const double steps = c.tile > 64 || c.waves == 1 ? k_tiles : std::ceil(k_tiles / c.waves);
     const double step = (c.step + c.full * std::min(1.0, there)) * (even ? 1.0 : 1.0 + c.any);
     const double x = rounds * (c.round + step * steps), y = mbytes * c.byte;
