@@ -214,8 +214,9 @@ struct ForwardTiles {
 //
 // A round's workgroups have one group or few, with few K-tiles each, and write as much as they read: the first K-tiles of a new group
 // would come from HBM behind the last round's outputs. So the workgroups ask for the group's rows while they are busy with the one
-// before it (warm), each for its part of the columns that its tile has: rows i * tiles_n + n of A's, i * tiles_m + m of B's, a lane
-// for a line of 128 bytes. 8192 rows over 16 groups of 4096 x 4096, inputs not in the caches: 339 us without.
+// before it (warm), two K-tiles before its end, each for its part of the columns that its tile has: rows i * tiles_n + n of A's,
+// i * tiles_m + m of B's, a lane for a line of 128 bytes. 8192 rows over 16 groups of 4096 x 4096: inputs in HBM 342 -> 315 us, in the
+// last-level cache 304 -> 302. (The forward products ask for K-tiles of their own weights in this way: 306 -> 330.)
 template <int BM, int BN>
 struct GradTiles {
   static constexpr bool kWarm = BM == 256;
@@ -387,12 +388,6 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
       lds_direct16(r.s, smem + at_s + st * next_s, off_s);
   };
 
-  const rsrc_t rw = [&]() {
-    if constexpr (kWarm)
-      return tiles.warm(wave);
-    else
-      return make_rsrc(smem, 0u);
-  }();
   f32x16 acc[TM][TN];
   u32x4 fa[2][TM] = {}, fb[2][TN] = {};
   uint32_t sa[TM] = {}, sb[TN] = {}, na[TM] = {}, nb[TN] = {};  // this K-tile's scales, and the next one's
@@ -436,14 +431,14 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
   };
 
   // One K-tile of stage st, whose row blocks from NI on are not multiplied, and the loads of `next` into that stage.
-  auto ktile = [&](auto ni_c, int st, const Source &next, uint32_t warm) {
+  auto ktile = [&](auto ni_c, int st, const Source &next) {
     constexpr int NI = decltype(ni_c)::value;
     constexpr int kReads = (TM + TN + 1) / 2, kLoadsPer = (kLoads + TM - 1) / TM;
     static_for<0, 4>([&](auto k_c) {
       constexpr int ks = decltype(k_c)::value;
       if constexpr (ks > 0) frag_wait<0>(fa[ks & 1], fb[ks & 1]);
       if constexpr (ks == 3) {
-        vm_wait<kWarm ? 1 : 0>();  // the load behind the next K-tile's may be in flight
+        vm_wait<0>();
         __builtin_amdgcn_s_barrier();
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -463,10 +458,6 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
         __builtin_amdgcn_sched_barrier(0);
       });
     });
-    if constexpr (kWarm) {  // one load whether there is something to ask for or not, so that the count above holds
-      lds_direct16(rw, smem + 2 * kStage, warm);
-      __builtin_amdgcn_sched_barrier(0);
-    }
     landed();  // nothing is in flight at the loop's back edge
   };
 
@@ -596,9 +587,7 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
     const Source s0 = source(cur, cur, 2, 0), s1 = source(cur, cur, 2, 1);
     static_for<0, kLoads>([&](auto q) { issue(q, s0, 0); });
     static_for<0, kLoads>([&](auto q) { issue(q, s1, 1); });
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (kWarm) lds_direct16(rw, smem + 2 * kStage, kOOBAny);
-    vm_wait<kLoads + (kWarm ? 1 : 0)>();  // the first K-tile's
+    vm_wait<kLoads>();  // the first K-tile's
     __builtin_amdgcn_s_barrier();
   }
   int st = 0;
@@ -606,8 +595,6 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
   for (int i = 0;; ++i) {
     const ExpertTile next = tiles.get(i + 1);
     const int n = max(cur.k_tiles, 2);
-    uint32_t warm = kOOBAny;
-    if constexpr (kWarm) warm = next.there && next.e != cur.e ? tiles.warm_off(next, wave, lane) : kOOBAny;
     clear();
     const int blocks = cur.cols > wave_n * WTN ? (cur.rows - wave_m * WTM + 31) >> 5 : 0;
     auto run = [&](auto ni_c) {
@@ -625,7 +612,7 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
 #pragma unroll 1
         for (; k < stop; ++k) {
           const Source s = source(cur, next, n, k + 2);
-          ktile(ni_c, st, s, k == n - 2 ? warm : kOOBAny);
+          ktile(ni_c, st, s);
           st ^= 1;
         }
       };
@@ -636,6 +623,13 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
           if (stop == n) break;
           cut(st, cur.K & 63);
           first();
+        }
+      } else if constexpr (kWarm) {
+#pragma unroll 1
+        for (int stop = next.there && next.e != cur.e ? n - 2 : n;; stop = n) {
+          upto(stop);
+          if (stop == n) break;
+          lds_direct16(tiles.warm(wave), smem + 2 * kStage, tiles.warm_off(next, wave, lane));
         }
       } else {
         upto(n);
