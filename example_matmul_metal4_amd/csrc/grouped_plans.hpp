@@ -2,6 +2,7 @@
 // choice and argument blocks. Part of runtime.cpp's translation unit, inside its unnamed namespace.
 
 constexpr int kMaxWidth = 1 << 22;  // N, K and leading dimensions: 256 rows of a tile, and 64 past an operand's end, stay in 32 bits
+constexpr int kMaxGroups = 1 << 14;  // a workgroup looks through all of them, 64 at a time
 
 bool is_grouped(const mtk_plan *p) { return p->kind >= PLAN_GROUPED && p->kind <= PLAN_MX_GEMM; }
 
@@ -12,14 +13,22 @@ int check_ld(int ld, int width, const char *name, int *out) {
   return MTK_OK;
 }
 
-int finish_plan(mtk_plan *p, mtk_plan **out) {
-  const int s = resolve(p);
-  if (s != MTK_OK) {
-    delete p;
-    return s;
+int finish_plan(std::unique_ptr<mtk_plan> p, mtk_plan **out) {
+  const int s = resolve(p.get());
+  if (s == MTK_OK) *out = p.release();
+  return s;
+}
+
+// No exception leaves a C entry point: making a plan allocates.
+template <typename F>
+int guarded(F f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc &) {
+    return fail(MTK_ERR_OOM, "out of memory");  // short enough for the error string to hold without allocating
+  } catch (...) {
+    return fail(MTK_ERR_INVALID, "unexpected exception");
   }
-  *out = p;
-  return MTK_OK;
 }
 
 template <typename T>
@@ -36,7 +45,7 @@ int check_grouped(const mtk_grouped_desc &d) {
   if (d.E <= 0 || d.T <= 0 || d.N <= 0 || d.K <= 0)
     return fail(MTK_ERR_INVALID, "E, T, N and K must be positive (got %d, %d, %d, %d)", d.E, d.T, d.N, d.K);
   if (d.N > kMaxWidth || d.K > kMaxWidth) return fail(MTK_ERR_UNSUPPORTED, "N and K above 2^22 are not supported (got %d, %d)", d.N, d.K);
-  if (d.E > (1 << 20)) return fail(MTK_ERR_UNSUPPORTED, "E above 2^20 is not supported (got %d)", d.E);
+  if (d.E > kMaxGroups) return fail(MTK_ERR_UNSUPPORTED, "E above 2^14 is not supported (got %d)", d.E);
   if (d.dtype != MTK_F16 && d.dtype != MTK_BF16) return fail(MTK_ERR_INVALID, "dtype must be MTK_F16 or MTK_BF16");
   return MTK_OK;
 }
@@ -152,20 +161,20 @@ int plan_grouped(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
   long long grid;
   if ((s = check_tiles(d.E, d.T, tile, a.tiles_n, &grid)) != MTK_OK) return s;
   grid = tile_grid(tile, cus, grid);
-  mtk_plan *p = new mtk_plan();
+  std::unique_ptr<mtk_plan> p(new mtk_plan());
   p->ctx = ctx;
   p->kind = PLAN_GROUPED;
   p->grouped = d;
   p->align_a = p->align_b = even ? 4 : 2;
   const std::string name = std::string("mtk_grouped_") + dtype_name(d.dtype) + (d.trans_b ? "_nt_" : "_nn_") + tile_name(kind, even);
-  add_launch(p, name, grid, 64 * kind.waves, a);
+  add_launch(p.get(), name, grid, 64 * kind.waves, a);
   p->flops = 2.0 * d.T * d.N * d.K;
   p->bytes = 2.0 * ((double)d.T * (d.N + d.K) + (double)std::min(d.E, d.T) * d.N * d.K);
   char desc[256];
   snprintf(desc, sizeof desc, "grouped gemm %s E=%d T=%d N=%d K=%d b=%s bias=%d tile=%d grid=%lld", dtype_name(d.dtype), d.E, d.T,
            d.N, d.K, d.trans_b ? "nk" : "kn", a.has_bias, tile, grid);
   p->description = desc;
-  return finish_plan(p, out);
+  return finish_plan(std::move(p), out);
 }
 
 int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
@@ -199,14 +208,14 @@ int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out
   if (grid > INT32_MAX / 512 || d.E * bias_tiles > INT32_MAX / 1024)
     return fail(MTK_ERR_UNSUPPORTED, "%d groups with these N and K are not supported", d.E);
   grid = tile_grid(tile, cus, grid);
-  mtk_plan *p = new mtk_plan();
+  std::unique_ptr<mtk_plan> p(new mtk_plan());
   p->ctx = ctx;
   p->kind = PLAN_GROUPED_GRAD;
   p->grouped = d;
   p->align_a = p->align_b = even ? 4 : 2;
   const std::string head = std::string("mtk_grouped_") + dtype_name(d.dtype);
   const std::string name = head + "_grad_" + tile_name(kind, even);
-  add_launch(p, name, grid, 64 * kind.waves, a);
+  add_launch(p.get(), name, grid, 64 * kind.waves, a);
   if (d.has_bias) {
     mtk_grouped_kargs b{};
     b.E = d.E;
@@ -214,7 +223,7 @@ int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out
     b.N = d.N;
     b.lda = d.ldc;
     b.tiles_n = (int)bias_tiles;
-    add_launch(p, head + "_bias_grad", d.E * bias_tiles, 1024, b);
+    add_launch(p.get(), head + "_bias_grad", d.E * bias_tiles, 1024, b);
     p->launches.back().role = ROLE_REDUCE;
   }
   p->flops = 2.0 * d.T * d.N * d.K;
@@ -223,7 +232,7 @@ int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out
   snprintf(desc, sizeof desc, "grouped gradient %s E=%d T=%d N=%d K=%d b=%s bias=%d out=%s tile=%d grid=%lld", dtype_name(d.dtype),
            d.E, d.T, d.N, d.K, d.trans_b ? "nk" : "kn", d.has_bias ? 1 : 0, d.out_f32 ? "f32" : "16", tile, grid);
   p->description = desc;
-  return finish_plan(p, out);
+  return finish_plan(std::move(p), out);
 }
 
 // ------------------------------------------------------------------ rows in few bits
@@ -258,7 +267,7 @@ int plan_mx_rows(mtk_ctx *ctx, const mtk_mx_rows_desc *d_in, bool quantize, mtk_
   if ((s = check_ld(d.ld, d.K, "ld", &d.ld)) != MTK_OK) return s;
   if (((long long)d.R + 15) / 16 * ((mx_k_tiles(d.K) + 1) / 2) > INT32_MAX / 256)
     return fail(MTK_ERR_UNSUPPORTED, "%d rows of %d are not supported", d.R, d.K);
-  mtk_plan *p = new mtk_plan();
+  std::unique_ptr<mtk_plan> p(new mtk_plan());
   p->ctx = ctx;
   p->kind = quantize ? PLAN_MX_QUANT : PLAN_MX_DEQUANT;
   p->mx_rows = d;
@@ -268,7 +277,7 @@ int plan_mx_rows(mtk_ctx *ctx, const mtk_mx_rows_desc *d_in, bool quantize, mtk_
   snprintf(desc, sizeof desc, "mx %s %s R=%d K=%d ld=%d grid=%u", quantize ? "quantize" : "dequantize", dtype_name(d.dtype), d.R, d.K, d.ld,
            p->launches[0].grid);
   p->description = desc;
-  return finish_plan(p, out);
+  return finish_plan(std::move(p), out);
 }
 
 int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
@@ -277,7 +286,7 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
   if (d.E < 0 || d.T <= 0 || d.N <= 0 || d.K <= 0)
     return fail(MTK_ERR_INVALID, "E must be 0 or more, T, N and K positive (got %d, %d, %d, %d)", d.E, d.T, d.N, d.K);
   if (d.N > kMaxWidth || d.K > kMaxWidth) return fail(MTK_ERR_UNSUPPORTED, "N and K above 2^22 are not supported (got %d, %d)", d.N, d.K);
-  if (d.E > (1 << 20)) return fail(MTK_ERR_UNSUPPORTED, "E above 2^20 is not supported (got %d)", d.E);
+  if (d.E > kMaxGroups) return fail(MTK_ERR_UNSUPPORTED, "E above 2^14 is not supported (got %d)", d.E);
   if (d.dtype != MTK_F16 && d.dtype != MTK_BF16) return fail(MTK_ERR_INVALID, "dtype must be MTK_F16 or MTK_BF16");
   if (!d.quantize_a && d.lda) return fail(MTK_ERR_INVALID, "lda is for 16-bit rows (quantize_a)");
   int s;
@@ -315,7 +324,7 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
   if ((s = check_tiles((int)groups, d.T, tile, a.tiles_n, &grid)) != MTK_OK) return s;
   if (!d.E) grid = (long long)((d.T + tile - 1) / tile) * a.tiles_n;
   grid = tile_grid(tile, cus, grid);
-  mtk_plan *p = new mtk_plan();
+  std::unique_ptr<mtk_plan> p(new mtk_plan());
   p->ctx = ctx;
   p->kind = PLAN_MX_GEMM;
   p->mx_gemm = d;
@@ -326,7 +335,7 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
     p->workspace = p->scales_at + mx_scale_bytes(d.T, k_tiles);
   }
   const std::string name = std::string("mtk_mx_gemm_") + dtype_name(d.dtype) + "_" + std::to_string(tile) + (inside ? "q" : "");
-  add_launch(p, name, grid, 64 * kind.waves, a);
+  add_launch(p.get(), name, grid, 64 * kind.waves, a);
   p->flops = 2.0 * d.T * d.N * d.K;
   p->bytes = 136.0 * k_tiles * ((d.quantize_a ? 0.0 : d.T) + (double)std::min<long long>(groups, d.T) * d.N) + 2.0 * d.T * d.N +
              (d.quantize_a ? 2.0 * d.T * d.K : 0.0);
@@ -334,7 +343,7 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
   snprintf(desc, sizeof desc, "mx gemm %s E=%d T=%d N=%d K=%d bias=%d quantize_a=%d tile=%d grid=%lld", dtype_name(d.dtype), d.E, d.T,
            d.N, d.K, a.has_bias, d.quantize_a ? 1 : 0, tile, grid);
   p->description = desc;
-  return finish_plan(p, out);
+  return finish_plan(std::move(p), out);
 }
 
 // ------------------------------------------------------------------ run-time arguments

@@ -21,7 +21,9 @@
 #include <cstdlib>
 #include <cstring>
 #include <map>
+#include <memory>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -1843,9 +1845,13 @@ int mtk_kv_write_run(const mtk_plan *plan, const mtk_kv_write_args *args) { retu
 int mtk_kv_read_run(const mtk_plan *plan, const mtk_kv_read_args *args) { return run_kv(plan, PLAN_KV_READ, args); }
 int mtk_kv_attn_run(const mtk_plan *plan, const mtk_kv_attn_args *args) { return run_kv(plan, PLAN_KV_ATTN, args); }
 
-int mtk_grouped_gemm_plan(mtk_ctx *ctx, const mtk_grouped_desc *desc, mtk_plan **out) { return plan_grouped(ctx, desc, out); }
+int mtk_grouped_gemm_plan(mtk_ctx *ctx, const mtk_grouped_desc *desc, mtk_plan **out) {
+  return guarded([&] { return plan_grouped(ctx, desc, out); });
+}
 int mtk_grouped_gemm_run(const mtk_plan *plan, const mtk_grouped_gemm_args *args) { return run_grouped(plan, PLAN_GROUPED, args); }
-int mtk_grouped_grad_plan(mtk_ctx *ctx, const mtk_grouped_desc *desc, mtk_plan **out) { return plan_grouped_grad(ctx, desc, out); }
+int mtk_grouped_grad_plan(mtk_ctx *ctx, const mtk_grouped_desc *desc, mtk_plan **out) {
+  return guarded([&] { return plan_grouped_grad(ctx, desc, out); });
+}
 int mtk_grouped_grad_run(const mtk_plan *plan, const mtk_grouped_grad_args *args) { return run_grouped(plan, PLAN_GROUPED_GRAD, args); }
 
 int mtk_mx_bytes(int R, int K, size_t *code_bytes, size_t *scale_bytes) {
@@ -1856,11 +1862,17 @@ int mtk_mx_bytes(int R, int K, size_t *code_bytes, size_t *scale_bytes) {
   *scale_bytes = mx_scale_bytes(R, mx_k_tiles(K));
   return MTK_OK;
 }
-int mtk_mx_quantize_plan(mtk_ctx *ctx, const mtk_mx_rows_desc *desc, mtk_plan **out) { return plan_mx_rows(ctx, desc, true, out); }
+int mtk_mx_quantize_plan(mtk_ctx *ctx, const mtk_mx_rows_desc *desc, mtk_plan **out) {
+  return guarded([&] { return plan_mx_rows(ctx, desc, true, out); });
+}
 int mtk_mx_quantize_run(const mtk_plan *plan, const mtk_mx_quantize_args *args) { return run_grouped(plan, PLAN_MX_QUANT, args); }
-int mtk_mx_dequantize_plan(mtk_ctx *ctx, const mtk_mx_rows_desc *desc, mtk_plan **out) { return plan_mx_rows(ctx, desc, false, out); }
+int mtk_mx_dequantize_plan(mtk_ctx *ctx, const mtk_mx_rows_desc *desc, mtk_plan **out) {
+  return guarded([&] { return plan_mx_rows(ctx, desc, false, out); });
+}
 int mtk_mx_dequantize_run(const mtk_plan *plan, const mtk_mx_dequantize_args *args) { return run_grouped(plan, PLAN_MX_DEQUANT, args); }
-int mtk_mx_gemm_plan(mtk_ctx *ctx, const mtk_mx_gemm_desc *desc, mtk_plan **out) { return plan_mx_gemm(ctx, desc, out); }
+int mtk_mx_gemm_plan(mtk_ctx *ctx, const mtk_mx_gemm_desc *desc, mtk_plan **out) {
+  return guarded([&] { return plan_mx_gemm(ctx, desc, out); });
+}
 int mtk_mx_gemm_run(const mtk_plan *plan, const mtk_mx_gemm_args *args) { return run_grouped(plan, PLAN_MX_GEMM, args); }
 
 size_t mtk_plan_workspace_bytes(const mtk_plan *plan) { return plan ? plan->workspace : 0; }

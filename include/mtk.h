@@ -424,8 +424,9 @@ int mtk_kv_attn_run(const mtk_plan *plan, const mtk_kv_attn_args *args);
  * inverted, over the same weights.
  *
  * Operands may be of any size but: 2 GiB for the weights of one group (forward), 2 GiB for A and dC (gradients of the weights),
- * leading dimensions, N and K up to 2^22. Even leading dimensions run the GEMM's kernels (A, B 4-byte aligned), odd ones
- * slower kernels that take rows at any 2-byte alignment. */
+ * E up to 2^14, leading dimensions, N and K up to 2^22. Where the leading dimensions of the two operands that are read are even,
+ * these are 4-byte aligned; with an odd one they may have any 2-byte alignment, and small tiles run, more slowly. C and the bias
+ * are 2-byte aligned. */
 typedef struct {
   int E, T, N, K;
   int lda, ldb, ldc; /* elements between rows; 0 = packed */
@@ -498,7 +499,7 @@ int mtk_mx_dequantize_run(const mtk_plan *plan, const mtk_mx_dequantize_args *ar
  * their sums fp32; C is in 16 bits, rounded once.
  * quantize_a: A are 16-bit rows [T][lda] that the run brings into the format first (in the workspace, or on chip), with the
  * result of mtk_mx_quantize; else codes and scales of T rows.
- * T x K and E x N x K up to 2^36, K, N and leading dimensions up to 2^22. */
+ * T x K and E x N x K up to 2^36, E up to 2^14, K, N and leading dimensions up to 2^22. */
 typedef struct {
   int E, T, N, K;
   int lda, ldc; /* 0 = packed; lda: with quantize_a only */

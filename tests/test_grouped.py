@@ -49,24 +49,24 @@ def few_bits(**kw):
 @pytest.mark.parametrize("make, kw, status", [
     *[(m, {n: v}, INVALID) for m in (product, gradient) for n in "ETNK" for v in (0, -1, -MOST - 1)],
     *[(m, {n: (1 << 22) + 1}, UNSUPPORTED) for m in (product, gradient) for n in "NK"],
-    *[(m, dict(E=(1 << 20) + 1), UNSUPPORTED) for m in (product, gradient)],
+    *[(m, dict(E=(1 << 14) + 1), UNSUPPORTED) for m in (product, gradient)],
     *[(m, {n: v}, INVALID) for m in (product, gradient) for n in ("lda", "ldc") for v in (63, -96)],
     *[(m, {n: (1 << 22) + 1}, UNSUPPORTED) for m in (product, gradient) for n in ("lda", "ldc")],
     (product, dict(ldb=95), INVALID), (product, dict(ldb=63, trans_b=False), INVALID), (product, dict(ldb=-1), INVALID),
     (product, dict(N=1 << 20, K=1 << 10), UNSUPPORTED), (product, dict(N=1 << 10, K=1 << 20, trans_b=False), UNSUPPORTED),  # 2 GiB a group
-    (product, dict(T=MOST), UNSUPPORTED), (product, dict(T=MOST, E=1, N=1, K=1), UNSUPPORTED), (product, dict(E=1 << 20, T=MOST, N=1 << 20, K=1), UNSUPPORTED),
+    (product, dict(T=MOST), UNSUPPORTED), (product, dict(T=MOST, E=1, N=1, K=1), UNSUPPORTED), (product, dict(E=1 << 14, T=MOST, N=1 << 20, K=1), UNSUPPORTED),
     (gradient, dict(T=MOST), UNSUPPORTED), (gradient, dict(T=1 << 24, lda=128), UNSUPPORTED), (gradient, dict(T=1 << 24, ldc=128), UNSUPPORTED),
-    (gradient, dict(E=1 << 20, T=1, N=1 << 20, K=1 << 20), UNSUPPORTED),
+    (gradient, dict(E=1 << 14, T=1, N=1 << 20, K=1 << 20), UNSUPPORTED),
     *[(m, {n: v}, INVALID) for m in (quantise, dequantise) for n in "RK" for v in (0, -1)],
     *[(m, dict(K=(1 << 22) + 1), UNSUPPORTED) for m in (quantise, dequantise)],
     *[(m, dict(ld=v), INVALID) for m in (quantise, dequantise) for v in (95, -96)],
     *[(m, dict(ld=(1 << 22) + 1), UNSUPPORTED) for m in (quantise, dequantise)],
     *[(m, dict(R=MOST), UNSUPPORTED) for m in (quantise, dequantise)],
     *[(few_bits, {n: v}, INVALID) for n in "TNK" for v in (0, -1)], (few_bits, dict(E=-1), INVALID),
-    (few_bits, dict(E=(1 << 20) + 1), UNSUPPORTED), (few_bits, dict(N=(1 << 22) + 1), UNSUPPORTED), (few_bits, dict(K=(1 << 22) + 1), UNSUPPORTED),
+    (few_bits, dict(E=(1 << 14) + 1), UNSUPPORTED), (few_bits, dict(N=(1 << 22) + 1), UNSUPPORTED), (few_bits, dict(K=(1 << 22) + 1), UNSUPPORTED),
     (few_bits, dict(lda=96), INVALID), (few_bits, dict(lda=95, quantize_a=True), INVALID), (few_bits, dict(ldc=63), INVALID),
     (few_bits, dict(ldc=(1 << 22) + 1), UNSUPPORTED), (few_bits, dict(T=MOST), UNSUPPORTED), (few_bits, dict(T=1 << 20, K=1 << 17), UNSUPPORTED),
-    (few_bits, dict(E=1 << 20, N=1 << 20), UNSUPPORTED), (few_bits, dict(N=1 << 22, K=1 << 22), UNSUPPORTED),
+    (few_bits, dict(E=1 << 14, N=1 << 20), UNSUPPORTED), (few_bits, dict(N=1 << 22, K=1 << 22), UNSUPPORTED),
 ], ids=lambda x: getattr(x, "__name__", str(x)))
 def test_plans_refuse(make, kw, status):
     with pytest.raises(mtk.MtkError) as e:
@@ -133,8 +133,19 @@ def test_workspaces():
 
 DRIVER = r"""
 #include "runtime.cpp"
+#include <new>
 #include <random>
 #include <set>
+
+static int allocations = -1;  // that succeed before one fails; below 0: all
+void *operator new(size_t n) {
+  if (allocations == 0) throw std::bad_alloc();
+  if (allocations > 0) --allocations;
+  if (void *p = malloc(n ? n : 1)) return p;
+  throw std::bad_alloc();
+}
+void operator delete(void *p) noexcept { free(p); }
+void operator delete(void *p, size_t) noexcept { free(p); }
 
 static int failures = 0;
 #define CHECK(x, ...) do { if (!(x)) { printf("failed: %s: ", #x); printf(__VA_ARGS__); printf("\n"); if (++failures > 20) exit(1); } } while (0)
@@ -328,7 +339,7 @@ static void plans() {
   int made = 0;
   for (int n = 0; n < 60000; ++n) {
     const bool large = n % 4 == 0;
-    const int E = large ? about(1 << 20) : about(200), T = large ? about(INT32_MAX - 8) : about(20000), N = about(large ? 1 << 22 : 16384), K = about(large ? 1 << 22 : 16384);
+    const int E = large ? about(1 << 14) : about(200), T = large ? about(INT32_MAX - 8) : about(20000), N = about(large ? 1 << 22 : 16384), K = about(large ? 1 << 22 : 16384);
     const int pad = n % 3 ? 0 : 1 + upto(9);
     mtk_plan *p = nullptr;
     mtk_grouped_desc d{};
@@ -353,8 +364,37 @@ static void plans() {
   CHECK(made > 100000, "%d plans", made);
 }
 
+// ---- every allocation of a plan's making fails once: an error, and no exception past the C entry
+static void no_memory() {
+  mtk_grouped_desc d{};
+  d.E = 3, d.T = 50, d.N = 64, d.K = 96, d.has_bias = 1;
+  mtk_mx_rows_desc r{50, 96, 0, MTK_F16};
+  mtk_mx_gemm_desc m{};
+  m.T = 5000, m.N = 640, m.K = 300, m.quantize_a = 1;
+  for (int which = 0; which < 5; ++which) {
+    int refused = 0;
+    for (int n = 0;; ++n) {
+      mtk_plan *p = nullptr;
+      allocations = n;
+      const int s = which == 0   ? mtk_grouped_gemm_plan(nullptr, &d, &p)
+                    : which == 1 ? mtk_grouped_grad_plan(nullptr, &d, &p)
+                    : which == 2 ? mtk_mx_quantize_plan(nullptr, &r, &p)
+                    : which == 3 ? mtk_mx_dequantize_plan(nullptr, &r, &p)
+                                 : mtk_mx_gemm_plan(nullptr, &m, &p);
+      allocations = -1;
+      if (s == MTK_OK) {
+        mtk_plan_destroy(p);
+        break;
+      }
+      CHECK(s == MTK_ERR_OOM && !p && strstr(mtk_last_error(), "memory"), "%d %d: %d", which, n, s);
+      ++refused;
+    }
+    CHECK(refused >= 3, "%d: %d", which, refused);
+  }
+}
+
 int main() {
-  groups(), tiles(), rows(), arguments(), plans();
+  groups(), tiles(), no_memory(), rows(), arguments(), plans();
   for (const std::string &n : names) puts(n.c_str());
   return failures != 0;
 }
