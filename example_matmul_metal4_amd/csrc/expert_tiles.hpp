@@ -138,7 +138,7 @@ struct GroupSearch {
     total = w.blocks();
 #pragma unroll 1
     for (int e0 = 64; e0 < E; e0 += 64) total += GroupWindow(row_start, E, T, BM, e0).blocks();
-    total *= tiles_n;
+    total = min(total, (int)group_max_blocks(E, T, BM)) * tiles_n;  // groups that do not ascend cost no more than those that do
   }
   __device__ __forceinline__ GroupTile get(int i, int &half) const {
     GroupTile r;
