@@ -1,6 +1,6 @@
 // Products grouped by expert: C[t] = A[t] op(B_e) + bias_e for the rows t of group e, and the weights' gradients
-// dB_e = sum over its rows of dC[t] x A[t]. The tiles are the GEMM's (tile_direct.hpp, quarter.hpp); here a workgroup
-// finds its group and tile, and narrows operands and buffer ranges to them.
+// dB_e = sum over its rows of dC[t] x A[t]. Few rows run the GEMM's quarter tiles (quarter.hpp): here a workgroup finds its
+// group and tile, and narrows operands and buffer ranges to them. Large tiles are in expert_tiles.hpp.
 //
 // Where the groups start lies on the device, so a launch's grid is what ascending groups need at most, and workgroups past
 // what they do need end at once. Every wavefront looks its tile up by itself: the groups' block counts, 64 groups to a
