@@ -87,6 +87,39 @@ __device__ __forceinline__ uint32_t range_of(const void *p, uint32_t exact, bool
   return (exact + (any ? (uint32_t)(uintptr_t)p & 2u : 0u) + 3u) & ~3u;
 }
 
+// Some 16-bit rows of K places, ld apart, as they lie in memory: at any 2-byte alignment. What lies behind the last row's end is out of
+// the buffer's range.
+struct AnyRows {
+  rsrc_t buf;
+  uint32_t mis, step;  // bytes from the buffer's start to the first row, and between rows
+  int K;
+  bool odd;            // rows start in the middle of dwords
+  __device__ __forceinline__ AnyRows(const void *first, int rows, int64_t ld, int K_) : K(K_) {
+    const uint32_t bytes = ((uint32_t)(rows - 1) * (uint32_t)ld + (uint32_t)K_) * 2u;
+    buf = make_rsrc_any(first, range_of(first, bytes, true), mis);
+    step = (uint32_t)ld * 2u;
+    odd = mis != 0 || (ld & 1) != 0;
+  }
+  __device__ __forceinline__ uint32_t at(int row, int k) const { return (uint32_t)row * step + (uint32_t)k * 2u + mis; }
+  // The 8 places of a row from k on, in two steps, so that many loads are in flight: the dwords that hold them ...
+  // (POLICY 2: past the caches)
+  template <int POLICY = 0>
+  __device__ __forceinline__ void load(int row, int k, u32x4 &v, uint32_t &e) const {
+    const uint32_t off = k < K ? at(row, k) : kOOBAny;
+    v = __builtin_amdgcn_raw_buffer_load_b128(buf, off & ~3u, 0, POLICY);
+    if (odd) e = buf_load4(buf, (off & ~3u) + 16u);
+  }
+  // ... and the places themselves, zeros from K on.
+  __device__ __forceinline__ u32x4 take(int row, int k, u32x4 v, uint32_t e) const {
+    if (odd) {
+      const uint32_t sh = (at(row, k) & 2u) << 3;
+      v = u32x4{__builtin_amdgcn_alignbit(v.y, v.x, sh), __builtin_amdgcn_alignbit(v.z, v.y, sh), __builtin_amdgcn_alignbit(v.w, v.z, sh),
+                __builtin_amdgcn_alignbit(e, v.w, sh)};
+    }
+    return K - k < 8 ? keep_halves(v, K - k) : v;
+  }
+};
+
 // The part of the GEMM's arguments that a tile of group e takes: `rows` rows of A from `row` on, one block at most.
 template <int BLOCK, bool ANY>
 __device__ __forceinline__ mtk_tile_args group_args(const mtk_grouped_kargs &g, int e, int row, int rows) {
@@ -154,59 +187,88 @@ __device__ __forceinline__ mtk_tile_args grad_args(const mtk_grouped_kargs &g, i
   return a;
 }
 
+// dbias_e[n] = sum over the group's rows of dC[t][n]: 64 columns from n0 on per workgroup, 8 neighbours a lane, 64 rows a step of a
+// wavefront, all in flight at once, the steps over the W wavefronts. Sums in 32 bits: a lane's rows in order, then rows apart by 1, 2
+// and 4 of 8, then the wavefronts in order. Latency bounds it: 343 rows of the largest of 24 groups, 1023 columns, a column a lane: 16
+// wavefronts 4.2 us, 8 15.3.
+template <int DT, int W>
+__device__ __forceinline__ void bias_columns(const mtk_grouped_kargs &g, const void *dC, int ld, int N, void *out, int e, int n0) {
+  __shared__ float sums[W][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int start = __builtin_amdgcn_readfirstlane(g.row_start[e]), next = __builtin_amdgcn_readfirstlane(g.row_start[e + 1]);
+  const group_rows r = group_of(start, next, g.T);
+  const int c = lane & 7, r0 = lane >> 3, k = n0 + 8 * c;
+  const AnyRows src((const uint16_t *)dC + (size_t)r.first * (size_t)ld, max(r.rows, 1), ld, N);
+  float s[8] = {};
+  for (int i = 64 * wave; i < r.rows; i += 64 * W) {
+    u32x4 v[8];
+    uint32_t x[8] = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int row = i + 8 * j + r0;
+      src.load(row, row < r.rows ? k : N, v[j], x[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const u32x4 w = src.take(i + 8 * j + r0, k, v[j], x[j]);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        s[2 * h] += from_bits<DT>((uint16_t)(w[h] & 0xffffu));
+        s[2 * h + 1] += from_bits<DT>((uint16_t)(w[h] >> 16));
+      }
+    }
+  }
+  float t = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float y = s[j];
+    y += __shfl_xor(y, 8);
+    y += __shfl_xor(y, 16);
+    y += __shfl_xor(y, 32);
+    t = r0 == j ? y : t;  // column 8 c + r0
+  }
+  if constexpr (W > 1) {
+    sums[wave][lane] = t;
+    __syncthreads();
+    if (wave > 0) return;
+    t = sums[0][lane];
+#pragma unroll
+    for (int w = 1; w < W; ++w) t += sums[w][lane];
+  }
+  const int col = n0 + 8 * c + r0;
+  if (col >= N) return;
+  const size_t at = (size_t)e * (size_t)N + (size_t)col;
+  if (g.C32)
+    ((float *)out)[at] = t;
+  else
+    ((uint16_t *)out)[at] = to_bits<DT>(t);
+}
+
+// The bias's gradient as a launch of its own, beside large tiles.
+constexpr int kBiasWaves = 16;
+template <int DT>
+__device__ __forceinline__ void grouped_bias_grad(const mtk_grouped_kargs &g) {
+  const int e = blockIdx.x / g.tiles_n;
+  bias_columns<DT, kBiasWaves>(g, g.A, g.lda, g.N, g.C32 ? (void *)g.C32 : g.C, e, 64 * (blockIdx.x - e * g.tiles_n));
+}
+
+// The first g.lead workgroups (a multiple of 8, or none) have the bias's gradient: dC is A (has_bias 1) or B (2).
 template <int DT, bool ANY, int W>
 __device__ __forceinline__ void grouped_grad_quarter(const mtk_grouped_kargs &g) {
+  int block = blockIdx.x;
+  if (block < g.lead) {
+    const bool a = g.has_bias == 1;
+    const int N = a ? g.M : g.N, across = (N + 63) >> 6, e = block / across;
+    if (e < g.E) bias_columns<DT, W>(g, a ? g.A : g.B, a ? g.lda : g.ldb, N, const_cast<void *>(g.bias), e, 64 * (block - e * across));
+    return;
+  }
+  block -= g.lead;
   // an XCD has 16 neighbours of every 128 tiles: those of a large group are spread over all of them
   const int tiles = g.tiles_m * g.tiles_n;
-  const int id = group_nth_tile((int)blockIdx.x & 127, 128, (int)blockIdx.x >> 7, (int)gridDim.x, 0).tile, e = id / tiles;
+  const int id = group_nth_tile(block & 127, 128, block >> 7, (int)gridDim.x - g.lead, 0).tile, e = id / tiles;
   const mtk_tile_args a = grad_args<ANY>(g, e);
   using A = std::conditional_t<ANY, QuarterAny<true>, QuarterOp<true, false>>;
   quarter_tile<DT, A, true, ANY, W, true>(a, A{}, tile_at<64, 64>(id - e * tiles, g.tiles_m, g.tiles_n));
-}
-
-// dbias_e[n] = sum over the group's rows of dC[t][n]: 64 columns per workgroup, one per lane; its 16 wavefronts take every 16th
-// row, 8 of them in flight at a time, and their sums in 32 bits are added in wavefront order. Latency bounds it: 343 rows of the
-// largest of 24 groups, 1023 columns: 8 wavefronts with two columns per lane 15.3 us.
-constexpr int kBiasWaves = 16, kBiasCols = 64;
-template <int DT>
-__device__ __forceinline__ void grouped_bias_grad(const mtk_grouped_kargs &g) {
-  __shared__ float sums[kBiasWaves][kBiasCols];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int e = blockIdx.x / g.tiles_n, n0 = (blockIdx.x - e * g.tiles_n) * kBiasCols;
-  const int start = __builtin_amdgcn_readfirstlane(g.row_start[e]), next = __builtin_amdgcn_readfirstlane(g.row_start[e + 1]);
-  const group_rows r = group_of(start, next, g.T);
-  const uint16_t *at = (const uint16_t *)g.A + (size_t)(r.first + wave) * (size_t)g.lda + min(n0 + lane, g.N - 1);
-  const size_t step = (size_t)kBiasWaves * (size_t)g.lda;
-  float s = 0.0f;
-  int i = wave;
-  constexpr int kAhead = 8;
-  for (; i + (kAhead - 1) * kBiasWaves < r.rows; i += kAhead * kBiasWaves, at += kAhead * step) {
-    uint16_t v[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) v[j] = at[j * step];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) s += from_bits<DT>(v[j]);
-  }
-  if (i < r.rows) {  // the rest, rows past the last read again and not added
-    uint16_t v[kAhead];
-    const int n = (r.rows - i + kBiasWaves - 1) / kBiasWaves;
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) v[j] = at[min(j, n - 1) * step];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) s += j < n ? from_bits<DT>(v[j]) : 0.0f;
-  }
-  sums[wave][lane] = s;
-  __syncthreads();
-  if (wave == 0 && n0 + lane < g.N) {
-    float t = sums[0][lane];
-#pragma unroll
-    for (int w = 1; w < kBiasWaves; ++w) t += sums[w][lane];
-    const size_t out = (size_t)e * (size_t)g.N + (size_t)(n0 + lane);
-    if (g.C32)
-      g.C32[out] = t;
-    else
-      ((uint16_t *)g.C)[out] = to_bits<DT>(t);
-  }
 }
 
 }  // namespace mtk

@@ -9,7 +9,7 @@
 
 #include <stdint.h>
 
-#define MTK_KARGS_VERSION 19
+#define MTK_KARGS_VERSION 20
 
 /* In-workgroup split-K: bytes of workspace slot per output tile of BM x BM (256 or 128). Each
  * wavefront keeps these accumulator blocks (32 x 32 fp32, 4 KB) of its running sum in the slot,
@@ -203,8 +203,9 @@ typedef struct {
   int32_t lda, ldb, ldc;
   uint32_t b_exact; /* bytes of the weights of a group */
   int32_t tiles_m, tiles_n, k_tiles;
-  int32_t has_bias;
-  int32_t b_once; /* weights that one row block reads are loaded past the caches */
+  int32_t has_bias; /* gradients on quarter tiles: dC is A (1) or B (2), dbias is `bias` */
+  int32_t lead;     /* ... and so many workgroups of the launch have it */
+  int32_t b_once;   /* weights that one row block reads are loaded past the caches */
 } mtk_grouped_kargs;
 
 /* Rows into blocks of 32 four-bit values with one scale, and back (mx.h has the layout). */

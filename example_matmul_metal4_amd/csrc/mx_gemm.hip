@@ -44,7 +44,7 @@ __device__ __forceinline__ void mx_few(const mtk_mx_gemm_kargs &g) {
   const uint32_t lane_s = 8u * (uint32_t)(lane & 31) + 4u * (uint32_t)(lane >> 5);
   // QUANT: load i has rows 2 i and 2 i + 1, 8 places per lane
   const int half = lane >> 5, place = 8 * (lane & 31), pairs = (rows + 1) >> 1;
-  const MxSource src(QUANT ? (const uint16_t *)g.A + first * g.lda : nullptr, rows, g.lda, g.K);
+  const AnyRows src(QUANT ? (const uint16_t *)g.A + first * g.lda : nullptr, rows, g.lda, g.K);
   u32x4 va[QUANT ? 16 : 4 * MB] = {}, vb[8];
   uint32_t ve[16] = {};
   uint32_t na[MB], nb[2];

@@ -12,39 +12,6 @@
 
 namespace mtk {
 
-// Some 16-bit rows of K places, ld apart, as they lie in memory: at any 2-byte alignment. What lies behind the last row's end is out of
-// the buffer's range.
-struct MxSource {
-  rsrc_t buf;
-  uint32_t mis, step;  // bytes from the buffer's start to the first row, and between rows
-  int K;
-  bool odd;            // rows start in the middle of dwords
-  __device__ __forceinline__ MxSource(const void *first, int rows, int64_t ld, int K_) : K(K_) {
-    const uint32_t bytes = ((uint32_t)(rows - 1) * (uint32_t)ld + (uint32_t)K_) * 2u;
-    buf = make_rsrc_any(first, range_of(first, bytes, true), mis);
-    step = (uint32_t)ld * 2u;
-    odd = mis != 0 || (ld & 1) != 0;
-  }
-  __device__ __forceinline__ uint32_t at(int row, int k) const { return (uint32_t)row * step + (uint32_t)k * 2u + mis; }
-  // The 8 places of a row from k on, in two steps, so that many loads are in flight: the dwords that hold them ...
-  // (POLICY 2: past the caches)
-  template <int POLICY = 0>
-  __device__ __forceinline__ void load(int row, int k, u32x4 &v, uint32_t &e) const {
-    const uint32_t off = k < K ? at(row, k) : kOOBAny;
-    v = __builtin_amdgcn_raw_buffer_load_b128(buf, off & ~3u, 0, POLICY);
-    if (odd) e = buf_load4(buf, (off & ~3u) + 16u);
-  }
-  // ... and the places themselves, zeros from K on.
-  __device__ __forceinline__ u32x4 take(int row, int k, u32x4 v, uint32_t e) const {
-    if (odd) {
-      const uint32_t sh = (at(row, k) & 2u) << 3;
-      v = u32x4{__builtin_amdgcn_alignbit(v.y, v.x, sh), __builtin_amdgcn_alignbit(v.z, v.y, sh), __builtin_amdgcn_alignbit(v.w, v.z, sh),
-                __builtin_amdgcn_alignbit(e, v.w, sh)};
-    }
-    return K - k < 8 ? keep_halves(v, K - k) : v;
-  }
-};
-
 // A lane's 8 values of a block that it shares with its three neighbours: their codes, the even place in the low half of a byte,
 // and the block's scale byte.
 template <int DT>

@@ -35,7 +35,7 @@ __device__ __forceinline__ void mx_quantise(const mtk_mx_rows_kargs &a) {
   const MxPlace p(a);
   if (p.r0 >= a.R) return;
   const int n = (int)min((int64_t)kMxRows, a.R - p.r0);
-  const MxSource src((const uint16_t *)a.src + p.r0 * a.ld, n, a.ld, a.K);
+  const AnyRows src((const uint16_t *)a.src + p.r0 * a.ld, n, a.ld, a.K);
   u32x4 v[kMxRows];
   uint32_t e[kMxRows] = {};
 #pragma unroll
