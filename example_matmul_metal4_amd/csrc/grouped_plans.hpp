@@ -209,8 +209,8 @@ int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out
     return fail(MTK_ERR_UNSUPPORTED, "%d groups with these N and K are not supported", d.E);
   grid = tile_grid(tile, cus, grid);
   // Quarter tiles have the bias's sums in their launch: 1000 rows over 24 groups of 1023 x 520 33.8 -> 29.9 us, 2000 over 4 of 300 x 301
-  // 16.6 -> 11.0 (1000 over 8 of 1024 x 512, whose workgroups fill a CU each, 9.9 -> 10.2). Beside large tiles a launch of 16 wavefronts
-  // each is cheaper than workgroups with those tiles' LDS.
+  // 16.6 -> 11.0 (1000 over 8 of 1024 x 512, whose workgroups fill a CU each, 9.9 -> 10.2). Large tiles are a
+  // persistent grid; beside them the bias has a launch of its own.
   const bool one_launch = d.has_bias && tile == 64;
   if (one_launch) {
     a.has_bias = d.trans_b ? 1 : 2;

@@ -312,6 +312,42 @@ def test_layers_in_4_bits(dev, E, T, D, F, dtype):
     down.close()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [1, 2000])  # few rows a workgroup, and large tiles
+def test_every_scale(dev, dtype, N):
+    # rows that somebody else has brought into the format: every scale byte, 0 (2^-127) among them, with every code
+    R, K = 256 if N == 1 else 4096, 256
+    codes = np.tile(np.arange(16, dtype=np.uint8) | (np.arange(16, dtype=np.uint8)[::-1] << 4), (R, 8))
+    scales = np.repeat((np.arange(R) % 256).astype(np.uint8)[None, :, None], 8, 2)
+    v = experts.values(codes, scales, K)
+    d = [dev.upload(x) for x in (codes, np.ascontiguousarray(scales))]
+    back = dev.upload(np.full((R, K), FILL, np.uint16))
+    mtk.MxDequantizePlan(dev, R, K, dtype=dtype).run(*d, back)
+    dev.sync()
+    with np.errstate(over="ignore"):  # the largest are infinities in 16 bits
+        want = kv.to_f64(kv.bits_of(v, dtype), dtype)
+    got = kv.to_f64(dev.download(back, (R, K), np.uint16), dtype)
+    assert np.array_equal(got, want, equal_nan=True), np.argwhere(~((got == want) | (np.isnan(got) & np.isnan(want))))[:5]
+    # times ones: the sum of each row's values; bf16 holds them all
+    if dtype == "bf16":
+        pick = np.r_[0:8]  # of a row, so that its sum is not zero
+        ones = np.zeros((N, K))
+        ones[:, pick] = 1
+        qw = experts.quantise(kv.bits_of(ones, dtype), dtype)
+        dw, out = [dev.upload(x) for x in qw], dev.empty(2 * R * N)
+        plan = mtk.MxGemmPlan(dev, R, N, K, dtype=dtype)
+        print(plan.describe(), flush=True)
+        plan.run(*d, *dw, None, None, out)
+        dev.sync()
+        got = kv.to_f64(dev.download(out, (R, N), np.uint16), dtype)
+        want, bound, _ = experts.mx_product(v, experts.values(*qw, K)[None], None, [0, R], dtype)
+        nan, large = np.isnan(want), np.abs(want) > 2.0 ** 127  # (past the type, or near it)
+        assert np.array_equal(np.isnan(got), nan)
+        agree(got[~nan & ~large], want[~nan & ~large], bound[~nan & ~large], "C")
+        free(out, *dw)
+    free(back, *d)
+
+
 # ------------------------------------------------------------------ streams, captures, several runs at once
 
 def test_other_streams_and_captures(dev):
