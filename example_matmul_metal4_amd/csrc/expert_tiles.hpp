@@ -170,6 +170,8 @@ struct GroupSearch {
 // C = A op(B_e) + bias_e
 template <int BM, int BN, bool KMAJOR>
 struct ForwardTiles {
+  static constexpr bool kTurned = !KMAJOR;
+  __device__ __forceinline__ int whole() const { return g.K >> 6; }
   static constexpr bool kWarm = false;
   const mtk_grouped_kargs &g;
   GroupSearch<BM> search;
@@ -219,6 +221,7 @@ struct ForwardTiles {
 // last-level cache 304 -> 302. (The forward products ask for K-tiles of their own weights in this way: 306 -> 330.)
 template <int BM, int BN>
 struct GradTiles {
+  static constexpr bool kTurned = false;
   static constexpr bool kWarm = BM == 256;
   const mtk_grouped_kargs &g;
   __device__ __forceinline__ explicit GradTiles(const mtk_grouped_kargs &g_) : g(g_) {}
@@ -271,6 +274,8 @@ struct GradTiles {
 // C = A B_e^T + bias_e, both in few bits; one group of all rows where there is no row_start.
 template <int BM, int BN>
 struct MxTiles {
+  static constexpr bool kTurned = true;
+  __device__ __forceinline__ int whole() const { return g.k_tiles; }
   static constexpr bool kWarm = false;
   const mtk_mx_gemm_kargs &g;
   GroupSearch<BM> search;
@@ -358,6 +363,8 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
   const int at_s = scales ? kCodes + wave * 1024 : 2 * kStage, next_s = scales ? kStage : 0;
   const uint32_t off_s = (uint32_t)(scales_a ? wave : wave - BM / 128) * 1024u + 16u * (uint32_t)lane;
 
+  int turn = 0;
+  if constexpr (TILES::kTurned) turn = tiles.g.turned ? group_turn((int)blockIdx.x, tiles.whole()) : 0;
   // The buffers of one K-tile's loads: K-tile k of t, or k - n of u where t has no more.
   struct Source {
     rsrc_t a, b, s;
@@ -365,6 +372,7 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
   auto source = [&](const ExpertTile &t, const ExpertTile &u, int n, int k) {
     const bool own = k < n;
     k = own ? k : k - n;
+    if constexpr (TILES::kTurned) k = group_turned(k, turn, tiles.whole());
     const int K = pick(own, t.K, u.K);
     const bool there = k < pick(own, t.k_tiles, u.there ? u.k_tiles : 0);
     Source r;

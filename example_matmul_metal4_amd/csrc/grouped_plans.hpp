@@ -99,6 +99,13 @@ constexpr TileCost kFewBits[] = {{256, 8, 1, 10.3, 0.43, 0.83, 1.50, 0.27, 0},
 // 30.3. Smaller ones may be there still: 14336 x 4096 in 4 bits, 16 rows, call after call 8.6 us, past the caches 9.5.
 constexpr double kLastLevelCache = 256e6;
 
+// Rows of weights that lie a power of two apart have the same place of K on few of the memory's channels, and workgroups that go through
+// K in step ask for it together: each XCD starts elsewhere in K. All of an XCD's workgroups alike, so that they share what its L2 holds.
+// 2048 rows over 64 groups of 2048 x 2048 143 -> 111 us, 8192 over 64 149 -> 137, 16 over 32 22.3 -> 19.9, 256 over 8 of 14336 x 4096
+// 166.6 -> 159.5; in 4 bits 64 over 64 of 2048 x 8192 64.3 -> 58.8. Groups of many rows read their rows' K-tiles from eight places then:
+// one group of 8192 rows, 4096 x 4096 214 -> 218, of 2048 rows and 8 of 1024 no slower. (Weights [K][N] are rows of other K-tiles.)
+constexpr double kTurnedRows = 2048;
+
 double busy_groups(int E, int T) { return E > 1 ? E * -std::expm1(-(double)T / E) : 1.0; }
 double tiles_across(int tile, int n) { return (double)(((long long)n + std::max(tile, 64) - 1) / std::max(tile, 64)); }
 
@@ -158,6 +165,7 @@ int plan_grouped(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
   a.k_tiles = (d.K + 63) / 64;
   a.has_bias = d.has_bias ? 1 : 0;
   a.b_once = 2.0 * d.E * d.N * d.K > kLastLevelCache ? 1 : 0;
+  a.turned = d.trans_b && d.T < kTurnedRows * busy ? 1 : 0;
   long long grid;
   if ((s = check_tiles(d.E, d.T, tile, a.tiles_n, &grid)) != MTK_OK) return s;
   grid = tile_grid(tile, cus, grid);
@@ -320,6 +328,7 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
   TileCost kind = choose_tile(kFewBits, true, cus, k_tiles, 1e-6 * (0.53 * (busy * d.N * d.K + (double)d.T * d.K) + 2.0 * d.T * d.N), [&](int t) {
     return (d.E ? std::max(busy, (double)d.T / t + 0.5 * busy) : (double)((d.T + t - 1) / t)) * tiles_across(t, d.N);
   });
+  a.turned = d.T < kTurnedRows * busy ? 1 : 0;
   // Few rows are brought into the format by the product's own workgroups, each of them all that it needs: 0.2 us for two rows and a
   // K-tile of a wavefront, against 2.4 for the launch. 14336 x 4096: 1 row 6.6 us (with the launch 8.3), 8 rows 8.5 (8.3), 16 10.2
   // (8.6); 2048 x 2048: 16 rows 7.0 (7.3); 4096 x 14336: 1 row 12.6 (12.1).

@@ -53,4 +53,13 @@ MTK_GROUP_FN group_place group_nth_tile(int block, int grid, int i, int total, i
   return p;
 }
 
+// K-tile k of `full` whole ones, taken from tile `turn` on; those behind them stay in their places.
+MTK_GROUP_FN int group_turned(int k, int turn, int full) {
+  if (k >= full) return k;
+  k += turn;
+  return k >= full ? k - full : k;
+}
+// Where XCD block % 8 starts.
+MTK_GROUP_FN int group_turn(int block, int full) { return (int)((int64_t)(block & 7) * full >> 3); }
+
 #endif

@@ -48,7 +48,9 @@ __device__ __forceinline__ void mx_few(const mtk_mx_gemm_kargs &g) {
   u32x4 va[QUANT ? 16 : 4 * MB] = {}, vb[8];
   uint32_t ve[16] = {};
   uint32_t na[MB], nb[2];
-  auto load = [&](int kt) {
+  const int turn = g.turned ? group_turn((int)blockIdx.x, g.k_tiles) : 0;
+  auto load = [&](int k) {
+    const int kt = group_turned(k, turn, g.k_tiles);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t off = lane_b + (uint32_t)i * 8u * B.row_b + (uint32_t)kt * 128u;
@@ -73,12 +75,13 @@ __device__ __forceinline__ void mx_few(const mtk_mx_gemm_kargs &g) {
   for (; kt < g.k_tiles; kt += W) {
     uint32_t sa[MB], sb[2];
     if constexpr (QUANT) {
+      const int k = group_turned(kt, turn, g.k_tiles) * 256 + place;
       static_for<0, 16>([&](auto i_c) {
         constexpr int i = decltype(i_c)::value;
         if (i < pairs) {
           uint32_t code;
           int byte;
-          mx_quantise8<DT>(src.take(2 * i + half, kt * 256 + place, va[i], ve[i]), code, byte);
+          mx_quantise8<DT>(src.take(2 * i + half, k, va[i], ve[i]), code, byte);
           const int row = 2 * i + half, block = place >> 5;
           *(uint32_t *)(la + lds_off(row, block) + 4 * (lane & 3)) = code;
           if ((lane & 3) == 0) *(uint8_t *)(ls + 8 * row + block) = (uint8_t)byte;

@@ -12,6 +12,7 @@
 // fragment reads, K-major operands with transposed reads. ANY: rows at any 2-byte alignment.
 #pragma once
 
+#include "groups.h"
 #include "tile_gemm.hpp"
 
 namespace mtk {
@@ -229,28 +230,34 @@ __device__ __forceinline__ void quarter_tile(const mtk_tile_args &a, AOp oa, con
   f32x16 acc[MB][2] = {};
   u32x4 sa[AOp::kLoads], sb[8];
   uint32_t ea[AOp::kLoads], eb[8];
+  auto place = [&](int k) {
+    if constexpr (PLACED)
+      return group_turned(k, at.turn, a.K / kBK);
+    else
+      return k;
+  };
   int kt = kt0 + wave;
   if (kt < kt1) {
-    oa.load(ra, kt, lane, sa, ea);
+    oa.load(ra, place(kt), lane, sa, ea);
     if constexpr (PLACED) {
       if (at.b_once)
-        ob.template load<2>(rb, kt, lane, sb, eb);
+        ob.template load<2>(rb, place(kt), lane, sb, eb);
       else
-        ob.load(rb, kt, lane, sb, eb);
+        ob.load(rb, place(kt), lane, sb, eb);
     } else {
       ob.load(rb, kt, lane, sb, eb);
     }
   }
   for (; kt < kt1; kt += W) {
-    oa.store(la, lane, kt, a.K - kt * kBK, sa, ea);
-    ob.store(lb, lane, kt, a.K - kt * kBK, sb, eb);
+    oa.store(la, lane, place(kt), a.K - place(kt) * kBK, sa, ea);
+    ob.store(lb, lane, place(kt), a.K - place(kt) * kBK, sb, eb);
     if (kt + W < kt1) {
-      oa.load(ra, kt + W, lane, sa, ea);
+      oa.load(ra, place(kt + W), lane, sa, ea);
       if constexpr (PLACED) {
         if (at.b_once)
-          ob.template load<2>(rb, kt + W, lane, sb, eb);
+          ob.template load<2>(rb, place(kt + W), lane, sb, eb);
         else
-          ob.load(rb, kt + W, lane, sb, eb);
+          ob.load(rb, place(kt + W), lane, sb, eb);
       } else {
         ob.load(rb, kt + W, lane, sb, eb);
       }

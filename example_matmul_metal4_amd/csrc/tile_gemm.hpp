@@ -38,10 +38,12 @@ constexpr int kBK = 64;
 constexpr int kThreads = 256;
 constexpr int kGroupM = 4;
 
-// The first row and column of an output tile; b_once: no other tile reads its columns of B.
+// The first row and column of an output tile; b_once: no other tile reads its columns of B; its whole K-tiles are taken from the
+// turn-th on.
 struct TileAt {
   int m0, n0;
   bool b_once;
+  int turn;
 };
 
 __device__ __forceinline__ uint32_t lds_off(int row, int chunk) {

@@ -196,6 +196,15 @@ static void tiles() {
     for (int t = 0; t < 2 * total; ++t) CHECK(had[t] == 1, "half %d of %d, grid %d: %d times", t, 2 * total, grid, had[t]);
     CHECK(rounds == (total + grid - 1) / grid, "%d rounds", rounds);
   }
+  for (int full = 0; full < 70; ++full)  // K-tiles from elsewhere on: each once, those behind the whole ones in their places
+    for (int b = 0; b < 16; ++b) {
+      const int turn = group_turn(b, full);
+      CHECK(turn >= 0 && (turn < full || full == 0), "%d of %d", turn, full);
+      std::set<int> seen;
+      for (int k = 0; k < full; ++k) seen.insert(group_turned(k, turn, full));
+      CHECK((int)seen.size() == full && (full == 0 || (*seen.begin() == 0 && *seen.rbegin() == full - 1)), "%d of %d", turn, full);
+      CHECK(group_turned(full, turn, full) == full && group_turned(full + 1, turn, full) == full + 1, "%d", full);
+    }
   for (int b = 0; b < 256; ++b) {  // no count passes 32 bits
     CHECK(group_nth_tile(b, 256, INT32_MAX / 256 - 1, INT32_MAX, 1).tile >= 0, " ");
     CHECK(group_nth_tile(b, 256, INT32_MAX / 256 + 1, INT32_MAX, 1).tile == -1, " ");
