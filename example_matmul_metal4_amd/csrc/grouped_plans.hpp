@@ -69,8 +69,8 @@ long long tile_grid(int tile, int cus, long long tiles) {
 // with 0.15 of the other. rounds: workgroups over those that are on the device at once, between that and the next whole number, at
 // least 1; part: that share, at most 1 (a full device's K-tiles take longer). The groups' sizes lie on the device: of E groups,
 // E (1 - exp(-T / E)) are taken to have rows, as if each row chose one of E, and each to have half a block that is not full. Fitted
-// to launches of 400 forward products, 400 gradients and 350 products in few bits, each by every kernel (random sizes, T to 16384,
-// N and K 64 to 14336): the kernel chosen takes 1.02, 1.02 and 1.01 times (geometric mean) the time of the fastest.
+// to launches of 400 forward products, 300 gradients and 350 products in few bits, each by every kernel (random sizes, T to 16384,
+// N and K 64 to 14336): the kernel chosen takes 1.02, 1.04 and 1.01 times (geometric mean) the time of the fastest.
 // Examples, us (tiles of 256, of 128, of 64 with 8, 4, 1 wavefronts): 256 rows over 8 groups of 14336 x 4096: 222, 207, 162, 156, 152;
 // 8192 over 16 of 4096 x 4096: 303, 345, 626, 563, 537; 16 over 32 of 2048 x 2048: 40, 31, 25, 22, 40. Gradients: 8192 over 16 of 4096
 // x 4096: 297, 357, 1294, 777, 601; 1000 over 24 of 1023 x 520 with the bias': -, -, 54, 35, 27.
@@ -84,11 +84,11 @@ constexpr TileCost kForward[] = {{256, 8, 1, 4.9, 0.0, 0.75, 1.06, 0.24, -1},
                                  {64, 8, 1, 1.7, 1.40, 1.35, 0.87, 0.17, 0.18},
                                  {64, 4, 2, 1.7, 2.18, 0.83, 1.06, 0.17, 0.27},
                                  {64, 1, 8, 0.0, 4.38, 0.77, 1.03, 0.17, 0.26}};
-constexpr TileCost kGradient[] = {{256, 8, 1, 5.3, 4.36, 1.13, 1.46, 0.22, -1},
-                                  {128, 4, 2, 3.9, 2.80, 0.62, 0.90, 0.21, -1},
-                                  {64, 8, 1, 3.2, 0.0, 1.96, 0.72, 0.36, 0.21},
-                                  {64, 4, 2, 3.8, 0.22, 1.22, 1.27, 0.34, 0.22},
-                                  {64, 1, 8, 3.1, 3.60, 0.92, 1.57, 0.23, 0.33}};
+constexpr TileCost kGradient[] = {{256, 8, 1, 5.7, 4.63, 1.26, 0.95, 0.22, -1},
+                                  {128, 4, 2, 4.0, 3.24, 0.67, 0.49, 0.21, -1},
+                                  {64, 8, 1, 2.5, 0.0, 1.67, 0.88, 0.58, 0.17},
+                                  {64, 4, 2, 2.9, 0.57, 0.98, 1.29, 0.35, 0.25},
+                                  {64, 1, 8, 2.1, 3.64, 0.90, 1.51, 0.23, 0.40}};
 constexpr TileCost kFewBits[] = {{256, 8, 1, 10.3, 0.43, 0.83, 1.50, 0.27, 0},
                                  {128, 4, 2, 7.0, 1.69, 0.48, 0.91, 0.26, 0},
                                  {64, 8, 1, 5.7, 0.29, 1.60, 1.34, 0.21, 0},
