@@ -20,8 +20,7 @@ __device__ __forceinline__ GroupTile mx_tile(const mtk_mx_gemm_kargs &g) {
 
 // 32 MB rows x 64 columns, the K-tiles over the workgroup's 8 wavefronts as in quarter.hpp: each has its own part of LDS, no
 // barrier until their sums are added, in wavefront order. QUANT: A are 16-bit rows, which every workgroup brings into the format
-// for itself as it stages them, a few instructions per row that the loads of B cover (a launch of its own before this one: 16 x
-// 14336 x 4096 11.6 us).
+// for itself as it stages them, a few instructions per row that the loads of B cover where rows are few (the plan has both sides).
 template <int DT, int MB, bool QUANT>
 __device__ __forceinline__ void mx_few(const mtk_mx_gemm_kargs &g) {
   constexpr int W = 8, ROWS = 32 * MB, kScaleB = QUANT ? ROWS * 8 : 0, kWaveB = (ROWS + 64) * 128 + kScaleB;

@@ -144,6 +144,64 @@ def test_few_bit_kernels(dev, kernel):
         free(*d)
 
 
+@functools.lru_cache(None)
+def halved():
+    """For each operator's 256 x 256 kernel the smallest of some problems of which the last round's tiles are half of the grid or fewer, so
+    that two workgroups share each."""
+    rng, found = rng_of(2), {}
+    size = lambda least, most: int(np.exp(rng.uniform(np.log(least), np.log(most))))
+    up = lambda x: -(-x // 256)
+    for i in range(20000):
+        E, T, N, K = size(1, 8), size(300, 9000), size(500, 9000), size(65, 6000) & ~1
+        N -= N % 2 if i % 3 else 0
+        if T * N * K > 1e11 or T * N > 3e7 or E * N * K > 6e7:
+            continue
+        starts = np.sort(np.r_[0, rng.integers(0, T + 1, E - 1), T])
+        blocks = sum(up(b - a) for a, b in zip(starts[:-1], starts[1:]))
+        dtype = DTYPES[i & 1]
+        makers = {"nt": (lambda: mtk.GroupedGemmPlan(None, E, T, N, K, dtype=dtype), blocks * up(N)),
+                  "nn": (lambda: mtk.GroupedGemmPlan(None, E, T, N, K, trans_b=False, dtype=dtype), blocks * up(N)),
+                  "grad": (lambda: mtk.GroupedGradPlan(None, E, T, N, K, dtype=dtype, out_f32=bool(i & 4)), E * up(N) * up(K)),
+                  "mx": (lambda: mtk.MxGemmPlan(None, T, N, K, E=E, dtype=dtype), blocks * up(N))}
+        for kind, (make, total) in makers.items():
+            if 0 < total % 256 <= 128 and make().describe().split("kernels: ")[1].endswith("_256"):
+                found[kind] = min(found.get(kind, (1e30,)), (T * N * K, i, E, T, N, K, dtype, tuple(starts.tolist()), bool(i & 4)))
+    return found
+
+
+@pytest.mark.parametrize("kind", ["nt", "nn", "grad", "mx"])
+def test_tiles_halved(dev, kind):
+    _, i, E, T, N, K, dtype, starts, out_f32 = halved()[kind]
+    rng, starts = rng_of(90), i32(starts)
+    A, bias = bits(rng, (T, K), dtype), bits(rng, (E, N), dtype)
+    if kind == "grad":
+        dC = bits(rng, (T, N), dtype)
+        plan = mtk.GroupedGradPlan(dev, E, T, N, K, dtype=dtype, out_f32=out_f32)
+        d = [dev.upload(x) for x in (A, dC, starts)] + [dev.empty((4 if out_f32 else 2) * E * N * K)]
+        want, bound = experts.grad(A, dC, starts, True, dtype, "f32" if out_f32 else dtype)[0]
+        args, shape = d, (E, N, K)
+    elif kind == "mx":
+        qa, qb = experts.quantise(A, dtype), experts.quantise(bits(rng, (E * N, K), dtype), dtype)
+        plan = mtk.MxGemmPlan(dev, T, N, K, E=E, dtype=dtype, has_bias=True)
+        d = [dev.upload(x) for x in (*qa, *qb, bias, starts)] + [dev.empty(2 * T * N)]
+        want, bound, _ = experts.mx_product(experts.values(*qa, K), experts.values(*qb, K).reshape(E, N, K), bias, starts, dtype)
+        args, shape = d, (T, N)
+    else:
+        B = bits(rng, (E, N, K) if kind == "nt" else (E, K, N), dtype)
+        plan = mtk.GroupedGemmPlan(dev, E, T, N, K, trans_b=kind == "nt", dtype=dtype, has_bias=True)
+        d = [dev.upload(x) for x in (A, B, bias, starts)] + [dev.empty(2 * T * N)]
+        want, bound, _ = experts.grouped(A, B, bias, starts, kind == "nt", dtype)
+        args, shape = d, (T, N)
+    print(plan.describe(), flush=True)
+    assert "_256" in plan.describe()
+    plan.run(*args)
+    dev.sync()
+    f32 = kind == "grad" and out_f32
+    got = dev.download(d[-1], shape, np.float32 if f32 else np.uint16)
+    agree(got.astype(np.float64) if f32 else kv.to_f64(got, dtype), want, bound, kind)
+    free(*d)
+
+
 # ------------------------------------------------------------------ layers
 
 class Layer:
