@@ -170,7 +170,7 @@ struct GroupSearch {
 // C = A op(B_e) + bias_e
 template <int BM, int BN, bool KMAJOR>
 struct ForwardTiles {
-  static constexpr bool kTurned = !KMAJOR;
+  static constexpr bool kTurned = !KMAJOR;  // the XCDs may start at different K-tiles (grouped_plans.hpp: kTurnedRows)
   __device__ __forceinline__ int whole() const { return g.K >> 6; }
   static constexpr bool kWarm = false;
   const mtk_grouped_kargs &g;
@@ -218,7 +218,7 @@ struct ForwardTiles {
 // would come from HBM behind the last round's outputs. So the workgroups ask for the group's rows while they are busy with the one
 // before it (warm), two K-tiles before its end, each for its part of the columns that its tile has: rows i * tiles_n + n of A's,
 // i * tiles_m + m of B's, a lane for a line of 128 bytes. 8192 rows over 16 groups of 4096 x 4096: inputs in HBM 342 -> 315 us, in the
-// last-level cache 304 -> 302. (The forward products ask for K-tiles of their own weights in this way: 306 -> 330.)
+// last-level cache 304 -> 302. (Forward products that ask for later K-tiles of their weights are slower: 306 -> 330.)
 template <int BM, int BN>
 struct GradTiles {
   static constexpr bool kTurned = false;
