@@ -124,6 +124,7 @@ struct ExpertTile {
   char *c;                   // its first output
   const uint16_t *bias;      // of its first column, or null
   int e, first, m, n;        // gradients: its group, the group's first row, and its block of rows and of columns
+  int turn;                  // its whole K-tiles are taken from this one on
   bool there;
 };
 
@@ -170,7 +171,7 @@ struct GroupSearch {
 // C = A op(B_e) + bias_e
 template <int BM, int BN, bool KMAJOR>
 struct ForwardTiles {
-  static constexpr bool kTurned = !KMAJOR;  // the XCDs may start at different K-tiles (grouped_plans.hpp: kTurnedRows)
+  static constexpr bool kTurned = !KMAJOR;  // tiles may start at different K-tiles (grouped_plans.hpp: kTurnedRows)
   __device__ __forceinline__ int whole() const { return g.K >> 6; }
   static constexpr bool kWarm = false;
   const mtk_grouped_kargs &g;
@@ -208,6 +209,7 @@ struct ForwardTiles {
     }
     t.c = (char *)g.C + ((size_t)row * (size_t)g.ldc + (size_t)at.n0) * 2;
     t.bias = g.has_bias ? (const uint16_t *)g.bias + (size_t)gt.e * (size_t)g.N + at.n0 : nullptr;
+    if constexpr (kTurned) t.turn = g.turned ? group_turn(group_turn_place(gt.e, at.n0 / BN, g.tiles_n, g.turned - 1), whole()) : 0;
     return t;
   }
 };
@@ -323,6 +325,7 @@ struct MxTiles {
     t.b_bytes = (uint32_t)t.cols * row_b;
     t.c = (char *)g.C + ((size_t)row * (size_t)g.ldc + (size_t)at.n0) * 2;
     t.bias = g.has_bias ? (const uint16_t *)g.bias + col : nullptr;
+    t.turn = g.turned ? group_turn(group_turn_place(gt.e, at.n0 / BN, g.tiles_n, g.turned - 1), whole()) : 0;
     return t;
   }
 };
@@ -363,8 +366,6 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
   const int at_s = scales ? kCodes + wave * 1024 : 2 * kStage, next_s = scales ? kStage : 0;
   const uint32_t off_s = (uint32_t)(scales_a ? wave : wave - BM / 128) * 1024u + 16u * (uint32_t)lane;
 
-  int turn = 0;
-  if constexpr (TILES::kTurned) turn = tiles.g.turned ? group_turn((int)blockIdx.x, tiles.whole()) : 0;
   // The buffers of one K-tile's loads: K-tile k of t, or k - n of u where t has no more.
   struct Source {
     rsrc_t a, b, s;
@@ -372,7 +373,7 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
   auto source = [&](const ExpertTile &t, const ExpertTile &u, int n, int k) {
     const bool own = k < n;
     k = own ? k : k - n;
-    if constexpr (TILES::kTurned) k = group_turned(k, turn, tiles.whole());
+    if constexpr (TILES::kTurned) k = group_turned(k, pick(own, t.turn, u.turn), tiles.whole());
     const int K = pick(own, t.K, u.K);
     const bool there = k < pick(own, t.k_tiles, u.there ? u.k_tiles : 0);
     Source r;

@@ -100,11 +100,21 @@ constexpr TileCost kFewBits[] = {{256, 8, 1, 10.3, 0.43, 0.83, 1.50, 0.27, 0},
 constexpr double kLastLevelCache = 256e6;
 
 // Rows of weights that lie a power of two apart have the same place of K on few of the memory's channels, and workgroups that go through
-// K in step ask for it together: each XCD starts elsewhere in K. All of an XCD's workgroups alike, so that they share what its L2 holds.
-// 2048 rows over 64 groups of 2048 x 2048 143 -> 111 us, 8192 over 64 149 -> 137, 16 over 32 22.3 -> 19.9, 256 over 8 of 14336 x 4096
-// 166.6 -> 159.5; in 4 bits 64 over 64 of 2048 x 8192 64.3 -> 58.8. Groups of many rows read their rows' K-tiles from eight places then:
-// one group of 8192 rows, 4096 x 4096 214 -> 218, of 2048 rows and 8 of 1024 no slower. (Weights [K][N] are rows of other K-tiles.)
+// K in step ask for it together: so groups, and parts of the columns where groups are few, start at different K-tiles (group_turn_place).
+// 2048 rows over 64 groups of 2048 x 2048 147 -> 115 us, 8192 over 64 147 -> 136, 16 over 32 21.8 -> 19.9, 16 rows by one of 14336 x 4096
+// 26.7 -> 23.5; in 4 bits 64 over 64 of 2048 x 8192 67.6 -> 60.5. Rows other lengths apart lose nothing by it, so they are not told apart:
+// 2048 over 64 of 2048 x 1536 93.1 -> 92.2, of 2048 x 2880 165.7 -> 165.5, 256 over 8 of 14336 x 5120 204.5 -> 204.3, 1000 rows by one
+// of 4096 x 5000 92.9 -> 84.6. Groups of many rows gain nothing, and have their rows read at several K-tiles: 16384 over 4 of 4096 x
+// 4096 475.7 -> 478.9, 8192 over 2 in 4 bits 101.4 -> 102.4. (Weights [K][N] are rows of other K-tiles.)
 constexpr double kTurnedRows = 2048;
+
+// Log2 of the parts of a group's columns that start apart. Groups start apart themselves; of one that has fewer than four row blocks (tile_at),
+// an XCD has an eighth of the columns, of more row blocks or groups more of them, and workgroups of one XCD that start together share
+// what its L2 holds: 8192 rows over 16 groups of 4096 x 4096 with eight parts 303 us, with one 294.
+int log_turn_parts(int E, int T, int tile) {
+  const long long blocks = ((long long)T + (long long)tile * E - 1) / ((long long)tile * E), runs = E * ((blocks + 3) / 4);
+  return runs == 1 ? 3 : runs == 2 ? 2 : runs <= 4 ? 1 : 0;
+}
 
 double busy_groups(int E, int T) { return E > 1 ? E * -std::expm1(-(double)T / E) : 1.0; }
 double tiles_across(int tile, int n) { return (double)(((long long)n + std::max(tile, 64) - 1) / std::max(tile, 64)); }
@@ -165,7 +175,7 @@ int plan_grouped(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
   a.k_tiles = (d.K + 63) / 64;
   a.has_bias = d.has_bias ? 1 : 0;
   a.b_once = 2.0 * d.E * d.N * d.K > kLastLevelCache ? 1 : 0;
-  a.turned = d.trans_b && d.T < kTurnedRows * busy ? 1 : 0;
+  a.turned = d.trans_b && d.T < kTurnedRows * busy ? 1 + log_turn_parts(d.E, d.T, tile) : 0;
   long long grid;
   if ((s = check_tiles(d.E, d.T, tile, a.tiles_n, &grid)) != MTK_OK) return s;
   grid = tile_grid(tile, cus, grid);
@@ -328,7 +338,6 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
   TileCost kind = choose_tile(kFewBits, true, cus, k_tiles, 1e-6 * (0.53 * (busy * d.N * d.K + (double)d.T * d.K) + 2.0 * d.T * d.N), [&](int t) {
     return (d.E ? std::max(busy, (double)d.T / t + 0.5 * busy) : (double)((d.T + t - 1) / t)) * tiles_across(t, d.N);
   });
-  a.turned = d.T < kTurnedRows * busy ? 1 : 0;
   // Few rows are brought into the format by the product's own workgroups, each of them all that it needs: 0.2 us for two rows and a
   // K-tile of a wavefront, against 2.4 for the launch. 14336 x 4096: 1 row 6.6 us (with the launch 8.3), 8 rows 8.5 (8.3), 16 10.2
   // (8.6); 2048 x 2048: 16 rows 7.0 (7.3); 4096 x 14336: 1 row 12.6 (12.1).
@@ -337,6 +346,7 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
   const bool inside = d.quantize_a && d.T <= 32.0 * busy && std::ceil(per / 2) * std::ceil(k_tiles / 8.0) * rounds <= 8;
   if (inside) kind = few;
   const int tile = kind.tile;
+  a.turned = d.T < kTurnedRows * busy ? 1 + log_turn_parts((int)groups, d.T, tile) : 0;
   a.tiles_n = (d.N + std::max(tile, 64) - 1) / std::max(tile, 64);
   long long grid;
   if ((s = check_tiles((int)groups, d.T, tile, a.tiles_n, &grid)) != MTK_OK) return s;

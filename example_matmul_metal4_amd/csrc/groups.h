@@ -59,7 +59,13 @@ MTK_GROUP_FN int group_turned(int k, int turn, int full) {
   k += turn;
   return k >= full ? k - full : k;
 }
-// Where XCD block % 8 starts.
-MTK_GROUP_FN int group_turn(int block, int full) { return (int)((int64_t)(block & 7) * full >> 3); }
+// Where the tiles of `place` (one of eight) start.
+MTK_GROUP_FN int group_turn(int place, int full) { return (int)((int64_t)(place & 7) * full >> 3); }
+// The place of group e's tiles that have column block n of `across`, where 2^log_parts parts of a group's columns start apart. Nothing of it
+// depends on how many rows any group has, so a row's sums have one order wherever its tile lies. Groups that follow each other start
+// far apart, and so do those that are eight apart, whose weights may lie a power of two apart as their rows do.
+MTK_GROUP_FN int group_turn_place(int e, int n, int across, int log_parts) {
+  return 5 * e + 3 * (e >> 3) + (log_parts ? (n << log_parts) / across << (3 - log_parts) : 0);
+}
 
 #endif

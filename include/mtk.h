@@ -417,7 +417,9 @@ int mtk_kv_attn_run(const mtk_plan *plan, const mtk_kv_attn_args *args);
  *   row_start[e] .. row_start[e + 1] - 1 (none allowed), ascending, within [0, T].
  * The kernels limit what row_start holds to [0, T]; a group whose end lies before its start has no rows. Rows of no group
  * are left as they were. Where the groups do not ascend, which of the rows are computed, and by which group, is undefined;
- * nothing outside of C is written. A row depends on its own values and its group's weights only.
+ * nothing outside of C is written. A row depends on its own values and its group's weights only, in every bit: a plan gives equal
+ * rows of a group equal results, wherever in the group they lie, wherever it starts and whatever rows the other groups have. (Plans
+ * of other sizes may add in another order.)
  * Sums in fp32, the bias added to them, one rounding.
  *
  * The input gradient of such a layer is the same product: dA = dC op(B_e)^T is a plan with N and K exchanged and trans_b

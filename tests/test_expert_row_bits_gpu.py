@@ -1,0 +1,95 @@
+"""A row of a grouped product has the same bits whatever rows the other groups have and wherever its own group starts: results of a
+serving batch do not depend on who else is in it. On every kernel whose tiles go through K from different places."""
+import numpy as np
+import pytest
+
+import example_matmul_metal4_amd as mtk
+from oracle import experts, kv
+
+FILL = 0x1234
+EQUAL = 16  # the group's rows repeat after so many
+
+# operator, kernel, E, T, N, K, dtype, 16-bit rows
+CASES = [
+    ("grouped", "nt_256", 10, 1976, 3250, 1104, "bf16", True), ("grouped", "nt_256", 11, 2494, 2574, 1080, "f16", True),
+    ("grouped", "nt_128", 28, 80, 1223, 1056, "f16", True), ("grouped", "nt_128", 48, 1807, 640, 1100, "bf16", True),
+    ("grouped", "nt_64_w8", 2, 60, 102, 2100, "bf16", True), ("grouped", "nt_64_w4", 51, 69, 408, 1088, "bf16", True),
+    ("grouped", "nt_64_w1", 24, 60, 3092, 1054, "f16", True), ("grouped", "nt_64_any_w8", 2, 60, 123, 2101, "f16", True),
+    ("grouped", "nt_64_any_w4", 59, 127, 257, 1121, "bf16", True), ("grouped", "nt_64_any_w1", 10, 21, 7537, 1189, "f16", True),
+    ("mx", "256", 4, 1676, 5345, 2304, "f16", True), ("mx", "128", 48, 1807, 624, 2200, "f16", False),
+    ("mx", "64", 34, 2459, 140, 2100, "bf16", False), ("mx", "32", 2, 60, 102, 4200, "bf16", False), ("mx", "32q", 2, 26, 125, 1120, "f16", True),
+]
+
+
+def plan_of(dev, op, E, T, N, K, dtype, rows16):
+    if op == "grouped":
+        return mtk.GroupedGemmPlan(dev, E, T, N, K, dtype=dtype, has_bias=True)
+    return mtk.MxGemmPlan(dev, T, N, K, E=E, dtype=dtype, has_bias=True, quantize_a=rows16)
+
+
+def routings(E, T, rows):
+    """Some row_start in which group E // 2 has `rows` rows, other rows lie before it and behind it, and the rows of the others vary."""
+    g, rest = E // 2, T - rows
+    for before in sorted({0, 1, min(37, rest // 2), rest // 2, rest - 1, rest}):
+        for groups in (1, g):  # in one group before it, or spread over all of them
+            starts = np.zeros(E + 1, int)
+            starts[g - groups:g + 1] = np.linspace(0, before, groups + 1).round()
+            starts[g + 1:] = np.linspace(before + rows, T, E - g).round() if E - g > 1 else T
+            starts[g + 1] = before + rows
+            yield starts.astype(np.int32)
+
+
+def test_the_kernels_are_those():
+    for op, kernel, *rest in CASES:
+        assert plan_of(None, op, *rest).describe().split("16_")[-1] == kernel, (op, kernel)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", CASES, ids=lambda c: f"{c[0]}-{c[1]}-{c[6]}")
+def test_bits_of_a_row(dev, case):
+    op, kernel, E, T, N, K, dtype, rows16 = case
+    rng = np.random.default_rng(K + T)
+    rows, g = max(1, T // 3), E // 2
+    # Places of very different sizes, whose second half takes the sum of the first one away again: what is left are the roundings on the
+    # way (and the few places behind), so that an order of the additions other than that of another run shows in the result's bits.
+    X, W = rng.standard_normal((EQUAL, K)), rng.standard_normal((E, N, K))
+    half = K // 512 * 256
+    size = np.exp2(rng.integers(0, 11, half // 32)).repeat(32)
+    X[:, :half] *= size
+    W[:, :, :half] *= size
+    X[:, half:2 * half] = -X[:, :half]
+    W[:, :, half:2 * half] = W[:, :, :half]
+    X, W = kv.bits_of(X, dtype), kv.bits_of(W.reshape(E * N, K), dtype)
+    X = X[np.arange(rows) % EQUAL]
+    A, bias = kv.bits_of(rng.standard_normal((T, K)), dtype), kv.bits_of(np.zeros((E, N)), dtype)
+    plan = plan_of(dev, op, E, T, N, K, dtype, rows16)
+    print(plan.describe(), flush=True)
+    weights = [dev.upload(x) for x in ([W] if op == "grouped" else experts.quantise(W, dtype))]
+    d_bias, C, ws = dev.upload(bias), dev.empty(2 * T * N), dev.empty(max(16, plan.workspace_bytes))
+    first = None
+    for starts in routings(E, T, rows):
+        at = starts[g]
+        assert starts[g + 1] - at == rows and (np.diff(starts) >= 0).all() and starts[-1] <= T
+        batch = A.copy()
+        batch[at:at + rows] = X
+        ds = dev.upload(starts)
+        dev.upload_into(C, np.full((T, N), FILL, np.uint16))
+        if op == "grouped":
+            a = [dev.upload(batch)]
+            plan.run(a[0], weights[0], d_bias, ds, C)
+        else:
+            a = [dev.upload(x) for x in ([batch] if rows16 else experts.quantise(batch, dtype))]
+            plan.run(a[0], None if rows16 else a[1], *weights, d_bias, ds, C, ws)
+        dev.sync()
+        got = dev.download(C, (T, N), np.uint16)[at:at + rows]
+        for x in (*a, ds):
+            x.free()
+        if first is None:
+            first = got
+            assert (got != 0).any()
+        off = np.argwhere(got != first)
+        assert len(off) == 0, f"{len(off)} of {got.size} values of the same rows differ, the first at {off[:3].tolist()}, behind {at} other rows"
+        off = np.argwhere(got != got[np.arange(rows) % EQUAL])
+        assert len(off) == 0, f"{len(off)} of {got.size} values of equal rows of the group differ, the first at {off[:3].tolist()}"
+    for x in (*weights, d_bias, C, ws):
+        x.free()
