@@ -3,6 +3,7 @@
 
 constexpr int kMaxWidth = 1 << 22;  // N, K and leading dimensions: 256 rows of a tile, and 64 past an operand's end, stay in 32 bits
 constexpr int kMaxGroups = 1 << 14;  // a workgroup looks through all of them, 64 at a time
+constexpr int kMaxRows = 1 << 30;    // counts of rows, rounded up to blocks, stay in 32 bits
 
 bool is_grouped(const mtk_plan *p) { return p->kind >= PLAN_GROUPED && p->kind <= PLAN_MX_GEMM; }
 
@@ -46,22 +47,30 @@ int check_grouped(const mtk_grouped_desc &d) {
     return fail(MTK_ERR_INVALID, "E, T, N and K must be positive (got %d, %d, %d, %d)", d.E, d.T, d.N, d.K);
   if (d.N > kMaxWidth || d.K > kMaxWidth) return fail(MTK_ERR_UNSUPPORTED, "N and K above 2^22 are not supported (got %d, %d)", d.N, d.K);
   if (d.E > kMaxGroups) return fail(MTK_ERR_UNSUPPORTED, "E above 2^14 is not supported (got %d)", d.E);
+  if (d.T > kMaxRows) return fail(MTK_ERR_UNSUPPORTED, "T above 2^30 is not supported (got %d)", d.T);
   if (d.dtype != MTK_F16 && d.dtype != MTK_BF16) return fail(MTK_ERR_INVALID, "dtype must be MTK_F16 or MTK_BF16");
-  return MTK_OK;
-}
-
-// The blocks of a launch that finds its tiles from row_start: at most `blocks` of them if the groups ascend, and no count
-// passes 32 bits whatever row_start holds.
-int check_tiles(int E, int T, int block, long long tiles_n, long long *grid) {
-  *grid = group_max_blocks(E, T, block) * tiles_n;
-  if ((long long)E * (((long long)T + block - 1) / block) * tiles_n > INT32_MAX || *grid > INT32_MAX / 512)
-    return fail(MTK_ERR_UNSUPPORTED, "%d groups of up to %d rows with this N are not supported", E, T);
   return MTK_OK;
 }
 
 // Workgroups of the tiles that expert_tiles.hpp runs: as many as are on the device at once, each with one tile after another.
 long long tile_grid(int tile, int cus, long long tiles) {
   return tile <= 64 ? tiles : std::min<long long>(tiles, (tile == 128 ? 2LL : 1LL) * cus);
+}
+
+// A launch has fewer than 2^32 threads.
+bool launches(long long grid, int threads) { return grid <= (long long)(UINT32_MAX / (unsigned)threads); }
+
+// A launch that finds its tiles from row_start: workgroups for all that ascending groups can have. fits: the launch can have so many, and no
+// count of tiles passes 32 bits whatever row_start holds (every group may have all rows).
+struct TileCount {
+  long long grid;
+  bool fits;
+};
+TileCount count_tiles(int E, int T, int tile, int waves, long long tiles_n, int cus) {
+  TileCount c;
+  c.grid = tile_grid(tile, cus, group_max_blocks(E, T, tile) * tiles_n);
+  c.fits = (long long)E * (((long long)T + tile - 1) / tile) * tiles_n <= INT32_MAX && launches(c.grid, 64 * waves);
+  return c;
 }
 
 // Which kernel runs a product, by the time that it is expected to take, in us: `start` and the larger of
@@ -117,15 +126,15 @@ int log_turn_parts(int E, int T, int tile) {
 }
 
 double busy_groups(int E, int T) { return E > 1 ? E * -std::expm1(-(double)T / E) : 1.0; }
-double tiles_across(int tile, int n) { return (double)(((long long)n + std::max(tile, 64) - 1) / std::max(tile, 64)); }
+int tiles_across(int tile, int n) { return (int)(((long long)n + std::max(tile, 64) - 1) / std::max(tile, 64)); }
 
-// wgs: workgroups with a tile of `tile`; k_tiles: of a tile
-template <int N, typename WGS>
-TileCost choose_tile(const TileCost (&costs)[N], bool even, int cus, double k_tiles, double mbytes, WGS wgs) {
+// wgs: workgroups with a tile of `tile`; k_tiles: of a tile; fits: a kernel's launch and counts can have this size. NULL: none can.
+template <int N, typename WGS, typename FITS>
+const TileCost *choose_tile(const TileCost (&costs)[N], bool even, int cus, double k_tiles, double mbytes, WGS wgs, FITS fits) {
   const TileCost *best = nullptr;
   double least = 0;
   for (const TileCost &c : costs) {
-    if (!even && c.any < 0) continue;
+    if ((!even && c.any < 0) || !fits(c)) continue;
     const double there = wgs(c.tile) / ((double)cus * c.per_cu), rounds = std::max(1.0, 0.5 * (there + std::ceil(there)));
     const double steps = c.tile > 64 || c.waves == 1 ? k_tiles : std::ceil(k_tiles / c.waves);
     const double step = (c.step + c.full * std::min(1.0, there)) * (even ? 1.0 : 1.0 + c.any);
@@ -133,7 +142,7 @@ TileCost choose_tile(const TileCost (&costs)[N], bool even, int cus, double k_ti
     const double t = c.start + std::max(x, y) + 0.15 * std::min(x, y);
     if (!best || t < least) best = &c, least = t;
   }
-  return *best;
+  return best;
 }
 
 std::string tile_name(const TileCost &c, bool even) {
@@ -157,9 +166,12 @@ int plan_grouped(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
   const int cus = ctx ? ctx->prop.multiProcessorCount : 256;
   const bool even = d.lda % 2 == 0 && d.ldb % 2 == 0;
   const double busy = busy_groups(d.E, d.T);
-  const TileCost kind = choose_tile(kForward, even, cus, (d.K + 63) / 64, 2e-6 * (busy * d.N * d.K + (double)d.T * ((double)d.N + d.K)), [&](int t) {
-    return std::max(busy, (double)d.T / t + 0.5 * busy) * tiles_across(t, d.N);
-  });
+  auto count = [&](const TileCost &c) { return count_tiles(d.E, d.T, c.tile, c.waves, tiles_across(c.tile, d.N), cus); };
+  const TileCost *chosen = choose_tile(kForward, even, cus, (d.K + 63) / 64, 2e-6 * (busy * d.N * d.K + (double)d.T * ((double)d.N + d.K)),
+                                       [&](int t) { return std::max(busy, (double)d.T / t + 0.5 * busy) * tiles_across(t, d.N); },
+                                       [&](const TileCost &c) { return count(c).fits; });
+  if (!chosen) return fail(MTK_ERR_UNSUPPORTED, "%d groups of up to %d rows with N %d have too many tiles", d.E, d.T, d.N);
+  const TileCost kind = *chosen;
   const int tile = kind.tile;
   mtk_grouped_kargs a{};
   a.E = d.E;
@@ -171,14 +183,12 @@ int plan_grouped(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
   a.ldc = d.ldc;
   a.b_stride = b_rows * d.ldb;
   a.b_exact = (uint32_t)b_exact;
-  a.tiles_n = (d.N + tile - 1) / tile;
+  a.tiles_n = tiles_across(tile, d.N);
   a.k_tiles = (d.K + 63) / 64;
   a.has_bias = d.has_bias ? 1 : 0;
   a.b_once = 2.0 * d.E * d.N * d.K > kLastLevelCache ? 1 : 0;
   a.turned = d.trans_b && d.T < kTurnedRows * busy ? 1 + log_turn_parts(d.E, d.T, tile) : 0;
-  long long grid;
-  if ((s = check_tiles(d.E, d.T, tile, a.tiles_n, &grid)) != MTK_OK) return s;
-  grid = tile_grid(tile, cus, grid);
+  const long long grid = count(kind).grid;
   std::unique_ptr<mtk_plan> p(new mtk_plan());
   p->ctx = ctx;
   p->kind = PLAN_GROUPED;
@@ -213,27 +223,29 @@ int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out
   a.N = d.trans_b ? d.K : d.N;
   a.lda = d.trans_b ? d.ldc : d.lda;
   a.ldb = d.trans_b ? d.lda : d.ldc;
-  auto tiles = [&](int tile, int n) { return (long long)((n + tile - 1) / tile); };
-  auto wgs = [&](int tile) { return d.E * tiles(tile, a.M) * tiles(tile, a.N); };
+  auto wgs = [&](int tile) { return (long long)d.E * tiles_across(tile, a.M) * tiles_across(tile, a.N); };
+  const long long bias_tiles = d.has_bias ? (long long)d.E * tiles_across(64, d.N) : 0, lead = (bias_tiles + 7) / 8 * 8;
+  auto fits = [&](const TileCost &c) {
+    if (c.tile == 64) return launches(wgs(64) + lead, 64 * c.waves);
+    return wgs(c.tile) <= INT32_MAX && launches(bias_tiles, 1024);
+  };
   const double k_tiles = std::max(1.0, d.T / busy_groups(d.E, d.T) / 64);
-  const TileCost kind = choose_tile(kGradient, even, cus, k_tiles, 1e-6 * ((d.out_f32 ? 4.0 : 2.0) * d.E * d.N * d.K + 2.0 * d.T * ((double)d.N + d.K)),
-                                    [&](int t) { return (double)wgs(t); });
+  const TileCost *chosen = choose_tile(kGradient, even, cus, k_tiles, 1e-6 * ((d.out_f32 ? 4.0 : 2.0) * d.E * d.N * d.K + 2.0 * d.T * ((double)d.N + d.K)),
+                                       [&](int t) { return (double)wgs(t); }, fits);
+  if (!chosen) return fail(MTK_ERR_UNSUPPORTED, "%d groups with N %d and K %d have too many tiles", d.E, d.N, d.K);
+  const TileCost kind = *chosen;
   const int tile = kind.tile;
-  a.tiles_m = (int)tiles(tile, a.M);
-  a.tiles_n = (int)tiles(tile, a.N);
-  long long grid = wgs(tile);
-  const long long bias_tiles = tiles(64, d.N);
-  if (grid > INT32_MAX / 512 || d.E * bias_tiles > INT32_MAX / 1024)
-    return fail(MTK_ERR_UNSUPPORTED, "%d groups with these N and K are not supported", d.E);
-  grid = tile_grid(tile, cus, grid);
+  a.tiles_m = tiles_across(tile, a.M);
+  a.tiles_n = tiles_across(tile, a.N);
+  long long grid = tile_grid(tile, cus, wgs(tile));
   // Quarter tiles have the bias's sums in their launch: 1000 rows over 24 groups of 1023 x 520 33.8 -> 29.9 us, 2000 over 4 of 300 x 301
   // 16.6 -> 11.0 (1000 over 8 of 1024 x 512, whose workgroups fill a CU each, 9.9 -> 10.2). Large tiles are a
   // persistent grid; beside them the bias has a launch of its own.
   const bool one_launch = d.has_bias && tile == 64;
   if (one_launch) {
     a.has_bias = d.trans_b ? 1 : 2;
-    a.lead = (int)((d.E * bias_tiles + 7) / 8 * 8);
-    grid += a.lead;
+    a.lead = (int)lead;
+    grid += lead;
   }
   std::unique_ptr<mtk_plan> p(new mtk_plan());
   p->ctx = ctx;
@@ -249,8 +261,8 @@ int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out
     b.T = d.T;
     b.N = d.N;
     b.lda = d.ldc;
-    b.tiles_n = (int)bias_tiles;
-    add_launch(p.get(), head + "_bias_grad", d.E * bias_tiles, 1024, b);
+    b.tiles_n = tiles_across(64, d.N);
+    add_launch(p.get(), head + "_bias_grad", bias_tiles, 1024, b);
     p->launches.back().role = ROLE_REDUCE;
   }
   p->flops = 2.0 * d.T * d.N * d.K;
@@ -335,23 +347,29 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
   a.b_once = 136.0 * k_tiles * groups * d.N > kLastLevelCache ? 1 : 0;
   const int cus = ctx ? ctx->prop.multiProcessorCount : 256;
   const double busy = busy_groups((int)groups, d.T);
-  TileCost kind = choose_tile(kFewBits, true, cus, k_tiles, 1e-6 * (0.53 * (busy * d.N * d.K + (double)d.T * d.K) + 2.0 * d.T * d.N), [&](int t) {
-    return (d.E ? std::max(busy, (double)d.T / t + 0.5 * busy) : (double)((d.T + t - 1) / t)) * tiles_across(t, d.N);
-  });
+  auto count = [&](const TileCost &c) {
+    TileCount n = count_tiles((int)groups, d.T, c.tile, c.waves, tiles_across(c.tile, d.N), cus);
+    if (!d.E) n.grid = tile_grid(c.tile, cus, ((long long)d.T + c.tile - 1) / c.tile * tiles_across(c.tile, d.N));
+    return n;
+  };
+  const TileCost *chosen = choose_tile(kFewBits, true, cus, k_tiles, 1e-6 * (0.53 * (busy * d.N * d.K + (double)d.T * d.K) + 2.0 * d.T * d.N),
+                                       [&](int t) {
+                                         return (d.E ? std::max(busy, (double)d.T / t + 0.5 * busy) : (double)((d.T + t - 1) / t)) * tiles_across(t, d.N);
+                                       },
+                                       [&](const TileCost &c) { return count(c).fits; });
+  if (!chosen) return fail(MTK_ERR_UNSUPPORTED, "%lld groups of up to %d rows with N %d have too many tiles", groups, d.T, d.N);
+  TileCost kind = *chosen;
   // Few rows are brought into the format by the product's own workgroups, each of them all that it needs: 0.2 us for two rows and a
   // K-tile of a wavefront, against 2.4 for the launch. 14336 x 4096: 1 row 6.6 us (with the launch 8.3), 8 rows 8.5 (8.3), 16 10.2
   // (8.6); 2048 x 2048: 16 rows 7.0 (7.3); 4096 x 14336: 1 row 12.6 (12.1).
   const TileCost &few = kFewBits[3];
   const double per = d.E ? std::max(1.0, d.T / busy) : d.T, rounds = std::ceil(busy * tiles_across(32, d.N) / cus);
-  const bool inside = d.quantize_a && d.T <= 32.0 * busy && std::ceil(per / 2) * std::ceil(k_tiles / 8.0) * rounds <= 8;
+  const bool inside = d.quantize_a && d.T <= 32.0 * busy && std::ceil(per / 2) * std::ceil(k_tiles / 8.0) * rounds <= 8 && count(few).fits;
   if (inside) kind = few;
   const int tile = kind.tile;
   a.turned = d.T < kTurnedRows * busy ? 1 + log_turn_parts((int)groups, d.T, tile) : 0;
-  a.tiles_n = (d.N + std::max(tile, 64) - 1) / std::max(tile, 64);
-  long long grid;
-  if ((s = check_tiles((int)groups, d.T, tile, a.tiles_n, &grid)) != MTK_OK) return s;
-  if (!d.E) grid = (long long)((d.T + tile - 1) / tile) * a.tiles_n;
-  grid = tile_grid(tile, cus, grid);
+  a.tiles_n = tiles_across(tile, d.N);
+  const long long grid = count(kind).grid;
   std::unique_ptr<mtk_plan> p(new mtk_plan());
   p->ctx = ctx;
   p->kind = PLAN_MX_GEMM;
