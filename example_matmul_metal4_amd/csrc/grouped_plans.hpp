@@ -304,8 +304,8 @@ int plan_mx_rows(mtk_ctx *ctx, const mtk_mx_rows_desc *d_in, bool quantize, mtk_
   if (s != MTK_OK) return s;
   if (d.dtype != MTK_F16 && d.dtype != MTK_BF16) return fail(MTK_ERR_INVALID, "dtype must be MTK_F16 or MTK_BF16");
   if ((s = check_ld(d.ld, d.K, "ld", &d.ld)) != MTK_OK) return s;
-  if (((long long)d.R + 15) / 16 * ((mx_k_tiles(d.K) + 1) / 2) > INT32_MAX / 256)
-    return fail(MTK_ERR_UNSUPPORTED, "%d rows of %d are not supported", d.R, d.K);
+  if (!launches(((long long)d.R + 15) / 16 * ((mx_k_tiles(d.K) + 1) / 2), 256))
+    return fail(MTK_ERR_UNSUPPORTED, "ceil(R / 16) x ceil(K / 512) has to be below 2^24 (got %d rows of %d)", d.R, d.K);
   std::unique_ptr<mtk_plan> p(new mtk_plan());
   p->ctx = ctx;
   p->kind = quantize ? PLAN_MX_QUANT : PLAN_MX_DEQUANT;
@@ -332,9 +332,10 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
   if ((s = check_ld(d.lda, d.K, "lda", &d.lda)) != MTK_OK || (s = check_ld(d.ldc, d.N, "ldc", &d.ldc)) != MTK_OK) return s;
   const long long groups = d.E ? d.E : 1;
   const int k_tiles = mx_k_tiles(d.K);
-  // scales of an operand are read with 32-bit offsets: 2^31 bytes
-  if ((double)d.T * k_tiles * 8 > 2147483392.0 || (double)groups * d.N * k_tiles * 8 > 2147483392.0)
-    return fail(MTK_ERR_UNSUPPORTED, "T x K and E x N x K up to 2^36 are supported");
+  // scales of an operand are read with 32-bit offsets, 8 bytes a row and K-tile; and the rows' own launch can have so many
+  constexpr long long kMostScales = (1ll << 28) - 32;
+  if ((long long)d.T * k_tiles > kMostScales || groups * d.N > kMostScales / k_tiles)
+    return fail(MTK_ERR_UNSUPPORTED, "T x ceil(K / 256) and E x N x ceil(K / 256) up to 2^28 - 32 are supported");
   mtk_mx_gemm_kargs a{};
   a.E = (int)groups;
   a.T = d.T;

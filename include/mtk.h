@@ -484,7 +484,8 @@ typedef struct {
   int dtype; /* MTK_F16 or MTK_BF16 */
 } mtk_mx_rows_desc;
 
-/* 16-bit rows [R][ld] into codes and scales. The weights [E][N][K] of a grouped product are E x N rows. */
+/* 16-bit rows [R][ld] into codes and scales. The weights [E][N][K] of a grouped product are E x N rows. K and ld up to 2^22,
+ * ceil(R / 16) x ceil(K / 512) below 2^24. */
 int mtk_mx_quantize_plan(mtk_ctx *ctx, const mtk_mx_rows_desc *desc, mtk_plan **out);
 typedef struct {
   const void *src;      /* 2-byte aligned; rows of 16-byte alignment (ld a multiple of 8) are read fastest */
@@ -505,7 +506,8 @@ int mtk_mx_dequantize_run(const mtk_plan *plan, const mtk_mx_dequantize_args *ar
  * their sums fp32; C is in 16 bits, rounded once.
  * quantize_a: A are 16-bit rows [T][lda] that the run brings into the format first (in the workspace, or on chip), with the
  * result of mtk_mx_quantize; else codes and scales of T rows.
- * T x K and E x N x K up to 2^36, E up to 2^14, K, N and leading dimensions up to 2^22. */
+ * T x ceil(K / 256) and E x N x ceil(K / 256) up to 2^28 - 32 (2^36 values), E up to 2^14, K, N and leading dimensions up to 2^22, tiles
+ * as in mtk_grouped_gemm with even leading dimensions. */
 typedef struct {
   int E, T, N, K;
   int lda, ldc; /* 0 = packed; lda: with quantize_a only */

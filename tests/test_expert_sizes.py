@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import example_matmul_metal4_amd as mtk
-from oracle import kv
+from oracle import experts, kv
 
 UNSUPPORTED = mtk.MTK_ERR_UNSUPPORTED
 FILL = 0x1234
@@ -76,6 +76,25 @@ def test_borders_of_gradients(odd, bias):
     assert kernels(gradient(E, T, N, less, has_bias=bias))
 
 
+@pytest.mark.parametrize("K", [1, 256, 257, 2048, 1 << 22])
+def test_borders_of_4_bits(K):
+    # rows x ceil(K / 256) up to 2^28 - 32, of A and of B, and what a product takes can be brought into the format and back
+    rows = ((1 << 28) - 32) // up(K, 256)
+    for quantize_a in (False, True):
+        assert kernels(mtk.MxGemmPlan(None, rows, 1, K, quantize_a=quantize_a))
+        message = refused(mtk.MxGemmPlan, None, rows + 1, 1, K, quantize_a=quantize_a)
+        assert "2^28 - 32" in message
+    E = up(rows, 1 << 22)
+    N = rows // E
+    assert kernels(mtk.MxGemmPlan(None, 1, N, K, E=E))
+    assert refused(mtk.MxGemmPlan, None, 1, N + 1 + 32 // E, K, E=E) or N == 1 << 22
+    for make in (mtk.MxQuantizePlan, mtk.MxDequantizePlan):
+        assert kernels(make(None, rows, K))
+        # ceil(R / 16) x ceil(K / 512) below 2^24
+        most = 16 * (((1 << 24) - 1) // up(K, 512))
+        assert kernels(make(None, most, K)) and refused(make, None, most + 1, K)
+
+
 @pytest.mark.gpu
 def test_rows_of_many_small_tiles(dev):
     # 2^22 tiles and more, of one row block and column each
@@ -131,3 +150,28 @@ def test_gradients_of_many_small_tiles(dev):
     assert not got[rest].any()
     for x in d:
         x.free()
+
+
+@pytest.mark.gpu
+def test_rows_into_4_bits_of_many_workgroups(dev):
+    # more than 2^23 workgroups, 2^31 threads: one value a row, of those that a block of one value holds exactly
+    R, K, dtype = (1 << 27) + 77, 1, "bf16"
+    rng = np.random.default_rng(3)
+    values = kv.bits_of(np.array([0.0, 1.0, -1.5, 2.0, -3.0, 2.0 ** -120, 1.5 * 2.0 ** 100]), dtype)
+    x = values[rng.integers(0, len(values), R, dtype=np.uint8)]
+    src, back = dev.upload(x), dev.empty(2 * (R + 64))
+    codes, scales = (dev.empty(n) for n in mtk.mx_bytes(R, K))  # 17 GB and 1 GB
+    dev.fill_u16(back, FILL, R + 64)
+    there, here = mtk.MxQuantizePlan(dev, R, K, dtype=dtype), mtk.MxDequantizePlan(dev, R, K, dtype=dtype)
+    print(there.describe(), here.describe(), flush=True)
+    there.run(src, codes, scales)
+    here.run(codes, scales, back)
+    dev.sync()
+    got = dev.download(back, (R + 64,), np.uint16)
+    assert (got[R:] == FILL).all() and np.array_equal(got[:R], x)
+    # the last rows' codes, padding and all
+    row = codes.nbytes // R
+    last = dev.download(mtk.DeviceBuffer(dev, codes.ptr + (R - 9) * row, 9 * row), (9, row), np.uint8)
+    assert np.array_equal(last, experts.quantise(x[R - 9:, None], dtype)[0])
+    for b in (src, back, codes, scales):
+        b.free()
