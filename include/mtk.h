@@ -460,7 +460,7 @@ typedef struct {
   const void *A, *dC;
   const int32_t *row_start;
   void *dB;        /* [E][N][K] or [E][K][N], 16-byte aligned; 16 bits, or fp32 with out_f32 */
-  void *dbias;     /* [E][N], the same type, with has_bias */
+  void *dbias;     /* [E][N], the same type, with has_bias; 4-byte aligned */
   void *workspace;
 } mtk_grouped_grad_args;
 int mtk_grouped_grad_run(const mtk_plan *plan, const mtk_grouped_grad_args *args);
@@ -496,8 +496,8 @@ int mtk_mx_quantize_run(const mtk_plan *plan, const mtk_mx_quantize_args *args);
 /* And back, each value exactly (f16 values below 2^-14 to the nearest subnormal). Places between K and ld are left. */
 int mtk_mx_dequantize_plan(mtk_ctx *ctx, const mtk_mx_rows_desc *desc, mtk_plan **out);
 typedef struct {
-  const void *codes, *scales;
-  void *dst;
+  const void *codes, *scales; /* 16-byte aligned */
+  void *dst;                  /* 2-byte aligned */
 } mtk_mx_dequantize_args;
 int mtk_mx_dequantize_run(const mtk_plan *plan, const mtk_mx_dequantize_args *args);
 
@@ -518,12 +518,12 @@ typedef struct {
 
 int mtk_mx_gemm_plan(mtk_ctx *ctx, const mtk_mx_gemm_desc *desc, mtk_plan **out);
 typedef struct {
-  const void *A, *a_scales; /* 16-bit rows and NULL with quantize_a */
+  const void *A, *a_scales; /* 16-bit rows (2-byte aligned) and NULL with quantize_a */
   const void *B, *b_scales; /* codes and scales: 16-byte aligned */
   const void *bias;
   const int32_t *row_start; /* [E + 1]; NULL where E is 0 */
-  void *C;
-  void *workspace;          /* runs that may overlap need one each */
+  void *C;                  /* C and bias: 2-byte aligned */
+  void *workspace;          /* 16-byte aligned; runs that may overlap need one each */
 } mtk_mx_gemm_args;
 int mtk_mx_gemm_run(const mtk_plan *plan, const mtk_mx_gemm_args *args);
 
