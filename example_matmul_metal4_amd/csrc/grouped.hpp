@@ -189,8 +189,8 @@ __device__ __forceinline__ mtk_tile_args grad_args(const mtk_grouped_kargs &g, i
 
 // dbias_e[n] = sum over the group's rows of dC[t][n]: 64 columns from n0 on per workgroup, 8 neighbours a lane, 64 rows a step of a
 // wavefront, all in flight at once, the steps over the W wavefronts. Sums in 32 bits: a lane's rows in order, then rows apart by 1, 2
-// and 4 of 8, then the wavefronts in order. Latency bounds it: 343 rows of the largest of 24 groups, 1023 columns, a column a lane: 16
-// wavefronts 4.2 us, 8 15.3.
+// and 4 of 8, then the wavefronts in order. Latency bounds it where groups have few rows, HBM where a launch of its own reads dC
+// again.
 template <int DT, int W>
 __device__ __forceinline__ void bias_columns(const mtk_grouped_kargs &g, const void *dC, int ld, int N, void *out, int e, int n0) {
   __shared__ float sums[W][64];
@@ -244,8 +244,9 @@ __device__ __forceinline__ void bias_columns(const mtk_grouped_kargs &g, const v
     ((uint16_t *)out)[at] = to_bits<DT>(t);
 }
 
-// The bias's gradient as a launch of its own, beside large tiles.
-constexpr int kBiasWaves = 16;
+// The bias's gradient as a launch of its own, beside large tiles. 4, 8 and 16 wavefronts, us of the launch: 8192 rows over 16 groups of 4096
+// columns 16.0, 15.6, 17.8; 16384 over 2 of 1024 40.7, 24.1, 24.7; 1000 over 24 of 1024 6.9, 6.5, 7.7; 30000 of one of 4096 -, 114, 118.
+constexpr int kBiasWaves = 8;
 template <int DT>
 __device__ __forceinline__ void grouped_bias_grad(const mtk_grouped_kargs &g) {
   const int e = blockIdx.x / g.tiles_n;

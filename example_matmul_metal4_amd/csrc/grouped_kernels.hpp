@@ -60,4 +60,4 @@ MTK_GROUPED(nt_128, 256, mtk_grouped_ops::nt_128)
 MTK_GROUPED(nn_128, 256, mtk_grouped_ops::nn_128)
 MTK_GROUPED(grad_256, 512, mtk_grouped_ops::grad_256)
 MTK_GROUPED(grad_128, 256, mtk_grouped_ops::grad_128)
-MTK_GROUPED(bias_grad, 1024, mtk::grouped_bias_grad<MTK_GROUPED_DT>)
+MTK_GROUPED(bias_grad, 512, mtk::grouped_bias_grad<MTK_GROUPED_DT>)

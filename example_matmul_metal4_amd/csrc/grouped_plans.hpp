@@ -227,7 +227,7 @@ int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out
   const long long bias_tiles = d.has_bias ? (long long)d.E * tiles_across(64, d.N) : 0, lead = (bias_tiles + 7) / 8 * 8;
   auto fits = [&](const TileCost &c) {
     if (c.tile == 64) return launches(wgs(64) + lead, 64 * c.waves);
-    return wgs(c.tile) <= INT32_MAX && launches(bias_tiles, 1024);
+    return wgs(c.tile) <= INT32_MAX && launches(bias_tiles, 512);
   };
   const double k_tiles = std::max(1.0, d.T / busy_groups(d.E, d.T) / 64);
   const TileCost *chosen = choose_tile(kGradient, even, cus, k_tiles, 1e-6 * ((d.out_f32 ? 4.0 : 2.0) * d.E * d.N * d.K + 2.0 * d.T * ((double)d.N + d.K)),
@@ -262,7 +262,7 @@ int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out
     b.N = d.N;
     b.lda = d.ldc;
     b.tiles_n = tiles_across(64, d.N);
-    add_launch(p.get(), head + "_bias_grad", bias_tiles, 1024, b);
+    add_launch(p.get(), head + "_bias_grad", bias_tiles, 512, b);
     p->launches.back().role = ROLE_REDUCE;
   }
   p->flops = 2.0 * d.T * d.N * d.K;

@@ -429,7 +429,7 @@ int mtk_kv_attn_run(const mtk_plan *plan, const mtk_kv_attn_args *args);
  * T up to 2^30, E up to 2^14, leading dimensions, N and K up to 2^22. Tiles are counted in 32 bits: E x ceil(T / t) x ceil(N / t)
  * (gradients: E x ceil(N / t) x ceil(K / t)) is below 2^31, t 256 where the leading dimensions of the two operands that are read are
  * even, else 64. With an odd one (T / 64 + E) x ceil(N / 64) is below 2^26, the workgroups of one launch (gradients:
- * E x ceil(N / 64) x (ceil(K / 64) + 1) up to 2^26 - 8); with even ones and a bias gradient E x ceil(N / 64) is below 2^22.
+ * E x ceil(N / 64) x (ceil(K / 64) + 1) up to 2^26 - 8); with even ones and a bias gradient E x ceil(N / 64) is below 2^23.
  * Where those leading dimensions are even, the two operands are 4-byte aligned; with an odd one they may have any 2-byte alignment,
  * and small tiles run, more slowly. C and the bias
  * are 2-byte aligned. */
