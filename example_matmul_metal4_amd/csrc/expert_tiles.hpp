@@ -185,7 +185,7 @@ struct ForwardTiles {
   __device__ __forceinline__ int ldc() const { return g.ldc; }
   __device__ __forceinline__ bool f32() const { return false; }
   // Through the caches, where the next operator finds them: a product in 4 bits of 4096 x 14336 x 4096 and the launch that reads its
-  // outputs 150 us, past them 158.
+  // outputs 151 us, past them 154.
   __device__ __forceinline__ bool streamed() const { return false; }
   __device__ __forceinline__ ExpertTile get(int i) const {
     ExpertTile t{};
@@ -220,8 +220,8 @@ struct ForwardTiles {
 // A round's workgroups have one group or few, with few K-tiles each, and write as much as they read: the first K-tiles of a new group
 // would come from HBM behind the last round's outputs. So the workgroups ask for the group's rows while they are busy with the one
 // before it (warm), two K-tiles before its end, each for its part of the columns that its tile has: rows i * tiles_n + n of A's,
-// i * tiles_m + m of B's, a lane for a line of 128 bytes. 8192 rows over 16 groups of 4096 x 4096: inputs in HBM 342 -> 315 us, in the
-// last-level cache 304 -> 302. (Forward products that ask for later K-tiles of their weights are slower: 306 -> 330.)
+// i * tiles_m + m of B's, a lane for a line of 128 bytes. 8192 rows over 16 groups of 4096 x 4096: inputs in HBM 340 -> 306 us, in the
+// last-level cache 293 -> 294. (Forward products that ask for later K-tiles of their weights are slower: 306 -> 330.)
 template <int BM, int BN>
 struct GradTiles {
   static constexpr bool kTurned = false;
@@ -498,8 +498,8 @@ __device__ __forceinline__ void expert_tiles(const TILES &tiles) {
     const size_t at = (size_t)(wave_m * WTM) * (size_t)ldc + (size_t)(wave_n * WTN);
     if (tiles.f32()) {
       float *C = (float *)t.c + at;
-      // Past the caches where rows are whole halves of lines: 7183 rows, 128 groups of 6640 x 128 206 -> 117 us; rows of other lengths
-      // leave parts of lines for the L2 to join: 471 rows, 128 of 256 x 2616 199 -> 104 through it.
+      // Past the caches where rows are whole halves of lines: 7183 rows, 128 groups of 6640 x 128 119 -> 85 us; rows of other lengths
+      // leave parts of lines for the L2 to join: 471 rows, 128 of 256 x 2616 190 -> 119 through it.
       const bool streamed = (ldc & 15) == 0 && ((uintptr_t)C & 63) == 0;
 #pragma unroll
       for (int j = 0; j < TN; ++j) {

@@ -80,9 +80,9 @@ TileCount count_tiles(int E, int T, int tile, int waves, long long tiles_n, int 
 // E (1 - exp(-T / E)) are taken to have rows, as if each row chose one of E, and each to have half a block that is not full. Fitted
 // to launches of 400 forward products, 300 gradients and 350 products in few bits, each by every kernel (random sizes, T to 16384,
 // N and K 64 to 14336): the kernel chosen takes 1.02, 1.04 and 1.01 times (geometric mean) the time of the fastest.
-// Examples, us (tiles of 256, of 128, of 64 with 8, 4, 1 wavefronts): 256 rows over 8 groups of 14336 x 4096: 222, 207, 162, 156, 152;
-// 8192 over 16 of 4096 x 4096: 303, 345, 626, 563, 537; 16 over 32 of 2048 x 2048: 40, 31, 25, 22, 40. Gradients: 8192 over 16 of 4096
-// x 4096: 297, 357, 1294, 777, 601; 1000 over 24 of 1023 x 520 with the bias': -, -, 54, 35, 27.
+// Examples, us (tiles of 256, of 128, of 64 with 8, 4, 1 wavefronts): 256 rows over 8 groups of 14336 x 4096: 191, 163, 157, 155, 149;
+// 8192 over 16 of 4096 x 4096: 292, 335, 605, 534, 518; 16 over 32 of 2048 x 2048: 29, 22, 22, 19, 39. Gradients: 8192 over 16 of 4096
+// x 4096: 294, 352, 1289, 777, 593; 1000 over 24 of 1023 x 520 with the bias': -, -, 56, 36, 27.
 struct TileCost {
   int tile, waves, per_cu;  // rows and columns of a tile (32: 64 columns); wavefronts and workgroups per CU
   double start, round, step, full, byte;
@@ -103,9 +103,10 @@ constexpr TileCost kFewBits[] = {{256, 8, 1, 10.3, 0.43, 0.83, 1.50, 0.27, 0},
                                  {64, 8, 1, 5.7, 0.29, 1.60, 1.34, 0.21, 0},
                                  {32, 8, 1, 5.3, 0.49, 1.04, 0.82, 0.18, 0}};
 
-// Weights that one row block reads are loaded past the caches where all groups' are more than the last-level cache holds, so that the
-// next call finds none of them: 256 rows over 8 groups of 14336 x 4096 165 -> 150 us (6.3 TB/s), 16 over 32 of 2048 x 2048 32.3 ->
-// 30.3. Smaller ones may be there still: 14336 x 4096 in 4 bits, 16 rows, call after call 8.6 us, past the caches 9.5.
+// Weights that one row block reads are loaded past the caches where all groups' are more than the last-level cache holds: 256 rows over 8
+// groups of 14336 x 4096 168 -> 151 us (6.2 TB/s), 64 over 64 of 2048 x 8192 in 4 bits 65.8 -> 58.9, 16 over 32 of 2048 x 2048, other
+// weights each call, 21.0 -> 19.4. Where the next call has the same few groups they could have stayed there (the last one, call after call:
+// 17.6 -> 18.4); smaller weights may be there still: 14336 x 4096 in 4 bits, 16 rows, call after call 9.5 us, past the caches 10.0.
 constexpr double kLastLevelCache = 256e6;
 
 // Rows of weights that lie a power of two apart have the same place of K on few of the memory's channels, and workgroups that go through
@@ -119,7 +120,7 @@ constexpr double kTurnedRows = 2048;
 
 // Log2 of the parts of a group's columns that start apart. Groups start apart themselves; of one that has fewer than four row blocks (tile_at),
 // an XCD has an eighth of the columns, of more row blocks or groups more of them, and workgroups of one XCD that start together share
-// what its L2 holds: 8192 rows over 16 groups of 4096 x 4096 with eight parts 303 us, with one 294.
+// what its L2 holds: 8192 rows over 16 groups of 4096 x 4096 with eight parts 301 us, with one 295.
 int log_turn_parts(int E, int T, int tile) {
   const long long blocks = ((long long)T + (long long)tile * E - 1) / ((long long)tile * E), runs = E * ((blocks + 3) / 4);
   return runs == 1 ? 3 : runs == 2 ? 2 : runs <= 4 ? 1 : 0;
@@ -238,9 +239,8 @@ int plan_grouped_grad(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out
   a.tiles_m = tiles_across(tile, a.M);
   a.tiles_n = tiles_across(tile, a.N);
   long long grid = tile_grid(tile, cus, wgs(tile));
-  // Quarter tiles have the bias's sums in their launch: 1000 rows over 24 groups of 1023 x 520 33.8 -> 29.9 us, 2000 over 4 of 300 x 301
-  // 16.6 -> 11.0 (1000 over 8 of 1024 x 512, whose workgroups fill a CU each, 9.9 -> 10.2). Large tiles are a
-  // persistent grid; beside them the bias has a launch of its own.
+  // Quarter tiles have the bias's sums in their launch: 1000 rows over 24 groups of 1023 x 520 33.2 -> 27.2 us, 2000 over 4 of 300 x 301
+  // 13.1 -> 8.3, 1000 over 8 of 1024 x 512 13.9 -> 11.7. Large tiles are a persistent grid; beside them the bias has a launch of its own.
   const bool one_launch = d.has_bias && tile == 64;
   if (one_launch) {
     a.has_bias = d.trans_b ? 1 : 2;
@@ -360,9 +360,9 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
                                        [&](const TileCost &c) { return count(c).fits; });
   if (!chosen) return fail(MTK_ERR_UNSUPPORTED, "%lld groups of up to %d rows with N %d have too many tiles", groups, d.T, d.N);
   TileCost kind = *chosen;
-  // Few rows are brought into the format by the product's own workgroups, each of them all that it needs: 0.2 us for two rows and a
-  // K-tile of a wavefront, against 2.4 for the launch. 14336 x 4096: 1 row 6.6 us (with the launch 8.3), 8 rows 8.5 (8.3), 16 10.2
-  // (8.6); 2048 x 2048: 16 rows 7.0 (7.3); 4096 x 14336: 1 row 12.6 (12.1).
+  // Few rows are brought into the format by the product's own workgroups, each of them all that it needs, which takes longer than the
+  // launch before it where a wavefront has many rows and K-tiles. 14336 x 4096: 1 row 7.7 us (with the launch 10.9), 8 rows 9.4 (11.3), 16
+  // 11.3 (11.2); 2048 x 2048: 16 rows 7.1 (8.4); 4096 x 14336: 1 row 12.7 (13.8); 64 over 64 groups of 2048 x 8192 66.8 (60.3).
   const TileCost &few = kFewBits[3];
   const double per = d.E ? std::max(1.0, d.T / busy) : d.T, rounds = std::ceil(busy * tiles_across(32, d.N) / cus);
   const bool inside = d.quantize_a && d.T <= 32.0 * busy && std::ceil(per / 2) * std::ceil(k_tiles / 8.0) * rounds <= 8 && count(few).fits;

@@ -44,14 +44,10 @@ def test_the_kernels_are_those():
         assert plan_of(None, op, *rest).describe().split("16_")[-1] == kernel, (op, kernel)
 
 
-@pytest.mark.gpu
-@pytest.mark.parametrize("case", CASES, ids=lambda c: f"{c[0]}-{c[1]}-{c[6]}")
-def test_bits_of_a_row(dev, case):
-    op, kernel, E, T, N, K, dtype, rows16 = case
-    rng = np.random.default_rng(K + T)
-    rows, g = max(1, T // 3), E // 2
-    # Places of very different sizes, whose second half takes the sum of the first one away again: what is left are the roundings on the
-    # way (and the few places behind), so that an order of the additions other than that of another run shows in the result's bits.
+def cancelling(rng, E, N, K, dtype):
+    """EQUAL rows and the weights of E groups, of places of very different sizes, whose second half takes the sum of the first one away again:
+    what is left are the roundings on the way (and the few places behind), so that another order of the additions shows in the result's
+    bits."""
     X, W = rng.standard_normal((EQUAL, K)), rng.standard_normal((E, N, K))
     half = K // 512 * 256
     size = np.exp2(rng.integers(0, 11, half // 32)).repeat(32)
@@ -59,7 +55,16 @@ def test_bits_of_a_row(dev, case):
     W[:, :, :half] *= size
     X[:, half:2 * half] = -X[:, :half]
     W[:, :, half:2 * half] = W[:, :, :half]
-    X, W = kv.bits_of(X, dtype), kv.bits_of(W.reshape(E * N, K), dtype)
+    return kv.bits_of(X, dtype), kv.bits_of(W.reshape(E * N, K), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", CASES, ids=lambda c: f"{c[0]}-{c[1]}-{c[6]}")
+def test_bits_of_a_row(dev, case):
+    op, kernel, E, T, N, K, dtype, rows16 = case
+    rng = np.random.default_rng(K + T)
+    rows, g = max(1, T // 3), E // 2
+    X, W = cancelling(rng, E, N, K, dtype)
     X = X[np.arange(rows) % EQUAL]
     A, bias = kv.bits_of(rng.standard_normal((T, K)), dtype), kv.bits_of(np.zeros((E, N)), dtype)
     plan = plan_of(dev, op, E, T, N, K, dtype, rows16)
@@ -92,4 +97,36 @@ def test_bits_of_a_row(dev, case):
         off = np.argwhere(got != got[np.arange(rows) % EQUAL])
         assert len(off) == 0, f"{len(off)} of {got.size} values of equal rows of the group differ, the first at {off[:3].tolist()}"
     for x in (*weights, d_bias, C, ws):
+        x.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op, E, T, N, K, dtype, rows16", [
+    ("grouped", 1, 1000, 700, 1100, "bf16", True), ("grouped", 1, 1900, 6000, 1100, "f16", True), ("grouped", 1, 300, 333, 1101, "f16", True),
+    ("mx", 0, 150, 700, 4200, "bf16", True), ("mx", 0, 1000, 2000, 2100, "f16", False), ("mx", 0, 1900, 9000, 2304, "bf16", True), ("mx", 1, 900, 640, 2304, "f16", False),
+], ids=str)
+def test_bits_of_equal_rows_of_one_group(dev, op, E, T, N, K, dtype, rows16):
+    rng = np.random.default_rng(K + T)
+    X, W = cancelling(rng, 1, N, K, dtype)
+    A = X[np.arange(T) % EQUAL]
+    plan = plan_of(dev, op, E, T, N, K, dtype, rows16)
+    print(plan.describe(), flush=True)
+    d = [dev.upload(x) for x in ([W] if op == "grouped" else experts.quantise(W, dtype))]
+    a = [dev.upload(x) for x in ([A] if rows16 else experts.quantise(A, dtype))]
+    bias, C, ws = dev.upload(np.zeros(N, np.uint16)), dev.empty(2 * T * N), dev.empty(max(16, plan.workspace_bytes))
+    got = []
+    for first in (0, 1, 5) if E else (0,):
+        starts = dev.upload(np.array([first, T], np.int32)) if E else None
+        if op == "grouped":
+            plan.run(a[0], d[0], bias, starts, C)
+        else:
+            plan.run(a[0], None if rows16 else a[1], *d, bias, starts, C, ws)
+        dev.sync()
+        out = dev.download(C, (T, N), np.uint16)[first:]
+        got.append(out[(np.arange(T - first) + first) % EQUAL == 0])
+        assert (out == out[(np.arange(T - first)) % EQUAL]).all(), f"equal rows differ behind {first} rows of no group"
+        if starts is not None:
+            starts.free()
+    assert all((g == got[0][0]).all() for g in got)
+    for x in (*d, *a, bias, C, ws):
         x.free()
