@@ -210,7 +210,7 @@ struct ForwardTiles {
     }
     t.c = (char *)g.C + ((size_t)row * (size_t)g.ldc + (size_t)at.n0) * 2;
     t.bias = g.has_bias ? (const uint16_t *)g.bias + (size_t)gt.e * (size_t)g.N + at.n0 : nullptr;
-    if constexpr (kTurned) t.turn = g.turned ? group_turn(group_turn_place(gt.e, at.n0 / BN, g.tiles_n, g.turned - 1), whole()) : 0;
+    if constexpr (kTurned) t.turn = g.turns.on ? group_turn(group_turn_place(gt.e, at.n0 / BN, g.turns), whole()) : 0;
     return t;
   }
 };
@@ -329,7 +329,7 @@ struct MxTiles {
     t.b_bytes = (uint32_t)t.cols * row_b;
     t.c = (char *)g.C + ((size_t)row * (size_t)g.ldc + (size_t)at.n0) * 2;
     t.bias = g.has_bias ? (const uint16_t *)g.bias + col : nullptr;
-    t.turn = g.turned ? group_turn(group_turn_place(gt.e, at.n0 / BN, g.tiles_n, g.turned - 1), whole()) : 0;
+    t.turn = g.turns.on ? group_turn(group_turn_place(gt.e, at.n0 / BN, g.turns), whole()) : 0;
     return t;
   }
 };

@@ -159,7 +159,7 @@ __device__ __forceinline__ void grouped_quarter(const mtk_grouped_kargs &g) {
   const TileAt at = tile_at<64, 64>(gt.t, gt.blocks, g.tiles_n);
   const mtk_tile_args a = group_args<64, ANY>(g, gt.e, gt.first + at.m0, gt.rows - at.m0);
   using A = std::conditional_t<ANY, QuarterAny<false>, QuarterOp<false, false>>;
-  quarter_tile<DT, A, BN, ANY, W, true>(a, A{}, TileAt{0, at.n0, g.b_once && gt.blocks == 1, g.turned ? group_turn(group_turn_place(gt.e, at.n0 / 64, g.tiles_n, g.turned - 1), g.K / kBK) : 0});
+  quarter_tile<DT, A, BN, ANY, W, true>(a, A{}, TileAt{0, at.n0, g.b_once && gt.blocks == 1, g.turns.on ? group_turn(group_turn_place(gt.e, at.n0 / 64, g.turns), g.K / kBK) : 0});
 }
 
 // Gradients: K runs over the group's rows, of which both operands hold K rows of M and of N columns. A group without a row has

@@ -188,7 +188,7 @@ int plan_grouped(mtk_ctx *ctx, const mtk_grouped_desc *d_in, mtk_plan **out) {
   a.k_tiles = (d.K + 63) / 64;
   a.has_bias = d.has_bias ? 1 : 0;
   a.b_once = 2.0 * d.E * d.N * d.K > kLastLevelCache ? 1 : 0;
-  a.turned = d.trans_b && d.T < kTurnedRows * busy ? 1 + log_turn_parts(d.E, d.T, tile) : 0;
+  if (d.trans_b && d.T < kTurnedRows * busy && d.K >= 128) a.turns = group_turns_of(log_turn_parts(d.E, d.T, tile), a.tiles_n);
   const long long grid = count(kind).grid;
   std::unique_ptr<mtk_plan> p(new mtk_plan());
   p->ctx = ctx;
@@ -368,8 +368,8 @@ int plan_mx_gemm(mtk_ctx *ctx, const mtk_mx_gemm_desc *d_in, mtk_plan **out) {
   const bool inside = d.quantize_a && d.T <= 32.0 * busy && std::ceil(per / 2) * std::ceil(k_tiles / 8.0) * rounds <= 8 && count(few).fits;
   if (inside) kind = few;
   const int tile = kind.tile;
-  a.turned = d.T < kTurnedRows * busy ? 1 + log_turn_parts((int)groups, d.T, tile) : 0;
   a.tiles_n = tiles_across(tile, d.N);
+  if (d.T < kTurnedRows * busy && k_tiles > 1) a.turns = group_turns_of(log_turn_parts((int)groups, d.T, tile), a.tiles_n);
   const long long grid = count(kind).grid;
   std::unique_ptr<mtk_plan> p(new mtk_plan());
   p->ctx = ctx;

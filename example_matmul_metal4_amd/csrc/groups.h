@@ -61,11 +61,19 @@ MTK_GROUP_FN int group_turned(int k, int turn, int full) {
 }
 // Where the tiles of `place` (one of eight) start.
 MTK_GROUP_FN int group_turn(int place, int full) { return (int)((int64_t)(place & 7) * full >> 3); }
-// The place of group e's tiles that have column block n of `across`, where 2^log_parts parts of a group's columns start apart. Nothing of it
-// depends on how many rows any group has, so a row's sums have one order wherever its tile lies. Groups that follow each other start
-// far apart, and so do those that are eight apart, whose weights may lie a power of two apart as their rows do.
-MTK_GROUP_FN int group_turn_place(int e, int n, int across, int log_parts) {
-  return 5 * e + 3 * (e >> 3) + (log_parts ? (n << log_parts) / across << (3 - log_parts) : 0);
+// Where tiles start: 2^log_parts parts of a group's columns start apart, and a column block is 1 / 65536 of `per_block` parts wide.
+typedef struct {
+  int32_t on, log_parts, per_block;
+} group_turns;
+MTK_GROUP_FN group_turns group_turns_of(int log_parts, int across) {
+  const group_turns t = {1, log_parts, (65536 << log_parts) / across};
+  return t;
+}
+// The place of group e's tiles that have column block n. Nothing of it depends on how many rows any group has, so a row's sums have one
+// order wherever its tile lies. Groups that follow each other start far apart, and so do those that are eight apart, whose weights
+// may lie a power of two apart as their rows do.
+MTK_GROUP_FN int group_turn_place(int e, int n, group_turns t) {
+  return 5 * e + 3 * (e >> 3) + ((n * t.per_block >> 16) << (3 - t.log_parts));
 }
 
 #endif

@@ -9,7 +9,9 @@
 
 #include <stdint.h>
 
-#define MTK_KARGS_VERSION 22
+#include "groups.h"
+
+#define MTK_KARGS_VERSION 23
 
 /* In-workgroup split-K: bytes of workspace slot per output tile of BM x BM (256 or 128). Each
  * wavefront keeps these accumulator blocks (32 x 32 fp32, 4 KB) of its running sum in the slot,
@@ -206,7 +208,7 @@ typedef struct {
   int32_t has_bias; /* gradients on quarter tiles: dC is A (1) or B (2), dbias is `bias` */
   int32_t lead;     /* ... and so many workgroups of the launch have it */
   int32_t b_once;   /* weights that one row block reads are loaded past the caches */
-  int32_t turned;   /* K-tiles are taken from different ones on: 1 + log_parts of group_turn_place; 0: all from the first */
+  group_turns turns; /* the K-tiles that tiles start at (groups.h) */
 } mtk_grouped_kargs;
 
 /* Rows into blocks of 32 four-bit values with one scale, and back (mx.h has the layout). */
@@ -230,7 +232,7 @@ typedef struct {
   int32_t E, T, N, K, k_tiles;
   int32_t ldc, tiles_n, has_bias;
   int32_t b_once; /* weights that one row block reads are loaded past the caches */
-  int32_t turned; /* as above */
+  group_turns turns;
 } mtk_mx_gemm_kargs;
 
 #endif

@@ -47,7 +47,7 @@ __device__ __forceinline__ void mx_few(const mtk_mx_gemm_kargs &g) {
   u32x4 va[QUANT ? 16 : 4 * MB] = {}, vb[8];
   uint32_t ve[16] = {};
   uint32_t na[MB], nb[2];
-  const int turn = g.turned ? group_turn(group_turn_place(gt.e, at.n0 / 64, g.tiles_n, g.turned - 1), g.k_tiles) : 0;
+  const int turn = g.turns.on ? group_turn(group_turn_place(gt.e, at.n0 / 64, g.turns), g.k_tiles) : 0;
   auto load = [&](int k) {
     const int kt = group_turned(k, turn, g.k_tiles);
 #pragma unroll

@@ -1,5 +1,9 @@
 """A row of a grouped product has the same bits whatever rows the other groups have and wherever its own group starts: results of a
 serving batch do not depend on who else is in it. On every kernel whose tiles go through K from different places."""
+import os
+import shutil
+import subprocess
+
 import numpy as np
 import pytest
 
@@ -56,6 +60,45 @@ def cancelling(rng, E, N, K, dtype):
     X[:, half:2 * half] = -X[:, :half]
     W[:, :, half:2 * half] = W[:, :, :half]
     return kv.bits_of(X, dtype), kv.bits_of(W.reshape(E * N, K), dtype)
+
+
+PLACES = r"""
+#include "groups.h"
+#include <cstdio>
+#include <initializer_list>
+int main() {
+  for (int log_parts = 0; log_parts < 4; ++log_parts)
+    for (int across : {1, 2, 3, 5, 7, 8, 9, 31, 32, 33, 100, 224, 1000, 4097, 40000, 65535, 65536}) {
+      const group_turns t = group_turns_of(log_parts, across);
+      const int step = 8 >> log_parts;
+      int last = -1, parts = 0;
+      for (int n = 0; n < across; ++n) {  // parts of neighbouring columns, in order, each about as wide as the others
+        const int p = group_turn_place(0, n, t);
+        if (!t.on || p % step || p < 0 || p >= 8 || p < last) return printf("%d of %d, %d parts: %d\n", n, across, 1 << log_parts, p), 1;
+        parts += p != last;
+        last = p;
+        if (group_turn_place(16383, n, t) - p != group_turn_place(16383, 0, t)) return 2;
+      }
+      if (across >= 1 << log_parts ? parts != 1 << log_parts : parts != across) return printf("%d: %d parts\n", across, parts), 3;
+    }
+  int had = 0;
+  for (int e = 0; e < 8; ++e) had |= 1 << (group_turn_place(e, 0, group_turns_of(0, 1)) & 7);
+  if (had != 255) return 4;  // eight groups in a row start at eight places
+  for (int e = 0; e < 64; ++e)
+    if (!((group_turn_place(e, 0, group_turns_of(0, 1)) - group_turn_place(e + 8, 0, group_turns_of(0, 1))) & 7)) return 5;
+  return 0;
+}
+"""
+
+
+def test_places(tmp_path):
+    if shutil.which("g++") is None:
+        pytest.skip("needs g++")
+    src, exe = tmp_path / "places.cpp", tmp_path / "places"
+    src.write_text(PLACES)
+    subprocess.run(["g++", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover=all", f"-I{os.path.join(mtk.PKG, 'csrc')}", str(src), "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0, (r.returncode, r.stdout, r.stderr)
 
 
 @pytest.mark.gpu
